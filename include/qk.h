@@ -46,6 +46,9 @@ extern "C" {
    Q6_K block is only 2-byte aligned at odd block indices).  Accepted
    wherever Q6_K is. */
 #define QK_TYPE_Q6_K_SPLIT 114
+/* Types of paged cache rows (besides QK_TYPE_F16); no weights have them. */
+#define QK_TYPE_I8 24
+#define QK_TYPE_F8_E4M3 120
 
 /* Status codes. */
 #define QK_OK 0
@@ -399,6 +402,149 @@ int qk_attention_split_f32(const float *q, const float *key_cache, const float *
 size_t qk_argmax_rows_workspace_bytes(int n, int rows);
 int qk_argmax_rows_f32(const float *v, int n, int64_t ldv, int rows, int32_t *out, void *workspace,
                        qk_stream stream);
+
+/* ------------------------------------- paged cache of a serving step -- */
+
+/* No reference counterpart (its one fp32 cache holds one sequence).  A step
+   over a paged cache: qk_rope_tables_f32 once, then per layer
+   qk_rope_paged_write and qk_paged_attention_f32, and qk_sample_rows_f32 over
+   the logits. */
+
+/* One layer's cache: a pool of pages.  Row `slot` of page `page` of KV head h
+   is the head_dim values from ((page * kv_heads + h) * page_rows + slot) *
+   head_dim of key (and of value), and the fp32 scale at (page * kv_heads + h)
+   * page_rows + slot of key_scale (value_scale):
+     QK_TYPE_F16      fp16, rounded to nearest even; no scales (NULL).
+     QK_TYPE_I8       int8 code * scale; written with scale = max|x| / 127 and
+                      code = x / scale rounded to nearest, ties to even.
+     QK_TYPE_F8_E4M3  float8 (4-bit exponent, 3-bit mantissa, no infinities)
+                      code * scale; written with scale the least power of two
+                      that keeps the row within 448, code = x / scale to
+                      nearest even.
+   A row whose largest magnitude is below 2^-100 is written as zeros with scale
+   1, one that holds a value that is not finite as zeros with scale NaN (I8,
+   E4M3).  head_dim 64, 96, 128 or 256; page_rows a power of two, 16 to 1024;
+   every base 16-byte aligned. */
+typedef struct qk_paged_kv {
+    int type;
+    int kv_heads, head_dim, page_rows;
+    int64_t pages;
+    void *key, *value;
+    float *key_scale, *value_scale;
+} qk_paged_kv;
+
+/* One sequence of a call: its new tokens are rows first .. first + count - 1
+   of q, k, v and out, at positions pos .. pos + count - 1; its row r lies in
+   page page_table[table * table_stride + r / page_rows]. */
+typedef struct qk_paged_seq {
+    int32_t first, count, pos, table;
+} qk_paged_seq;
+
+/* The sequences of a call.  page_table is a device array [table_rows]
+   [table_stride]; an entry outside [0, pages) is a page that is absent.  seqs
+   is a device array of n_seqs entries, n_tokens the token rows of q, k, v and
+   out, max_count and max_rows bounds of count and of pos + count: a call may
+   take time and workspace by them.  A sequence with count < 1 or a negative
+   entry, with more than max_count tokens or max_rows rows, with tokens beyond
+   n_tokens, with rows beyond the table's stride or a table row beyond
+   table_rows is left out: nothing of it is read or written. */
+typedef struct qk_paged_batch {
+    const int32_t *page_table;
+    int table_rows, table_stride;
+    const qk_paged_seq *seqs;
+    int n_seqs, n_tokens, max_count, max_rows;
+} qk_paged_batch;
+
+/* How the rotary frequencies of rot_dim / 2 pairs, theta^(-2 i / rot_dim), are
+   scaled for contexts longer than the trained one:
+     QK_ROPE_NONE    as they are
+     QK_ROPE_LINEAR  / factor
+     QK_ROPE_LLAMA3  / factor where they turn less than low_freq_factor times
+                     over original_context, as they are from high_freq_factor
+                     turns on, in between mixed by the turns
+     QK_ROPE_YARN    from pair low to pair high a linear ramp from unscaled to
+                     / factor, low and high the pairs that turn beta_fast and
+                     beta_slow times over original_context (rounded outwards,
+                     within 0 .. rot_dim - 1); cosines and sines times
+                     attention_factor (0: 0.1 ln(factor) + 1) */
+#define QK_ROPE_NONE 0
+#define QK_ROPE_LINEAR 1
+#define QK_ROPE_LLAMA3 2
+#define QK_ROPE_YARN 3
+typedef struct qk_rope_scaling {
+    int type;
+    float factor, low_freq_factor, high_freq_factor, original_context, beta_fast, beta_slow, attention_factor;
+} qk_rope_scaling;
+
+/* cosine[p * rot_dim / 2 + i] and sine[...] of (first_pos + p) * f_i for p <
+   positions, in 64 bits, rounded once: the tables that qk_rope_kv_write*,
+   qk_rope_paged_write and the decode drivers' own rotation take.  scaling may
+   be NULL (QK_ROPE_NONE); freq_factors (device, rot_dim / 2 values, or NULL)
+   divide the frequencies before the scaling (a GGUF file's rope_freqs.weight).
+   rot_dim even, at most 512. */
+int qk_rope_tables_f32(float theta, int rot_dim, const qk_rope_scaling *scaling, const float *freq_factors,
+                       int first_pos, int positions, float *cosine, float *sine, qk_stream stream);
+
+/* Rotates every new token's q and k at its position and writes k and v into
+   the pages.  q is [n_tokens] rows of heads * head_dim values, ldq apart, its
+   rotation goes to q_out (which may be q with ldq_out = ldq, or NULL with q
+   NULL: no queries); k and v are rows of kv_heads * head_dim.  The first
+   rot_dim values of a head rotate (0: none, and no tables), in pairs (2 i, 2 i
+   + 1) or, with `half`, (i, i + rot_dim / 2), by the tables' row of the token's
+   position, in 64 bits, rounded once.  Tables have `positions` rows of rot_dim
+   / 2 values; a sequence that reaches beyond them is left out.  A token whose
+   page is absent writes no row (its q is rotated).  No two tokens of a call may
+   have the same row.  q, q_out, k, v 16-byte aligned with leading dimensions
+   multiples of 4. */
+int qk_rope_paged_write(const qk_paged_kv *kv, const qk_paged_batch *batch, const float *q, int ldq, float *q_out,
+                        int ldq_out, const float *k, int ldk, const float *v, int ldv, int heads, const float *cosine,
+                        const float *sine, int positions, int rot_dim, int half, qk_stream stream);
+
+/* The rows of every sequence's count tokens as fp32: row pos + i of a sequence
+   goes to row first + i of key_out and value_out (rows of kv_heads * head_dim,
+   ldk and ldv apart; either may be NULL).  Rows of absent pages are 0.
+   16-byte aligned, leading dimensions multiples of 4. */
+int qk_paged_read_f32(const qk_paged_kv *kv, const qk_paged_batch *batch, float *key_out, int ldk, float *value_out,
+                      int ldv, qk_stream stream);
+
+/* GQA attention of every new token over its sequence's rows 0 .. its own
+   position (which hold them already): out = softmax(scale q K^T) V, scale 1 /
+   sqrt(head_dim) when 0.  q and out are [n_tokens] rows of heads * head_dim,
+   ldq and ldout apart.  Rows of absent pages take no part; a token that sees
+   no row gets zeros.  Products keep 22 bits of q and of the probabilities, and
+   every bit of the cache.  A key or value that is not finite makes the outputs
+   of the tokens that see it not finite, and reaches no other.  workspace holds
+   partial results when a sequence's rows are split over workgroups; with less
+   than the queried bytes (or none) the call takes fewer splits.  Calls sharing
+   a workspace must not overlap.  Base alignments 16 bytes, leading dimensions
+   multiples of 4. */
+size_t qk_paged_attention_workspace_bytes(const qk_paged_batch *batch, int heads, int kv_heads, int head_dim);
+int qk_paged_attention_f32(const qk_paged_kv *kv, const qk_paged_batch *batch, const float *q, int ldq, float *out,
+                           int ldout, int heads, float scale, void *workspace, size_t workspace_bytes,
+                           qk_stream stream);
+
+/* The next token of each of `rows` rows of n logits (row r at logits + r *
+   ldv).  Of row r, with w_i = exp((logit_i - max) / temperature[r]) rounded to
+   a multiple of 2^-44, tokens in descending order of their logits (equal ones
+   by index):
+     top_k[r]  keeps the first top_k (<= 0: all),
+     top_p[r]  of those the shortest run whose weights reach top_p of their sum
+               (1: all),
+     min_p[r]  of those the tokens with w_i >= min_p (0: all),
+   and the first always; out[r] is the first token in index order at which the
+   running sum of the kept weights exceeds uniform[r] (in [0, 1)) of their sum.
+   prob (or NULL) receives its share of that sum.  temperature[r] <= 0, or a
+   parameter that is NaN, keeps the first alone.  NaN logits count as -inf;
+   where a logit is +inf, those that are share the weight.  A row without a
+   logit above -inf gives 0 with prob 0.  The sums are of integers: a row's
+   token does not depend on the other rows or the launch.  All arrays are on
+   the device; temperature, top_k, top_p and min_p hold `rows` values, or are
+   NULL: 1, and no filter.  workspace: qk_sample_rows_workspace_bytes(n, rows)
+   bytes, 256-byte aligned; calls sharing it must not overlap. */
+size_t qk_sample_rows_workspace_bytes(int n, int rows);
+int qk_sample_rows_f32(const float *logits, int n, int64_t ldv, int rows, const float *temperature,
+                       const int32_t *top_k, const float *top_p, const float *min_p, const float *uniform,
+                       int32_t *out, float *prob, void *workspace, size_t workspace_bytes, qk_stream stream);
 
 /* ---------------------------------------------------- decode-step driver -- */
 

@@ -28,6 +28,9 @@ BLOCK_BYTES = {Q4_K: 144, Q6_K: 210, Q6_K_SPLIT: 210}
 QUANT_TYPES = (Q4_K, Q6_K, Q6_K_SPLIT)
 STORAGE_NAMES = {F32: "FP32", F16: "FP16", Q4_K: "Q4_K", Q6_K: "Q6_K", Q6_K_SPLIT: "Q6_K (split)"}
 MAX_FUSED = 8
+# Types of paged cache rows, besides F16.
+I8, F8_E4M3 = 24, 120
+ROPE_SCALING = {"none": 0, "linear": 1, "llama3": 2, "yarn": 3}
 
 QK_OK = 0
 QK_ERR_INVALID_ARG = 1
@@ -86,6 +89,31 @@ class qk_gguf_tensor(ctypes.Structure):
                 ("host", ctypes.c_void_p), ("device", ctypes.c_void_p)]
 
 
+class qk_paged_kv(ctypes.Structure):
+    """One layer's paged cache (include/qk.h)."""
+    _fields_ = [(n, ctypes.c_int) for n in ("type", "kv_heads", "head_dim", "page_rows")] + \
+               [("pages", ctypes.c_int64)] + [(n, ctypes.c_void_p) for n in ("key", "value", "key_scale", "value_scale")]
+
+
+class qk_paged_seq(ctypes.Structure):
+    """One sequence of a call over a paged cache (include/qk.h)."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("first", "count", "pos", "table")]
+
+
+class qk_paged_batch(ctypes.Structure):
+    """The sequences of a call over a paged cache (include/qk.h)."""
+    _fields_ = [("page_table", ctypes.c_void_p), ("table_rows", ctypes.c_int), ("table_stride", ctypes.c_int),
+                ("seqs", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int) for n in ("n_seqs", "n_tokens", "max_count", "max_rows")]
+
+
+class qk_rope_scaling(ctypes.Structure):
+    """Scaling of rotary frequencies (include/qk.h)."""
+    _fields_ = [("type", ctypes.c_int)] + \
+               [(n, ctypes.c_float) for n in ("factor", "low_freq_factor", "high_freq_factor", "original_context",
+                                              "beta_fast", "beta_slow", "attention_factor")]
+
+
 _i, _vp, _f = ctypes.c_int, ctypes.c_void_p, ctypes.c_float
 # name -> (restype, argtypes), exactly the declarations of include/qk.h.
 SIGNATURES = {
@@ -123,6 +151,16 @@ SIGNATURES = {
     "qk_silu_mul_f32": (_i, [_vp, _vp, _i, _vp]),
     "qk_argmax_workspace_bytes": (ctypes.c_size_t, [_i]),
     "qk_argmax_f32": (_i, [_vp, _i, _vp, _vp, _vp]),
+    "qk_rope_tables_f32": (_i, [_f, _i, ctypes.POINTER(qk_rope_scaling), _vp, _i, _i, _vp, _vp, _vp]),
+    "qk_rope_paged_write": (_i, [ctypes.POINTER(qk_paged_kv), ctypes.POINTER(qk_paged_batch), _vp, _i, _vp, _i, _vp,
+                                 _i, _vp, _i, _i, _vp, _vp, _i, _i, _i, _vp]),
+    "qk_paged_read_f32": (_i, [ctypes.POINTER(qk_paged_kv), ctypes.POINTER(qk_paged_batch), _vp, _i, _vp, _i, _vp]),
+    "qk_paged_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(qk_paged_batch), _i, _i, _i]),
+    "qk_paged_attention_f32": (_i, [ctypes.POINTER(qk_paged_kv), ctypes.POINTER(qk_paged_batch), _vp, _i, _vp, _i, _i,
+                                    _f, _vp, ctypes.c_size_t, _vp]),
+    "qk_sample_rows_workspace_bytes": (ctypes.c_size_t, [_i, _i]),
+    "qk_sample_rows_f32": (_i, [_vp, _i, ctypes.c_int64, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t,
+                                _vp]),
     "qk_llama_create": (_i, [ctypes.POINTER(qk_llama_config), ctypes.POINTER(qk_llama_weights), _vp,
                              ctypes.POINTER(ctypes.c_void_p)]),
     "qk_llama_destroy": (_i, [_vp]),
@@ -382,6 +420,211 @@ def matvec_i8(t: Tensor, xq, xscale, out, cols: int, rows: int, n_tokens: int = 
     ldy = rows if ldy is None else ldy
     check(lib().qk_gemv_i8(t.type, t.gpu, ptr(xq), ldxq, ptr(xscale), ldscale, ptr(out), ldy, cols, rows,
                            n_tokens, stream_handle(stream)), "INT8 matrix launch")
+
+
+# ------------------------------------------ paged cache of a serving step --
+
+_KV_DTYPES = {F16: "torch.float16", I8: "torch.int8", F8_E4M3: "torch.float8_e4m3fn"}
+
+
+def _want(where: str, name: str, t, dtypes, shape=None, last_contiguous: bool = False):
+    """Check a torch tensor's device, type and shape: dense (QKError otherwise),
+    or with last_contiguous of rows that are.  None in shape takes any size."""
+    if not getattr(t, "is_cuda", False):
+        raise QKError(where, QK_ERR_INVALID_ARG, f"{name} must be a GPU tensor")
+    if str(t.dtype) not in dtypes:
+        raise QKError(where, QK_ERR_TYPE, f"{name} must be {' or '.join(dtypes)}, got {t.dtype}")
+    if shape is not None and (t.dim() != len(shape) or any(w is not None and w != n for w, n in zip(shape, t.shape))):
+        raise QKError(where, QK_ERR_SHAPE, f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    rows = last_contiguous and t.dim() == 2 and (t.shape[1] < 2 or t.stride(1) == 1) and \
+        (t.shape[0] < 2 or t.stride(0) >= t.shape[1])
+    if not (rows or t.is_contiguous()):
+        raise QKError(where, QK_ERR_INVALID_ARG, f"{name} must be contiguous{' in its rows' if last_contiguous else ''}")
+
+
+def _ld(t) -> int:
+    """Leading dimension of a matrix of contiguous rows."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _on(where: str, first, stream, *others):
+    """The device of a call's tensors (one for all of them, QKError otherwise)
+    as the current one, and the stream: the given one, or the device's current
+    torch stream."""
+    import torch
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise QKError(where, QK_ERR_INVALID_ARG, f"tensors on {first.device} and {t.device}")
+    guard = torch.cuda.device(first.device)
+    return guard, stream_handle(torch.cuda.current_stream(first.device) if stream is None else stream)
+
+
+class PagedKV:
+    """One layer's paged cache (qk_paged_kv): key and value are tensors [pages]
+    [kv_heads][page_rows][head_dim] of the type's dtype (F16 float16, I8 int8,
+    F8_E4M3 float8_e4m3fn), the scales [pages][kv_heads][page_rows] float32 (I8,
+    F8_E4M3)."""
+
+    def __init__(self, type: int, key, value, key_scale=None, value_scale=None):
+        where = "PagedKV"
+        if type not in _KV_DTYPES:
+            raise QKError(where, QK_ERR_TYPE, f"cache type {type} is not F16, I8 or F8_E4M3")
+        _want(where, "key", key, (_KV_DTYPES[type],), (None,) * 4)
+        _want(where, "value", value, (_KV_DTYPES[type],), tuple(key.shape))
+        if (type == F16) != (key_scale is None) or (type == F16) != (value_scale is None):
+            raise QKError(where, QK_ERR_INVALID_ARG, "scales belong to I8 and F8_E4M3 caches, and only to them")
+        for name, t in (("key_scale", key_scale), ("value_scale", value_scale)):
+            if t is not None:
+                _want(where, name, t, ("torch.float32",), tuple(key.shape[:3]))
+        for t in (value, key_scale, value_scale):
+            if t is not None and t.device != key.device:
+                raise QKError(where, QK_ERR_INVALID_ARG, f"tensors on {key.device} and {t.device}")
+        self.type, self.key, self.value, self.key_scale, self.value_scale = type, key, value, key_scale, value_scale
+        self.pages, self.kv_heads, self.page_rows, self.head_dim = (int(n) for n in key.shape)
+        self.desc = qk_paged_kv(type, self.kv_heads, self.head_dim, self.page_rows, self.pages, ptr(key), ptr(value),
+                                ptr(key_scale), ptr(value_scale))
+
+    @classmethod
+    def empty(cls, type: int, pages: int, kv_heads: int, page_rows: int, head_dim: int, device="cuda") -> "PagedKV":
+        """A cache whose rows are not written yet."""
+        import torch
+        if type not in _KV_DTYPES:
+            raise QKError("PagedKV", QK_ERR_TYPE, f"cache type {type} is not F16, I8 or F8_E4M3")
+        dtype = getattr(torch, _KV_DTYPES[type].split(".")[1])
+        new = lambda: torch.empty(pages, kv_heads, page_rows, head_dim, dtype=dtype, device=device)
+        scale = lambda: None if type == F16 else torch.empty(pages, kv_heads, page_rows, device=device)
+        return cls(type, new(), new(), scale(), scale())
+
+
+class PagedBatch:
+    """The sequences of a call over a paged cache (qk_paged_batch): page_table
+    [table_rows][table_stride] int32, seqs [n_seqs][4] int32 of (first, count,
+    pos, table), both on the GPU; n_tokens token rows; max_count and max_rows
+    bound count and pos + count."""
+
+    def __init__(self, page_table, seqs, n_tokens: int, max_count: int, max_rows: int):
+        where = "PagedBatch"
+        _want(where, "page_table", page_table, ("torch.int32",), (None, None))
+        _want(where, "seqs", seqs, ("torch.int32",), (None, 4))
+        if page_table.device != seqs.device:
+            raise QKError(where, QK_ERR_INVALID_ARG, f"tensors on {page_table.device} and {seqs.device}")
+        self.page_table, self.seqs, self.n_tokens = page_table, seqs, int(n_tokens)
+        self.max_count, self.max_rows = int(max_count), int(max_rows)
+        self.desc = qk_paged_batch(ptr(page_table), page_table.shape[0], page_table.shape[1], ptr(seqs), seqs.shape[0],
+                                   self.n_tokens, self.max_count, self.max_rows)
+
+
+def rope_tables(theta: float, rot_dim: int, cosine, sine, first_pos: int = 0, scaling: dict | None = None,
+                freq_factors=None, stream=None) -> None:
+    """qk_rope_tables_f32: cosine and sine, [positions][rot_dim / 2] float32, of
+    positions first_pos, first_pos + 1, ...  scaling: {"type": "none", "linear",
+    "llama3" or "yarn", "factor": ..., ...} with the fields of qk_rope_scaling;
+    freq_factors: rot_dim / 2 values that divide the frequencies."""
+    where = "rope_tables"
+    _want(where, "cosine", cosine, ("torch.float32",), (None, rot_dim // 2))
+    _want(where, "sine", sine, ("torch.float32",), tuple(cosine.shape))
+    if freq_factors is not None:
+        _want(where, "freq_factors", freq_factors, ("torch.float32",), (rot_dim // 2,))
+    c = None
+    if scaling is not None:
+        fields = dict(scaling)
+        kind = fields.pop("type", "none")
+        unknown = set(fields) - {n for n, _ in qk_rope_scaling._fields_}
+        if kind not in ROPE_SCALING or unknown:
+            raise QKError(where, QK_ERR_INVALID_ARG, f"unknown scaling {kind!r} {sorted(unknown)}")
+        c = ctypes.byref(qk_rope_scaling(type=ROPE_SCALING[kind], **{n: float(v) for n, v in fields.items()}))
+    guard, st = _on(where, cosine, stream, sine, freq_factors)
+    with guard:
+        check(lib().qk_rope_tables_f32(theta, rot_dim, c, ptr(freq_factors), first_pos, cosine.shape[0], ptr(cosine),
+                                       ptr(sine), st), "rotary table launch")
+
+
+def rope_paged_write(kv: PagedKV, batch: PagedBatch, q, q_out, k, v, cosine, sine, heads: int,
+                     rot_dim: int | None = None, half: bool = False, stream=None) -> None:
+    """qk_rope_paged_write: q [n_tokens][heads * head_dim] rotated into q_out
+    (both may be None, or the same), k and v [n_tokens][kv_heads * head_dim]
+    into the pages, k rotated.  rot_dim: head_dim when None; 0 needs no tables."""
+    where = "rope_paged_write"
+    rot_dim = kv.head_dim if rot_dim is None else rot_dim
+    f32, n, width = ("torch.float32",), batch.n_tokens, kv.kv_heads * kv.head_dim
+    for name, t, w in (("q", q, heads * kv.head_dim), ("q_out", q_out, heads * kv.head_dim), ("k", k, width),
+                       ("v", v, width)):
+        if t is not None or name in "kv":
+            _want(where, name, t, f32, (n, w), last_contiguous=True)
+    positions = 0
+    if rot_dim:
+        _want(where, "cosine", cosine, f32, (None, rot_dim // 2))
+        _want(where, "sine", sine, f32, tuple(cosine.shape))
+        positions = cosine.shape[0]
+    guard, st = _on(where, kv.key, stream, batch.seqs, q, q_out, k, v, *((cosine, sine) if rot_dim else ()))
+    with guard:
+        check(lib().qk_rope_paged_write(ctypes.byref(kv.desc), ctypes.byref(batch.desc), ptr(q),
+                                        0 if q is None else _ld(q), ptr(q_out), 0 if q_out is None else _ld(q_out),
+                                        ptr(k), _ld(k), ptr(v), _ld(v), heads, ptr(cosine) if rot_dim else None,
+                                        ptr(sine) if rot_dim else None, positions, rot_dim, int(half), st),
+              "paged cache write launch")
+
+
+def paged_read(kv: PagedKV, batch: PagedBatch, key_out, value_out, stream=None) -> None:
+    """qk_paged_read_f32: the rows of the batch's tokens as fp32, [n_tokens]
+    [kv_heads * head_dim] each (either may be None)."""
+    where = "paged_read"
+    for name, t in (("key_out", key_out), ("value_out", value_out)):
+        if t is not None:
+            _want(where, name, t, ("torch.float32",), (batch.n_tokens, kv.kv_heads * kv.head_dim), last_contiguous=True)
+    guard, st = _on(where, kv.key, stream, batch.seqs, key_out, value_out)
+    with guard:
+        check(lib().qk_paged_read_f32(ctypes.byref(kv.desc), ctypes.byref(batch.desc), ptr(key_out),
+                                      0 if key_out is None else _ld(key_out), ptr(value_out),
+                                      0 if value_out is None else _ld(value_out), st), "paged cache read launch")
+
+
+def paged_attention_workspace_bytes(batch: PagedBatch, heads: int, kv_heads: int, head_dim: int) -> int:
+    """Workspace bytes of paged_attention."""
+    return int(lib().qk_paged_attention_workspace_bytes(ctypes.byref(batch.desc), heads, kv_heads, head_dim))
+
+
+def paged_attention(kv: PagedKV, batch: PagedBatch, q, out, heads: int, scale: float = 0.0, workspace=None,
+                    stream=None) -> None:
+    """qk_paged_attention_f32: attention of every new token (rows of q, [n_tokens]
+    [heads * head_dim]) over its sequence's pages up to its own position, into
+    out.  scale: 1 / sqrt(head_dim) when 0."""
+    where = "paged_attention"
+    for name, t in (("q", q), ("out", out)):
+        _want(where, name, t, ("torch.float32",), (batch.n_tokens, heads * kv.head_dim), last_contiguous=True)
+    nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    guard, st = _on(where, kv.key, stream, batch.seqs, q, out, workspace)
+    with guard:
+        check(lib().qk_paged_attention_f32(ctypes.byref(kv.desc), ctypes.byref(batch.desc), ptr(q), _ld(q), ptr(out),
+                                           _ld(out), heads, scale, ptr(workspace), nbytes, st),
+              "paged attention launch")
+
+
+def sample_workspace_bytes(n: int, rows: int) -> int:
+    """Workspace bytes of sample_rows for rows of n logits."""
+    return int(lib().qk_sample_rows_workspace_bytes(n, rows))
+
+
+def sample_rows(logits, uniform, out, temperature=None, top_k=None, top_p=None, min_p=None, prob=None, workspace=None,
+                stream=None) -> None:
+    """qk_sample_rows_f32: the next token of each row of logits [rows][n], out
+    int32 [rows], by uniform float32 [rows] in [0, 1).  temperature, top_p, min_p
+    (float32) and top_k (int32) hold a value a row, or are None: 1, and no
+    filter.  prob (float32 [rows] or None) receives the token's probability."""
+    where = "sample_rows"
+    _want(where, "logits", logits, ("torch.float32",), (None, None), last_contiguous=True)
+    rows, n = logits.shape
+    for name, t, dt in (("uniform", uniform, "float32"), ("out", out, "int32"), ("temperature", temperature, "float32"),
+                        ("top_k", top_k, "int32"), ("top_p", top_p, "float32"), ("min_p", min_p, "float32"),
+                        ("prob", prob, "float32")):
+        if t is not None or name in ("uniform", "out"):
+            _want(where, name, t, ("torch." + dt,), (rows,))
+    nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    guard, st = _on(where, logits, stream, uniform, out, temperature, top_k, top_p, min_p, prob, workspace)
+    with guard:
+        check(lib().qk_sample_rows_f32(ptr(logits), n, _ld(logits), rows, ptr(temperature), ptr(top_k), ptr(top_p),
+                                       ptr(min_p), ptr(uniform), ptr(out), ptr(prob), ptr(workspace), nbytes, st),
+              "sampling launch")
 
 
 def _upload_weights(owner, cfg: dict, weights: dict):

@@ -1,0 +1,269 @@
+"""qk_paged_attention_f32 against softmax attention in 64 bits over the values
+that the pages stand for."""
+import numpy as np
+import pytest
+
+import paged_ref
+from conftest import rel_l2, to_dev
+
+pytestmark = pytest.mark.gpu
+KINDS = ["f16", "i8", "e4m3"]
+# A score is sum q k / sqrt(hd) of normal values: |q| |k| / sqrt(hd) is about
+# sqrt(hd), 16 at most.  q keeps 2^-22 of its largest value, products and sums
+# of hd / 32 steps in fp32 2^-24 each, so a score is within 16 * 1.45 * (2^-22 +
+# 8 * 2^-24) in base 2 were all errors alike, e.g. 1.7e-5; they are not (32 and
+# more independent ones): a sixth of it, 3e-6, bounds what a probability is off
+# by, and the output, an average of them.
+TOL = 3e-6
+LAYOUTS = [(32, 8, 64), (6, 6, 64), (16, 2, 96), (5, 1, 96), (24, 8, 128), (8, 8, 128), (20, 1, 128), (8, 1, 256), (4, 2, 256)]
+
+
+def run(qk, t, pool, q, heads, workspace=True, scale=0.0, **over):
+    kv, batch = pool.dev(qk, t, **over)
+    out = t.full((batch.n_tokens, heads * pool.hd), np.nan, device="cuda")
+    nb = qk.paged_attention_workspace_bytes(batch, heads, pool.kvh, pool.hd) if workspace is True else workspace
+    ws = t.full((nb,), 0xFF, dtype=t.uint8, device="cuda") if nb else None   # stale partials are not numbers
+    qk.paged_attention(kv, batch, to_dev(t, q), out, heads, scale=scale, workspace=ws)
+    t.cuda.synchronize()
+    return out.cpu().numpy()
+
+
+def queries(rng, pool, heads):
+    return rng.standard_normal((pool.n, heads * pool.hd)).astype(np.float32)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kvh,hd", LAYOUTS)
+@pytest.mark.parametrize("page_rows", [16, 64])
+def test_decoding_sequences(qk, torch_gpu, kind, heads, kvh, hd, page_rows):
+    """One token each, lengths around the tiles and the pages, unused rows not
+    finite."""
+    rng = np.random.default_rng(hd)
+    pool = paged_ref.Pool(rng, kind, kvh, hd, page_rows, [(1, n - 1) for n in (1, 2, 15, 16, 17, 31, 32, 33, 64, 127, 129, 400)])
+    pool.poison(pool.unused())
+    q = queries(rng, pool, heads)
+    assert rel_l2(run(qk, torch_gpu, pool, q, heads), pool.attention(q, heads)) < TOL
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kvh,hd", LAYOUTS)
+@pytest.mark.parametrize("seqs", [[(70, 0)], [(3, 90), (33, 31), (1, 64), (64, 0)]], ids=["fresh", "mixed"])
+def test_chunks(qk, torch_gpu, kind, heads, kvh, hd, seqs):
+    rng = np.random.default_rng(hd + len(seqs))
+    pool = paged_ref.Pool(rng, kind, kvh, hd, 32, seqs)
+    pool.poison(pool.unused())
+    q = queries(rng, pool, heads)
+    assert rel_l2(run(qk, torch_gpu, pool, q, heads), pool.attention(q, heads)) < TOL
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kvh,hd,count,pos", [(32, 8, 64, 1, 5000), (24, 8, 128, 1, 9000), (8, 1, 256, 3, 4000),
+                                                    (16, 2, 96, 2, 3001), (8, 2, 128, 300, 1200), (8, 8, 64, 517, 300)])
+def test_long_rows_and_chunks(qk, torch_gpu, kind, heads, kvh, hd, count, pos):
+    """Rows split over workgroups, and long chunks: a few tokens against the
+    oracle, all of them against the call without a workspace (one split)."""
+    rng = np.random.default_rng(pos)
+    pool = paged_ref.Pool(rng, kind, kvh, hd, 128, [(count, pos)])
+    pool.poison(pool.unused())
+    q = queries(rng, pool, heads)
+    got = run(qk, torch_gpu, pool, q, heads)
+    assert rel_l2(got, run(qk, torch_gpu, pool, q, heads, workspace=0)) < TOL
+    k, v, _ = pool.rows(0, pos + count)
+    for i in sorted({0, count // 3, count - 1}):
+        for h in (0, heads - 1):
+            s = k[: pos + i + 1, h * kvh // heads] @ q[i, h * hd:(h + 1) * hd].astype(np.float64) / np.sqrt(hd)
+            p = np.exp(s - s.max())
+            assert rel_l2(got[i, h * hd:(h + 1) * hd], p @ v[: pos + i + 1, h * kvh // heads] / p.sum()) < 2 * TOL
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_smaller_workspaces(qk, torch_gpu, kind):
+    """Fewer splits where fewer fit; a few bytes are none."""
+    rng = np.random.default_rng(3)
+    pool = paged_ref.Pool(rng, kind, 2, 64, 64, [(1, 3000), (1, 100), (2, 1500)])
+    q = queries(rng, pool, 8)
+    want = pool.attention(q, 8)
+    for nb in (0, 100, 3 * pool.n * 8 * 68 * 4 + 16, 5 * pool.n * 8 * 68 * 4):
+        assert rel_l2(run(qk, torch_gpu, pool, q, 8, workspace=nb), want) < TOL
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd,heads,kvh", [(64, 8, 2), (128, 4, 4)])
+def test_absent_pages(qk, torch_gpu, kind, hd, heads, kvh):
+    """Rows of absent pages take no part: in the middle, all of a sequence
+    (zeros), all that the chunk's first tokens see, entries beyond the pool."""
+    rng = np.random.default_rng(4)
+    pool = paged_ref.Pool(rng, kind, kvh, hd, 16, [(1, 200), (1, 40), (40, 0), (5, 30), (1, 900)])
+    pool.table[0, 3:7] = -1
+    pool.table[1, :] = -1
+    pool.table[2, 0] = pool.pages
+    pool.table[3, 1] = -2 ** 31
+    pool.table[4, ::2] = 2 ** 31 - 1
+    pool.poison(pool.unused())
+    pool.poison(np.arange(pool.pages)[:, None] * 0 + np.zeros((1, 16)) > 1)
+    q = queries(rng, pool, heads)
+    got, want = run(qk, torch_gpu, pool, q, heads), pool.attention(q, heads)
+    assert not got[1].any() and not want[1].any() and not got[2:18].any()
+    assert rel_l2(got, want) < TOL
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("count,pos", [(1, 300), (40, 60), (200, 0)])
+def test_left_out_sequences(qk, torch_gpu, kind, count, pos):
+    """A sequence that does not fit the batch leaves its outputs as they were,
+    and so do tokens that no sequence holds."""
+    rng = np.random.default_rng(4)
+    pool = paged_ref.Pool(rng, kind, 2, 64, 16, [(2, 5), (count, pos), (3, 9)])
+    q = queries(rng, pool, 4)
+    want = pool.attention(q, 4)
+    for bad in ((2, -1), (3, 3), (0, pool.n), (1, 0), (2, 2 ** 31 - 2)):
+        keep = pool.seqs[1].copy()
+        pool.seqs[1, bad[0]] = bad[1]
+        got = run(qk, torch_gpu, pool, q, 4)
+        pool.seqs[1] = keep
+        rows = np.r_[0:2, 2 + count: pool.n]
+        assert rel_l2(got[rows], want[rows]) < TOL and np.isnan(got[2: 2 + count]).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_strides_scale_and_streams(qk, torch_gpu, kind):
+    """q and out inside wider rows, a scale of the caller's, another stream."""
+    t = torch_gpu
+    rng = np.random.default_rng(6)
+    pool = paged_ref.Pool(rng, kind, 2, 64, 32, [(1, 100), (9, 20)])
+    q = queries(rng, pool, 8)
+    kv, batch = pool.dev(qk, t)
+    wide = t.full((pool.n, 8 * 64 + 12), 7.0, device="cuda")
+    wide[:, : 8 * 64] = to_dev(t, q)
+    out = t.full((pool.n, 8 * 64 + 4), 7.0, device="cuda")
+    side = t.cuda.Stream()
+    side.wait_stream(t.cuda.current_stream())
+    with t.cuda.stream(side):
+        qk.paged_attention(kv, batch, wide[:, : 8 * 64], out[:, : 8 * 64], 8, scale=0.03)
+    side.synchronize()
+    assert rel_l2(out[:, : 8 * 64].cpu().numpy(), pool.attention(q, 8, 0.03)) < TOL
+    assert (out[:, 8 * 64:] == 7).all() and (wide[:, 8 * 64:] == 7).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("gain", [1e-30, 1e-4, 30.0])
+@pytest.mark.parametrize("spread", [0.0, 4.0])
+@pytest.mark.parametrize("count", [1, 130])
+def test_magnitudes(qk, torch_gpu, kind, gain, spread, count):
+    """Small and large queries, rows whose magnitudes differ by e^+-8 (the value
+    scales' exponents with them)."""
+    rng = np.random.default_rng(7)
+    row_gain = lambda *s: rng.standard_normal(s).astype(np.float32) * np.exp(spread * rng.standard_normal(s[:-1] + (1,)) / 2).astype(np.float32)
+    pool = paged_ref.Pool(rng, kind, 2, 64, 16, [(count, 350)], draw=row_gain)
+    q = queries(rng, pool, 4) * np.float32(gain)
+    got, want = run(qk, torch_gpu, pool, q, 4), pool.attention(q, 4)
+    # Scores of up to |q| |k| / 8 in natural units, each within a few 2^-23 of
+    # its size: gain 30 and rows of e^4 give scores of some thousands, of which
+    # the largest decides; their error moves probabilities by itself.
+    k = pool.rows(0, 350 + count)[0]
+    size = np.linalg.norm(q.reshape(-1, 64), axis=1).max() * np.linalg.norm(k, axis=-1).max() / 8
+    assert rel_l2(got, want) < max(TOL, size * 2.0 ** -23 * 2)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("count", [1, 200])
+def test_scales_of_other_writers(qk, torch_gpu, kind, count):
+    """Rows of zeros (scale 1 and scale 0), scales far apart."""
+    rng = np.random.default_rng(8)
+    pool = paged_ref.Pool(rng, kind, 1, 64, 16, [(count, 200)])
+    if kind != "f16":
+        for part in (pool.value, pool.key):
+            part[0][:, :, 3] = 0
+            part[2][:, :, 3] = 0
+            part[1][:, :, 3] = 0
+        f = np.float32(2.0) ** rng.integers(-60, 40, pool.value[1].shape).astype(np.float32)
+        pool.value[1] = pool.value[1] * f
+        pool.value[2] = pool.value[2] * f[..., None].astype(np.float64)
+    q = queries(rng, pool, 2)
+    assert rel_l2(run(qk, torch_gpu, pool, q, 2), pool.attention(q, 2)) < TOL
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("count,pos", [(40, 30), (300, 10)])
+def test_not_finite_rows_reach_only_those_who_see_them(qk, torch_gpu, kind, count, pos):
+    rng = np.random.default_rng(9)
+    at = pos + count // 2
+    for part in ("key", "value"):
+        for bad in (np.nan, np.inf):
+            pool = paged_ref.Pool(rng, kind, 2, 64, 16, [(count, pos)])
+            codes, scale, _ = getattr(pool, part)
+            page = pool.table[0, at // 16]
+            if kind == "f16":
+                codes[page, 1, at % 16, 5] = bad
+            elif kind == "i8":
+                scale[page, 1, at % 16] = np.nan
+            else:
+                codes[page, 1, at % 16, 5] = 0x7F
+            clean = paged_ref.Pool(np.random.default_rng(9), kind, 2, 64, 16, [(count, pos)])
+            q = queries(np.random.default_rng(1), pool, 4)
+            got = run(qk, torch_gpu, pool, q, 4).reshape(count, 4, 64)
+            sees = np.arange(pos, pos + count) >= at
+            assert np.isfinite(got[~sees]).all() and np.isfinite(got[:, :2]).all()
+            assert (~np.isfinite(got[sees][:, 2:])).any(-1).all()
+            pool_ok = pool.attention(q, 4).reshape(count, 4, 64)
+            assert rel_l2(got[~sees], pool_ok[~sees]) < TOL and rel_l2(got[:, :2], pool_ok[:, :2]) < TOL
+            del clean
+
+
+@pytest.mark.parametrize("count", [1, 200])
+def test_not_finite_queries(qk, torch_gpu, count):
+    rng = np.random.default_rng(10)
+    pool = paged_ref.Pool(rng, "i8", 2, 64, 16, [(count, 30), (2, 9)])
+    q = queries(rng, pool, 4)
+    q[0, 70], q[count, 3], q[count + 1, 255] = np.nan, np.inf, -np.inf
+    got, want = run(qk, torch_gpu, pool, q, 4).reshape(-1, 4, 64), None
+    q2 = np.where(np.isfinite(q), q, 0)
+    want = pool.attention(q2, 4).reshape(-1, 4, 64)
+    bad = [(0, 1), (count, 0), (count + 1, 3)]
+    for b in bad:
+        assert np.isnan(got[b]).all()
+        got[b] = want[b]
+    assert rel_l2(got, want) < TOL
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_the_same_call_twice_and_captured(qk, torch_gpu, kind):
+    """Bit for bit the same again, and in a graph replayed over new inputs,
+    between eager calls on another workspace."""
+    t = torch_gpu
+    rng = np.random.default_rng(11)
+    pool = paged_ref.Pool(rng, kind, 2, 64, 32, [(1, 2000), (1, 50), (130, 20)])
+    kv, batch = pool.dev(qk, t)
+    nb = qk.paged_attention_workspace_bytes(batch, 8, 2, 64)
+    ws = [t.empty(max(nb, 16), dtype=t.uint8, device="cuda") for _ in range(2)]
+    q = to_dev(t, queries(rng, pool, 8))
+    out, eager = t.empty_like(q), t.empty_like(q)
+    call = lambda o, w: qk.paged_attention(kv, batch, q, o, 8, workspace=w)
+    call(out, ws[0])
+    call(eager, ws[1])
+    assert t.equal(out, eager)
+    g = t.cuda.CUDAGraph()
+    with t.cuda.graph(g):
+        call(out, ws[0])
+    for i in range(4):
+        q.copy_(to_dev(t, queries(rng, pool, 8)))
+        out.fill_(7)
+        g.replay()
+        call(eager, ws[1])
+        t.cuda.synchronize()
+        assert t.equal(out, eager)
+
+
+def test_refusals(qk, torch_gpu):
+    t = torch_gpu
+    pool = paged_ref.Pool(np.random.default_rng(1), "i8", 2, 64, 16, [(1, 3)])
+    kv, batch = pool.dev(qk, t)
+    x = t.zeros(1, 256, device="cuda")
+    with pytest.raises(qk.QKError, match="shape"):
+        qk.paged_attention(kv, batch, x, x.clone(), 3)
+    with pytest.raises(qk.QKError, match="multiple of kv_heads"):
+        qk.paged_attention(kv, batch, x[:, :192], x.clone()[:, :192], 3)
+    with pytest.raises(qk.QKError, match="float32"):
+        qk.paged_attention(kv, batch, x.half(), x.clone(), 4)
+    with pytest.raises(qk.QKError, match="GPU"):
+        qk.paged_attention(kv, batch, x.cpu(), x.clone(), 4)

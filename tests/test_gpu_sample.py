@@ -1,0 +1,227 @@
+"""qk_sample_rows_f32 against the definition in numpy: the token's interval of
+the kept weights' running sum holds the given random number."""
+import numpy as np
+import pytest
+
+from conftest import to_dev
+
+pytestmark = pytest.mark.gpu
+UNIT = 2.0 ** 44
+
+
+def kept_weights(x, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Integer weights of the kept tokens (0: dropped), by a sort."""
+    x = np.where(np.isnan(x), -np.inf, x.astype(np.float64))
+    n, top = len(x), x.max()
+    order = np.argsort(-x, kind="stable")
+    if top == -np.inf:
+        return None
+    if not temperature > 0 or not top_p > 0 or not min_p <= 1 or top_k == 1:
+        w = np.zeros(n)
+        w[order[0]] = UNIT
+        return w
+    if top == np.inf:
+        w = np.where(x == np.inf, UNIT, 0)
+    else:
+        with np.errstate(over="ignore", invalid="ignore"):
+            w = np.rint(np.exp((x - top) / np.float64(temperature)) * UNIT)
+        w = np.where(x == -np.inf, 0, w)
+    keep = np.ones(n, dtype=bool)
+    if top_k > 0:
+        keep[top_k:] = False
+    ws = w[order] * keep
+    if top_p < 1:
+        before = np.cumsum(ws) - ws
+        keep &= before < np.float64(top_p) * ws.sum()
+    keep &= ws >= np.float64(min_p) * UNIT
+    keep[0] = True
+    out = np.zeros(n)
+    out[order[keep]] = ws[keep]
+    return out
+
+
+def check(qk, t, x, u, ldv=None, **params):
+    """Tokens of rows x by u; params: a list a row each."""
+    rows, n = x.shape
+    buf = t.full((rows, ldv or n), 9e30, device="cuda")
+    buf[:, :n] = to_dev(t, x)
+    dev = {k: to_dev(t, np.asarray(v, dtype=np.int32 if k == "top_k" else np.float32)) for k, v in params.items()}
+    out = t.full((rows + 1,), -7, dtype=t.int32, device="cuda")
+    prob = t.full((rows + 1,), -7.0, device="cuda")
+    ws = t.full((max(1, qk.sample_workspace_bytes(n, rows)),), 0xFF, dtype=t.uint8, device="cuda")
+    uu = to_dev(t, np.asarray(u, dtype=np.float32))
+    qk.sample_rows(buf[:, :n], uu, out[:rows], prob=prob[:rows], workspace=ws, **dev)
+    only = t.empty(rows, dtype=t.int32, device="cuda")
+    qk.sample_rows(buf[:, :n], uu, only, workspace=ws, **dev)   # without prob, over a used workspace
+    got, pr = out.cpu().numpy(), prob.cpu().numpy()
+    assert got[rows] == -7 and pr[rows] == -7 and np.array_equal(only.cpu().numpy(), got[:rows])
+    for r in range(rows):
+        w = kept_weights(x[r], **{k: (v[r] if k == "top_k" else np.float32(v[r])) for k, v in params.items()})
+        if w is None:
+            assert got[r] == 0 and pr[r] == 0
+            continue
+        i, c, total = got[r], np.cumsum(w), w.sum()
+        assert 0 <= i < n and w[i] > 0, (r, i)
+        # Each weight is one unit off at most where exp rounds the other way,
+        # sums in 64 bits 2^-53 of themselves a step: 2^-36 of the sum.
+        eps = total * 2.0 ** -36
+        uv = min(max(np.float64(np.float32(u[r])), 0), 1) if u[r] == u[r] else 0.0
+        target = min(uv * total, total - 1)
+        assert c[i] - w[i] <= target + eps and c[i] > target - eps, (r, i, c[i] / total, uv)
+        assert abs(pr[r] - w[i] / total) <= 2.0 ** -23 * w[i] / total
+    return got[:rows]
+
+
+def logits(rng, rows, n, spread=2.2):
+    x = rng.standard_normal((rows, n)).astype(np.float32) * np.float32(spread)
+    for r in range(rows):
+        at = rng.integers(0, n, min(n, 30))
+        x[r, at] = 8 + 3 * rng.standard_normal(len(at))
+    return x
+
+
+PARAMS = {
+    "plain": dict(),
+    "temperature": dict(temperature=[0.3, 1.7, 1e-6, 50.0]),
+    "top_k": dict(top_k=[2, 50, 999, 5000]),
+    "top_p": dict(top_p=[0.1, 0.9, 0.999, 1e-6]),
+    "min_p": dict(min_p=[0.01, 0.5, 1.0, 1e-6]),
+    "all": dict(temperature=[0.7, 0.0, 1.2, 0.9], top_k=[40, 0, 7, 200], top_p=[0.9, 1.0, 0.5, 0.99],
+                min_p=[0.05, 0.0, 0.0, 0.001]),
+    "off": dict(temperature=[1.0, 1.0, -1.0, 0.0], top_k=[0, -3, 1 << 30, 1], top_p=[1.0, 2.0, 1.0, 1.0],
+                min_p=[0.0, -1.0, 0.0, 0.0]),
+    "greedy": dict(top_p=[0.0, -1.0, np.nan, 0.5], min_p=[0.0, 0.0, 0.0, 1.5]),
+    "not numbers": dict(temperature=[np.nan, np.inf, 1.0, 1.0], min_p=[0.0, 0.0, np.nan, 0.0]),
+}
+
+
+@pytest.mark.parametrize("n", [1, 2, 63, 1000, 4097, 32003, 128256])
+@pytest.mark.parametrize("which", PARAMS)
+def test_rows(qk, torch_gpu, n, which):
+    rng = np.random.default_rng(n)
+    p = PARAMS[which]
+    for u in ([0.0, 0.25, 0.7, 1 - 2.0 ** -24], rng.random(4).astype(np.float32)):
+        check(qk, torch_gpu, logits(rng, 4, n), u, **p)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 17, 64, 300])
+def test_batches(qk, torch_gpu, rows):
+    """Each row by its own parameters, whatever the rows beside it; the same
+    row alone gives the same token."""
+    rng = np.random.default_rng(rows)
+    x, u = logits(rng, rows, 5003), rng.random(rows).astype(np.float32)
+    p = dict(temperature=rng.uniform(0, 1.5, rows), top_k=rng.integers(-5, 300, rows), top_p=rng.uniform(0.3, 1.1, rows),
+             min_p=rng.uniform(-0.1, 0.2, rows))
+    got = check(qk, torch_gpu, x, u, **p)
+    for r in {0, rows // 2, rows - 1}:
+        alone = check(qk, torch_gpu, x[r:r + 1], u[r:r + 1], **{k: v[r:r + 1] for k, v in p.items()})
+        assert alone[0] == got[r]
+
+
+@pytest.mark.parametrize("spread", [0.0, 0.01, 30.0])
+@pytest.mark.parametrize("n", [1000, 50001])
+def test_flat_and_peaked_rows(qk, torch_gpu, spread, n):
+    """Equal logits (every filter cuts among ties), nearly equal ones, and rows
+    where a few tokens hold everything."""
+    rng = np.random.default_rng(1)
+    x = (rng.standard_normal((6, n)) * spread).astype(np.float32)
+    check(qk, torch_gpu, x, [0.0, 0.2, 0.5, 0.9, 0.99, 0.4], top_k=[0, n // 3, 77, n - 1, 2, 0],
+          top_p=[0.5, 0.75, 1.0, 0.25, 0.9, 0.999], min_p=[0, 0, 0, 0, 0, 0.5])
+
+
+def test_ties_go_by_index(qk, torch_gpu):
+    """Quantised logits: many ties at every threshold, signed zeros among them."""
+    rng = np.random.default_rng(2)
+    x = np.rint(rng.standard_normal((8, 9001)) * 2).astype(np.float32)
+    x[:, ::3] *= np.float32(-1)
+    assert (np.signbit(x) & (x == 0)).any()
+    check(qk, torch_gpu, x, rng.random(8), top_k=[5, 50, 500, 5000, 0, 0, 3000, 9000], top_p=[1, 1, 1, 1, 0.1, 0.7, 0.6, 0.9])
+
+
+def test_masked_rows(qk, torch_gpu):
+    """-inf, the type's lowest value, NaN, +inf, and rows that leave nothing."""
+    low = np.finfo(np.float32).min
+    n = 5000
+    x = np.full((10, n), -np.inf, dtype=np.float32)
+    x[1, 4321] = -3
+    x[2] = low
+    x[3] = np.nan
+    x[4, [7, 4000]] = np.inf
+    x[4, 8] = 5
+    x[5, :100], x[5, 200] = np.nan, 1
+    x[6] = low
+    x[6, [10, 20]] = [low / 2, 3e38]
+    x[7, 1000:1003] = [1, 2, 3]
+    x[8], x[8, 17] = low, 0
+    x[9, ::2] = 0
+    for params in (dict(), dict(top_k=[3] * 10), dict(top_p=[0.6] * 10), dict(min_p=[0.3] * 10),
+                   dict(top_k=[4000] * 10, top_p=[0.95] * 10, temperature=[0.5] * 10), dict(temperature=[1e30] * 10)):
+        for u in (0.0, 0.6, 1 - 2.0 ** -24):
+            check(qk, torch_gpu, x, [u] * 10, **params)
+
+
+def test_random_numbers_out_of_range(qk, torch_gpu):
+    rng = np.random.default_rng(3)
+    x = logits(rng, 5, 700)
+    check(qk, torch_gpu, x, [-1.0, 1.0, 5.0, np.nan, np.inf], top_p=[0.9] * 5)
+
+
+@pytest.mark.parametrize("n,ldv", [(1000, 1001), (4097, 5000), (7, 9)])
+def test_strides(qk, torch_gpu, n, ldv):
+    rng = np.random.default_rng(4)
+    check(qk, torch_gpu, logits(rng, 5, n), rng.random(5), ldv=ldv, top_p=[0.9] * 5, top_k=[30] * 5)
+
+
+def test_frequencies(qk, torch_gpu):
+    """Over 4096 evenly spaced numbers a token is drawn in proportion to its
+    weight: its interval holds that many of them, to one at either end."""
+    rng = np.random.default_rng(5)
+    x = np.repeat(logits(rng, 1, 300), 4096, 0)
+    u = (np.arange(4096) + 0.5) / 4096
+    p = dict(temperature=[0.9] * 4096, top_p=[0.95] * 4096)
+    got = np.bincount(check(qk, torch_gpu, x, u, **p), minlength=300)
+    w = kept_weights(x[0], 0.9 * np.float32(1), 0, np.float32(0.95))
+    assert np.abs(got - 4096 * w / w.sum()).max() <= 1.001
+
+
+def test_captured(qk, torch_gpu):
+    """Two captured graphs with workspaces of their own, replayed in turn over
+    new logits."""
+    t = torch_gpu
+    rng = np.random.default_rng(6)
+    x, u = t.empty(20, 30000, device="cuda"), t.empty(20, device="cuda")
+    p = t.full((20,), 0.9, device="cuda")
+    outs = [t.empty(20, dtype=t.int32, device="cuda") for _ in range(3)]
+    ws = [t.empty(max(1, qk.sample_workspace_bytes(30000, 20)), dtype=t.uint8, device="cuda") for _ in range(3)]
+    call = lambda i: qk.sample_rows(x, u, outs[i], top_p=p, workspace=ws[i])
+    x.copy_(to_dev(t, logits(rng, 20, 30000)))
+    u.uniform_()
+    graphs = []
+    call(2)
+    for i in range(2):
+        graphs.append(t.cuda.CUDAGraph())
+        with t.cuda.graph(graphs[i]):
+            call(i)
+    for i in range(5):
+        x.copy_(to_dev(t, logits(rng, 20, 30000)))
+        u.uniform_()
+        graphs[i % 2].replay()
+        graphs[1 - i % 2].replay()
+        call(2)
+        t.cuda.synchronize()
+        assert t.equal(outs[0], outs[2]) and t.equal(outs[1], outs[2])
+
+
+def test_refusals(qk, torch_gpu):
+    t = torch_gpu
+    x, u, o = t.zeros(2, 10, device="cuda"), t.zeros(2, device="cuda"), t.zeros(2, dtype=t.int32, device="cuda")
+    with pytest.raises(qk.QKError, match="int32"):
+        qk.sample_rows(x, u, o.long())
+    with pytest.raises(qk.QKError, match="shape"):
+        qk.sample_rows(x, u[:1], o)
+    with pytest.raises(qk.QKError, match="int32"):
+        qk.sample_rows(x, u, o, top_k=u)
+    with pytest.raises(qk.QKError, match="float32"):
+        qk.sample_rows(x.half(), u, o)
+    with pytest.raises(qk.QKError, match="contiguous"):
+        qk.sample_rows(x.t().contiguous().t(), u, o)
