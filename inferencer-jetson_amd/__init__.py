@@ -442,21 +442,67 @@ def _want(where: str, name: str, t, dtypes, shape=None, last_contiguous: bool = 
         raise QKError(where, QK_ERR_INVALID_ARG, f"{name} must be contiguous{' in its rows' if last_contiguous else ''}")
 
 
-def _ld(t) -> int:
-    """Leading dimension of a matrix of contiguous rows."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+_SCALING_FIELDS = {n for n, _ in qk_rope_scaling._fields_} - {"type"}
+_TORCH = None
 
 
-def _on(where: str, first, stream, *others):
-    """The device of a call's tensors (one for all of them, QKError otherwise)
-    as the current one, and the stream: the given one, or the device's current
-    torch stream."""
-    import torch
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise QKError(where, QK_ERR_INVALID_ARG, f"tensors on {first.device} and {t.device}")
-    guard = torch.cuda.device(first.device)
-    return guard, stream_handle(torch.cuda.current_stream(first.device) if stream is None else stream)
+def _torch():
+    global _TORCH
+    if _TORCH is None:
+        import torch
+        _TORCH = torch
+    return _TORCH
+
+
+def _gpu(where: str, name: str, t):
+    """The GPU a tensor is on (QKError if it is on none)."""
+    if not t.is_cuda:
+        raise QKError(where, QK_ERR_INVALID_ARG, f"{name} must be a GPU tensor")
+    return t.device
+
+
+def _rows(where: str, name: str, t, n: int, w: int, device) -> int:
+    """The leading dimension of a float32 matrix [n][w] of contiguous rows on
+    the device (QKError for anything else)."""
+    if t is not None and t.dtype is _TORCH.float32 and t.device == device and t.shape == (n, w):
+        ld, one = t.stride()
+        if (one == 1 or w == 1) and (ld >= w or n == 1):
+            return ld if ld >= w else w
+    _want(where, name, t, ("torch.float32",), (n, w), last_contiguous=True)
+    raise QKError(where, QK_ERR_INVALID_ARG, f"{name} is on {t.device}, the call's other tensors on {device}")
+
+
+def _dense(where: str, name: str, t, dtype, shape, device) -> int:
+    """The address of a contiguous tensor of the type and shape on the device
+    (QKError for anything else)."""
+    if t is not None and t.dtype is dtype and t.device == device and t.shape == shape and t.is_contiguous():
+        return t.data_ptr()
+    _want(where, name, t, (str(dtype),), shape)
+    raise QKError(where, QK_ERR_INVALID_ARG, f"{name} is on {t.device}, the call's other tensors on {device}")
+
+
+def _space(where: str, t, device) -> tuple[int | None, int]:
+    """Address and bytes of a workspace tensor (None: none) on the device."""
+    if t is None:
+        return None, 0
+    if t.device != device or not t.is_contiguous():
+        raise QKError(where, QK_ERR_INVALID_ARG, f"workspace must be a contiguous tensor on {device}")
+    return t.data_ptr(), t.numel() * t.element_size()
+
+
+def _launch(device, stream, fn, *args) -> int:
+    """fn(*args, stream) with the tensors' device current: on the given stream,
+    or on the device's current torch stream."""
+    cuda = _TORCH.cuda
+    index = device.index
+    if stream is None:
+        stream = _TORCH._C._cuda_getCurrentRawStream(index)
+    elif not isinstance(stream, int):
+        stream = stream.cuda_stream
+    if cuda.current_device() == index:
+        return fn(*args, stream)
+    with cuda.device(index):
+        return fn(*args, stream)
 
 
 class PagedKV:
@@ -467,6 +513,7 @@ class PagedKV:
 
     def __init__(self, type: int, key, value, key_scale=None, value_scale=None):
         where = "PagedKV"
+        _torch()
         if type not in _KV_DTYPES:
             raise QKError(where, QK_ERR_TYPE, f"cache type {type} is not F16, I8 or F8_E4M3")
         _want(where, "key", key, (_KV_DTYPES[type],), (None,) * 4)
@@ -483,11 +530,12 @@ class PagedKV:
         self.pages, self.kv_heads, self.page_rows, self.head_dim = (int(n) for n in key.shape)
         self.desc = qk_paged_kv(type, self.kv_heads, self.head_dim, self.page_rows, self.pages, ptr(key), ptr(value),
                                 ptr(key_scale), ptr(value_scale))
+        self.ref, self.device, self.width = ctypes.byref(self.desc), key.device, self.kv_heads * self.head_dim
 
     @classmethod
     def empty(cls, type: int, pages: int, kv_heads: int, page_rows: int, head_dim: int, device="cuda") -> "PagedKV":
         """A cache whose rows are not written yet."""
-        import torch
+        torch = _torch()
         if type not in _KV_DTYPES:
             raise QKError("PagedKV", QK_ERR_TYPE, f"cache type {type} is not F16, I8 or F8_E4M3")
         dtype = getattr(torch, _KV_DTYPES[type].split(".")[1])
@@ -512,6 +560,13 @@ class PagedBatch:
         self.max_count, self.max_rows = int(max_count), int(max_rows)
         self.desc = qk_paged_batch(ptr(page_table), page_table.shape[0], page_table.shape[1], ptr(seqs), seqs.shape[0],
                                    self.n_tokens, self.max_count, self.max_rows)
+        self.ref, self.device = ctypes.byref(self.desc), seqs.device
+
+
+def _one_device(where: str, kv: PagedKV, batch: PagedBatch):
+    if kv.device != batch.device:
+        raise QKError(where, QK_ERR_INVALID_ARG, f"cache on {kv.device}, batch on {batch.device}")
+    return kv.device
 
 
 def rope_tables(theta: float, rot_dim: int, cosine, sine, first_pos: int = 0, scaling: dict | None = None,
@@ -519,24 +574,25 @@ def rope_tables(theta: float, rot_dim: int, cosine, sine, first_pos: int = 0, sc
     """qk_rope_tables_f32: cosine and sine, [positions][rot_dim / 2] float32, of
     positions first_pos, first_pos + 1, ...  scaling: {"type": "none", "linear",
     "llama3" or "yarn", "factor": ..., ...} with the fields of qk_rope_scaling;
-    freq_factors: rot_dim / 2 values that divide the frequencies."""
+    freq_factors: rot_dim / 2 values that divide the frequencies.  Like every
+    call of this section it runs on the tensors' device, on the given stream or
+    else on that device's current torch stream."""
     where = "rope_tables"
-    _want(where, "cosine", cosine, ("torch.float32",), (None, rot_dim // 2))
-    _want(where, "sine", sine, ("torch.float32",), tuple(cosine.shape))
-    if freq_factors is not None:
-        _want(where, "freq_factors", freq_factors, ("torch.float32",), (rot_dim // 2,))
+    f32 = _torch().float32
+    positions = cosine.shape[0] if cosine.dim() == 2 else -1
+    device = _gpu(where, "cosine", cosine)
+    c_ptr = _dense(where, "cosine", cosine, f32, (positions, rot_dim // 2), device)
+    s_ptr = _dense(where, "sine", sine, f32, (positions, rot_dim // 2), device)
+    f_ptr = None if freq_factors is None else _dense(where, "freq_factors", freq_factors, f32, (rot_dim // 2,), device)
     c = None
     if scaling is not None:
         fields = dict(scaling)
         kind = fields.pop("type", "none")
-        unknown = set(fields) - {n for n, _ in qk_rope_scaling._fields_}
-        if kind not in ROPE_SCALING or unknown:
-            raise QKError(where, QK_ERR_INVALID_ARG, f"unknown scaling {kind!r} {sorted(unknown)}")
-        c = ctypes.byref(qk_rope_scaling(type=ROPE_SCALING[kind], **{n: float(v) for n, v in fields.items()}))
-    guard, st = _on(where, cosine, stream, sine, freq_factors)
-    with guard:
-        check(lib().qk_rope_tables_f32(theta, rot_dim, c, ptr(freq_factors), first_pos, cosine.shape[0], ptr(cosine),
-                                       ptr(sine), st), "rotary table launch")
+        if kind not in ROPE_SCALING or not fields.keys() <= _SCALING_FIELDS:
+            raise QKError(where, QK_ERR_INVALID_ARG, f"unknown scaling {scaling}")
+        c = ctypes.byref(qk_rope_scaling(ROPE_SCALING[kind], **fields))
+    check(_launch(device, stream, lib().qk_rope_tables_f32, theta, rot_dim, c, f_ptr, first_pos, positions, c_ptr,
+                  s_ptr), "rotary table launch")
 
 
 def rope_paged_write(kv: PagedKV, batch: PagedBatch, q, q_out, k, v, cosine, sine, heads: int,
@@ -545,43 +601,42 @@ def rope_paged_write(kv: PagedKV, batch: PagedBatch, q, q_out, k, v, cosine, sin
     (both may be None, or the same), k and v [n_tokens][kv_heads * head_dim]
     into the pages, k rotated.  rot_dim: head_dim when None; 0 needs no tables."""
     where = "rope_paged_write"
-    rot_dim = kv.head_dim if rot_dim is None else rot_dim
-    f32, n, width = ("torch.float32",), batch.n_tokens, kv.kv_heads * kv.head_dim
-    for name, t, w in (("q", q, heads * kv.head_dim), ("q_out", q_out, heads * kv.head_dim), ("k", k, width),
-                       ("v", v, width)):
-        if t is not None or name in "kv":
-            _want(where, name, t, f32, (n, w), last_contiguous=True)
-    positions = 0
+    device, n, w, hd = _one_device(where, kv, batch), batch.n_tokens, kv.width, kv.head_dim
+    rot_dim = hd if rot_dim is None else rot_dim
+    q_ptr = qo_ptr = c_ptr = s_ptr = None
+    ldq = ldq_out = positions = 0
+    if q is not None or q_out is not None:
+        ldq = _rows(where, "q", q, n, heads * hd, device)
+        ldq_out = _rows(where, "q_out", q_out, n, heads * hd, device)
+        q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
+    ldk, ldv = _rows(where, "k", k, n, w, device), _rows(where, "v", v, n, w, device)
     if rot_dim:
-        _want(where, "cosine", cosine, f32, (None, rot_dim // 2))
-        _want(where, "sine", sine, f32, tuple(cosine.shape))
-        positions = cosine.shape[0]
-    guard, st = _on(where, kv.key, stream, batch.seqs, q, q_out, k, v, *((cosine, sine) if rot_dim else ()))
-    with guard:
-        check(lib().qk_rope_paged_write(ctypes.byref(kv.desc), ctypes.byref(batch.desc), ptr(q),
-                                        0 if q is None else _ld(q), ptr(q_out), 0 if q_out is None else _ld(q_out),
-                                        ptr(k), _ld(k), ptr(v), _ld(v), heads, ptr(cosine) if rot_dim else None,
-                                        ptr(sine) if rot_dim else None, positions, rot_dim, int(half), st),
-              "paged cache write launch")
+        f32 = _TORCH.float32
+        positions = cosine.shape[0] if cosine is not None and cosine.dim() == 2 else -1
+        c_ptr = _dense(where, "cosine", cosine, f32, (positions, rot_dim // 2), device)
+        s_ptr = _dense(where, "sine", sine, f32, (positions, rot_dim // 2), device)
+    check(_launch(device, stream, lib().qk_rope_paged_write, kv.ref, batch.ref, q_ptr, ldq, qo_ptr, ldq_out,
+                  k.data_ptr(), ldk, v.data_ptr(), ldv, heads, c_ptr, s_ptr, positions, rot_dim, int(half)),
+          "paged cache write launch")
 
 
 def paged_read(kv: PagedKV, batch: PagedBatch, key_out, value_out, stream=None) -> None:
     """qk_paged_read_f32: the rows of the batch's tokens as fp32, [n_tokens]
     [kv_heads * head_dim] each (either may be None)."""
     where = "paged_read"
-    for name, t in (("key_out", key_out), ("value_out", value_out)):
-        if t is not None:
-            _want(where, name, t, ("torch.float32",), (batch.n_tokens, kv.kv_heads * kv.head_dim), last_contiguous=True)
-    guard, st = _on(where, kv.key, stream, batch.seqs, key_out, value_out)
-    with guard:
-        check(lib().qk_paged_read_f32(ctypes.byref(kv.desc), ctypes.byref(batch.desc), ptr(key_out),
-                                      0 if key_out is None else _ld(key_out), ptr(value_out),
-                                      0 if value_out is None else _ld(value_out), st), "paged cache read launch")
+    device, n, w = _one_device(where, kv, batch), batch.n_tokens, kv.width
+    ldk = ldv = 0
+    if key_out is not None:
+        ldk = _rows(where, "key_out", key_out, n, w, device)
+    if value_out is not None:
+        ldv = _rows(where, "value_out", value_out, n, w, device)
+    check(_launch(device, stream, lib().qk_paged_read_f32, kv.ref, batch.ref, ptr(key_out), ldk, ptr(value_out), ldv),
+          "paged cache read launch")
 
 
 def paged_attention_workspace_bytes(batch: PagedBatch, heads: int, kv_heads: int, head_dim: int) -> int:
     """Workspace bytes of paged_attention."""
-    return int(lib().qk_paged_attention_workspace_bytes(ctypes.byref(batch.desc), heads, kv_heads, head_dim))
+    return int(lib().qk_paged_attention_workspace_bytes(batch.ref, heads, kv_heads, head_dim))
 
 
 def paged_attention(kv: PagedKV, batch: PagedBatch, q, out, heads: int, scale: float = 0.0, workspace=None,
@@ -590,14 +645,11 @@ def paged_attention(kv: PagedKV, batch: PagedBatch, q, out, heads: int, scale: f
     [heads * head_dim]) over its sequence's pages up to its own position, into
     out.  scale: 1 / sqrt(head_dim) when 0."""
     where = "paged_attention"
-    for name, t in (("q", q), ("out", out)):
-        _want(where, name, t, ("torch.float32",), (batch.n_tokens, heads * kv.head_dim), last_contiguous=True)
-    nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    guard, st = _on(where, kv.key, stream, batch.seqs, q, out, workspace)
-    with guard:
-        check(lib().qk_paged_attention_f32(ctypes.byref(kv.desc), ctypes.byref(batch.desc), ptr(q), _ld(q), ptr(out),
-                                           _ld(out), heads, scale, ptr(workspace), nbytes, st),
-              "paged attention launch")
+    device, n, w = _one_device(where, kv, batch), batch.n_tokens, heads * kv.head_dim
+    ldq, ldout = _rows(where, "q", q, n, w, device), _rows(where, "out", out, n, w, device)
+    ws, nbytes = _space(where, workspace, device)
+    check(_launch(device, stream, lib().qk_paged_attention_f32, kv.ref, batch.ref, q.data_ptr(), ldq, out.data_ptr(),
+                  ldout, heads, scale, ws, nbytes), "paged attention launch")
 
 
 def sample_workspace_bytes(n: int, rows: int) -> int:
@@ -612,19 +664,19 @@ def sample_rows(logits, uniform, out, temperature=None, top_k=None, top_p=None, 
     (float32) and top_k (int32) hold a value a row, or are None: 1, and no
     filter.  prob (float32 [rows] or None) receives the token's probability."""
     where = "sample_rows"
-    _want(where, "logits", logits, ("torch.float32",), (None, None), last_contiguous=True)
+    torch = _torch()
+    if logits.dim() != 2:
+        raise QKError(where, QK_ERR_SHAPE, f"logits has shape {tuple(logits.shape)}, expected rows of logits")
     rows, n = logits.shape
-    for name, t, dt in (("uniform", uniform, "float32"), ("out", out, "int32"), ("temperature", temperature, "float32"),
-                        ("top_k", top_k, "int32"), ("top_p", top_p, "float32"), ("min_p", min_p, "float32"),
-                        ("prob", prob, "float32")):
-        if t is not None or name in ("uniform", "out"):
-            _want(where, name, t, ("torch." + dt,), (rows,))
-    nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    guard, st = _on(where, logits, stream, uniform, out, temperature, top_k, top_p, min_p, prob, workspace)
-    with guard:
-        check(lib().qk_sample_rows_f32(ptr(logits), n, _ld(logits), rows, ptr(temperature), ptr(top_k), ptr(top_p),
-                                       ptr(min_p), ptr(uniform), ptr(out), ptr(prob), ptr(workspace), nbytes, st),
-              "sampling launch")
+    device = _gpu(where, "logits", logits)
+    ldv = _rows(where, "logits", logits, rows, n, device)
+    f32, i32, shape = torch.float32, torch.int32, (rows,)
+    of = lambda name, t, dt: None if t is None else _dense(where, name, t, dt, shape, device)
+    u_ptr, o_ptr = _dense(where, "uniform", uniform, f32, shape, device), _dense(where, "out", out, i32, shape, device)
+    ws, nbytes = _space(where, workspace, device)
+    check(_launch(device, stream, lib().qk_sample_rows_f32, logits.data_ptr(), n, ldv, rows,
+                  of("temperature", temperature, f32), of("top_k", top_k, i32), of("top_p", top_p, f32),
+                  of("min_p", min_p, f32), u_ptr, o_ptr, of("prob", prob, f32), ws, nbytes), "sampling launch")
 
 
 def _upload_weights(owner, cfg: dict, weights: dict):
