@@ -524,9 +524,9 @@ int qk_paged_attention_f32(const qk_paged_kv *kv, const qk_paged_batch *batch, c
                            qk_stream stream);
 
 /* The next token of each of `rows` rows of n logits (row r at logits + r *
-   ldv).  Of row r, with w_i = exp((logit_i - max) / temperature[r]) rounded to
-   a multiple of 2^-44, tokens in descending order of their logits (equal ones
-   by index):
+   ldv).  Of row r, with w_i = exp((logit_i - max) / temperature[r]) held to
+   2^-45 (a token below that may have no weight), tokens in descending order of
+   their logits (equal ones by index):
      top_k[r]  keeps the first top_k (<= 0: all),
      top_p[r]  of those the shortest run whose weights reach top_p of their sum
                (1: all),
