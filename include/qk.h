@@ -525,8 +525,8 @@ int qk_paged_attention_f32(const qk_paged_kv *kv, const qk_paged_batch *batch, c
 
 /* The next token of each of `rows` rows of n logits (row r at logits + r *
    ldv).  Of row r, with w_i = exp((logit_i - max) / temperature[r]) held to
-   2^-45 (a token below that may have no weight), tokens in descending order of
-   their logits (equal ones by index):
+   2^-30 of itself (a token below 2^-45 may have no weight), tokens in descending
+   order of their logits (equal ones by index):
      top_k[r]  keeps the first top_k (<= 0: all),
      top_p[r]  of those the shortest run whose weights reach top_p of their sum
                (1: all),
@@ -536,8 +536,8 @@ int qk_paged_attention_f32(const qk_paged_kv *kv, const qk_paged_batch *batch, c
    prob (or NULL) receives its share of that sum.  temperature[r] <= 0, or a
    parameter that is NaN, keeps the first alone.  NaN logits count as -inf;
    where a logit is +inf, those that are share the weight.  A row without a
-   logit above -inf gives 0 with prob 0.  The sums are of integers: a row's
-   token does not depend on the other rows or the launch.  All arrays are on
+   logit above -inf gives 0 with prob 0.  A row's
+   token does not depend on the other rows.  All arrays are on
    the device; temperature, top_k, top_p and min_p hold `rows` values, or are
    NULL: 1, and no filter.  workspace: qk_sample_rows_workspace_bytes(n, rows)
    bytes, 256-byte aligned; calls sharing it must not overlap. */

@@ -2,31 +2,66 @@
 // min-p and the pick by a given random number.
 //
 // The filters keep a prefix of the row in descending order (equal logits by
-// index), so what they leave is the tokens from one of them on: the cut.  Two
+// index), so what they leave is the tokens down to one of them: the cut.  Four
 // launches:
 //   sample_scan_kernel, a workgroup per 16384 logits (a segment): its largest,
 //     and a histogram over 16 bins an octave of the weights 2^(x log2(e) / T)
-//     below the segment's own power of two 2^E, as integers in units of
-//     2^(E - 46), so the order of adding does not matter;
-//   sample_pick_kernel, a workgroup per row: adds up the segments' histograms,
-//     finds the bin in which the cut lies, reads the row again for that bin's
-//     tokens (some hundreds at most, or with top-k all that it leaves), sorts
-//     them and finds the cut; then the segment that holds the random number's
-//     token from the histograms, and the token by looking that segment over.
-// A row is thus read once from memory and once from the cache, and each
-// weight's exponential (in 64 bits: 32 would move the borders between tokens by
-// 1e-8 of the sum, and with them one token in some thousands of rows) is taken
-// once.  Rows that this does not serve -- an infinite logit, more tokens in the
-// cut's bin than its list holds (thousands of equal logits, or a temperature
-// that leaves all of them alike), |x log2(e) / T| of 2^20 and more -- go through
-// sample_plain, which finds the cut digit by digit from histograms of the
-// floats' order.
+//     below the segment's own power of two, as integers, so the order of adding
+//     does not matter;
+//   sample_plan_kernel, a workgroup per row: adds up the segments' histograms
+//     and finds the bin in which the cut lies;
+//   sample_collect_kernel, per segment again: lists that bin's tokens (some
+//     hundreds at most; with top-k, where they fit, all that it leaves);
+//   sample_pick_kernel, a workgroup per row: sorts the list and finds the cut,
+//     then from the histograms the segment that holds the random number's token,
+//     and the token by looking that segment over.
+// A row is thus read once from memory and once from the cache, and its
+// exponentials are taken once.  They are held to 2^-30 of themselves: with the 24
+// bits of a float the borders between 10^5 tokens of like weight would move by
+// some 10^-5 of a token's width, and with them one token in some ten thousand
+// rows; in 64 bits (half the rate, its conversions a quarter) the scan of 512
+// rows of 128256 took 100 us.  Rows that this does not serve -- an infinite
+// logit, more tokens in the cut's bin than its list holds (thousands of equal
+// logits, or a temperature that leaves all of them alike), |x log2(e) / T| of 4096
+// and more -- go through sample_plain, which finds the cut digit by digit from
+// histograms of the floats' order.
 #include "qk_internal.h"
 
 namespace qk {
 namespace {
 
 hipStream_t S(qk_stream s) { return static_cast<hipStream_t>(s); }
+
+constexpr int kThreads = 512, kWaves = kThreads / 64;
+constexpr int kSegment = 32 * kThreads;
+constexpr int kMaxSegments = (1 << 19) / kSegment;
+constexpr int kOctave = 16, kBins = 48 * kOctave;
+constexpr int kFine = 128;   // steps of an octave in the weights' table
+constexpr int kList = 2048;
+constexpr int kGather = 8;   // segments whose bins a thread loads at once
+constexpr int kCopies = 2;   // of a segment's histogram in LDS: half the conflicts
+constexpr double kUnit = 17592186044416.;   // 2^44: sample_plain's weights, of which 2^19 stay below 2^64
+
+// A segment's largest logit, its lowest index (of greedy rows), and the power of
+// two that its weights are below (kNone: no logit above -inf, kFar: out of range).
+struct SegmentHead {
+    float best;
+    int at, e, pad;
+};
+constexpr int kNone = -0x40000000, kFar = 0x40000000;
+
+// A row as its segments leave it.
+struct RowPlan {
+    double least;    // the weight that min-p asks for, in units of 2^(e - 31)
+    float best;
+    int e;           // the row's power of two
+    int way;         // kDone: the token is out; kPlain: for sample_plain; kBinned
+    int counted;     // top-k leaves tokens out
+    int bin_k;       // the bin of top-k's last token, kBins without
+    int bin_m, m_hi; // the bins around `least` (two where it is near a border), kBins without
+    int lo, hi;      // the bins to list first (lo > hi: none)
+};
+constexpr int kDone = 0, kPlain = 1, kBinned = 2;
 
 struct SampleArgs {
     const float *logits;
@@ -36,31 +71,21 @@ struct SampleArgs {
     const int32_t *top_k;
     int32_t *out;
     float *prob;
-    struct SegmentHead *heads;   // [rows][segments]
-    uint64_t *mass;              // [rows][segments][kBins]
-    uint32_t *count;             // the same, of rows with top-k
-    int segments, wide;          // wide: rows are 16-byte aligned
+    SegmentHead *heads;   // [rows][segments]
+    RowPlan *plans;       // [rows]
+    uint64_t *mass;       // [rows][segments][kBins]: of bin i in units of 2^(segment's e - 31 - i / 16)
+    double *cum;          // [rows][kBins]: sums of the row's bins up to each, in units of 2^(e - 31)
+    uint64_t *list;       // [rows][kList] tokens of the bins asked for
+    uint32_t *count;      // [rows][segments][kBins] tokens, of rows with top-k
+    uint32_t *counts;     // [rows][kBins]: sums up to each
+    int *listed;          // [rows]
+    int segments, wide;   // wide: rows are 16-byte aligned
 };
 
-// A segment's largest logit, its lowest index, and the power of two that its
-// weights are below (kNone: no logit above -inf, kFar: out of range).
-struct SegmentHead {
-    float best;
-    int at, e, pad;
-};
-constexpr int kNone = -0x40000000, kFar = 0x40000000;
-
-constexpr int kThreads = 512, kWaves = kThreads / 64;   // of sample_pick_kernel
-constexpr int kScanThreads = 1024, kSegment = 16 * kScanThreads;
-constexpr int kMaxSegments = (1 << 19) / kSegment;
-constexpr int kBins = 768, kOctave = 16;   // 48 octaves; a weight has 46 bits
-constexpr int kList = 2048;
-constexpr double kUnit = 17592186044416.;   // 2^44: sample_plain's weights, of which 2^19 stay below 2^64
-
-// Order-preserving key; NaN as -inf, -0 as 0.
-__device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x + 0.f; }
+// NaN as -inf; -0 as 0 in the order-preserving key.
+__device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY); }
 __device__ __forceinline__ uint32_t key_of(float x) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, x);
+    const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t k) {
@@ -80,6 +105,37 @@ __device__ __forceinline__ RowParams row_params(const SampleArgs &a, int row) {
     return r;
 }
 
+// Inclusive sums over a wave's lanes of a 64-bit type: the rows of 16 by DPP
+// shifts, then the rows before (a lane without a source adds 0).
+template <int CTRL, int ROWS, class T>
+__device__ __forceinline__ T dpp_part(T v) {
+    static_assert(sizeof(T) == 8, "two dwords");
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(b), CTRL, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), CTRL, ROWS, 0xF, false);
+    return __builtin_bit_cast(T, static_cast<uint64_t>(hi) << 32 | lo);
+}
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {
+    v += dpp_part<0x111, 0xF>(v);   // row_shr 1, 2, 4, 8
+    v += dpp_part<0x112, 0xF>(v);
+    v += dpp_part<0x114, 0xF>(v);
+    v += dpp_part<0x118, 0xF>(v);
+    v += dpp_part<0x142, 0xA>(v);   // row_bcast 15 into rows 1 and 3
+    v += dpp_part<0x143, 0xC>(v);   // row_bcast 31 into rows 2 and 3
+    return v;
+}
+// The last lane's value of a 64-bit type.
+template <class T>
+__device__ __forceinline__ T wave_last(T v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(b), 63);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(b >> 32), 63);
+    return __builtin_bit_cast(T, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// -------------------------------------------------- rows digit by digit --
+
 struct RowScale {
     float top;
     double t;
@@ -91,9 +147,7 @@ __device__ __forceinline__ uint64_t weight(float x, const RowScale &r) {
 }
 
 __device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
-    #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
-    return v;
+    return wave_last(wave_scan(v));
 }
 // Sum over the workgroup, to every thread.
 __device__ __forceinline__ uint64_t block_sum_u64(uint64_t v, uint64_t *scratch) {
@@ -263,12 +317,7 @@ __device__ __forceinline__ void sample_plain(const SampleArgs &a, const RowParam
     for (int i0 = 0; i0 < a.n; i0 += kThreads) {
         const int i = i0 + tid;
         const uint64_t w = i < a.n ? kept(i) : 0;
-        uint64_t upto = w;
-        #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const uint64_t o = __shfl_up(upto, off);
-            if (lane >= off) upto += o;
-        }
+        uint64_t upto = wave_scan(w);
         __syncthreads();
         if (lane == 63) scratch[wave] = upto;
         __syncthreads();
@@ -291,30 +340,58 @@ __device__ __forceinline__ void sample_plain(const SampleArgs &a, const RowParam
 
 constexpr double kLog2E = 1.4426950408889634074;
 
-// 2^-d in units of 2^-46, d = i / 16 + r below 47 and bin i: 2^-(i % 16 + 1/2)/16
-// from the table, e^(-y ln 2) of |y| <= 1/32 by its Taylor polynomial to y^6
-// (the next term is 4e-16), the power of two into the exponent, rounded by
-// adding 2^52.
-__device__ __forceinline__ uint64_t unit_weight(double d, int i, const double *table) {
-    const double y = fma(static_cast<double>(i), -1. / kOctave, d) - 0.5 / kOctave;
-    double p = 1.5403530393381609954e-4;
-    p = fma(p, y, -1.3333558146428443423e-3);
-    p = fma(p, y, 9.6181291076284771619e-3);
-    p = fma(p, y, -5.5504108664821579953e-2);
-    p = fma(p, y, 2.4022650695910071233e-1);
-    p = fma(p, y, -6.9314718055994530942e-1);
-    p = fma(p, y, 1.);
-    const double v = p * table[i & (kOctave - 1)];
-    const uint64_t scaled = __builtin_bit_cast(uint64_t, v) + (static_cast<uint64_t>(46 - i / kOctave) << 52);
-    return __builtin_bit_cast(uint64_t, __builtin_bit_cast(double, scaled) + 4503599627370496.) - 0x4330000000000000ull;
+// log2(e) / T as two floats.
+struct Slope {
+    float hi, lo;
+};
+__device__ __forceinline__ Slope slope_of(float t) {
+    const double c = kLog2E / static_cast<double>(t);
+    const float hi = static_cast<float>(c);
+    return {hi, static_cast<float>(c - static_cast<double>(hi))};
 }
 
-// How far a logit's weight lies below 2^e, in octaves (inf for none).
-__device__ __forceinline__ double octaves_below(float x, double c, int e) {
-    return fma(-static_cast<double>(x), c, static_cast<double>(e));
+// The power of two above a segment's weights by its largest logit: t = x c is
+// below it for every x, since p is monotone.
+__device__ __forceinline__ int exponent_of(float best, const Slope &c) {
+    const float p = best * c.hi;
+    return best == -INFINITY ? kNone : !(fabsf(p) < 4096.f) ? kFar : static_cast<int>(floorf(p)) + 1;
 }
-constexpr double kDepth = 47.;   // from here on a weight rounds to 0
-__device__ __forceinline__ int bin_of(double d) { return static_cast<int>(fmax(d, 0.) * kOctave); }
+
+// t = x c = p + lo to some 48 bits, p = (g + 1/2) / 128 + y with y exact, f = 128
+// e - 1 - g >= 0 the fine step below 2^e, or -1 from 47 octaves on (and for
+// -inf).  y with lo stays within 1/256 + 2^-12.
+struct Depth {
+    float y;
+    int f;
+    __device__ __forceinline__ int bin() const { return f >> 3; }
+};
+static_assert(kFine == 8 * kOctave, "Depth::bin");
+__device__ __forceinline__ Depth depth_of(float x, const Slope &c, int e) {
+    const float p = x * c.hi, lo = fmaf(x, c.lo, fmaf(x, c.hi, -p));
+    const float g = floorf(p * kFine);
+    const float y = fmaf(g, -1.f / kFine, p) + (lo - 0.5f / kFine);
+    const int top = kFine * e;
+    const bool in = g >= static_cast<float>(top - 47 * kFine);
+    return {y, in ? top - 1 - static_cast<int>(g) : -1};
+}
+
+// The weight of a step f in units of 2^(e - 31 - f / 128): 2^-((f % 128) + 1/2)/128
+// from the table (as an integer and as a float), times 1 + z with z = e^(y ln 2) -
+// 1 by its Taylor polynomial (the next term is 2^-38), which is so small that 24
+// bits of it are 32 of the weight.
+__device__ __forceinline__ uint32_t unit_weight(const Depth &d, const uint2 *table) {
+    const uint2 t = table[d.f & (kFine - 1)];
+    float z = fmaf(d.y, 5.5504108664821580e-2f, 2.4022650695910072e-1f);
+    z = fmaf(d.y, z, 6.9314718055994531e-1f) * d.y;
+    return t.x + static_cast<uint32_t>(static_cast<int>(z * __builtin_bit_cast(float, t.y)));
+}
+
+__device__ __forceinline__ void fill_table(uint2 *table) {
+    if (threadIdx.x < kFine) {
+        const double w = exp2(31. - (static_cast<double>(threadIdx.x) + 0.5) / kFine);
+        table[threadIdx.x] = make_uint2(static_cast<uint32_t>(rint(w)), __builtin_bit_cast(uint32_t, static_cast<float>(w)));
+    }
+}
 
 __device__ __forceinline__ void load_quad(const float *x, int i, int n, int wide, float (&v)[4]) {
     if (wide && i + 3 < n) {
@@ -326,125 +403,298 @@ __device__ __forceinline__ void load_quad(const float *x, int i, int n, int wide
     }
 }
 
-__device__ __forceinline__ void fill_table(double *table) {
-    if (threadIdx.x < kOctave) table[threadIdx.x] = exp2(-(static_cast<double>(threadIdx.x) + 0.5) / kOctave);
+constexpr int kQuads = kSegment / (4 * kThreads);
+__device__ __forceinline__ int quad_at(int seg, int j) {
+    return seg * kSegment + (j * kThreads + static_cast<int>(threadIdx.x)) * 4;
 }
 
 // --------------------------------------------------------------- scan --
 
-__global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleArgs a) {
-    __shared__ unsigned long long mass[kBins];
+__global__ __launch_bounds__(kThreads) void sample_scan_kernel(SampleArgs a) {
+    __shared__ unsigned long long mass[kCopies][kBins];
     __shared__ uint32_t count[kBins];
-    __shared__ double table[kOctave];
-    __shared__ uint64_t best_of[kScanThreads / 64];
+    __shared__ uint2 table[kFine];
+    __shared__ float best_of[kWaves];
+    __shared__ int lowest;
     const int row = blockIdx.y, seg = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float *x = a.logits + static_cast<int64_t>(row) * a.ldv;
-    float v[4][4];
+    float v[kQuads][4];
     #pragma unroll
-    for (int j = 0; j < 4; ++j) load_quad(x, seg * kSegment + (j * kScanThreads + tid) * 4, a.n, a.wide, v[j]);
+    for (int j = 0; j < kQuads; ++j) load_quad(x, quad_at(seg, j), a.n, a.wide, v[j]);
     const RowParams r = row_params(a, row);
     fill_table(table);
-    for (int i = tid; i < kBins; i += kScanThreads) mass[i] = 0, count[i] = 0;
-    float best = -INFINITY;
-    int at = 0x7FFFFFFF;
-    #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int i = tid; i < kBins; i += kThreads) {
         #pragma unroll
-        for (int e = 0; e < 4; ++e) arg_better(best, at, v[j][e], seg * kSegment + (j * kScanThreads + tid) * 4 + e);
+        for (int k = 0; k < kCopies; ++k) mass[k][i] = 0;
+        count[i] = 0;
+    }
+    if (tid == 0) {
+        lowest = 0x7FFFFFFF;
+        if (seg == 0) a.listed[row] = 0;
+    }
+    float best = -INFINITY;
     #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) arg_better(best, at, __shfl_xor(best, off), __shfl_xor(at, off));
-    if (lane == 0) best_of[wave] = static_cast<uint64_t>(key_of(best)) << 32 | static_cast<uint32_t>(at);
+    for (int j = 0; j < kQuads; ++j)
+        #pragma unroll
+        for (int k = 0; k < 4; ++k) best = fmaxf(best, v[j][k]);
+    #pragma unroll
+    for (int off = 32; off > 0; off >>= 1) best = fmaxf(best, __shfl_xor(best, off));
+    if (lane == 0) best_of[wave] = best;
     __syncthreads();
-    for (int w = 0; w < kScanThreads / 64; ++w)
-        arg_better(best, at, value_of(static_cast<uint32_t>(best_of[w] >> 32)),
-                   static_cast<int>(best_of[w] & 0xFFFFFFFFu));
-    const double c = kLog2E / static_cast<double>(r.t), top = static_cast<double>(best) * c;
-    const int e = best == -INFINITY ? kNone : !(fabs(top) < 1048576.) ? kFar : static_cast<int>(ceil(top));
-    const int64_t me = static_cast<int64_t>(row) * a.segments + seg;
-    if (tid == 0) a.heads[me] = SegmentHead{best, at, e, 0};
-    if (r.greedy || e == kNone || e == kFar) return;
-    const bool counted = r.k > 0 && r.k < a.n;
     #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int w = 0; w < kWaves; ++w) best = fmaxf(best, best_of[w]);
+    const Slope c = slope_of(r.t);
+    const int e = exponent_of(best, c);
+    const int64_t me = static_cast<int64_t>(row) * a.segments + seg;
+    if (r.greedy) {
+        int at = 0x7FFFFFFF;
+        #pragma unroll
+        for (int j = kQuads - 1; j >= 0; --j)
+            #pragma unroll
+            for (int k = 3; k >= 0; --k) at = v[j][k] == best ? quad_at(seg, j) + k : at;
+        if (at < a.n) atomicMin(&lowest, at);
+        __syncthreads();
+        if (tid == 0) a.heads[me] = SegmentHead{best, lowest, kNone, 0};
+        return;
+    }
+    if (tid == 0) a.heads[me] = SegmentHead{best, 0, e, 0};
+    if (e == kNone || e == kFar) return;
+    const bool counted = r.k > 0 && r.k < a.n;
+    unsigned long long *const mine = mass[lane % kCopies];
+    #pragma unroll
+    for (int j = 0; j < kQuads; ++j)
         #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const double d = octaves_below(v[j][k], c, e);
-            if (d < kDepth) {
-                const int bin = bin_of(d);
-                atomicAdd(&mass[bin], static_cast<unsigned long long>(unit_weight(d, bin, table)));
-                if (counted) atomicAdd(&count[bin], 1u);
+            const Depth d = depth_of(v[j][k], c, e);
+            if (d.f >= 0) {
+                atomicAdd(&mine[d.bin()], static_cast<unsigned long long>(unit_weight(d, table)));
+                if (counted) atomicAdd(&count[d.bin()], 1u);
             }
         }
     __syncthreads();
-    for (int i = tid; i < kBins; i += kScanThreads) {
-        a.mass[me * kBins + i] = mass[i];
+    for (int i = tid; i < kBins; i += kThreads) {
+        uint64_t sum = 0;
+        #pragma unroll
+        for (int k = 0; k < kCopies; ++k) sum += mass[k][i];
+        a.mass[me * kBins + i] = sum;
         if (counted) a.count[me * kBins + i] = count[i];
     }
 }
 
-// --------------------------------------------------------------- pick --
+// --------------------------------------------------------------- plan --
 
-struct PickShared {
-    double cum[kBins];            // sums of the row's bins up to each, in units of 2^(e - 46)
-    uint64_t list[kList];         // tokens: the key's bits, then the index's complement
-    double sorted[kList];         // sums of the list's weights up to each
-    double table[kOctave];
-    SegmentHead head[kMaxSegments];
-    uint64_t kept[kMaxSegments];  // kept weight of each segment, in its own units
-    uint64_t part[8][kWaves];
-    double wave_sum[kWaves];
-    uint32_t wave_count[kWaves];
-    uint32_t counts[kBins];       // tokens of the row's bins up to each
-    int listed, bin_k, bin_p, cut, found;
-};
-
-// Inclusive sums over kBins values, two a thread, in a fixed order.
-template <class T>
-__device__ __forceinline__ void scan_bins(T *v, T *waves) {
-    static_assert(kBins <= 2 * kThreads, "two bins a thread");
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = 2 * tid;
-    T a = i < kBins ? v[i] : T(0), b = i + 1 < kBins ? v[i + 1] : T(0);
-    T sum = a + b;
-    #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const T o = __shfl_up(sum, off);
-        if (lane >= off) sum += o;
-    }
-    __syncthreads();
-    if (lane == 63) waves[wave] = sum;
-    __syncthreads();
-    T base = T(0);
-    for (int w = 0; w < wave; ++w) base += waves[w];
-    const T before = base + (sum - (a + b));
-    if (i < kBins) v[i] = before + a;
-    if (i + 1 < kBins) v[i + 1] = base + sum;
-    __syncthreads();
+// Octaves and bins from a segment's power of two down to the row's (64: no bin
+// of it is left).
+__device__ __forceinline__ int octaves_down(int e, int segment_e) {
+    return segment_e == kNone ? 64 : min(e - segment_e, 64);
 }
 
-// The first of kBins non-decreasing sums to reach target, kBins if none does.
-template <class T>
+// The first of kBins sums to reach target (rounding may leave two such steps:
+// the lower), kBins if none does; by kBins threads or fewer, several bins each.
+template <int THREADS, class T>
 __device__ __forceinline__ int first_reaching(const T *cum, double target, int *found) {
+    __syncthreads();
     if (threadIdx.x == 0) *found = kBins;
     __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += kThreads)
+    #pragma unroll
+    for (int i = threadIdx.x; i < kBins; i += THREADS)
         if (static_cast<double>(cum[i]) >= target && (i == 0 || static_cast<double>(cum[i - 1]) < target))
-            atomicMin(found, i);   // rounding may leave two such steps
+            atomicMin(found, i);
     __syncthreads();
-    const int r = *found;
-    __syncthreads();
-    return r;
+    return *found;
 }
+
+__global__ __launch_bounds__(kBins) void sample_plan_kernel(SampleArgs a) {
+    __shared__ SegmentHead head[kMaxSegments];
+    __shared__ double cum[kBins];
+    __shared__ uint32_t counts[kBins];
+    __shared__ uint2 table[kFine];
+    __shared__ double sums[kBins / 64];
+    __shared__ uint64_t tokens[kBins / 64];
+    __shared__ int found;
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const RowParams r = row_params(a, row);
+    const int64_t first = static_cast<int64_t>(row) * a.segments;
+    if (tid < a.segments) head[tid] = a.heads[first + tid];
+    fill_table(table);
+    __syncthreads();
+    RowPlan st{0., -INFINITY, kNone, kBinned, r.k > 0 && r.k < a.n, kBins, kBins, kBins, 0, -1};
+    int at = 0x7FFFFFFF;
+    bool far = false;
+    for (int g = 0; g < a.segments; ++g) {
+        const SegmentHead h = head[g];
+        arg_better(st.best, at, h.best, h.at);
+        far = far || h.e == kFar;
+        if (h.e != kFar) st.e = max(st.e, h.e);
+    }
+    if (st.best == -INFINITY || r.greedy) {
+        if (tid == 0) {
+            a.out[row] = st.best == -INFINITY ? 0 : at;
+            if (a.prob) a.prob[row] = st.best == -INFINITY ? 0.f : 1.f;
+        }
+        st.way = kDone;
+    } else if (far) {
+        st.way = kPlain;
+    } else {
+        // Bin tid of the row: of a segment m octaves lower, its bin tid - 16 m.
+        // The integers of one bin have one unit, so they add up exactly.
+        uint64_t sum = 0, n = 0;
+        for (int g0 = 0; g0 < a.segments; g0 += kGather) {
+            uint64_t w[kGather];
+            uint32_t m[kGather];
+            #pragma unroll
+            for (int k = 0; k < kGather; ++k) {   // all loads first
+                const int g = min(g0 + k, a.segments - 1), from = tid - kOctave * octaves_down(st.e, head[g].e);
+                const bool in = g0 + k < a.segments && from >= 0;
+                const int64_t i = (first + g) * kBins + max(from, 0);
+                w[k] = in ? a.mass[i] : 0;
+                m[k] = in && st.counted ? a.count[i] : 0;
+            }
+            #pragma unroll
+            for (int k = 0; k < kGather; ++k) {
+                sum += w[k];
+                n += m[k];
+            }
+        }
+        const double mine = wave_scan(ldexp(static_cast<double>(sum), -(tid / kOctave)));
+        const uint64_t upto = wave_scan(n);
+        if (lane == 63) {
+            sums[wave] = mine;
+            tokens[wave] = upto;
+        }
+        __syncthreads();
+        double before = 0.;
+        uint64_t earlier = 0;
+        for (int w = 0; w < wave; ++w) {
+            before += sums[w];
+            earlier += tokens[w];
+        }
+        cum[tid] = before + mine;
+        counts[tid] = static_cast<uint32_t>(earlier + upto);
+        a.cum[static_cast<int64_t>(row) * kBins + tid] = cum[tid];
+        if (st.counted) {
+            a.counts[static_cast<int64_t>(row) * kBins + tid] = counts[tid];
+            st.bin_k = first_reaching<kBins>(counts, static_cast<double>(r.k), &found);
+        }
+        if (r.mp > 0.f) {
+            const Depth d = depth_of(st.best, slope_of(r.t), st.e);
+            st.least = ldexp(static_cast<double>(r.mp) * unit_weight(d, table), -(d.f / kFine));
+            const double below = (d.f + 0.5) / kFine - d.y - log2(static_cast<double>(r.mp));
+            // A token's bin goes by p alone, which is off by 2^-12 octaves at most.
+            auto bin_at = [](double d) { return static_cast<int>(fmin(fmax(d, 0.), 48.) * kOctave); };
+            st.bin_m = bin_at(below - 0x1p-11);
+            st.m_hi = bin_at(below + 0x1p-11);
+        }
+        if (st.bin_k < kBins) {
+            st.lo = counts[st.bin_k] <= kList ? 0 : st.bin_k;   // all that top-k leaves, where it fits the list
+            st.hi = st.bin_k;
+        } else {
+            __syncthreads();
+            const double target = static_cast<double>(r.p) * cum[kBins - 1];
+            const int bin = min(st.bin_m, r.p < 1.f ? first_reaching<kBins>(cum, target, &found) : kBins);
+            if (bin < kBins) {
+                st.lo = bin;
+                st.hi = bin == st.bin_m ? st.m_hi : bin;
+            }
+        }
+    }
+    if (tid == 0) a.plans[row] = st;
+}
+
+// ------------------------------------------------------------ collect --
 
 __device__ __forceinline__ uint64_t packed(float x, int i) {
     return static_cast<uint64_t>(key_of(x)) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(i));
 }
 
-// Descending bitonic sort of list[0 .. size), size a power of two.
-__device__ __forceinline__ void sort_list(uint64_t *list, int size) {
+// Logits that may lie in a segment's bins lo .. hi: their interval, widened by
+// more than the roundings of the bins' arithmetic, so few get the exact test.
+struct Range {
+    Slope c;
+    int e, lo, hi;
+    float low, high;
+};
+__device__ __forceinline__ Range range_of(int lo, int hi, float t, int e) {
+    const double c = kLog2E / static_cast<double>(t);
+    const double high = (e - lo * (1. / kOctave)) / c, low = (e - (hi + 1) * (1. / kOctave)) / c;
+    return {slope_of(t), e, lo, hi, static_cast<float>(low - 1e-6 * (fabs(low) + 1e-20)),
+            static_cast<float>(high + 1e-6 * (fabs(high) + 1e-20))};
+}
+
+// The tokens of a quad within a range, into a list of the workgroup.
+__device__ __forceinline__ void list_quad(const float (&v)[4], int i, const Range &in, uint64_t *list, int *listed) {
+    #pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if (!(v[k] >= in.low && v[k] <= in.high)) continue;
+        const Depth d = depth_of(v[k], in.c, in.e);
+        if (d.f >= 0 && d.bin() >= in.lo && d.bin() <= in.hi) {
+            const int slot = atomicAdd(listed, 1);
+            if (slot < kList) list[slot] = packed(v[k], i + k);
+        }
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleArgs a) {
+    __shared__ uint64_t list[kList];
+    __shared__ int listed, base;
+    const int row = blockIdx.y, seg = blockIdx.x, tid = threadIdx.x;
+    const float *x = a.logits + static_cast<int64_t>(row) * a.ldv;
+    const RowPlan &st = a.plans[row];
+    const SegmentHead &head = a.heads[static_cast<int64_t>(row) * a.segments + seg];
+    if (st.way != kBinned || st.lo > st.hi || head.e == kNone) return;
+    const int shift = kOctave * octaves_down(st.e, head.e);
+    if (st.hi < shift) return;
+    float v[kQuads][4];
+    #pragma unroll
+    for (int j = 0; j < kQuads; ++j) load_quad(x, quad_at(seg, j), a.n, a.wide, v[j]);
+    const Range in = range_of(st.lo - shift, st.hi - shift, a.temperature ? a.temperature[row] : 1.f, head.e);
+    if (tid == 0) listed = 0;
+    __syncthreads();
+    #pragma unroll
+    for (int j = 0; j < kQuads; ++j) list_quad(v[j], quad_at(seg, j), in, list, &listed);
+    __syncthreads();
+    const int n = listed;
+    if (n == 0) return;
+    if (tid == 0) base = atomicAdd(&a.listed[row], n);
+    __syncthreads();
+    for (int i = tid; i < min(n, kList); i += kThreads)
+        if (base + i < kList) a.list[static_cast<int64_t>(row) * kList + base + i] = list[i];
+}
+
+// --------------------------------------------------------------- pick --
+
+struct PickShared {
+    uint64_t list[kList];         // tokens: the key's bits, then the index's complement
+    double sorted[kList];         // sums of the list's weights up to each
+    double cum[kBins];
+    uint2 table[kFine];
+    SegmentHead head[kMaxSegments];
+    double kept[kMaxSegments];    // kept weight of each segment, in units of the row's 2^(e - 31)
+    double wave_sum[kWaves];
+    uint64_t part[kQuads][kWaves];
+    int listed, found, cut;
+};
+
+// Descending order of list[0 .. n): by counting the larger ones of each where
+// they are few, else a bitonic sort (of a power of two, the rest zeros).
+__device__ __forceinline__ void sort_list(uint64_t *list, int n) {
+    const int tid = threadIdx.x;
+    if (n <= 256) {
+        const uint64_t mine = tid < n ? list[tid] : 0;
+        int rank = 0;
+        for (int i = 0; i < n; ++i) rank += list[i] > mine;
+        __syncthreads();
+        if (tid < n) list[rank] = mine;
+        __syncthreads();
+        return;
+    }
+    int size = 512;
+    while (size < n) size <<= 1;
+    for (int i = n + tid; i < size; i += kThreads) list[i] = 0;
     for (int k = 2; k <= size; k <<= 1)
         for (int j = k >> 1; j > 0; j >>= 1) {
             __syncthreads();
-            for (int t = threadIdx.x; t < size / 2; t += kThreads) {
+            for (int t = tid; t < size / 2; t += kThreads) {
                 const int i = 2 * t - (t & (j - 1)), o = i + j;
                 const uint64_t p = list[i], q = list[o];
                 if ((p < q) == ((i & k) == 0)) list[i] = q, list[o] = p;
@@ -453,98 +703,54 @@ __device__ __forceinline__ void sort_list(uint64_t *list, int size) {
     __syncthreads();
 }
 
-// A row by its segments' histograms, by all threads of the workgroup; false:
-// it is one for sample_plain, with its largest logit in best.
-__device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowParams &r, int row, float &best,
+// A row by its segments' histograms and its list, by all threads of the
+// workgroup; false: it is one for sample_plain.
+__device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowParams &r, const RowPlan &st, int row,
                                               PickShared &s) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float *x = a.logits + static_cast<int64_t>(row) * a.ldv;
     const int64_t first = static_cast<int64_t>(row) * a.segments;
-    best = -INFINITY;
-    int at = 0x7FFFFFFF, e = kNone;
-    bool far = false;
-    for (int g = 0; g < a.segments; ++g) {
-        const SegmentHead h = a.heads[first + g];
-        arg_better(best, at, h.best, h.at);
-        far = far || h.e == kFar;
-        if (h.e != kFar) e = max(e, h.e);
-        if (tid == 0) s.head[g] = h;
-    }
-    if (best == -INFINITY || r.greedy) {
-        if (tid == 0) {
-            a.out[row] = best == -INFINITY ? 0 : at;
-            if (a.prob) a.prob[row] = best == -INFINITY ? 0.f : 1.f;
-        }
-        return true;
-    }
-    if (far) return false;
-
-    // The row's bins: of a segment whose power of two lies m octaves lower,
-    // bin i - 16 m.
-    const bool counted = r.k > 0 && r.k < a.n;
+    const int e = st.e, listed = a.listed[row];
+    const Slope c = slope_of(r.t);
+    if (st.lo <= st.hi && listed > kList) return false;
     fill_table(s.table);
-    for (int i = tid; i < kBins; i += kThreads) {
-        double sum = 0.;
-        uint32_t n = 0;
-        for (int g = 0; g < a.segments; ++g) {
-            const int eg = a.heads[first + g].e;
-            const int lower = min(e - eg, 64), from = i - kOctave * lower;
-            if (eg == kNone || from < 0) continue;
-            sum += ldexp(static_cast<double>(a.mass[(first + g) * kBins + from]), -lower);
-            if (counted) n += a.count[(first + g) * kBins + from];
-        }
-        s.cum[i] = sum;
-        s.counts[i] = n;
-    }
+    if (tid < a.segments) s.head[tid] = a.heads[first + tid];
+    if (tid == 0) s.listed = st.lo <= st.hi ? listed : 0;
+    if (st.lo <= st.hi)
+        for (int i = tid; i < listed; i += kThreads) s.list[i] = a.list[static_cast<int64_t>(row) * kList + i];
+    for (int i = tid; i < kBins; i += kThreads) s.cum[i] = a.cum[static_cast<int64_t>(row) * kBins + i];
     __syncthreads();
-    scan_bins(s.cum, s.wave_sum);
-    if (counted) scan_bins(s.counts, s.wave_count);
-    const double c = kLog2E / static_cast<double>(r.t);
+    sort_list(s.list, s.listed);
 
-    // Tokens of bins lo .. hi into the list; false: more than it holds.
+    // Tokens of other bins, by reading the row; false: more than the list holds.
     auto collect = [&](int lo, int hi) {
         __syncthreads();
         if (tid == 0) s.listed = 0;
         __syncthreads();
         for (int g = 0; g < a.segments; ++g) {
-            const int eg = s.head[g].e, lower = min(e - eg, 64) * kOctave;
-            if (eg == kNone) continue;
-            const int end = min(a.n, (g + 1) * kSegment);
-            #pragma unroll 2
-            for (int i = g * kSegment + tid * 4; i < end; i += kThreads * 4) {
+            const int down = octaves_down(e, s.head[g].e) * kOctave;
+            if (s.head[g].e == kNone || hi < down) continue;
+            const Range in = range_of(lo - down, hi - down, r.t, s.head[g].e);
+            #pragma unroll 1
+            for (int j = 0; j < kQuads; ++j) {
                 float v[4];
-                load_quad(x, i, a.n, a.wide, v);
-                #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const double d = octaves_below(v[k], c, eg);
-                    if (!(d < kDepth)) continue;
-                    const int bin = bin_of(d) + lower;
-                    if (bin >= lo && bin <= hi) {
-                        const int slot = atomicAdd(&s.listed, 1);
-                        if (slot < kList) s.list[slot] = packed(v[k], i + k);
-                    }
-                }
+                load_quad(x, quad_at(g, j), a.n, a.wide, v);
+                list_quad(v, quad_at(g, j), in, s.list, &s.listed);
             }
         }
         __syncthreads();
         if (s.listed > kList) return false;
-        int size = 2;
-        while (size < s.listed) size <<= 1;
-        for (int i = s.listed + tid; i < size; i += kThreads) s.list[i] = 0;
-        sort_list(s.list, size);
+        sort_list(s.list, s.listed);
         return true;
     };
-    // A listed token's weight in its segment's units, and in the row's.
-    auto listed_weight = [&](int i, int &g) -> uint64_t {
-        const uint64_t t = s.list[i];
-        g = static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(t)) / kSegment;
-        const double d = octaves_below(value_of(static_cast<uint32_t>(t >> 32)), c, s.head[g].e);
-        return unit_weight(d, bin_of(d), s.table);
+    // A listed token's segment, and its weight in the row's units.
+    auto segment_of = [&](int i) {
+        return static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(s.list[i])) / kSegment;
     };
     auto row_weight = [&](int i) {
-        int g;
-        const uint64_t w = listed_weight(i, g);
-        return ldexp(static_cast<double>(w), s.head[g].e - e);
+        const int eg = s.head[segment_of(i)].e;
+        const Depth d = depth_of(value_of(static_cast<uint32_t>(s.list[i] >> 32)), c, eg);
+        return ldexp(static_cast<double>(unit_weight(d, s.table)), eg - e - d.f / kFine);
     };
     // Sums of the list's weights up to each, four a thread.
     auto sum_list = [&]() {
@@ -556,12 +762,7 @@ __device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowPara
             w[k] = i < s.listed ? row_weight(i) : 0.;
             sum += w[k];
         }
-        double upto = sum;
-        #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const double o = __shfl_up(upto, off);
-            if (lane >= off) upto += o;
-        }
+        const double upto = wave_scan(sum);
         if (lane == 63) s.wave_sum[wave] = upto;
         __syncthreads();
         double base = 0.;
@@ -575,35 +776,29 @@ __device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowPara
         __syncthreads();
     };
 
-    const int last = kBins - 1;
-    int bin_k = kBins, lo = 0, left = 0;   // top-k: the bin of its last token, and how many of the list are left
-    bool listed = false;
-    if (counted) bin_k = first_reaching(s.counts, static_cast<double>(r.k), &s.found);
-    double total = s.cum[last];
-    if (bin_k < kBins) {
-        const bool all = s.counts[bin_k] <= kList;   // the whole of what top-k leaves fits the list
-        lo = all ? 0 : bin_k;
-        if (!collect(lo, bin_k)) return false;
+    auto left_of = [&](int lo) {
+        if (st.bin_k == kBins) return s.listed;
+        return min(s.listed, r.k - (lo > 0 ? static_cast<int>(a.counts[static_cast<int64_t>(row) * kBins + lo - 1]) : 0));
+    };
+    double total = s.cum[kBins - 1];
+    int lo = kBins, left = 0;   // the list's first bin, and how many of the list top-k leaves
+    if (st.lo <= st.hi) {
         sum_list();
-        listed = true;
-        left = r.k - (lo > 0 ? static_cast<int>(s.counts[lo - 1]) : 0);
-        total = (lo > 0 ? s.cum[lo - 1] : 0.) + s.sorted[left - 1];
+        lo = st.lo;
+        left = left_of(lo);
+        if (st.bin_k < kBins) total = (lo > 0 ? s.cum[lo - 1] : 0.) + s.sorted[left - 1];
     }
     const double target = r.p < 1.f ? static_cast<double>(r.p) * total : INFINITY;
-    // The largest token's weight, and the least one that min-p keeps.
-    const double dbest = octaves_below(best, c, e);
-    const double least = r.mp > 0.f ? static_cast<double>(r.mp) * static_cast<double>(unit_weight(dbest, bin_of(dbest), s.table)) : 0.;
-    int bin = bin_k;
-    if (r.p < 1.f) bin = min(bin, first_reaching(s.cum, target, &s.found));
-    if (r.mp > 0.f) bin = min(bin, bin_of(fmin(dbest - log2(static_cast<double>(r.mp)), 48.)));
+    int bin = min(st.bin_k, st.bin_m);
+    if (r.p < 1.f) bin = min(bin, first_reaching<kThreads>(s.cum, target, &s.found));
     int whole = kBins, keep = 0;   // kept: bins below `whole`, and the list's first `keep` tokens
     uint64_t cut = ~0ull;          // the last of these
     if (bin < kBins) {
-        if (!listed || bin < lo) {
-            if (!collect(bin, bin)) return false;
+        if (bin < lo) {   // a smaller nucleus within a top-k beyond the list
+            if (!collect(bin, bin == st.bin_m ? st.m_hi : bin)) return false;
             sum_list();
             lo = bin;
-            left = s.listed;
+            left = left_of(lo);
         }
         whole = lo;
         const double above = lo > 0 ? s.cum[lo - 1] : 0.;
@@ -614,7 +809,7 @@ __device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowPara
         int mine = 0;
         for (int i = tid; i < left; i += kThreads) {
             const double before = above + (i > 0 ? s.sorted[i - 1] : 0.);
-            if (before < target && (least == 0. || row_weight(i) >= least)) mine = i + 1;
+            if (before < target && (st.least == 0. || row_weight(i) >= st.least)) mine = i + 1;
         }
         if (mine) atomicMax(&s.cut, mine);
         __syncthreads();
@@ -622,77 +817,75 @@ __device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowPara
         if (keep > 0) cut = s.list[keep - 1];
     }
 
-    // Kept weight of each segment, in its own units.
+    // Kept weight of each segment: its whole bins, and its listed tokens in the
+    // list's order.
     for (int g = wave; g < a.segments; g += kWaves) {
-        const int eg = s.head[g].e;
-        uint64_t sum = 0;
-        if (eg != kNone)
-            for (int i = lane; i < min(whole, kBins) - kOctave * min(e - eg, 64); i += 64) sum += a.mass[(first + g) * kBins + i];
-        sum = wave_sum_u64(sum);
+        const int down = octaves_down(e, s.head[g].e), n = whole - kOctave * down;
+        double sum = 0.;
+        #pragma unroll
+        for (int i = 0; i < kBins; i += 64) {
+            const uint64_t w = n > 0 ? a.mass[(first + g) * kBins + i + lane] : 0;
+            sum += i + lane < n ? ldexp(static_cast<double>(w), -down - (i + lane) / kOctave) : 0.;
+        }
+        for (int i = lane; i < keep; i += 64) sum += segment_of(i) == g ? row_weight(i) : 0.;
+        sum = wave_last(wave_scan(sum));
         if (lane == 0) s.kept[g] = sum;
     }
     __syncthreads();
-    for (int i = tid; i < keep; i += kThreads) {
-        int g;
-        const uint64_t w = listed_weight(i, g);
-        atomicAdd(reinterpret_cast<unsigned long long *>(&s.kept[g]), static_cast<unsigned long long>(w));
-    }
-    __syncthreads();
     double z = 0.;
-    for (int g = 0; g < a.segments; ++g)
-        if (s.head[g].e != kNone) z += ldexp(static_cast<double>(s.kept[g]), max(s.head[g].e - e, -64));
-    // The segment of the random number's token, and how much of its weight
-    // lies before that token.
+    for (int g = 0; g < a.segments; ++g) z += s.kept[g];
+    // The segment of the random number's token, and how much of its weight lies
+    // before that token.
     const double u = a.uniform[row], goal = u > 0. ? fmin(u, 1.) * z : 0.;
-    double sum = 0.;
-    int seg = -1;
-    uint64_t want = 0;
+    double sum = 0., share = 0.;
+    int seg = 0;
     for (int g = 0; g < a.segments; ++g) {
-        const uint64_t w = s.head[g].e == kNone ? 0 : s.kept[g];
-        if (!w) continue;
-        const int lower = max(s.head[g].e - e, -64);
-        const double part = ldexp(static_cast<double>(w), lower);
+        const double w = s.kept[g];
+        if (!(w > 0.)) continue;
         seg = g;
-        const double inside = ldexp(fmax(goal - sum, 0.), -lower);
-        want = inside < static_cast<double>(w) ? min(static_cast<uint64_t>(inside), w - 1) : w - 1;
-        if (goal < sum + part) break;
-        sum += part;
+        share = (goal - sum) / w;
+        if (goal < sum + w) break;
+        sum += w;
     }
-    // The segment again: thread sums by tiles of 4 * kThreads tokens, then the
-    // wave and the token.
-    constexpr int kTiles = kSegment / (4 * kThreads);
-    static_assert(kTiles == 8, "s.part");
-    const int eg = s.head[seg].e;
-    auto weights = [&](int i, uint64_t (&w)[4]) {
-        float v[4];
-        load_quad(x, i, a.n, a.wide, v);
+    // The segment again, weights as integers of 2^-47: thread sums by quads, then
+    // the wave and the token.
+    const int eg = s.head[seg].e, down = kOctave * octaves_down(e, eg);
+    const float cut_x = keep > 0 ? value_of(static_cast<uint32_t>(cut >> 32)) : INFINITY;
+    const int cut_i = keep > 0 ? static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(cut)) : -1;
+    auto weights = [&](const float (&v)[4], int i, uint64_t (&w)[4]) {
         uint64_t sum = 0;
         #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const double d = octaves_below(v[k], c, eg);
-            const bool kept = d < kDepth && (bin_of(d) + kOctave * (e - eg) < whole || packed(v[k], i + k) >= cut);
-            w[k] = kept ? unit_weight(d, bin_of(d), s.table) : 0;
+            const Depth d = depth_of(v[k], c, eg);
+            const bool kept = d.f >= 0 && (d.bin() + down < whole || v[k] > cut_x || (v[k] == cut_x && i + k <= cut_i));
+            w[k] = kept ? static_cast<uint64_t>(unit_weight(d, s.table)) << 16 >> (d.f / kFine) : 0;
             sum += w[k];
         }
         return sum;
     };
-    uint64_t tile_sum[kTiles];
-    #pragma unroll
-    for (int j = 0; j < kTiles; ++j) {
-        uint64_t w[4];
-        const int i = seg * kSegment + (j * kThreads + tid) * 4;
-        tile_sum[j] = i < a.n ? weights(i, w) : 0;
-    }
-    #pragma unroll
-    for (int j = 0; j < kTiles; ++j) {
-        const uint64_t t = wave_sum_u64(tile_sum[j]);
-        if (lane == 0) s.part[j][wave] = t;
+    // Half of the quads in flight at a time, in a loop: short code.
+    #pragma unroll 1
+    for (int j0 = 0; j0 < kQuads; j0 += kQuads / 2) {
+        float v[kQuads / 2][4];
+        #pragma unroll
+        for (int j = 0; j < kQuads / 2; ++j) load_quad(x, quad_at(seg, j0 + j), a.n, a.wide, v[j]);
+        #pragma unroll
+        for (int j = 0; j < kQuads / 2; ++j) {
+            uint64_t w[4];
+            const uint64_t t = wave_scan(weights(v[j], quad_at(seg, j0 + j), w));
+            if (lane == 63) s.part[j0 + j][wave] = t;
+        }
     }
     __syncthreads();
+    uint64_t all = 0;
+    for (int j = 0; j < kQuads; ++j)
+        for (int w = 0; w < kWaves; ++w) all += s.part[j][w];
+    const double inside = fmax(share, 0.) * static_cast<double>(all);
+    const uint64_t want = inside < static_cast<double>(all) ? min(static_cast<uint64_t>(inside), all - 1) : all - 1;
     int tile = 0, mine = 0;
     uint64_t before = 0;
     bool done = false;
-    for (int j = 0; j < kTiles && !done; ++j)
+    for (int j = 0; j < kQuads && !done; ++j)
         for (int w = 0; w < kWaves; ++w) {
             if (before + s.part[j][w] > want) {
                 tile = j;
@@ -702,21 +895,21 @@ __device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowPara
             }
             before += s.part[j][w];
         }
-    if (wave != mine || !done) return true;
+    if (wave != mine) return true;
     uint64_t w[4];
-    const int i = seg * kSegment + (tile * kThreads + tid) * 4;
-    uint64_t own = i < a.n ? weights(i, w) : 0, upto = own;
-    #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const uint64_t o = __shfl_up(upto, off);
-        if (lane >= off) upto += o;
-    }
-    uint64_t b = before + upto - own;
-    if (own && b <= want && want < b + own)
+    float v[4];
+    const int i = quad_at(seg, tile);
+    load_quad(x, i, a.n, a.wide, v);
+    const uint64_t own = weights(v, i, w);
+    uint64_t b = before + wave_scan(own) - own;
+    if (b <= want && want < b + own)
         for (int k = 0; k < 4; ++k) {
             if (w[k] && b <= want && want < b + w[k]) {
                 a.out[row] = i + k;
-                if (a.prob) a.prob[row] = static_cast<float>(ldexp(static_cast<double>(w[k]), max(eg - e, -64)) / z);
+                const Depth d = depth_of(v[k], c, eg);
+                if (a.prob)
+                    a.prob[row] = static_cast<float>(
+                        ldexp(static_cast<double>(unit_weight(d, s.table)), eg - e - d.f / kFine) / z);
             }
             b += w[k];
         }
@@ -728,12 +921,33 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
         PickShared pick;
         PlainShared plain;
     } s;
-    const RowParams r = row_params(a, blockIdx.x);
-    float best;
-    if (!sample_binned(a, r, blockIdx.x, best, s.pick)) sample_plain(a, r, blockIdx.x, best, s.plain);
+    const int row = blockIdx.x;
+    const RowPlan st = a.plans[row];
+    if (st.way == kDone) return;
+    const RowParams r = row_params(a, row);
+    if (st.way == kPlain || !sample_binned(a, r, st, row, s.pick)) sample_plain(a, r, row, st.best, s.plain);
 }
 
 size_t round256(size_t b) { return (b + 255) / 256 * 256; }
+
+// A call's arrays in its workspace; returns their bytes.
+size_t lay_out(SampleArgs &a, int rows, char *ws) {
+    const size_t segments = static_cast<size_t>(rows) * a.segments;
+    size_t at = 0;
+    auto take = [&](auto *&p, size_t n) {
+        p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(ws + at);
+        at += round256(n * sizeof(*p));
+    };
+    take(a.heads, segments);
+    take(a.plans, rows);
+    take(a.mass, segments * kBins);
+    take(a.cum, static_cast<size_t>(rows) * kBins);
+    take(a.list, static_cast<size_t>(rows) * kList);
+    take(a.count, segments * kBins);
+    take(a.counts, static_cast<size_t>(rows) * kBins);
+    take(a.listed, rows);
+    return at;
+}
 
 }  // namespace
 }  // namespace qk
@@ -742,8 +956,9 @@ extern "C" {
 
 size_t qk_sample_rows_workspace_bytes(int n, int rows) {
     if (n < 1 || n > 1 << 19 || rows < 1) return 0;
-    const size_t segments = static_cast<size_t>(rows) * ((n + qk::kSegment - 1) / qk::kSegment);
-    return qk::round256(segments * sizeof(qk::SegmentHead)) + segments * qk::kBins * (sizeof(uint64_t) + sizeof(uint32_t));
+    qk::SampleArgs a{};
+    a.segments = (n + qk::kSegment - 1) / qk::kSegment;
+    return qk::lay_out(a, rows, nullptr);
 }
 
 int qk_sample_rows_f32(const float *logits, int n, int64_t ldv, int rows, const float *temperature,
@@ -761,13 +976,12 @@ int qk_sample_rows_f32(const float *logits, int n, int64_t ldv, int rows, const 
     qk::SampleArgs a{logits, ldv, n, temperature, top_p, min_p, uniform, top_k, out, prob};
     a.segments = (n + qk::kSegment - 1) / qk::kSegment;
     a.wide = qk::aligned(logits, 16) && ldv % 4 == 0;
-    const size_t segments = static_cast<size_t>(rows) * a.segments;
-    char *ws = static_cast<char *>(workspace);
-    a.heads = reinterpret_cast<qk::SegmentHead *>(ws);
-    a.mass = reinterpret_cast<uint64_t *>(ws + qk::round256(segments * sizeof(qk::SegmentHead)));
-    a.count = reinterpret_cast<uint32_t *>(a.mass + segments * qk::kBins);
-    hipLaunchKernelGGL(qk::sample_scan_kernel, dim3(a.segments, rows), dim3(qk::kScanThreads), 0, qk::S(stream), a);
-    hipLaunchKernelGGL(qk::sample_pick_kernel, dim3(rows), dim3(qk::kThreads), 0, qk::S(stream), a);
+    qk::lay_out(a, rows, static_cast<char *>(workspace));
+    const dim3 grid(a.segments, rows), block(qk::kThreads);
+    hipLaunchKernelGGL(qk::sample_scan_kernel, grid, block, 0, qk::S(stream), a);
+    hipLaunchKernelGGL(qk::sample_plan_kernel, dim3(rows), dim3(qk::kBins), 0, qk::S(stream), a);
+    hipLaunchKernelGGL(qk::sample_collect_kernel, grid, block, 0, qk::S(stream), a);
+    hipLaunchKernelGGL(qk::sample_pick_kernel, dim3(rows), block, 0, qk::S(stream), a);
     return qk::launch_status("qk_sample_rows_f32 launch");
 }
 

@@ -61,13 +61,14 @@ def check(qk, t, x, u, ldv=None, **params):
             continue
         i, c, total = got[r], np.cumsum(w), w.sum()
         assert 0 <= i < n and w[i] > 0, (r, i)
-        # Each of n weights is held to half a unit of 2^-44 of the largest at
-        # least, and sums in 64 bits are off by 2^-53 of themselves a step.
-        eps = n * 2.0 ** -45 + total * 2.0 ** -36
+        # Each of n weights is held to 2^-30 of itself, or has none below 2^-45
+        # of the largest; sums in 64 bits add nothing to that.
+        eps = n * 2.0 ** -45 + total * 2.0 ** -29
         uv = min(max(np.float64(np.float32(u[r])), 0), 1) if u[r] == u[r] else 0.0
         target = uv * total
         assert c[i] - w[i] <= target + eps and c[i] > target - eps, (r, i, c[i] / total, uv)
-        # One rounding to fp32 of a share whose weight is off by half a unit.
+        # One rounding to fp32 of a quotient whose parts are off by 2^-30, and by
+        # what the tokens without weight leave out.
         assert abs(pr[r] - w[i] / total) <= (2.0 ** -23 * w[i] + 2.0 ** -45 + n * 2.0 ** -45 * w[i]) / total
     return got[:rows]
 
