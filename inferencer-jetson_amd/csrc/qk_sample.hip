@@ -665,42 +665,38 @@ __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleArgs a) 
 
 struct PickShared {
     uint64_t list[kList];         // tokens: the key's bits, then the index's complement
-    double sorted[kList];         // sums of the list's weights up to each
+    uint64_t some[kList];         // those of them that are ordered
+    uint64_t ordered[kList];
     double cum[kBins];
+    uint64_t part_mass[kThreads]; // of the list in kThreads parts of its logits' range
+    uint32_t part_count[kThreads];
     uint2 table[kFine];
     SegmentHead head[kMaxSegments];
-    double kept[kMaxSegments];    // kept weight of each segment, in units of the row's 2^(e - 31)
-    double wave_sum[kWaves];
-    uint64_t part[kQuads][kWaves];
-    int listed, found, cut;
+    unsigned long long kept[kMaxSegments];   // listed kept weight of each segment
+    double kept_all[kMaxSegments];           // kept weight of each segment
+    uint64_t wave_mass[kWaves], wave_count[kWaves];
+    uint64_t quads[kQuads * kWaves];
+    uint64_t base_mass, base_count;
+    uint32_t key_high, key_low;
+    int listed, found, picked;
 };
 
-// Descending order of list[0 .. n): by counting the larger ones of each where
-// they are few, else a bitonic sort (of a power of two, the rest zeros).
-__device__ __forceinline__ void sort_list(uint64_t *list, int n) {
-    const int tid = threadIdx.x;
-    if (n <= 256) {
-        const uint64_t mine = tid < n ? list[tid] : 0;
-        int rank = 0;
-        for (int i = 0; i < n; ++i) rank += list[i] > mine;
-        __syncthreads();
-        if (tid < n) list[rank] = mine;
-        __syncthreads();
-        return;
-    }
-    int size = 512;
-    while (size < n) size <<= 1;
-    for (int i = n + tid; i < size; i += kThreads) list[i] = 0;
-    for (int k = 2; k <= size; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            __syncthreads();
-            for (int t = tid; t < size / 2; t += kThreads) {
-                const int i = 2 * t - (t & (j - 1)), o = i + j;
-                const uint64_t p = list[i], q = list[o];
-                if ((p < q) == ((i & k) == 0)) list[i] = q, list[o] = p;
-            }
-        }
+// Sums over the workgroup's threads up to each (inclusive) of a pair.
+__device__ __forceinline__ void block_scan(uint64_t &mass, uint64_t &count, PickShared &s) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    mass = wave_scan(mass);
+    count = wave_scan(count);
     __syncthreads();
+    if (lane == 63) {
+        s.wave_mass[wave] = mass;
+        s.wave_count[wave] = count;
+    }
+    __syncthreads();
+    #pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        mass += w < wave ? s.wave_mass[w] : 0;
+        count += w < wave ? s.wave_count[w] : 0;
+    }
 }
 
 // A row by its segments' histograms and its list, by all threads of the
@@ -710,17 +706,16 @@ __device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowPara
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float *x = a.logits + static_cast<int64_t>(row) * a.ldv;
     const int64_t first = static_cast<int64_t>(row) * a.segments;
-    const int e = st.e, listed = a.listed[row];
-    const Slope c = slope_of(r.t);
-    if (st.lo <= st.hi && listed > kList) return false;
+    const int e = st.e, listed = st.lo <= st.hi ? a.listed[row] : 0;
+    if (listed > kList) return false;
     fill_table(s.table);
     if (tid < a.segments) s.head[tid] = a.heads[first + tid];
-    if (tid == 0) s.listed = st.lo <= st.hi ? listed : 0;
-    if (st.lo <= st.hi)
-        for (int i = tid; i < listed; i += kThreads) s.list[i] = a.list[static_cast<int64_t>(row) * kList + i];
+    if (tid < kMaxSegments) s.kept[tid] = 0;
+    if (tid == 0) s.listed = listed;
+    for (int i = tid; i < listed; i += kThreads) s.list[i] = a.list[static_cast<int64_t>(row) * kList + i];
     for (int i = tid; i < kBins; i += kThreads) s.cum[i] = a.cum[static_cast<int64_t>(row) * kBins + i];
+    const Slope c = slope_of(r.t);
     __syncthreads();
-    sort_list(s.list, s.listed);
 
     // Tokens of other bins, by reading the row; false: more than the list holds.
     auto collect = [&](int lo, int hi) {
@@ -739,119 +734,229 @@ __device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowPara
             }
         }
         __syncthreads();
-        if (s.listed > kList) return false;
-        sort_list(s.list, s.listed);
+        return s.listed <= kList;
+    };
+    // A listed token's segment, and its weight in the row's units of 2^(e - 31)
+    // (exact, for min-p) and as an integer of 2^(e - 47).
+    auto segment_of = [&](uint64_t t) { return static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(t)) / kSegment; };
+    auto weight_of = [&](uint64_t t, uint64_t &whole) {
+        const int eg = s.head[segment_of(t)].e;
+        const Depth d = depth_of(value_of(static_cast<uint32_t>(t >> 32)), c, eg);
+        const uint32_t m = unit_weight(d, s.table);
+        const int below = e - eg + d.f / kFine;
+        whole = below < 48 ? static_cast<uint64_t>(m) << 16 >> below : 0;
+        return ldexp(static_cast<double>(m), -below);
+    };
+    constexpr double kWhole = 0x1p-16;   // 2^(e - 47) in units of 2^(e - 31)
+    // The last listed token that is kept, in the tokens' order: as many as
+    // `left`, while the sum before is below the target and the weight is not
+    // below the least; ~0 if none is.  A list of some hundreds is cut into
+    // kThreads parts of its range first, of which one then holds the cut and is
+    // ordered by counting the larger tokens of each.
+    auto cut_of = [&](double above, double target, int left, double least) -> uint64_t {
+        const int n = s.listed;
+        auto stays = [&](uint64_t t, uint64_t &w) { return weight_of(t, w) >= least; };
+        float high = 0.f, scale = 0.f;
+        auto part_of = [&](uint64_t t) {
+            return min(static_cast<int>((high - value_of(static_cast<uint32_t>(t >> 32))) * scale), kThreads - 1);
+        };
+        const bool parts = n > 128;
+        uint64_t base_mass = 0, base_count = 0;
+        int part = 0;
+        if (parts) {
+            __syncthreads();
+            s.part_mass[tid] = 0;
+            s.part_count[tid] = 0;
+            if (tid == 0) {
+                s.key_high = 0;
+                s.key_low = ~0u;
+                s.found = -1;
+            }
+            __syncthreads();
+            uint32_t top = 0, low = ~0u;
+            for (int i = tid; i < n; i += kThreads) {
+                const uint32_t k = static_cast<uint32_t>(s.list[i] >> 32);
+                top = max(top, k);
+                low = min(low, k);
+            }
+            if (tid < n) {
+                atomicMax(&s.key_high, top);
+                atomicMin(&s.key_low, low);
+            }
+            __syncthreads();
+            high = value_of(s.key_high);
+            scale = fminf((kThreads - 1) / (high - value_of(s.key_low)), 1e30f);   // 1e30: all alike, one part
+            for (int i = tid; i < n; i += kThreads) {
+                uint64_t w;
+                if (!stays(s.list[i], w)) continue;
+                atomicAdd(reinterpret_cast<unsigned long long *>(&s.part_mass[part_of(s.list[i])]), static_cast<unsigned long long>(w));
+                atomicAdd(&s.part_count[part_of(s.list[i])], 1u);
+            }
+            __syncthreads();
+            uint64_t mass = s.part_mass[tid], count = s.part_count[tid];
+            const uint64_t own_mass = mass, own_count = count;
+            block_scan(mass, count, s);
+            const uint64_t mass0 = mass - own_mass, count0 = count - own_count;
+            if (own_count > 0 && count0 < static_cast<uint64_t>(left) && above + static_cast<double>(mass0) * kWhole < target)
+                atomicMax(&s.found, tid);
+            __syncthreads();
+            part = s.found;
+            if (part < 0) return ~0ull;
+            if (tid == part) {
+                s.base_mass = mass0;
+                s.base_count = count0;
+            }
+        }
+        __syncthreads();
+        if (parts) {
+            base_mass = s.base_mass;
+            base_count = s.base_count;
+        }
+        if (tid == 0) s.picked = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += kThreads) {
+            uint64_t w;
+            if (stays(s.list[i], w) && (!parts || part_of(s.list[i]) == part)) s.some[atomicAdd(&s.picked, 1)] = s.list[i];
+        }
+        __syncthreads();
+        const int m = s.picked;
+        for (int i = tid; i < m; i += kThreads) {
+            const uint64_t t = s.some[i];
+            int rank = 0;
+            for (int k = 0; k < m; ++k) rank += s.some[k] > t;
+            s.ordered[rank] = t;
+        }
+        __syncthreads();
+        if (tid == 0) s.found = -1;
+        for (int i0 = 0; i0 < m; i0 += kThreads) {
+            const int i = i0 + tid;
+            uint64_t own = 0, count = i < m;
+            if (i < m) weight_of(s.ordered[i], own);
+            uint64_t mass = own;
+            block_scan(mass, count, s);
+            mass += base_mass;
+            if (i < m && base_count + i < static_cast<uint64_t>(left) &&
+                above + static_cast<double>(mass - own) * kWhole < target)
+                atomicMax(&s.found, i);
+            base_mass = s.wave_mass[kWaves - 1] + base_mass;   // of full rounds only: the last has no next
+            #pragma unroll
+            for (int w = 0; w < kWaves - 1; ++w) base_mass += s.wave_mass[w];
+        }
+        __syncthreads();
+        return s.found < 0 ? ~0ull : s.ordered[s.found];
+    };
+    // All that top-k leaves is listed, a token a thread: both cuts from one order,
+    // and the token from the kept ones themselves.
+    if (st.bin_k < kBins && st.lo == 0 && listed <= kThreads) {
+        const uint64_t t = tid < listed ? s.list[tid] : 0;
+        int rank = 0;
+        for (int k = 0; k < listed; ++k) rank += s.list[k] > t;
+        if (tid < listed) s.ordered[rank] = t;
+        __syncthreads();
+        const uint64_t mine = tid < listed ? s.ordered[tid] : 0;
+        uint64_t own = 0, upto = 0, none = 0;
+        bool stays = false;
+        if (tid < listed) stays = weight_of(mine, own) >= st.least && tid < r.k;
+        if (tid >= r.k) own = 0;
+        upto = own;
+        block_scan(upto, none, s);
+        uint64_t total = 0;
+        #pragma unroll
+        for (int w = 0; w < kWaves; ++w) total += s.wave_mass[w];
+        if (r.p < 1.f) stays = stays && static_cast<double>(upto - own) < static_cast<double>(r.p) * static_cast<double>(total);
+        s.some[tid] = stays ? own : 0;
+        if (tid == 0) s.picked = 0;
+        __syncthreads();
+        if (stays) atomicMax(&s.picked, tid + 1);
+        __syncthreads();
+        const int keep = s.picked;
+        uint64_t z = 0, before = 0;
+        for (int k = 0; k < keep; ++k) {   // in index order: those with a larger complement
+            const uint64_t w = s.some[k];
+            z += w;
+            before += static_cast<uint32_t>(s.ordered[k]) > static_cast<uint32_t>(mine) ? w : 0;
+        }
+        const double goal = a.uniform[row] * static_cast<double>(z);
+        const uint64_t want = goal > 0. ? min(goal < static_cast<double>(z) ? static_cast<uint64_t>(goal) : z, z - 1) : 0;
+        if (stays && before <= want && want < before + own) {
+            a.out[row] = static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(mine));
+            if (a.prob) a.prob[row] = static_cast<float>(static_cast<double>(own) / static_cast<double>(z));
+        }
         return true;
-    };
-    // A listed token's segment, and its weight in the row's units.
-    auto segment_of = [&](int i) {
-        return static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(s.list[i])) / kSegment;
-    };
-    auto row_weight = [&](int i) {
-        const int eg = s.head[segment_of(i)].e;
-        const Depth d = depth_of(value_of(static_cast<uint32_t>(s.list[i] >> 32)), c, eg);
-        return ldexp(static_cast<double>(unit_weight(d, s.table)), eg - e - d.f / kFine);
-    };
-    // Sums of the list's weights up to each, four a thread.
-    auto sum_list = [&]() {
-        static_assert(kList == 4 * kThreads, "four tokens a thread");
-        double w[4], sum = 0.;
-        #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int i = tid * 4 + k;
-            w[k] = i < s.listed ? row_weight(i) : 0.;
-            sum += w[k];
-        }
-        const double upto = wave_scan(sum);
-        if (lane == 63) s.wave_sum[wave] = upto;
-        __syncthreads();
-        double base = 0.;
-        for (int v = 0; v < wave; ++v) base += s.wave_sum[v];
-        base += upto - sum;
-        #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            base += w[k];
-            s.sorted[tid * 4 + k] = base;
-        }
-        __syncthreads();
-    };
-
+    }
     auto left_of = [&](int lo) {
         if (st.bin_k == kBins) return s.listed;
         return min(s.listed, r.k - (lo > 0 ? static_cast<int>(a.counts[static_cast<int64_t>(row) * kBins + lo - 1]) : 0));
     };
-    double total = s.cum[kBins - 1];
-    int lo = kBins, left = 0;   // the list's first bin, and how many of the list top-k leaves
-    if (st.lo <= st.hi) {
-        sum_list();
-        lo = st.lo;
-        left = left_of(lo);
-        if (st.bin_k < kBins) total = (lo > 0 ? s.cum[lo - 1] : 0.) + s.sorted[left - 1];
+    auto above_of = [&](int lo) { return lo > 0 ? s.cum[lo - 1] : 0.; };
+
+    double target = INFINITY;
+    int lo = st.lo <= st.hi ? st.lo : kBins;   // the list's first bin
+    if (r.p < 1.f) {
+        double total = s.cum[kBins - 1];
+        if (st.bin_k < kBins) {   // of what top-k leaves
+            const uint64_t last = cut_of(above_of(lo), INFINITY, left_of(lo), 0.);
+            uint64_t mass = 0, none = 0;
+            for (int i = tid; i < s.listed; i += kThreads) {
+                uint64_t w;
+                weight_of(s.list[i], w);
+                mass += s.list[i] >= last ? w : 0;
+            }
+            block_scan(mass, none, s);
+            mass = 0;
+            #pragma unroll
+            for (int w = 0; w < kWaves; ++w) mass += s.wave_mass[w];
+            total = above_of(lo) + static_cast<double>(mass) * kWhole;
+        }
+        target = static_cast<double>(r.p) * total;
     }
-    const double target = r.p < 1.f ? static_cast<double>(r.p) * total : INFINITY;
     int bin = min(st.bin_k, st.bin_m);
     if (r.p < 1.f) bin = min(bin, first_reaching<kThreads>(s.cum, target, &s.found));
-    int whole = kBins, keep = 0;   // kept: bins below `whole`, and the list's first `keep` tokens
-    uint64_t cut = ~0ull;          // the last of these
+    int whole = kBins;      // kept: bins below `whole`, and the list's tokens down to `cut`
+    uint64_t cut = ~0ull;
     if (bin < kBins) {
         if (bin < lo) {   // a smaller nucleus within a top-k beyond the list
             if (!collect(bin, bin == st.bin_m ? st.m_hi : bin)) return false;
-            sum_list();
             lo = bin;
-            left = left_of(lo);
         }
         whole = lo;
-        const double above = lo > 0 ? s.cum[lo - 1] : 0.;
-        if (tid == 0) s.cut = 0;
-        __syncthreads();
-        // Kept: as many as top-k leaves, while the sum before is below the
-        // target and the weight not below the least.
-        int mine = 0;
-        for (int i = tid; i < left; i += kThreads) {
-            const double before = above + (i > 0 ? s.sorted[i - 1] : 0.);
-            if (before < target && (st.least == 0. || row_weight(i) >= st.least)) mine = i + 1;
-        }
-        if (mine) atomicMax(&s.cut, mine);
-        __syncthreads();
-        keep = s.cut;
-        if (keep > 0) cut = s.list[keep - 1];
+        cut = cut_of(above_of(lo), target, left_of(lo), st.least);
+        for (int i = tid; i < s.listed; i += kThreads)
+            if (s.list[i] >= cut) {
+                uint64_t w;
+                weight_of(s.list[i], w);
+                atomicAdd(&s.kept[segment_of(s.list[i])], static_cast<unsigned long long>(w));
+            }
     }
+    __syncthreads();
 
-    // Kept weight of each segment: its whole bins, and its listed tokens in the
-    // list's order.
+    // Kept weight of each segment: its whole bins and its listed tokens.
     for (int g = wave; g < a.segments; g += kWaves) {
         const int down = octaves_down(e, s.head[g].e), n = whole - kOctave * down;
         double sum = 0.;
-        #pragma unroll
-        for (int i = 0; i < kBins; i += 64) {
-            const uint64_t w = n > 0 ? a.mass[(first + g) * kBins + i + lane] : 0;
-            sum += i + lane < n ? ldexp(static_cast<double>(w), -down - (i + lane) / kOctave) : 0.;
+        if (n > 0) {
+            #pragma unroll
+            for (int i = 0; i < kBins; i += 64) {
+                const uint64_t w = a.mass[(first + g) * kBins + i + lane];
+                sum += i + lane < n ? ldexp(static_cast<double>(w), -down - (i + lane) / kOctave) : 0.;
+            }
+            sum = wave_last(wave_scan(sum));
         }
-        for (int i = lane; i < keep; i += 64) sum += segment_of(i) == g ? row_weight(i) : 0.;
-        sum = wave_last(wave_scan(sum));
-        if (lane == 0) s.kept[g] = sum;
+        if (lane == 0) s.kept_all[g] = sum + static_cast<double>(s.kept[g]) * kWhole;
     }
     __syncthreads();
-    double z = 0.;
-    for (int g = 0; g < a.segments; ++g) z += s.kept[g];
-    // The segment of the random number's token, and how much of its weight lies
-    // before that token.
+    // The segment of the random number's token, and the share of its weight that
+    // lies before that token.
+    const double mine = lane < a.segments ? s.kept_all[lane] : 0., upto = wave_scan(mine), z = wave_last(upto);
     const double u = a.uniform[row], goal = u > 0. ? fmin(u, 1.) * z : 0.;
-    double sum = 0., share = 0.;
-    int seg = 0;
-    for (int g = 0; g < a.segments; ++g) {
-        const double w = s.kept[g];
-        if (!(w > 0.)) continue;
-        seg = g;
-        share = (goal - sum) / w;
-        if (goal < sum + w) break;
-        sum += w;
-    }
-    // The segment again, weights as integers of 2^-47: thread sums by quads, then
-    // the wave and the token.
+    const uint64_t some = __builtin_amdgcn_ballot_w64(mine > 0.), over = __builtin_amdgcn_ballot_w64(mine > 0. && goal < upto);
+    const int seg = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : 0;
+    const double share = (goal - (__shfl(upto, seg) - __shfl(mine, seg))) / __shfl(mine, seg);
+    // The segment again, weights as integers: wave sums by quads, then the token.
     const int eg = s.head[seg].e, down = kOctave * octaves_down(e, eg);
-    const float cut_x = keep > 0 ? value_of(static_cast<uint32_t>(cut >> 32)) : INFINITY;
-    const int cut_i = keep > 0 ? static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(cut)) : -1;
+    const bool any = cut != ~0ull;
+    const float cut_x = any ? value_of(static_cast<uint32_t>(cut >> 32)) : INFINITY;
+    const int cut_i = any ? static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(cut)) : -1;
     auto weights = [&](const float (&v)[4], int i, uint64_t (&w)[4]) {
         uint64_t sum = 0;
         #pragma unroll
@@ -863,50 +968,33 @@ __device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowPara
         }
         return sum;
     };
-    // Half of the quads in flight at a time, in a loop: short code.
-    #pragma unroll 1
-    for (int j0 = 0; j0 < kQuads; j0 += kQuads / 2) {
-        float v[kQuads / 2][4];
-        #pragma unroll
-        for (int j = 0; j < kQuads / 2; ++j) load_quad(x, quad_at(seg, j0 + j), a.n, a.wide, v[j]);
-        #pragma unroll
-        for (int j = 0; j < kQuads / 2; ++j) {
-            uint64_t w[4];
-            const uint64_t t = wave_scan(weights(v[j], quad_at(seg, j0 + j), w));
-            if (lane == 63) s.part[j0 + j][wave] = t;
-        }
+    float v[kQuads][4];
+    #pragma unroll
+    for (int j = 0; j < kQuads; ++j) load_quad(x, quad_at(seg, j), a.n, a.wide, v[j]);
+    #pragma unroll
+    for (int j = 0; j < kQuads; ++j) {
+        uint64_t w[4];
+        const uint64_t t = wave_scan(weights(v[j], quad_at(seg, j), w));
+        if (lane == 63) s.quads[j * kWaves + wave] = t;
     }
     __syncthreads();
-    uint64_t all = 0;
-    for (int j = 0; j < kQuads; ++j)
-        for (int w = 0; w < kWaves; ++w) all += s.part[j][w];
+    static_assert(kQuads * kWaves == 64, "a lane for each sum");
+    const uint64_t sum = s.quads[lane], sums = wave_scan(sum), all = wave_last(sums);
     const double inside = fmax(share, 0.) * static_cast<double>(all);
     const uint64_t want = inside < static_cast<double>(all) ? min(static_cast<uint64_t>(inside), all - 1) : all - 1;
-    int tile = 0, mine = 0;
-    uint64_t before = 0;
-    bool done = false;
-    for (int j = 0; j < kQuads && !done; ++j)
-        for (int w = 0; w < kWaves; ++w) {
-            if (before + s.part[j][w] > want) {
-                tile = j;
-                mine = w;
-                done = true;
-                break;
-            }
-            before += s.part[j][w];
-        }
-    if (wave != mine) return true;
+    const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sums > want));
+    if (wave != at % kWaves) return true;
     uint64_t w[4];
-    float v[4];
-    const int i = quad_at(seg, tile);
-    load_quad(x, i, a.n, a.wide, v);
-    const uint64_t own = weights(v, i, w);
-    uint64_t b = before + wave_scan(own) - own;
+    float q[4];
+    const int i = quad_at(seg, at / kWaves);
+    load_quad(x, i, a.n, a.wide, q);
+    const uint64_t own = weights(q, i, w);
+    uint64_t b = __shfl(sums - sum, at) + wave_scan(own) - own;
     if (b <= want && want < b + own)
         for (int k = 0; k < 4; ++k) {
             if (w[k] && b <= want && want < b + w[k]) {
                 a.out[row] = i + k;
-                const Depth d = depth_of(v[k], c, eg);
+                const Depth d = depth_of(q[k], c, eg);
                 if (a.prob)
                     a.prob[row] = static_cast<float>(
                         ldexp(static_cast<double>(unit_weight(d, s.table)), eg - e - d.f / kFine) / z);
