@@ -36,7 +36,11 @@ struct PagedAttn {
     const float *q;
     float *out, *parts;
     int64_t ldq, ldout;
-    int heads, page_shift, splits, split_rows;
+    int heads, page_shift;
+    // Splits of the rows of a sequence of few query rows a KV head and of one of
+    // many (more than few_rows, which the chunk kernel takes).
+    int splits[2], split_rows[2], part_splits;
+    int few_rows;
     float scale;   // log2(e) * the softmax scale
 };
 
@@ -143,29 +147,30 @@ struct ValueTile {   // 8 rows a lane: slot j < 4 row 4 g + j, else 16 + 4 g + j
             __builtin_memcpy(w[j], row + i * kB, kB);
         }
     }
-    // Operand of dimension c: its codes of the 8 rows, slot order.
-    __device__ __forceinline__ half8 operand(int c) const {
-        half2v p[4];
+    // Operands of four dimensions (two of the rest of 96) from one dword of each
+    // row: rows are interleaved in pairs, and a pair's bytes are as they stand
+    // what a conversion takes.
+    __device__ __forceinline__ void operands(int d, half8 (&v)[4]) const {
         if constexpr (TYPE == QK_TYPE_F16) {
-            const uint32_t sel = c & 1 ? 0x07060302u : 0x05040100u;
             #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                p[k] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(w[2 * k + 1][c / 2], w[2 * k][c / 2], sel));
-            return join(p[0], p[1], p[2], p[3]);
-        } else {
-            // Byte c % 4 of four rows into one dword, then as key codes.
-            const int b = c & 3, d = c / 4;
-            const uint32_t pair = static_cast<uint32_t>(b | (4 + b) << 8) | 0x0c0c0000u;
-            uint32_t q[2];
-            #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const uint32_t lo = __builtin_amdgcn_perm(w[4 * k + 1][d], w[4 * k][d], pair);
-                const uint32_t hi = __builtin_amdgcn_perm(w[4 * k + 3][d], w[4 * k + 2][d], pair);
-                q[k] = lo | hi << 16;
+            for (int c = 0; c < 4 && 4 * d + c < HD / 16; ++c) {
+                const uint32_t sel = c & 1 ? 0x07060302u : 0x05040100u;
+                half2v p[4];
+                #pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    p[k] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(w[2 * k + 1][2 * d + c / 2], w[2 * k][2 * d + c / 2], sel));
+                v[c] = join(p[0], p[1], p[2], p[3]);
             }
-            codes4<TYPE>(q[0], p[0], p[1]);
-            codes4<TYPE>(q[1], p[2], p[3]);
-            return join(p[0], p[1], p[2], p[3]);
+        } else {
+            half2v p[4][4];
+            #pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t x = w[2 * k][d], y = w[2 * k + 1][d];
+                codes4<TYPE>(__builtin_amdgcn_perm(y, x, 0x05010400u), p[0][k], p[1][k]);
+                codes4<TYPE>(__builtin_amdgcn_perm(y, x, 0x07030602u), p[2][k], p[3][k]);
+            }
+            #pragma unroll
+            for (int c = 0; c < 4; ++c) v[c] = join(p[c][0], p[c][1], p[c][2], p[c][3]);
         }
     }
 };
@@ -185,9 +190,16 @@ __device__ __forceinline__ void clear_not_finite(half8 &v, uint32_t &bad) {
     v = __builtin_bit_cast(half8, w);
 }
 
-__device__ __forceinline__ void split_half(float x, _Float16 &hi, _Float16 &lo) {
-    hi = static_cast<_Float16>(x);
-    lo = static_cast<_Float16>(x - static_cast<float>(hi));
+// Two values as halves each: hi rounded, lo what is left (one mixed fma a value).
+// The values are pinned: a product that ends here would otherwise be rounded to
+// fp16 at once where hi is used and by way of fp32 where lo is made of it, and the
+// two differ by a step now and then.
+__device__ __forceinline__ void split_pair(float x, float y, half2v &hi, half2v &lo) {
+    float minus = -1.f;   // a constant here would make two conversions and a difference of the fma
+    asm("" : "+v"(x), "+v"(y), "+s"(minus));
+    hi = half2v{static_cast<_Float16>(x), static_cast<_Float16>(y)};
+    lo = half2v{static_cast<_Float16>(fmaf(static_cast<float>(hi[0]), minus, x)),
+                static_cast<_Float16>(fmaf(static_cast<float>(hi[1]), minus, y))};
 }
 
 // A workgroup: 16 query rows of one (sequence, KV head) over a split's rows,
@@ -201,10 +213,12 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttn a) {
     const qk_paged_seq s = a.b.seqs[blockIdx.y];
     if (!paged_seq_ok(s, a.b, a.page_shift)) return;
     const int kvh = a.kv.kv_heads, G = a.heads / kvh;
-    const int split = blockIdx.x % a.splits, unit = blockIdx.x / a.splits;
+    // A chip's XCDs take workgroups in turn: the splits rotate, or the first ones
+    // (which every sequence has) would all fall to the same XCDs.
+    const int splits = a.splits[0], unit = blockIdx.x / splits, split = (blockIdx.x + unit + blockIdx.y) % splits;
     const int h = unit % kvh, row0 = unit / kvh * kRowTile;
     const int rows = s.count * G;
-    if (row0 >= rows) return;
+    if (row0 >= rows || rows > a.few_rows) return;
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
@@ -214,9 +228,9 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttn a) {
     const int mine = have ? s.pos + tok : -1;
     const int last = s.pos + min(row0 + kRowTile - 1, rows - 1) / G;   // of the tile's last token
     const int seen = s.pos + row0 / G;                                // of its first
-    const int64_t begin64 = static_cast<int64_t>(split) * a.split_rows;
+    const int64_t begin64 = static_cast<int64_t>(split) * a.split_rows[0];
     if (begin64 > last) return;   // the merge takes the splits that reach a token
-    const int begin = static_cast<int>(begin64), end = static_cast<int>(min(begin64 + a.split_rows, int64_t(last) + 1));
+    const int begin = static_cast<int>(begin64), end = static_cast<int>(min(begin64 + a.split_rows[0], int64_t(last) + 1));
 
     half8 qh[NS], ql[NS];
     float qscale;
@@ -246,14 +260,14 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttn a) {
         const int e = fin && top > 0.f ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
         qscale = fin ? ldexpf(a.scale, -e) : __builtin_nanf("");
         #pragma unroll
-        for (int st = 0; st < NS; ++st)
+        for (int st = 0; st < NS; ++st) {
+            half2v u[4], w[4];
             #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                _Float16 hi, lo;
-                split_half(fin ? ldexpf(v[st][k], e) : 0.f, hi, lo);
-                qh[st][k] = hi;
-                ql[st][k] = lo;
-            }
+            for (int k = 0; k < 4; ++k)
+                split_pair(fin ? ldexpf(v[st][2 * k], e) : 0.f, fin ? ldexpf(v[st][2 * k + 1], e) : 0.f, u[k], w[k]);
+            qh[st] = join(u[0], u[1], u[2], u[3]);
+            ql[st] = join(w[0], w[1], w[2], w[3]);
+        }
     }
 
     float4v o[NC];
@@ -264,59 +278,86 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttn a) {
 
     const int32_t *table = a.b.page_table + static_cast<int64_t>(s.table) * a.b.table_stride;
     const int64_t page_stride = static_cast<int64_t>(kvh) * a.kv.page_rows, head_row = static_cast<int64_t>(h) * a.kv.page_rows;
-    for (int t0 = begin + wave * kTile; t0 < end; t0 += 4 * kTile) {
-        // Each half of a tile lies in one page; rows past the sequence's last
-        // are read from the first page (in bounds, masked).
-        KeyTile<HD, TYPE> kt;
-        ValueTile<HD, TYPE> vt;
+    // Each half of a tile lies in one page; rows past the sequence's last are
+    // read from the first page (in bounds, masked).  A tile's pages are looked up
+    // two tiles ahead, its rows loaded one ahead.
+    struct Pages {
+        int64_t id[2];
+    };
+    struct Tile {
+        KeyTile<HD, TYPE> k;
+        ValueTile<HD, TYPE> v;
         float4v ks[2], vs[2];
         bool present[2];
+    };
+    auto pages_of = [&](int t0) {
+        Pages p;
         #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-            const int r = t0 + 16 * hf;
-            const int64_t page = r <= last ? paged_page(table, r >> a.page_shift, a.kv.pages) : -1;
-            present[hf] = page >= 0;
-            const int64_t base = max(page, int64_t(0)) * page_stride + head_row + (r & (a.kv.page_rows - 1));
-            kt.load(hf, static_cast<const char *>(a.kv.key) + (base + n) * (HD * kCode), g);
+            const int r = min(t0 + 16 * hf, last);
+            const int64_t page = paged_page(table, r >> a.page_shift, a.kv.pages);
+            p.id[hf] = t0 + 16 * hf <= last ? page : -1;
+        }
+        return p;
+    };
+    auto load = [&](Tile &t, int t0, const Pages &p) {
+        #pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+            t.present[hf] = p.id[hf] >= 0;
+            const int64_t base = max(p.id[hf], int64_t(0)) * page_stride + head_row + ((t0 + 16 * hf) & (a.kv.page_rows - 1));
+            t.k.load(hf, static_cast<const char *>(a.kv.key) + (base + n) * (HD * kCode), g);
             #pragma unroll
             for (int j = 0; j < 4; ++j)
-                vt.load(4 * hf + j, static_cast<const char *>(a.kv.value) + (base + 4 * g + j) * (HD * kCode), n);
+                t.v.load(4 * hf + j, static_cast<const char *>(a.kv.value) + (base + 4 * g + j) * (HD * kCode), n);
             if constexpr (kScaled) {
-                ks[hf] = *reinterpret_cast<const float4v *>(a.kv.key_scale + base + 4 * g);
-                vs[hf] = *reinterpret_cast<const float4v *>(a.kv.value_scale + base + 4 * g);
+                t.ks[hf] = *reinterpret_cast<const float4v *>(a.kv.key_scale + base + 4 * g);
+                t.vs[hf] = *reinterpret_cast<const float4v *>(a.kv.value_scale + base + 4 * g);
             }
         }
+    };
+    auto take = [&](Tile &t, int t0) {
         float4v st[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
         #pragma unroll
         for (int x = 0; x < NS; ++x)
             #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
-                const half8 k = kt.operand(hf, x);
+                const half8 k = t.k.operand(hf, x);
                 st[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[x], st[hf], 0, 0, 0);
                 st[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[x], st[hf], 0, 0, 0);
             }
         // Register r of half hf: row t0 + 16 hf + 4 g + r.
         float mx = -INFINITY, vtop = 0.f;
+        const bool edge = t0 + kTile - 1 > seen || !t.present[0] || !t.present[1];
         #pragma unroll
         for (int hf = 0; hf < 2; ++hf)
             #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int at = t0 + 16 * hf + 4 * g + r;
                 float x = st[hf][r] * qscale;
                 if constexpr (kScaled)
-                    x *= ks[hf][r];
+                    x *= t.ks[hf][r];
                 else
                     x = fmaf(x, 0.f, x);   // an infinite key's score: not a number, whatever its sign
-                st[hf][r] = present[hf] && at <= mine ? x : -INFINITY;
-                mx = fmaxf(mx, st[hf][r]);
-                if constexpr (kScaled) {
-                    vs[hf][r] = present[hf] && at <= last ? vs[hf][r] : 0.f;
-                    vtop = fmaxf(vtop, vs[hf][r]);
+                st[hf][r] = x;
+            }
+        if (edge) {
+            #pragma unroll
+            for (int hf = 0; hf < 2; ++hf)
+                #pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int at = t0 + 16 * hf + 4 * g + r;
+                    st[hf][r] = t.present[hf] && at <= mine ? st[hf][r] : -INFINITY;
+                    if constexpr (kScaled) t.vs[hf][r] = t.present[hf] && at <= last ? t.vs[hf][r] : 0.f;
                 }
+        }
+        #pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+            #pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                mx = fmaxf(mx, st[hf][r]);
+                if constexpr (kScaled) vtop = fmaxf(vtop, t.vs[hf][r]);
             }
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        float f = 1.f;
         const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn;
         int en = ev;
         if constexpr (kScaled) {
@@ -325,40 +366,48 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttn a) {
             en = max(ev, vtop > 0.f ? __builtin_amdgcn_frexp_expf(vtop) : -126);
             en = __builtin_amdgcn_readfirstlane(en);
         }
-        f = __builtin_amdgcn_exp2f(m - ref);
-        m = mn;
-        l *= f;
-        const float fo = kScaled ? ldexpf(f, ev - en) : f;
-        ev = en;
-        #pragma unroll
-        for (int c = 0; c < NC; ++c)
+        // The sums follow a larger maximum or exponent, of which there are few.
+        if (en != ev || __builtin_amdgcn_ballot_w64(mn > m)) {
+            const float f = __builtin_amdgcn_exp2f(m - ref);
+            l *= f;
+            const float fo = kScaled ? ldexpf(f, ev - en) : f;
             #pragma unroll
-            for (int r = 0; r < 4; ++r) o[c][r] *= fo;
-        half8 ph, pl;
+            for (int c = 0; c < NC; ++c)
+                #pragma unroll
+                for (int r = 0; r < 4; ++r) o[c][r] *= fo;
+            m = mn;
+            ev = en;
+        }
+        half2v pu[4], pw[4];
         #pragma unroll
-        for (int hf = 0; hf < 2; ++hf)
+        for (int hf = 0; hf < 2; ++hf) {
+            float y[4];
             #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float w = __builtin_amdgcn_exp2f(st[hf][r] - ref);
                 l += w;
-                float x = w * (kScaled ? ldexpf(vs[hf][r], 14 - ev) : 0x1p14f);
-                if constexpr (kScaled) x = st[hf][r] == -INFINITY ? 0.f : x;   // a masked row's scale may be NaN
-                _Float16 hi, lo;
-                split_half(x, hi, lo);
-                ph[4 * hf + r] = hi;
-                pl[4 * hf + r] = lo;
+                y[r] = w * (kScaled ? ldexpf(t.vs[hf][r], 14 - ev) : 0x1p14f);
+                if constexpr (kScaled) y[r] = st[hf][r] == -INFINITY ? 0.f : y[r];   // a masked row's scale may be NaN
             }
+            split_pair(y[0], y[1], pu[2 * hf], pw[2 * hf]);
+            split_pair(y[2], y[3], pu[2 * hf + 1], pw[2 * hf + 1]);
+        }
+        const half8 ph = join(pu[0], pu[1], pu[2], pu[3]), pl = join(pw[0], pw[1], pw[2], pw[3]);
         // A row that some token does not see meets it as 0 * value.
-        const bool edge = TYPE != QK_TYPE_I8 && (t0 + kTile - 1 > seen || !present[0] || !present[1]);
         uint32_t bad = 0;
         #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            half8 v = vt.operand(c);
-            if (edge) clear_not_finite(v, bad);
-            o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, o[c], 0, 0, 0);
-            o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, o[c], 0, 0, 0);
+        for (int d = 0; d < (NC + 3) / 4; ++d) {
+            half8 v[4];
+            t.v.operands(d, v);
+            #pragma unroll
+            for (int k = 0; k < 4 && 4 * d + k < NC; ++k) {
+                if (TYPE != QK_TYPE_I8 && edge) clear_not_finite(v[k], bad);
+                float4v &c = o[4 * d + k];
+                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[k], pl, c, 0, 0, 0);
+                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[k], ph, c, 0, 0, 0);
+            }
         }
-        if (edge && __builtin_amdgcn_ballot_w64(bad != 0)) {
+        if (TYPE != QK_TYPE_I8 && edge && __builtin_amdgcn_ballot_w64(bad != 0)) {
             // The tokens that see such a row: not finite.
             #pragma unroll
             for (int off = 1; off < 16; off <<= 1) bad |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(bad), off));
@@ -366,8 +415,22 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttn a) {
             for (int hf = 0; hf < 2; ++hf)
                 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if ((bad >> (4 * hf + r) & 1) && present[hf] && t0 + 16 * hf + 4 * g + r <= mine)
+                    if ((bad >> (4 * hf + r) & 1) && t.present[hf] && t0 + 16 * hf + 4 * g + r <= mine)
                         l = __builtin_nanf("");
+        }
+    };
+    constexpr int kStep = 4 * kTile;
+    int t0 = begin + wave * kTile;
+    if (t0 < end) {
+        Tile cur;
+        load(cur, t0, pages_of(t0));
+        Pages ahead = pages_of(t0 + kStep);
+        for (; t0 < end; t0 += kStep) {
+            Tile next;
+            if (t0 + kStep < end) load(next, t0 + kStep, ahead);
+            ahead = pages_of(t0 + 2 * kStep);
+            take(cur, t0);
+            cur = next;
         }
     }
     l += __shfl_xor(l, 16);
@@ -408,8 +471,8 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttn a) {
     const int head = h * G + row % G;
     float *dst;
     float norm = 1.f;
-    if (a.splits > 1) {
-        dst = a.parts + ((static_cast<int64_t>(s.first + tok) * a.heads + head) * a.splits + split) * part_floats(HD);
+    if (splits > 1) {
+        dst = a.parts + ((static_cast<int64_t>(s.first + tok) * a.heads + head) * a.part_splits + split) * part_floats(HD);
         if (g == 0) *reinterpret_cast<float4 *>(dst) = make_float4(m, l, 0.f, 0.f);
         dst += 4;
     } else {
@@ -420,6 +483,400 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttn a) {
     for (int r = 0; r < 4; ++r)
         #pragma unroll
         for (int c = 0; c < NC; ++c) dst[value_dim<HD, TYPE>(4 * g + r, c)] = o[c][r] * norm;
+}
+
+// -------------------------------------------------------------- chunks --
+//
+// Sequences of many query rows: a workgroup takes 128 of them (32 a wave) over
+// tiles of 64 cache rows, which all four waves read from LDS as fp16, converted
+// once.  Keys lie there as they are, values transposed, [dimension][row], so both
+// are operands of v_mfma_f32_32x32x16_f16 as 16-byte reads.  The rows of a tile
+// are permuted as the scores' registers hold them: lane half hi has, of each 16
+// rows, 4 hi .. + 3 and 8 + 4 hi .. + 3.  While a tile is multiplied the next one
+// is in registers on its way from memory; two LDS buffers, a barrier a tile.
+constexpr int kChunkTile = 64, kChunkRows = 128;
+
+template <int HD, int TYPE>
+struct Chunk {
+    static constexpr int kCode = code_bytes(TYPE);
+    static constexpr int kKeyCols = 16 / kCode, kKeyTasks = kChunkTile * HD / kKeyCols, kKeys = (kKeyTasks + 255) / 256;
+    static constexpr int kValCols = HD == 64 ? 4 : 8, kValTasks = kChunkTile / 4 * HD / kValCols, kVals = (kValTasks + 255) / 256;
+    static constexpr int kValBytes = kValCols * kCode;
+    // Keys: 16 bytes between rows put the 8 rows of a read into different
+    // banks.  Values: 128 bytes a dimension, 16-byte pieces exchanged by it.
+    static constexpr int kKeyStride = 2 * HD + 16;
+    static constexpr int kKeyBytes = kChunkTile * kKeyStride, kValueBytes = HD * 2 * kChunkTile;
+    static constexpr int kHead = 2 * kChunkTile * 4 + 32;   // the scales; absent and not finite rows; the exponent
+    static constexpr int kBuffer = kKeyBytes + kValueBytes + kHead;
+
+    struct Head {
+        float ks[kChunkTile], vs[kChunkTile];   // vs times 2^(14 - ev)
+        uint64_t absent;
+        uint32_t bad[2];
+        int ev, pad[3];
+    };
+    static_assert(sizeof(Head) == kHead, "Head");
+
+    static __device__ __forceinline__ int value_at(int d, int piece) {
+        return d * 2 * kChunkTile + ((piece ^ ((d ^ (d >> 3)) & 7)) << 4);
+    }
+};
+
+typedef float float16v __attribute__((ext_vector_type(16)));
+typedef _Float16 half4v __attribute__((ext_vector_type(4)));
+
+template <int HD, int TYPE>
+__global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
+    using C = Chunk<HD, TYPE>;
+    constexpr int NS = HD / 16, ND = HD / 32, kCode = C::kCode;
+    constexpr bool kScaled = TYPE != QK_TYPE_F16;
+    extern __shared__ __align__(16) char lds[];
+    const qk_paged_seq s = a.b.seqs[blockIdx.y];
+    if (!paged_seq_ok(s, a.b, a.page_shift)) return;
+    const int kvh = a.kv.kv_heads, G = a.heads / kvh;
+    const int splits = a.splits[1], unit = blockIdx.x / splits, split = (blockIdx.x + unit + blockIdx.y) % splits;
+    const int rows = s.count * G, tiles = (rows + kChunkRows - 1) / kChunkRows;
+    if (unit / kvh >= tiles || rows <= a.few_rows) return;
+    // The last tiles first: they see the most rows.
+    const int h = unit % kvh, row0 = (tiles - 1 - unit / kvh) * kChunkRows;
+    const int lane = threadIdx.x & 63, n = lane & 31, hi = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int last = s.pos + min(row0 + kChunkRows - 1, rows - 1) / G, seen = s.pos + row0 / G;
+    const int64_t begin64 = static_cast<int64_t>(split) * a.split_rows[1];
+    if (begin64 > last) return;
+    const int begin = static_cast<int>(begin64), end = static_cast<int>(min(begin64 + a.split_rows[1], int64_t(last) + 1));
+
+    const int wrow = row0 + 32 * wave, row = wrow + n, tok = row / G;
+    const bool have = row < rows;
+    const int mine = have ? s.pos + tok : -1;
+    const int wave_seen = s.pos + wrow / G, wave_last = wrow < rows ? s.pos + min(wrow + 31, rows - 1) / G : -1;
+
+    // ------------------------------------------------------ staging ------
+    const int32_t *table = a.b.page_table + static_cast<int64_t>(s.table) * a.b.table_stride;
+    const int64_t page_stride = static_cast<int64_t>(kvh) * a.kv.page_rows, head_row = static_cast<int64_t>(h) * a.kv.page_rows;
+    const int mask = a.kv.page_rows - 1;
+    // Renewed every tile: what follows from it is then computed anew, instead of
+    // kept in registers through the loop (30 of them, which spilled).
+    int tid = threadIdx.x;
+    auto key_row = [&](int i) { return (tid + 256 * i) / (HD / C::kKeyCols); };
+    auto key_col = [&](int i) { return (tid + 256 * i) % (HD / C::kKeyCols) * C::kKeyCols; };
+    auto value_quad = [&](int i) { return (tid + 256 * i) / (HD / C::kValCols); };
+    auto value_col = [&](int i) { return (tid + 256 * i) % (HD / C::kValCols) * C::kValCols; };
+    struct Pages {
+        int32_t key[C::kKeys], value[C::kVals], scale;
+    };
+    auto pages_of = [&](int t0) {
+        Pages p;
+        #pragma unroll
+        for (int i = 0; i < C::kKeys; ++i) p.key[i] = table[min(t0 + min(key_row(i), kChunkTile - 1), last) >> a.page_shift];
+        #pragma unroll
+        for (int i = 0; i < C::kVals; ++i) p.value[i] = table[min(t0 + min(4 * value_quad(i), kChunkTile - 1), last) >> a.page_shift];
+        p.scale = table[min(t0 + lane, last) >> a.page_shift];
+        return p;
+    };
+    // Whether a row is there; its place in the pool (the first page's, masked,
+    // if not).
+    auto place = [&](int r, int32_t page, bool &there) {
+        there = r <= last && page >= 0 && page < a.kv.pages;
+        return (there ? page : 0) * page_stride + head_row + (r & mask);
+    };
+    struct Stage {
+        uint4v key[C::kKeys];
+        uint32_t value[C::kVals][4][C::kValBytes / 4];
+        float scale;
+        bool there[C::kVals], scale_there;
+    };
+    auto load = [&](Stage &g, int t0, const Pages &p) {
+        bool there;
+        #pragma unroll
+        for (int i = 0; i < C::kKeys; ++i) {
+            const int64_t at = place(t0 + min(key_row(i), kChunkTile - 1), p.key[i], there);
+            g.key[i] = *reinterpret_cast<const uint4v *>(static_cast<const char *>(a.kv.key) + (at * HD + key_col(i)) * kCode);
+        }
+        #pragma unroll
+        for (int i = 0; i < C::kVals; ++i) {
+            const int quad = min(value_quad(i), kChunkTile / 4 - 1);
+            // Four rows that start in a page are all in it; of them some may lie
+            // past the last, which is written page memory.
+            const int64_t at = place(t0 + 4 * quad, p.value[i], g.there[i]);
+            const char *from = static_cast<const char *>(a.kv.value) + (at * HD + value_col(i)) * kCode;
+            #pragma unroll
+            for (int r = 0; r < 4; ++r) __builtin_memcpy(g.value[i][r], from + r * HD * kCode, C::kValBytes);
+        }
+        const int64_t at = place(t0 + lane, p.scale, g.scale_there);
+        if constexpr (kScaled)
+            if (wave < 2) g.scale = (wave == 0 ? a.kv.value_scale : a.kv.key_scale)[at];
+    };
+    int top_ev = -126;   // wave 0's: the exponent of the largest value scale so far
+    auto store = [&](const Stage &g, int t0, char *buf) {
+        auto &head = *reinterpret_cast<typename C::Head *>(buf + C::kKeyBytes + C::kValueBytes);
+        if (wave == 0) {
+            const uint64_t absent = __builtin_amdgcn_ballot_w64(!g.scale_there);
+            if constexpr (kScaled) {
+                // A row that some token does not see meets it as 0 * value: what
+                // is not finite counts as 0 there, and is flagged.
+                const bool bad = g.scale_there && !isfinite(g.scale) && t0 + kChunkTile - 1 > seen;
+                const uint64_t all_bad = __builtin_amdgcn_ballot_w64(bad);
+                if (lane < 2 && all_bad) atomicOr(&head.bad[lane], static_cast<uint32_t>(all_bad >> (32 * lane)));
+                const float v = g.scale_there && !bad ? g.scale : 0.f;
+                float top = v;
+                #pragma unroll
+                for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+                top_ev = max(top_ev, top > 0.f ? __builtin_amdgcn_frexp_expf(top) : -126);
+                head.vs[lane] = ldexpf(v, 14 - top_ev);
+            }
+            if (lane == 0) {
+                head.absent = absent;
+                head.ev = top_ev;
+            }
+        } else if (wave == 1) {
+            if constexpr (kScaled) head.ks[lane] = g.scale;
+        }
+        #pragma unroll
+        for (int i = 0; i < C::kKeys; ++i) {
+            if (C::kKeyTasks % 256 && tid + 256 * i >= C::kKeyTasks) continue;
+            char *at = buf + key_row(i) * C::kKeyStride + key_col(i) * 2;
+            if constexpr (TYPE == QK_TYPE_F16) {
+                *reinterpret_cast<uint4v *>(at) = g.key[i];
+            } else {
+                half2v c[8];
+                #pragma unroll
+                for (int w = 0; w < 4; ++w) codes4<TYPE>(g.key[i][w], c[2 * w], c[2 * w + 1]);
+                *reinterpret_cast<half8 *>(at) = join(c[0], c[1], c[2], c[3]);
+                *reinterpret_cast<half8 *>(at + 16) = join(c[4], c[5], c[6], c[7]);
+            }
+        }
+        const bool edge = TYPE != QK_TYPE_I8 && t0 + kChunkTile - 1 > seen;
+        #pragma unroll
+        for (int i = 0; i < C::kVals; ++i) {
+            if (C::kValTasks % 256 && tid + 256 * i >= C::kValTasks) continue;
+            const int quad = value_quad(i), piece = quad / 4 * 2 + (quad & 1), half = quad >> 1 & 1;
+            uint32_t bad = 0;
+            #pragma unroll
+            for (int d4 = 0; d4 < C::kValCols / 4; ++d4) {
+                half2v p[4][2];   // of four dimensions: rows 0 and 1, rows 2 and 3
+                if constexpr (TYPE == QK_TYPE_F16) {
+                    #pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        #pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            p[c][k] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(g.value[i][2 * k + 1][2 * d4 + c / 2],
+                                                                                       g.value[i][2 * k][2 * d4 + c / 2],
+                                                                                       c & 1 ? 0x07060302u : 0x05040100u));
+                } else {
+                    #pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const uint32_t x = g.value[i][2 * k][d4], y = g.value[i][2 * k + 1][d4];
+                        codes4<TYPE>(__builtin_amdgcn_perm(y, x, 0x05010400u), p[0][k], p[1][k]);
+                        codes4<TYPE>(__builtin_amdgcn_perm(y, x, 0x07030602u), p[2][k], p[3][k]);
+                    }
+                }
+                #pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t w[2] = {__builtin_bit_cast(uint32_t, p[c][0]), __builtin_bit_cast(uint32_t, p[c][1])};
+                    if (TYPE != QK_TYPE_I8 && !g.there[i]) w[0] = w[1] = 0;
+                    if (edge) {
+                        #pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            if ((w[k] & 0x7C00u) == 0x7C00u) w[k] &= 0xFFFF0000u, bad |= 1u << (2 * k);
+                            if ((w[k] & 0x7C000000u) == 0x7C000000u) w[k] &= 0xFFFFu, bad |= 2u << (2 * k);
+                        }
+                    }
+                    const int d = value_col(i) + 4 * d4 + c;
+                    *reinterpret_cast<uint2 *>(buf + C::kKeyBytes + C::value_at(d, piece) + 8 * half) = make_uint2(w[0], w[1]);
+                }
+            }
+            if (edge && bad) atomicOr(&head.bad[quad / 8], bad << (4 * quad % 32));
+        }
+    };
+
+    // ------------------------------------------------------- queries -----
+    half8 qh[NS], ql[NS];
+    float qscale;
+    {
+        const float *qrow = a.q + (s.first + tok) * a.ldq + static_cast<int64_t>(h * G + row % G) * HD + 8 * hi;
+        float top = 0.f;
+        int fin = 1;
+        #pragma unroll
+        for (int x = 0; x < NS; ++x)
+            #pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (have) v = *reinterpret_cast<const float4 *>(qrow + 16 * x + e);
+                top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+                fin &= isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w);
+            }
+        top = fmaxf(top, __shfl_xor(top, 32));
+        fin &= __shfl_xor(fin, 32);
+        const int e = fin && top > 0.f ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
+        // Scores in units of 2^-e; one that underflows is as good as 2^-126.
+        qscale = ldexpf(fabsf(a.scale), -e);
+        qscale = fin ? (qscale < 0x1p-126f ? 0x1p-126f : qscale) : __builtin_nanf("");
+        const float sign = a.scale < 0.f ? -1.f : 1.f;
+        #pragma unroll
+        for (int x = 0; x < NS; ++x) {
+            half2v u[4], w[4];
+            #pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (have && fin) v = *reinterpret_cast<const float4 *>(qrow + 16 * x + 4 * k);
+                split_pair(ldexpf(sign * v.x, e), ldexpf(sign * v.y, e), u[2 * k], w[2 * k]);
+                split_pair(ldexpf(sign * v.z, e), ldexpf(sign * v.w, e), u[2 * k + 1], w[2 * k + 1]);
+            }
+            qh[x] = join(u[0], u[1], u[2], u[3]);
+            ql[x] = join(w[0], w[1], w[2], w[3]);
+        }
+    }
+
+    float16v o[ND];
+    #pragma unroll
+    for (int d = 0; d < ND; ++d)
+        #pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+    // The largest score so far in the products' units, and in base 2 (-c).
+    float m = -INFINITY, c = INFINITY, l = 0.f;
+    int ev = -126;
+
+    auto take = [&](const char *buf, int t0) {
+        const auto &head = *reinterpret_cast<const typename C::Head *>(buf + C::kKeyBytes + C::kValueBytes);
+        const int en = kScaled ? __builtin_amdgcn_readfirstlane(head.ev) : ev;
+        const bool edge = t0 + kChunkTile - 1 > wave_seen || head.absent;   // some token does not see it whole
+        // Half a tile at a time: 32 scores a lane left too few registers.
+        #pragma unroll 1
+        for (int hf = 0; hf < 2; ++hf) {
+            float16v st;
+            #pragma unroll
+            for (int r = 0; r < 16; ++r) st[r] = 0.f;
+            const char *keys = buf + (32 * hf + n) * C::kKeyStride + 16 * hi;
+            #pragma unroll
+            for (int x = 0; x < NS; ++x) {
+                const half8 k = *reinterpret_cast<const half8 *>(keys + 32 * x);
+                st = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[x], st, 0, 0, 0);
+                st = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[x], st, 0, 0, 0);
+            }
+            // Register r: row t0 + 32 hf + 8 (r / 4) + 4 hi + r % 4.
+            #pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+                if constexpr (kScaled) {
+                    const float4v ks = *reinterpret_cast<const float4v *>(head.ks + 32 * hf + 8 * r4 + 4 * hi);
+                    #pragma unroll
+                    for (int r = 0; r < 4; ++r) st[4 * r4 + r] *= ks[r];
+                } else {
+                    #pragma unroll
+                    for (int r = 0; r < 4; ++r)   // an infinite key's score: not a number, whatever its sign
+                        st[4 * r4 + r] = fmaf(st[4 * r4 + r], 0.f, st[4 * r4 + r]);
+                }
+            }
+            if (edge) {
+                const uint32_t hide = static_cast<uint32_t>(head.absent >> (32 * hf)) >> (4 * hi);
+                const int left = mine - t0 - 32 * hf - 4 * hi;
+                #pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int at = 8 * (r / 4) + r % 4;
+                    st[r] = at <= left && !(hide >> at & 1) ? st[r] : -INFINITY;
+                }
+            }
+            float mx = fmaxf(fmaxf(st[0], st[1]), st[2]);
+            #pragma unroll
+            for (int r = 3; r < 15; r += 2) mx = fmaxf(mx, fmaxf(st[r], st[r + 1]));
+            mx = fmaxf(mx, st[15]);
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float mn = fmaxf(m, mx);
+            if (en != ev || __builtin_amdgcn_ballot_w64(mn > m)) {
+                // c is what the weights so far were taken with, rounding and all.
+                const float cn = mn == -INFINITY ? INFINITY : -mn * qscale;
+                const float f = cn == INFINITY ? 1.f : __builtin_amdgcn_exp2f(cn - c);
+                l *= f;
+                const float fo = kScaled ? ldexpf(f, ev - en) : f;
+                #pragma unroll
+                for (int d = 0; d < ND; ++d)
+                    #pragma unroll
+                    for (int r = 0; r < 16; ++r) o[d][r] *= fo;
+                m = mn;
+                c = cn;
+                ev = en;
+            }
+            const float ref = c == INFINITY ? 0.f : c;   // nothing seen: weights of exp2(-inf)
+            if (edge && t0 + kChunkTile - 1 > seen) {
+                const uint32_t bad = head.bad[hf] >> (4 * hi);
+                if (__builtin_amdgcn_ballot_w64(bad != 0)) {
+                    #pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if ((bad >> (8 * (r / 4) + r % 4) & 1) && st[r] != -INFINITY) l = __builtin_nanf("");
+                }
+            }
+            const char *values = buf + C::kKeyBytes;
+            #pragma unroll
+            for (int b = 0; b < 2; ++b) {   // 16 rows
+                half2v pu[4], pw[4];
+                #pragma unroll
+                for (int r4 = 0; r4 < 2; ++r4) {
+                    float4v vs;
+                    if constexpr (kScaled)
+                        vs = *reinterpret_cast<const float4v *>(head.vs + 32 * hf + 16 * b + 8 * r4 + 4 * hi);
+                    float y[4];
+                    #pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float x = st[8 * b + 4 * r4 + r];
+                        const float w = __builtin_amdgcn_exp2f(fmaf(x, qscale, ref));
+                        l += w;
+                        y[r] = w * (kScaled ? vs[r] : 0x1p14f);
+                    }
+                    split_pair(y[0], y[1], pu[2 * r4], pw[2 * r4]);
+                    split_pair(y[2], y[3], pu[2 * r4 + 1], pw[2 * r4 + 1]);
+                }
+                const half8 ph = join(pu[0], pu[1], pu[2], pu[3]), pl = join(pw[0], pw[1], pw[2], pw[3]);
+                #pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    const half8 v = *reinterpret_cast<const half8 *>(values + C::value_at(32 * d + n, 4 * hf + 2 * b + hi));
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[d], 0, 0, 0);
+                }
+            }
+        }
+    };
+
+    Stage g;
+    load(g, begin, pages_of(begin));
+    Pages ahead = pages_of(begin + kChunkTile);
+    int b = 0;
+    for (int t0 = begin; t0 < end; t0 += kChunkTile, b ^= 1) {
+        char *buf = lds + b * C::kBuffer;
+        asm volatile("" : "+v"(tid));
+        if (t0 + kChunkTile - 1 > seen) {   // flags that all waves may set
+            auto &head = *reinterpret_cast<typename C::Head *>(buf + C::kKeyBytes + C::kValueBytes);
+            if (tid == 0) head.bad[0] = head.bad[1] = 0;
+            __syncthreads();
+        }
+        store(g, t0, buf);
+        __syncthreads();   // the tile is in; every wave is done with the one before
+        if (t0 + kChunkTile < end) {
+            load(g, t0 + kChunkTile, ahead);
+            ahead = pages_of(t0 + 2 * kChunkTile);
+        }
+        if (t0 <= wave_last) take(buf, t0);
+    }
+    l += __shfl_xor(l, 32);
+    if (!have) return;
+    const int head = h * G + row % G;
+    const bool none = m == -INFINITY && l == 0.f;
+    float *dst;
+    float norm = kScaled ? ldexpf(1.f, ev - 14) : 0x1p-14f;
+    if (splits > 1) {
+        dst = a.parts + ((static_cast<int64_t>(s.first + tok) * a.heads + head) * a.part_splits + split) * part_floats(HD);
+        if (hi == 0) *reinterpret_cast<float4 *>(dst) = make_float4(-c, l, 0.f, 0.f);
+        dst += 4;
+    } else {
+        dst = a.out + (s.first + tok) * a.ldout + static_cast<int64_t>(head) * HD;
+        norm = none ? 0.f : norm / l;
+    }
+    #pragma unroll
+    for (int d = 0; d < ND; ++d)
+        #pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+            float4 v = make_float4(o[d][4 * r4] * norm, o[d][4 * r4 + 1] * norm, o[d][4 * r4 + 2] * norm, o[d][4 * r4 + 3] * norm);
+            *reinterpret_cast<float4 *>(dst + 32 * d + 8 * r4 + 4 * hi) = v;
+        }
 }
 
 // The splits that reach a token, in order; one wave a (token, head).
@@ -433,8 +890,10 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
     const int tok = static_cast<int>(at / a.heads), head = static_cast<int>(at % a.heads);
     // As the kernel's: a tile's splits go to its last token's last row, and
     // those beyond this token's own hold nothing of it.
-    const int live = min(a.splits, (s.pos + tok) / a.split_rows + 1);
-    const float *p = a.parts + (static_cast<int64_t>(s.first + tok) * a.heads + head) * a.splits * part_floats(HD);
+    const int many = static_cast<int64_t>(s.count) * (a.heads / a.kv.kv_heads) > a.few_rows;
+    if (a.splits[many] == 1) return;
+    const int live = min(a.splits[many], (s.pos + tok) / a.split_rows[many] + 1);
+    const float *p = a.parts + (static_cast<int64_t>(s.first + tok) * a.heads + head) * a.part_splits * part_floats(HD);
     constexpr int kD = HD > 64 ? (HD + 63) / 64 : 1;
     float m = -INFINITY, l = 0.f, o[kD] = {};
     for (int i = 0; i < live; ++i) {
@@ -454,13 +913,35 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
         if (d * 64 + lane < HD) out[d * 64 + lane] = o[d] * norm;
 }
 
-// Splits of a call's rows: enough workgroups for the chip, at least two tiles
-// a wave.
-int wanted_splits(const qk_paged_batch &b, int heads, int kv_heads) {
-    const int64_t tiles = (static_cast<int64_t>(b.max_count) * (heads / kv_heads) + kRowTile - 1) / kRowTile;
-    const int64_t units = std::max<int64_t>(1, tiles * kv_heads * b.n_seqs);
-    const int64_t most = (b.max_rows + 8 * kTile - 1) / (8 * kTile);
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({1024 / units, most, 64})));
+// A sequence of more query rows a KV head than this takes the chunk kernel.
+constexpr int kFewRows = 64;
+// The chunk kernel's queries and sums of a head fit the registers up to here
+// (at 256 it spilled 58 and more).
+constexpr int kChunkDim = 128;
+
+// Splits of a call's rows.  Few query rows: some 8 workgroups a CU, so that
+// sequences of different lengths even out, of at least 512 rows each while there
+// are enough of them to go round, at least one tile a wave.  Chunks: two
+// workgroups a CU of at least four tiles.
+struct Splits {
+    int few, many;
+};
+// Query rows a KV head up to which a sequence of this call takes the first
+// kernel: one sequence has the chunk kernel alone, if its bound calls for it.
+int few_rows(const qk_paged_batch &b, int heads, int kv_heads, int head_dim) {
+    if (head_dim > kChunkDim || static_cast<int64_t>(b.max_count) * (heads / kv_heads) <= kFewRows) return INT32_MAX;
+    return b.n_seqs == 1 ? 0 : kFewRows;
+}
+Splits wanted_splits(const qk_paged_batch &b, int heads, int kv_heads, int head_dim) {
+    const int64_t few = few_rows(b, heads, kv_heads, head_dim), rows = static_cast<int64_t>(b.max_count) * (heads / kv_heads);
+    const int64_t per_tile = static_cast<int64_t>(kv_heads) * b.n_seqs;
+    auto fit = [&](int64_t query_rows, int tile, int64_t want, int64_t least) {
+        const int64_t units = std::max<int64_t>((query_rows + tile - 1) / tile * per_tile, 1);
+        if (least == 0) least = units * b.max_rows >= 512 * 1024 ? 512 : 4 * kTile;
+        return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want / units, (b.max_rows + least - 1) / least, 64})));
+    };
+    return {few > 0 ? fit(std::min(rows, few), kRowTile, 2048, 0) : 1,
+            rows > few ? fit(rows, kChunkRows, 512, 4 * kChunkTile) : 1};
 }
 
 size_t split_bytes(const qk_paged_batch &b, int heads, int hd) {
@@ -469,12 +950,20 @@ size_t split_bytes(const qk_paged_batch &b, int heads, int hd) {
 
 template <int HD, int TYPE>
 int launch(const PagedAttn &a, hipStream_t stream) {
-    const int64_t G = a.heads / a.kv.kv_heads;
-    const int64_t tiles = (a.b.max_count * G + kRowTile - 1) / kRowTile;
-    hipLaunchKernelGGL((paged_attention_kernel<HD, TYPE>),
-                       dim3(static_cast<unsigned>(tiles * a.kv.kv_heads * a.splits), a.b.n_seqs), dim3(256), 0,
-                       stream, a);
-    if (a.splits > 1)
+    const int64_t rows = static_cast<int64_t>(a.b.max_count) * (a.heads / a.kv.kv_heads);
+    auto grid = [&](int64_t n, int tile, int splits) {
+        return dim3(static_cast<unsigned>((n + tile - 1) / tile * a.kv.kv_heads * splits), a.b.n_seqs);
+    };
+    if (a.few_rows > 0)
+        hipLaunchKernelGGL((paged_attention_kernel<HD, TYPE>),
+                           grid(std::min<int64_t>(rows, a.few_rows), kRowTile, a.splits[0]), dim3(256), 0, stream, a);
+    if constexpr (HD <= kChunkDim) {
+        constexpr size_t kLds = 2 * Chunk<HD, TYPE>::kBuffer;
+        if (rows > a.few_rows)
+            hipLaunchKernelGGL((paged_chunk_kernel<HD, TYPE>), grid(rows, kChunkRows, a.splits[1]), dim3(256), kLds,
+                               stream, a);
+    }
+    if (a.part_splits > 1)
         hipLaunchKernelGGL((paged_merge_kernel<HD>),
                            dim3(static_cast<unsigned>((static_cast<int64_t>(a.b.max_count) * a.heads + 3) / 4),
                                 a.b.n_seqs),
@@ -498,8 +987,9 @@ size_t qk_paged_attention_workspace_bytes(const qk_paged_batch *batch, int heads
     if (qk::check_paged_batch("qk_paged_attention_workspace_bytes", batch) || heads < 1 || kv_heads < 1 ||
         heads % kv_heads || head_dim < 1 || head_dim > 256 || batch->n_seqs == 0 || batch->n_tokens == 0)
         return 0;
-    const int splits = qk::wanted_splits(*batch, heads, kv_heads);
-    return splits > 1 ? splits * qk::split_bytes(*batch, heads, head_dim) : 0;
+    const qk::Splits splits = qk::wanted_splits(*batch, heads, kv_heads, head_dim);
+    const int most = std::max(splits.few, splits.many);
+    return most > 1 ? most * qk::split_bytes(*batch, heads, head_dim) : 0;
 }
 
 int qk_paged_attention_f32(const qk_paged_kv *kv, const qk_paged_batch *batch, const float *q, int ldq, float *out,
@@ -534,10 +1024,17 @@ int qk_paged_attention_f32(const qk_paged_kv *kv, const qk_paged_batch *batch, c
     a.scale = 1.4426950408889634f * (scale != 0.f ? scale : 1.f / std::sqrt(static_cast<float>(kv->head_dim)));
     const size_t per = qk::split_bytes(*batch, heads, kv->head_dim);
     const int64_t fit = workspace ? static_cast<int64_t>(workspace_bytes / per) : 0;
-    a.splits = static_cast<int>(std::min<int64_t>(qk::wanted_splits(*batch, heads, kv->kv_heads), fit < 2 ? 1 : fit));
-    // Splits of whole rounds of the four waves' tiles.
-    a.split_rows = ((batch->max_rows + a.splits - 1) / a.splits + 4 * qk::kTile - 1) / (4 * qk::kTile) * (4 * qk::kTile);
-    a.splits = (batch->max_rows + a.split_rows - 1) / a.split_rows;
+    const qk::Splits wanted = qk::wanted_splits(*batch, heads, kv->kv_heads, kv->head_dim);
+    // Splits of whole rounds of a workgroup's tiles.
+    auto plan = [&](int kind, int splits, int round) {
+        const int n = static_cast<int>(std::min<int64_t>(splits, fit < 2 ? 1 : fit));
+        a.split_rows[kind] = ((batch->max_rows + n - 1) / n + round - 1) / round * round;
+        a.splits[kind] = (batch->max_rows + a.split_rows[kind] - 1) / a.split_rows[kind];
+    };
+    a.few_rows = qk::few_rows(*batch, heads, kv->kv_heads, kv->head_dim);
+    plan(0, wanted.few, 4 * qk::kTile);
+    plan(1, wanted.many, qk::kChunkTile);
+    a.part_splits = std::max(a.splits[0], a.splits[1]);
     switch (kv->head_dim) {
         case 64: return qk::launch_type<64>(a, qk::S(stream));
         case 96: return qk::launch_type<96>(a, qk::S(stream));
