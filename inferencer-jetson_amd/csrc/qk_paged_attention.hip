@@ -190,14 +190,14 @@ __device__ __forceinline__ void clear_not_finite(half8 &v, uint32_t &bad) {
     v = __builtin_bit_cast(half8, w);
 }
 
-// Two values as halves each: hi rounded, lo what is left (one mixed fma a value).
+// Two values as halves each: hi cut off, lo what is left (one mixed fma a value).
 // The values are pinned: a product that ends here would otherwise be rounded to
 // fp16 at once where hi is used and by way of fp32 where lo is made of it, and the
 // two differ by a step now and then.
 __device__ __forceinline__ void split_pair(float x, float y, half2v &hi, half2v &lo) {
     float minus = -1.f;   // a constant here would make two conversions and a difference of the fma
     asm("" : "+v"(x), "+v"(y), "+s"(minus));
-    hi = half2v{static_cast<_Float16>(x), static_cast<_Float16>(y)};
+    hi = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(x, y));
     lo = half2v{static_cast<_Float16>(fmaf(static_cast<float>(hi[0]), minus, x)),
                 static_cast<_Float16>(fmaf(static_cast<float>(hi[1]), minus, y))};
 }
@@ -235,22 +235,25 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttn a) {
     half8 qh[NS], ql[NS];
     float qscale;
     {
-        const float *qrow = a.q + (s.first + tok) * a.ldq + static_cast<int64_t>(h * G + row % G) * HD;
+        // (The last row again past it: a load under a condition is one at a time.)
+        const int at = min(row, rows - 1);
+        const float *qrow = a.q + (s.first + at / G) * a.ldq + static_cast<int64_t>(h * G + at % G) * HD;
         float v[NS][8], top = 0.f;
         bool finite = true;
         #pragma unroll
         for (int st = 0; st < NS; ++st)
             #pragma unroll
             for (int e = 0; e < 8; e += 4) {
-                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (have) x = *reinterpret_cast<const float4 *>(qrow + key_dim<HD, TYPE>(st, g) + e);
-                const float y[4] = {x.x, x.y, x.z, x.w};
-                #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    v[st][e + k] = y[k];
-                    top = fmaxf(top, fabsf(y[k]));
-                    finite = finite && isfinite(y[k]);
-                }
+                const float4 x = *reinterpret_cast<const float4 *>(qrow + key_dim<HD, TYPE>(st, g) + e);
+                v[st][e] = x.x, v[st][e + 1] = x.y, v[st][e + 2] = x.z, v[st][e + 3] = x.w;
+            }
+        #pragma unroll
+        for (int st = 0; st < NS; ++st)
+            #pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                v[st][k] = have ? v[st][k] : 0.f;
+                top = fmaxf(top, fabsf(v[st][k]));
+                finite = finite && isfinite(v[st][k]);
             }
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
@@ -498,28 +501,26 @@ constexpr int kChunkTile = 64, kChunkRows = 128;
 
 template <int HD, int TYPE>
 struct Chunk {
-    static constexpr int kCode = code_bytes(TYPE);
-    static constexpr int kKeyCols = 16 / kCode, kKeyTasks = kChunkTile * HD / kKeyCols, kKeys = (kKeyTasks + 255) / 256;
-    static constexpr int kValCols = HD == 64 ? 4 : 8, kValTasks = kChunkTile / 4 * HD / kValCols, kVals = (kValTasks + 255) / 256;
-    static constexpr int kValBytes = kValCols * kCode;
+    static constexpr int kCode = code_bytes(TYPE), kWidth = HD == 96 ? 128 : HD;
+    // A thread's share of a tile: 16 bytes of kKeys key rows, kValCols values of
+    // four rows (of 96 dimensions as of 128, a quarter of the threads idle, so that
+    // a wave's rows lie within 16 of one page).
+    static constexpr int kKeyCols = 16 / kCode, kKeyLine = kWidth / kKeyCols, kKeys = kChunkTile * kKeyLine / 256;
+    static constexpr int kValCols = kWidth / 16, kValBytes = kValCols * kCode;
+    static_assert(kValCols % 4 == 0, "values go by four");
     // Keys: 16 bytes between rows put the 8 rows of a read into different
     // banks.  Values: 128 bytes a dimension, 16-byte pieces exchanged by it.
     static constexpr int kKeyStride = 2 * HD + 16;
     static constexpr int kKeyBytes = kChunkTile * kKeyStride, kValueBytes = HD * 2 * kChunkTile;
-    static constexpr int kHead = 2 * kChunkTile * 4 + 32;   // the scales; absent and not finite rows; the exponent
-    static constexpr int kBuffer = kKeyBytes + kValueBytes + kHead;
 
     struct Head {
         float ks[kChunkTile], vs[kChunkTile];   // vs times 2^(14 - ev)
-        uint64_t absent;
-        uint32_t bad[2];
-        int ev, pad[3];
+        uint32_t bad[2];                        // rows that are not finite
+        int ev, pad;
     };
-    static_assert(sizeof(Head) == kHead, "Head");
+    static constexpr int kBuffer = kKeyBytes + kValueBytes + sizeof(Head);
 
-    static __device__ __forceinline__ int value_at(int d, int piece) {
-        return d * 2 * kChunkTile + ((piece ^ ((d ^ (d >> 3)) & 7)) << 4);
-    }
+    static __device__ __forceinline__ int exchange(int d) { return (d ^ (d >> 3)) & 7; }
 };
 
 typedef float float16v __attribute__((ext_vector_type(16)));
@@ -558,84 +559,70 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
     // Renewed every tile: what follows from it is then computed anew, instead of
     // kept in registers through the loop (30 of them, which spilled).
     int tid = threadIdx.x;
-    auto key_row = [&](int i) { return (tid + 256 * i) / (HD / C::kKeyCols); };
-    auto key_col = [&](int i) { return (tid + 256 * i) % (HD / C::kKeyCols) * C::kKeyCols; };
-    auto value_quad = [&](int i) { return (tid + 256 * i) / (HD / C::kValCols); };
-    auto value_col = [&](int i) { return (tid + 256 * i) % (HD / C::kValCols) * C::kValCols; };
-    struct Pages {
-        int32_t key[C::kKeys], value[C::kVals], scale;
-    };
-    auto pages_of = [&](int t0) {
-        Pages p;
-        #pragma unroll
-        for (int i = 0; i < C::kKeys; ++i) p.key[i] = table[min(t0 + min(key_row(i), kChunkTile - 1), last) >> a.page_shift];
-        #pragma unroll
-        for (int i = 0; i < C::kVals; ++i) p.value[i] = table[min(t0 + min(4 * value_quad(i), kChunkTile - 1), last) >> a.page_shift];
-        p.scale = table[min(t0 + lane, last) >> a.page_shift];
-        return p;
-    };
-    // Whether a row is there; its place in the pool (the first page's, masked,
-    // if not).
-    auto place = [&](int r, int32_t page, bool &there) {
-        there = r <= last && page >= 0 && page < a.kv.pages;
-        return (there ? page : 0) * page_stride + head_row + (r & mask);
-    };
+    // The pages of a tile's four 16 rows (past the last row: of the last), one a
+    // lane: it is read a tile ahead, and as a uniform value it would be waited for,
+    // with all loads before it, as soon as it was asked for.
+    auto pages_of = [&](int t0) { return table[min(t0 + 16 * (lane & 3), last) >> a.page_shift]; };
     struct Stage {
         uint4v key[C::kKeys];
-        uint32_t value[C::kVals][4][C::kValBytes / 4];
+        uint32_t value[4][C::kValBytes / 4];
         float scale;
-        bool there[C::kVals], scale_there;
+        uint32_t absent;   // of the 16 rows that there are, those whose page is not
     };
-    auto load = [&](Stage &g, int t0, const Pages &p) {
-        bool there;
+    auto load = [&](Stage &g, int t0, int32_t pages) {
+        int64_t at[4];
+        g.absent = 0;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int32_t page = __builtin_amdgcn_readlane(pages, i);
+            const bool there = page >= 0 && page < a.kv.pages;
+            if (!there && t0 + 16 * i <= last) g.absent |= 1u << i;
+            at[i] = (there ? page : 0) * page_stride + head_row + ((t0 + 16 * i) & mask);
+        }
+        auto row_of = [&](int i) { return i == 0 ? at[0] : i == 1 ? at[1] : i == 2 ? at[2] : at[3]; };
         #pragma unroll
         for (int i = 0; i < C::kKeys; ++i) {
-            const int64_t at = place(t0 + min(key_row(i), kChunkTile - 1), p.key[i], there);
-            g.key[i] = *reinterpret_cast<const uint4v *>(static_cast<const char *>(a.kv.key) + (at * HD + key_col(i)) * kCode);
+            const int row = tid / C::kKeyLine + i * (256 / C::kKeyLine), col = min(tid % C::kKeyLine * C::kKeyCols, HD - C::kKeyCols);
+            const char *base = static_cast<const char *>(a.kv.key) +
+                               row_of((64 * wave / C::kKeyLine + i * (256 / C::kKeyLine)) / 16) * (HD * kCode);
+            g.key[i] = *reinterpret_cast<const uint4v *>(base + ((row & 15) * HD + col) * kCode);
         }
+        const int quad = tid / 16, col = min(tid % 16 * C::kValCols, HD - C::kValCols);
+        const char *base = static_cast<const char *>(a.kv.value) + row_of(wave) * (HD * kCode);
         #pragma unroll
-        for (int i = 0; i < C::kVals; ++i) {
-            const int quad = min(value_quad(i), kChunkTile / 4 - 1);
-            // Four rows that start in a page are all in it; of them some may lie
-            // past the last, which is written page memory.
-            const int64_t at = place(t0 + 4 * quad, p.value[i], g.there[i]);
-            const char *from = static_cast<const char *>(a.kv.value) + (at * HD + value_col(i)) * kCode;
-            #pragma unroll
-            for (int r = 0; r < 4; ++r) __builtin_memcpy(g.value[i][r], from + r * HD * kCode, C::kValBytes);
-        }
-        const int64_t at = place(t0 + lane, p.scale, g.scale_there);
+        for (int r = 0; r < 4; ++r)
+            __builtin_memcpy(g.value[r], base + ((4 * (quad & 3) + r) * HD + col) * kCode, C::kValBytes);
         if constexpr (kScaled)
-            if (wave < 2) g.scale = (wave == 0 ? a.kv.value_scale : a.kv.key_scale)[at];
+            if (wave < 2) g.scale = (wave == 0 ? a.kv.value_scale : a.kv.key_scale)[row_of(tid >> 4 & 3) + (tid & 15)];
     };
     int top_ev = -126;   // wave 0's: the exponent of the largest value scale so far
     auto store = [&](const Stage &g, int t0, char *buf) {
         auto &head = *reinterpret_cast<typename C::Head *>(buf + C::kKeyBytes + C::kValueBytes);
-        if (wave == 0) {
-            const uint64_t absent = __builtin_amdgcn_ballot_w64(!g.scale_there);
-            if constexpr (kScaled) {
+        const bool edge = t0 + kChunkTile - 1 > seen;
+        if constexpr (kScaled) {
+            if (wave == 0) {
                 // A row that some token does not see meets it as 0 * value: what
                 // is not finite counts as 0 there, and is flagged.
-                const bool bad = g.scale_there && !isfinite(g.scale) && t0 + kChunkTile - 1 > seen;
+                const bool there = t0 + lane <= last && !(g.absent >> (lane >> 4) & 1);
+                const bool bad = there && edge && !isfinite(g.scale);
                 const uint64_t all_bad = __builtin_amdgcn_ballot_w64(bad);
                 if (lane < 2 && all_bad) atomicOr(&head.bad[lane], static_cast<uint32_t>(all_bad >> (32 * lane)));
-                const float v = g.scale_there && !bad ? g.scale : 0.f;
+                const float v = there && !bad ? g.scale : 0.f;
                 float top = v;
                 #pragma unroll
                 for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
                 top_ev = max(top_ev, top > 0.f ? __builtin_amdgcn_frexp_expf(top) : -126);
                 head.vs[lane] = ldexpf(v, 14 - top_ev);
+                if (lane == 0) head.ev = top_ev;
+            } else if (wave == 1) {
+                head.ks[lane] = g.scale;
             }
-            if (lane == 0) {
-                head.absent = absent;
-                head.ev = top_ev;
-            }
-        } else if (wave == 1) {
-            if constexpr (kScaled) head.ks[lane] = g.scale;
         }
         #pragma unroll
         for (int i = 0; i < C::kKeys; ++i) {
-            if (C::kKeyTasks % 256 && tid + 256 * i >= C::kKeyTasks) continue;
-            char *at = buf + key_row(i) * C::kKeyStride + key_col(i) * 2;
+            const int row = tid / C::kKeyLine + i * (256 / C::kKeyLine), col = tid % C::kKeyLine * C::kKeyCols;
+            if (HD != C::kWidth && col >= HD) continue;
+            char *at = buf + row * C::kKeyStride + col * 2;
             if constexpr (TYPE == QK_TYPE_F16) {
                 *reinterpret_cast<uint4v *>(at) = g.key[i];
             } else {
@@ -646,65 +633,72 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
                 *reinterpret_cast<half8 *>(at + 16) = join(c[4], c[5], c[6], c[7]);
             }
         }
-        const bool edge = TYPE != QK_TYPE_I8 && t0 + kChunkTile - 1 > seen;
+        const int quad = tid / 16, col = tid % 16 * C::kValCols;
+        if (HD != C::kWidth && col >= HD) return;
+        const int piece = quad / 4 * 2 + (quad & 1), half = quad >> 1 & 1;
+        const int exchanged = (piece ^ C::exchange(col)) << 4;
+        char *const at = buf + C::kKeyBytes + col * 2 * kChunkTile + 8 * half;
+        uint2 w[C::kValCols];   // of a dimension: rows 0 and 1, rows 2 and 3
         #pragma unroll
-        for (int i = 0; i < C::kVals; ++i) {
-            if (C::kValTasks % 256 && tid + 256 * i >= C::kValTasks) continue;
-            const int quad = value_quad(i), piece = quad / 4 * 2 + (quad & 1), half = quad >> 1 & 1;
-            uint32_t bad = 0;
-            #pragma unroll
-            for (int d4 = 0; d4 < C::kValCols / 4; ++d4) {
-                half2v p[4][2];   // of four dimensions: rows 0 and 1, rows 2 and 3
-                if constexpr (TYPE == QK_TYPE_F16) {
-                    #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        #pragma unroll
-                        for (int k = 0; k < 2; ++k)
-                            p[c][k] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(g.value[i][2 * k + 1][2 * d4 + c / 2],
-                                                                                       g.value[i][2 * k][2 * d4 + c / 2],
-                                                                                       c & 1 ? 0x07060302u : 0x05040100u));
-                } else {
-                    #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const uint32_t x = g.value[i][2 * k][d4], y = g.value[i][2 * k + 1][d4];
-                        codes4<TYPE>(__builtin_amdgcn_perm(y, x, 0x05010400u), p[0][k], p[1][k]);
-                        codes4<TYPE>(__builtin_amdgcn_perm(y, x, 0x07030602u), p[2][k], p[3][k]);
-                    }
-                }
+        for (int d4 = 0; d4 < C::kValCols / 4; ++d4) {
+            half2v p[4][2];
+            if constexpr (TYPE == QK_TYPE_F16) {
                 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t w[2] = {__builtin_bit_cast(uint32_t, p[c][0]), __builtin_bit_cast(uint32_t, p[c][1])};
-                    if (TYPE != QK_TYPE_I8 && !g.there[i]) w[0] = w[1] = 0;
-                    if (edge) {
-                        #pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            if ((w[k] & 0x7C00u) == 0x7C00u) w[k] &= 0xFFFF0000u, bad |= 1u << (2 * k);
-                            if ((w[k] & 0x7C000000u) == 0x7C000000u) w[k] &= 0xFFFFu, bad |= 2u << (2 * k);
-                        }
-                    }
-                    const int d = value_col(i) + 4 * d4 + c;
-                    *reinterpret_cast<uint2 *>(buf + C::kKeyBytes + C::value_at(d, piece) + 8 * half) = make_uint2(w[0], w[1]);
+                for (int c = 0; c < 4; ++c)
+                    #pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        p[c][k] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(g.value[2 * k + 1][2 * d4 + c / 2],
+                                                                                   g.value[2 * k][2 * d4 + c / 2],
+                                                                                   c & 1 ? 0x07060302u : 0x05040100u));
+            } else {
+                #pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t x = g.value[2 * k][d4], y = g.value[2 * k + 1][d4];
+                    codes4<TYPE>(__builtin_amdgcn_perm(y, x, 0x05010400u), p[0][k], p[1][k]);
+                    codes4<TYPE>(__builtin_amdgcn_perm(y, x, 0x07030602u), p[2][k], p[3][k]);
                 }
             }
-            if (edge && bad) atomicOr(&head.bad[quad / 8], bad << (4 * quad % 32));
+            #pragma unroll
+            for (int c = 0; c < 4; ++c)
+                w[4 * d4 + c] = make_uint2(__builtin_bit_cast(uint32_t, p[c][0]), __builtin_bit_cast(uint32_t, p[c][1]));
         }
+        const bool gone = g.absent >> wave & 1;
+        if (TYPE != QK_TYPE_I8 && (edge || gone)) {
+            uint32_t bad = 0;
+            #pragma unroll
+            for (int d = 0; d < C::kValCols; ++d) {
+                if ((w[d].x & 0x7C00u) == 0x7C00u) w[d].x &= 0xFFFF0000u, bad |= 1u;
+                if ((w[d].x & 0x7C000000u) == 0x7C000000u) w[d].x &= 0xFFFFu, bad |= 2u;
+                if ((w[d].y & 0x7C00u) == 0x7C00u) w[d].y &= 0xFFFF0000u, bad |= 4u;
+                if ((w[d].y & 0x7C000000u) == 0x7C000000u) w[d].y &= 0xFFFFu, bad |= 8u;
+            }
+            if (bad && !gone) atomicOr(&head.bad[quad / 8], bad << (4 * quad % 32));
+        }
+        #pragma unroll
+        for (int d = 0; d < C::kValCols; ++d)
+            *reinterpret_cast<uint2 *>(at + (exchanged ^ (d << 4)) + d * 2 * kChunkTile) = w[d];
     };
 
     // ------------------------------------------------------- queries -----
     half8 qh[NS], ql[NS];
     float qscale;
     {
-        const float *qrow = a.q + (s.first + tok) * a.ldq + static_cast<int64_t>(h * G + row % G) * HD + 8 * hi;
+        const int at = min(row, rows - 1);
+        const float *qrow = a.q + (s.first + at / G) * a.ldq + static_cast<int64_t>(h * G + at % G) * HD + 8 * hi;
+        float4 v[NS][2];
         float top = 0.f;
         int fin = 1;
         #pragma unroll
         for (int x = 0; x < NS; ++x)
             #pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (have) v = *reinterpret_cast<const float4 *>(qrow + 16 * x + e);
-                top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
-                fin &= isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w);
+            for (int k = 0; k < 2; ++k) v[x][k] = *reinterpret_cast<const float4 *>(qrow + 16 * x + 4 * k);
+        #pragma unroll
+        for (int x = 0; x < NS; ++x)
+            #pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const float4 y = v[x][k];
+                top = fmaxf(fmaxf(top, fmaxf(fabsf(y.x), fabsf(y.y))), fmaxf(fabsf(y.z), fabsf(y.w)));
+                fin &= isfinite(y.x) && isfinite(y.y) && isfinite(y.z) && isfinite(y.w);
             }
         top = fmaxf(top, __shfl_xor(top, 32));
         fin &= __shfl_xor(fin, 32);
@@ -718,10 +712,9 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
             half2v u[4], w[4];
             #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (have && fin) v = *reinterpret_cast<const float4 *>(qrow + 16 * x + 4 * k);
-                split_pair(ldexpf(sign * v.x, e), ldexpf(sign * v.y, e), u[2 * k], w[2 * k]);
-                split_pair(ldexpf(sign * v.z, e), ldexpf(sign * v.w, e), u[2 * k + 1], w[2 * k + 1]);
+                const float4 y = have && fin ? v[x][k] : make_float4(0.f, 0.f, 0.f, 0.f);
+                split_pair(ldexpf(sign * y.x, e), ldexpf(sign * y.y, e), u[2 * k], w[2 * k]);
+                split_pair(ldexpf(sign * y.z, e), ldexpf(sign * y.w, e), u[2 * k + 1], w[2 * k + 1]);
             }
             qh[x] = join(u[0], u[1], u[2], u[3]);
             ql[x] = join(w[0], w[1], w[2], w[3]);
@@ -737,23 +730,25 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
     float m = -INFINITY, c = INFINITY, l = 0.f;
     int ev = -126;
 
-    auto take = [&](const char *buf, int t0) {
+    auto take = [&](const char *buf, int t0, uint32_t absent) {
         const auto &head = *reinterpret_cast<const typename C::Head *>(buf + C::kKeyBytes + C::kValueBytes);
         const int en = kScaled ? __builtin_amdgcn_readfirstlane(head.ev) : ev;
-        const bool edge = t0 + kChunkTile - 1 > wave_seen || head.absent;   // some token does not see it whole
+        const bool edge = t0 + kChunkTile - 1 > wave_seen || absent;   // some token does not see it whole
         // Half a tile at a time: 32 scores a lane left too few registers.
         #pragma unroll 1
         for (int hf = 0; hf < 2; ++hf) {
-            float16v st;
+            float16v st, lo;   // two chains: a product's result is ready for the next but one
             #pragma unroll
-            for (int r = 0; r < 16; ++r) st[r] = 0.f;
+            for (int r = 0; r < 16; ++r) st[r] = lo[r] = 0.f;
             const char *keys = buf + (32 * hf + n) * C::kKeyStride + 16 * hi;
             #pragma unroll
             for (int x = 0; x < NS; ++x) {
                 const half8 k = *reinterpret_cast<const half8 *>(keys + 32 * x);
-                st = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[x], st, 0, 0, 0);
+                lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[x], lo, 0, 0, 0);
                 st = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[x], st, 0, 0, 0);
             }
+            #pragma unroll
+            for (int r = 0; r < 16; ++r) st[r] += lo[r];
             // Register r: row t0 + 32 hf + 8 (r / 4) + 4 hi + r % 4.
             #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
@@ -768,7 +763,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
                 }
             }
             if (edge) {
-                const uint32_t hide = static_cast<uint32_t>(head.absent >> (32 * hf)) >> (4 * hi);
+                const uint32_t two = absent >> (2 * hf), hide = ((two & 1 ? 0xFFFFu : 0) | (two & 2 ? 0xFFFF0000u : 0)) >> (4 * hi);
                 const int left = mine - t0 - 32 * hf - 4 * hi;
                 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
@@ -826,19 +821,22 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
                     split_pair(y[2], y[3], pu[2 * r4 + 1], pw[2 * r4 + 1]);
                 }
                 const half8 ph = join(pu[0], pu[1], pu[2], pu[3]), pl = join(pw[0], pw[1], pw[2], pw[3]);
+                half8 v[ND];
                 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
-                    const half8 v = *reinterpret_cast<const half8 *>(values + C::value_at(32 * d + n, 4 * hf + 2 * b + hi));
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[d], 0, 0, 0);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[d], 0, 0, 0);
+                    v[d] = *reinterpret_cast<const half8 *>(
+                        values + (32 * d + n) * 2 * kChunkTile + (((4 * hf + 2 * b + hi) ^ C::exchange(32 * d + n)) << 4));
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], pl, o[d], 0, 0, 0);
                 }
+                #pragma unroll
+                for (int d = 0; d < ND; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], ph, o[d], 0, 0, 0);
             }
         }
     };
 
     Stage g;
     load(g, begin, pages_of(begin));
-    Pages ahead = pages_of(begin + kChunkTile);
+    int32_t ahead = pages_of(begin + kChunkTile);
     int b = 0;
     for (int t0 = begin; t0 < end; t0 += kChunkTile, b ^= 1) {
         char *buf = lds + b * C::kBuffer;
@@ -849,12 +847,13 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
             __syncthreads();
         }
         store(g, t0, buf);
+        const uint32_t absent = g.absent;
         __syncthreads();   // the tile is in; every wave is done with the one before
         if (t0 + kChunkTile < end) {
             load(g, t0 + kChunkTile, ahead);
             ahead = pages_of(t0 + 2 * kChunkTile);
         }
-        if (t0 <= wave_last) take(buf, t0);
+        if (t0 <= wave_last) take(buf, t0, absent);
     }
     l += __shfl_xor(l, 32);
     if (!have) return;
