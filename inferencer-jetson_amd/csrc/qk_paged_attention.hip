@@ -202,6 +202,36 @@ __device__ __forceinline__ void split_pair(float x, float y, half2v &hi, half2v 
                 static_cast<_Float16>(fmaf(static_cast<float>(hi[1]), minus, y))};
 }
 
+// The largest of three, without the steps that make a signalling NaN quiet first
+// (results of arithmetic are quiet already); NaN only of three.  The compiler does
+// not see that a vector instruction wrote the result: one that it does see has to
+// come between this and a lane exchange, which needs wait states behind it.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
+}
+
+// Both halves' maximum, of a lane and the one 32 from it.
+__device__ __forceinline__ float max_halves(float v) {
+    const uint32_t bits = __builtin_bit_cast(uint32_t, v);
+    const auto both = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
+    const uint32_t low = both[0], high = both[1];
+    return fmaxf(__builtin_bit_cast(float, low), __builtin_bit_cast(float, high));
+}
+
+// A wave's largest value, none below 0, in every lane.
+__device__ __forceinline__ float wave_max(float v) {
+    int bits = __builtin_bit_cast(int, v);   // ordered as the values are
+    bits = max(bits, __builtin_amdgcn_update_dpp(0, bits, 0x111, 0xF, 0xF, false));   // row_shr 1, 2, 4, 8
+    bits = max(bits, __builtin_amdgcn_update_dpp(0, bits, 0x112, 0xF, 0xF, false));
+    bits = max(bits, __builtin_amdgcn_update_dpp(0, bits, 0x114, 0xF, 0xF, false));
+    bits = max(bits, __builtin_amdgcn_update_dpp(0, bits, 0x118, 0xF, 0xF, false));
+    bits = max(bits, __builtin_amdgcn_update_dpp(0, bits, 0x142, 0xA, 0xF, false));   // row_bcast 15 into rows 1 and 3
+    bits = max(bits, __builtin_amdgcn_update_dpp(0, bits, 0x143, 0xC, 0xF, false));   // row_bcast 31 into rows 2 and 3
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(bits, 63));
+}
+
 // A workgroup: 16 query rows of one (sequence, KV head) over a split's rows,
 // its four waves every fourth tile of 32 rows each; the waves' states meet in
 // LDS.
@@ -357,7 +387,7 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttn a) {
             #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 mx = fmaxf(mx, st[hf][r]);
-                if constexpr (kScaled) vtop = fmaxf(vtop, t.vs[hf][r]);
+                if constexpr (kScaled) vtop = fmaxf(vtop, fabsf(t.vs[hf][r]));
             }
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
@@ -524,7 +554,6 @@ struct Chunk {
 };
 
 typedef float float16v __attribute__((ext_vector_type(16)));
-typedef _Float16 half4v __attribute__((ext_vector_type(4)));
 
 template <int HD, int TYPE>
 __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
@@ -559,10 +588,10 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
     // Renewed every tile: what follows from it is then computed anew, instead of
     // kept in registers through the loop (30 of them, which spilled).
     int tid = threadIdx.x;
-    // The pages of a tile's four 16 rows (past the last row: of the last), one a
-    // lane: it is read a tile ahead, and as a uniform value it would be waited for,
-    // with all loads before it, as soon as it was asked for.
-    auto pages_of = [&](int t0) { return table[min(t0 + 16 * (lane & 3), last) >> a.page_shift]; };
+    // The page of each lane's row of a tile, 16 rows of one page (past the last
+    // row: of the last): it is read a tile ahead, and as uniform values the four
+    // would be waited for, with all loads before them, as soon as asked for.
+    auto pages_of = [&](int t0) { return table[min(t0 + (lane & 48), last) >> a.page_shift]; };
     struct Stage {
         uint4v key[C::kKeys];
         uint32_t value[4][C::kValBytes / 4];
@@ -570,16 +599,15 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
         uint32_t absent;   // of the 16 rows that there are, those whose page is not
     };
     auto load = [&](Stage &g, int t0, int32_t pages) {
-        int64_t at[4];
-        g.absent = 0;
-        #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int32_t page = __builtin_amdgcn_readlane(pages, i);
-            const bool there = page >= 0 && page < a.kv.pages;
-            if (!there && t0 + 16 * i <= last) g.absent |= 1u << i;
-            at[i] = (there ? page : 0) * page_stride + head_row + ((t0 + 16 * i) & mask);
-        }
-        auto row_of = [&](int i) { return i == 0 ? at[0] : i == 1 ? at[1] : i == 2 ? at[2] : at[3]; };
+        const bool there = pages >= 0 && pages < a.kv.pages;
+        const int group = t0 + (lane & 48);
+        const uint64_t gone = __builtin_amdgcn_ballot_w64(!there && group <= last);
+        g.absent = (gone & 1) | (gone >> 15 & 2) | (gone >> 30 & 4) | (gone >> 45 & 8);
+        const int page = there ? pages : 0;
+        // First row of 16 rows i, a uniform number.
+        auto row_of = [&](int i) {
+            return __builtin_amdgcn_readlane(page, 16 * i) * page_stride + head_row + ((t0 + 16 * i) & mask);
+        };
         #pragma unroll
         for (int i = 0; i < C::kKeys; ++i) {
             const int row = tid / C::kKeyLine + i * (256 / C::kKeyLine), col = min(tid % C::kKeyLine * C::kKeyCols, HD - C::kKeyCols);
@@ -593,7 +621,8 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
         for (int r = 0; r < 4; ++r)
             __builtin_memcpy(g.value[r], base + ((4 * (quad & 3) + r) * HD + col) * kCode, C::kValBytes);
         if constexpr (kScaled)
-            if (wave < 2) g.scale = (wave == 0 ? a.kv.value_scale : a.kv.key_scale)[row_of(tid >> 4 & 3) + (tid & 15)];
+            if (wave < 2)
+                g.scale = (wave == 0 ? a.kv.value_scale : a.kv.key_scale)[page * page_stride + head_row + (group & mask) + (tid & 15)];
     };
     int top_ev = -126;   // wave 0's: the exponent of the largest value scale so far
     auto store = [&](const Stage &g, int t0, char *buf) {
@@ -608,9 +637,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
                 const uint64_t all_bad = __builtin_amdgcn_ballot_w64(bad);
                 if (lane < 2 && all_bad) atomicOr(&head.bad[lane], static_cast<uint32_t>(all_bad >> (32 * lane)));
                 const float v = there && !bad ? g.scale : 0.f;
-                float top = v;
-                #pragma unroll
-                for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+                const float top = wave_max(fabsf(v));
                 top_ev = max(top_ev, top > 0.f ? __builtin_amdgcn_frexp_expf(top) : -126);
                 head.vs[lane] = ldexpf(v, 14 - top_ev);
                 if (lane == 0) head.ev = top_ev;
@@ -737,18 +764,16 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
         // Half a tile at a time: 32 scores a lane left too few registers.
         #pragma unroll 1
         for (int hf = 0; hf < 2; ++hf) {
-            float16v st, lo;   // two chains: a product's result is ready for the next but one
+            float16v st;
             #pragma unroll
-            for (int r = 0; r < 16; ++r) st[r] = lo[r] = 0.f;
+            for (int r = 0; r < 16; ++r) st[r] = 0.f;
             const char *keys = buf + (32 * hf + n) * C::kKeyStride + 16 * hi;
             #pragma unroll
             for (int x = 0; x < NS; ++x) {
                 const half8 k = *reinterpret_cast<const half8 *>(keys + 32 * x);
-                lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[x], lo, 0, 0, 0);
+                st = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[x], st, 0, 0, 0);
                 st = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[x], st, 0, 0, 0);
             }
-            #pragma unroll
-            for (int r = 0; r < 16; ++r) st[r] += lo[r];
             // Register r: row t0 + 32 hf + 8 (r / 4) + 4 hi + r % 4.
             #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
@@ -771,12 +796,10 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
                     st[r] = at <= left && !(hide >> at & 1) ? st[r] : -INFINITY;
                 }
             }
-            float mx = fmaxf(fmaxf(st[0], st[1]), st[2]);
+            float mn = m;
             #pragma unroll
-            for (int r = 3; r < 15; r += 2) mx = fmaxf(mx, fmaxf(st[r], st[r + 1]));
-            mx = fmaxf(mx, st[15]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float mn = fmaxf(m, mx);
+            for (int r = 0; r < 14; r += 2) mn = max3(mn, st[r], st[r + 1]);
+            mn = max_halves(fmaxf(fmaxf(mn, st[14]), st[15]));
             if (en != ev || __builtin_amdgcn_ballot_w64(mn > m)) {
                 // c is what the weights so far were taken with, rounding and all.
                 const float cn = mn == -INFINITY ? INFINITY : -mn * qscale;
