@@ -36,7 +36,7 @@ struct PagedAttn {
     const float *q;
     float *out, *parts;
     int64_t ldq, ldout;
-    int heads, page_shift;
+    int heads, group, page_shift;   // group: query heads a KV head
     // Splits of the rows of a sequence of few query rows a KV head and of one of
     // many (more than few_rows, which the chunk kernel takes).
     int splits[2], split_rows[2], part_splits;
@@ -232,6 +232,19 @@ __device__ __forceinline__ float wave_max(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(bits, 63));
 }
 
+// |v| as an integer, ordered as the values are, infinity and NaN above them.
+__device__ __forceinline__ int magnitude(float v) { return __builtin_bit_cast(int, v) & 0x7FFFFFFF; }
+
+// What a query row of largest magnitude top is multiplied by (a power of two that
+// brings that below 2^14) and what its scores are.  All scores of a row that is
+// not finite are not numbers.
+__device__ __forceinline__ void query_units(int top, float scale, float &factor, float &qscale) {
+    const int e = top > 0 ? min(14 - __builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, top)), 126) : 0;
+    const bool fin = top < 0x7F800000;
+    factor = fin ? ldexpf(1.f, e) : __builtin_nanf("");
+    qscale = fin ? ldexpf(scale, -e) : 1.f;
+}
+
 // A workgroup: 16 query rows of one (sequence, KV head) over a split's rows,
 // its four waves every fourth tile of 32 rows each; the waves' states meet in
 // LDS.
@@ -242,7 +255,7 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttn a) {
     __shared__ float meet[3][HD * 16 + 64];
     const qk_paged_seq s = a.b.seqs[blockIdx.y];
     if (!paged_seq_ok(s, a.b, a.page_shift)) return;
-    const int kvh = a.kv.kv_heads, G = a.heads / kvh;
+    const int kvh = a.kv.kv_heads, G = a.group;
     // A chip's XCDs take workgroups in turn: the splits rotate, or the first ones
     // (which every sequence has) would all fall to the same XCDs.
     const int splits = a.splits[0], unit = blockIdx.x / splits, split = (blockIdx.x + unit + blockIdx.y) % splits;
@@ -253,11 +266,12 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttn a) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
     // This lane's query row, the last row it sees, and the rows the tile sees.
-    const int row = row0 + n, tok = row / G;
+    // (Past the last row: that one again, masked and not written.)
+    const int row = row0 + n, tok = min(row, rows - 1) / G, own = min(row, rows - 1) - tok * G;
     const bool have = row < rows;
     const int mine = have ? s.pos + tok : -1;
-    const int last = s.pos + min(row0 + kRowTile - 1, rows - 1) / G;   // of the tile's last token
-    const int seen = s.pos + row0 / G;                                // of its first
+    const int last = s.pos + __builtin_amdgcn_readlane(tok, 15);   // of the tile's last token
+    const int seen = s.pos + __builtin_amdgcn_readlane(tok, 0);    // of its first
     const int64_t begin64 = static_cast<int64_t>(split) * a.split_rows[0];
     if (begin64 > last) return;   // the merge takes the splits that reach a token
     const int begin = static_cast<int>(begin64), end = static_cast<int>(min(begin64 + a.split_rows[0], int64_t(last) + 1));
@@ -265,11 +279,8 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttn a) {
     half8 qh[NS], ql[NS];
     float qscale;
     {
-        // (The last row again past it: a load under a condition is one at a time.)
-        const int at = min(row, rows - 1);
-        const float *qrow = a.q + (s.first + at / G) * a.ldq + static_cast<int64_t>(h * G + at % G) * HD;
-        float v[NS][8], top = 0.f;
-        bool finite = true;
+        const float *qrow = a.q + (s.first + tok) * a.ldq + static_cast<int64_t>(h * G + own) * HD;
+        float v[NS][8];
         #pragma unroll
         for (int st = 0; st < NS; ++st)
             #pragma unroll
@@ -277,27 +288,21 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttn a) {
                 const float4 x = *reinterpret_cast<const float4 *>(qrow + key_dim<HD, TYPE>(st, g) + e);
                 v[st][e] = x.x, v[st][e + 1] = x.y, v[st][e + 2] = x.z, v[st][e + 3] = x.w;
             }
+        int top = 0;
         #pragma unroll
         for (int st = 0; st < NS; ++st)
             #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                v[st][k] = have ? v[st][k] : 0.f;
-                top = fmaxf(top, fabsf(v[st][k]));
-                finite = finite && isfinite(v[st][k]);
-            }
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        int fin = finite;
-        fin &= __shfl_xor(fin, 16);
-        fin &= __shfl_xor(fin, 32);
-        const int e = fin && top > 0.f ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
-        qscale = fin ? ldexpf(a.scale, -e) : __builtin_nanf("");
+            for (int k = 0; k < 8; ++k) top = max(top, magnitude(v[st][k]));
+        top = max(top, __shfl_xor(top, 16));
+        top = max(top, __shfl_xor(top, 32));
+        float factor;
+        query_units(top, a.scale, factor, qscale);
         #pragma unroll
         for (int st = 0; st < NS; ++st) {
             half2v u[4], w[4];
             #pragma unroll
             for (int k = 0; k < 4; ++k)
-                split_pair(fin ? ldexpf(v[st][2 * k], e) : 0.f, fin ? ldexpf(v[st][2 * k + 1], e) : 0.f, u[k], w[k]);
+                split_pair(factor * v[st][2 * k], factor * v[st][2 * k + 1], u[k], w[k]);
             qh[st] = join(u[0], u[1], u[2], u[3]);
             ql[st] = join(w[0], w[1], w[2], w[3]);
         }
@@ -501,7 +506,7 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttn a) {
         }
     }
     if (!have) return;
-    const int head = h * G + row % G;
+    const int head = h * G + own;
     float *dst;
     float norm = 1.f;
     if (splits > 1) {
@@ -563,7 +568,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
     extern __shared__ __align__(16) char lds[];
     const qk_paged_seq s = a.b.seqs[blockIdx.y];
     if (!paged_seq_ok(s, a.b, a.page_shift)) return;
-    const int kvh = a.kv.kv_heads, G = a.heads / kvh;
+    const int kvh = a.kv.kv_heads, G = a.group;
     const int splits = a.splits[1], unit = blockIdx.x / splits, split = (blockIdx.x + unit + blockIdx.y) % splits;
     const int rows = s.count * G, tiles = (rows + kChunkRows - 1) / kChunkRows;
     if (unit / kvh >= tiles || rows <= a.few_rows) return;
@@ -576,10 +581,12 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
     if (begin64 > last) return;
     const int begin = static_cast<int>(begin64), end = static_cast<int>(min(begin64 + a.split_rows[1], int64_t(last) + 1));
 
-    const int wrow = row0 + 32 * wave, row = wrow + n, tok = row / G;
+    // Of a row past the last one: that one again, masked and not written.
+    const int wrow = row0 + 32 * wave, row = wrow + n, tok = min(row, rows - 1) / G, own = min(row, rows - 1) - tok * G;
     const bool have = row < rows;
     const int mine = have ? s.pos + tok : -1;
-    const int wave_seen = s.pos + wrow / G, wave_last = wrow < rows ? s.pos + min(wrow + 31, rows - 1) / G : -1;
+    const int wave_seen = s.pos + __builtin_amdgcn_readlane(tok, 0);
+    const int wave_last = wrow < rows ? s.pos + __builtin_amdgcn_readlane(tok, 31) : -1;
 
     // ------------------------------------------------------ staging ------
     const int32_t *table = a.b.page_table + static_cast<int64_t>(s.table) * a.b.table_stride;
@@ -710,38 +717,35 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
     half8 qh[NS], ql[NS];
     float qscale;
     {
-        const int at = min(row, rows - 1);
-        const float *qrow = a.q + (s.first + at / G) * a.ldq + static_cast<int64_t>(h * G + at % G) * HD + 8 * hi;
+        const float *qrow = a.q + (s.first + tok) * a.ldq + static_cast<int64_t>(h * G + own) * HD + 8 * hi;
         float4 v[NS][2];
-        float top = 0.f;
-        int fin = 1;
         #pragma unroll
         for (int x = 0; x < NS; ++x)
             #pragma unroll
             for (int k = 0; k < 2; ++k) v[x][k] = *reinterpret_cast<const float4 *>(qrow + 16 * x + 4 * k);
+        int top = 0;
         #pragma unroll
         for (int x = 0; x < NS; ++x)
             #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const float4 y = v[x][k];
-                top = fmaxf(fmaxf(top, fmaxf(fabsf(y.x), fabsf(y.y))), fmaxf(fabsf(y.z), fabsf(y.w)));
-                fin &= isfinite(y.x) && isfinite(y.y) && isfinite(y.z) && isfinite(y.w);
+                top = max(max(top, max(magnitude(y.x), magnitude(y.y))), max(magnitude(y.z), magnitude(y.w)));
             }
-        top = fmaxf(top, __shfl_xor(top, 32));
-        fin &= __shfl_xor(fin, 32);
-        const int e = fin && top > 0.f ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
-        // Scores in units of 2^-e; one that underflows is as good as 2^-126.
-        qscale = ldexpf(fabsf(a.scale), -e);
-        qscale = fin ? (qscale < 0x1p-126f ? 0x1p-126f : qscale) : __builtin_nanf("");
-        const float sign = a.scale < 0.f ? -1.f : 1.f;
+        top = max(top, __shfl_xor(top, 32));
+        // The running maximum is one of the products, whose order a negative scale
+        // would turn: its sign goes to the queries.
+        float factor;
+        query_units(top, fabsf(a.scale), factor, qscale);
+        qscale = fmaxf(qscale, 0x1p-126f);   // one that underflows is as good as 2^-126
+        factor = a.scale < 0.f ? -factor : factor;
         #pragma unroll
         for (int x = 0; x < NS; ++x) {
             half2v u[4], w[4];
             #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const float4 y = have && fin ? v[x][k] : make_float4(0.f, 0.f, 0.f, 0.f);
-                split_pair(ldexpf(sign * y.x, e), ldexpf(sign * y.y, e), u[2 * k], w[2 * k]);
-                split_pair(ldexpf(sign * y.z, e), ldexpf(sign * y.w, e), u[2 * k + 1], w[2 * k + 1]);
+                const float4 y = v[x][k];
+                split_pair(factor * y.x, factor * y.y, u[2 * k], w[2 * k]);
+                split_pair(factor * y.z, factor * y.w, u[2 * k + 1], w[2 * k + 1]);
             }
             qh[x] = join(u[0], u[1], u[2], u[3]);
             ql[x] = join(w[0], w[1], w[2], w[3]);
@@ -880,7 +884,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
     }
     l += __shfl_xor(l, 32);
     if (!have) return;
-    const int head = h * G + row % G;
+    const int head = h * G + own;
     const bool none = m == -INFINITY && l == 0.f;
     float *dst;
     float norm = kScaled ? ldexpf(1.f, ev - 14) : 0x1p-14f;
@@ -912,7 +916,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
     const int tok = static_cast<int>(at / a.heads), head = static_cast<int>(at % a.heads);
     // As the kernel's: a tile's splits go to its last token's last row, and
     // those beyond this token's own hold nothing of it.
-    const int many = static_cast<int64_t>(s.count) * (a.heads / a.kv.kv_heads) > a.few_rows;
+    const int many = static_cast<int64_t>(s.count) * a.group > a.few_rows;
     if (a.splits[many] == 1) return;
     const int live = min(a.splits[many], (s.pos + tok) / a.split_rows[many] + 1);
     const float *p = a.parts + (static_cast<int64_t>(s.first + tok) * a.heads + head) * a.part_splits * part_floats(HD);
@@ -935,35 +939,47 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
         if (d * 64 + lane < HD) out[d * 64 + lane] = o[d] * norm;
 }
 
-// A sequence of more query rows a KV head than this takes the chunk kernel.
+// A sequence of more query rows a KV head than this takes the chunk kernel, if the
+// call has at least so many pairs of a query row and a cache row.
 constexpr int kFewRows = 64;
+constexpr int64_t kFewPairs = 3 << 19;
 // The chunk kernel's queries and sums of a head fit the registers up to here
 // (at 256 it spilled 58 and more).
 constexpr int kChunkDim = 128;
 
-// Splits of a call's rows.  Few query rows: some 8 workgroups a CU, so that
-// sequences of different lengths even out, of at least 512 rows each while there
-// are enough of them to go round, at least one tile a wave.  Chunks: two
-// workgroups a CU of at least four tiles.
-struct Splits {
-    int few, many;
-};
 // Query rows a KV head up to which a sequence of this call takes the first
 // kernel: one sequence has the chunk kernel alone, if its bound calls for it.
 int few_rows(const qk_paged_batch &b, int heads, int kv_heads, int head_dim) {
-    if (head_dim > kChunkDim || static_cast<int64_t>(b.max_count) * (heads / kv_heads) <= kFewRows) return INT32_MAX;
+    if (head_dim > kChunkDim || static_cast<int64_t>(b.max_count) * (heads / kv_heads) <= kFewRows ||
+        static_cast<double>(b.n_tokens) * heads * b.max_rows < kFewPairs)
+        return INT32_MAX;
     return b.n_seqs == 1 ? 0 : kFewRows;
 }
+
+// Splits of a call's rows.  Few query rows: some 8 workgroups a CU, so that
+// sequences of different lengths even out, of at least 512 rows each while there
+// are enough of them to go round, at least one tile a wave.  Chunks: two
+// workgroups a CU, all at once, of at least four tiles; those that lie behind
+// all that a chunk's first tokens see end at once and do not count.
+struct Splits {
+    int few, many;
+};
 Splits wanted_splits(const qk_paged_batch &b, int heads, int kv_heads, int head_dim) {
     const int64_t few = few_rows(b, heads, kv_heads, head_dim), rows = static_cast<int64_t>(b.max_count) * (heads / kv_heads);
     const int64_t per_tile = static_cast<int64_t>(kv_heads) * b.n_seqs;
-    auto fit = [&](int64_t query_rows, int tile, int64_t want, int64_t least) {
-        const int64_t units = std::max<int64_t>((query_rows + tile - 1) / tile * per_tile, 1);
-        if (least == 0) least = units * b.max_rows >= 512 * 1024 ? 512 : 4 * kTile;
-        return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want / units, (b.max_rows + least - 1) / least, 64})));
-    };
-    return {few > 0 ? fit(std::min(rows, few), kRowTile, 2048, 0) : 1,
-            rows > few ? fit(rows, kChunkRows, 512, 4 * kChunkTile) : 1};
+    Splits splits{1, 1};
+    if (few > 0) {
+        const int64_t units = std::max<int64_t>((std::min(rows, few) + kRowTile - 1) / kRowTile * per_tile, 1);
+        const int64_t least = units * b.max_rows >= 512 * 1024 ? 512 : 4 * kTile;
+        splits.few = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({2048 / units, (b.max_rows + least - 1) / least, 64})));
+    }
+    if (rows > few) {
+        const int64_t units = (rows + kChunkRows - 1) / kChunkRows * per_tile;
+        const double mean = b.max_rows - 0.5 * std::min(b.max_count, b.max_rows);
+        auto live = [&](int n) { return units * std::min<double>(n, mean * n / b.max_rows + 0.5); };
+        while (splits.many < 64 && live(splits.many + 1) <= 512 && b.max_rows > splits.many * 4 * kChunkTile) ++splits.many;
+    }
+    return splits;
 }
 
 size_t split_bytes(const qk_paged_batch &b, int heads, int hd) {
@@ -1042,6 +1058,7 @@ int qk_paged_attention_f32(const qk_paged_kv *kv, const qk_paged_batch *batch, c
     a.ldq = ldq;
     a.ldout = ldout;
     a.heads = heads;
+    a.group = heads / kv->kv_heads;
     a.page_shift = __builtin_ctz(kv->page_rows);
     a.scale = 1.4426950408889634f * (scale != 0.f ? scale : 1.f / std::sqrt(static_cast<float>(kv->head_dim)));
     const size_t per = qk::split_bytes(*batch, heads, kv->head_dim);
