@@ -220,16 +220,24 @@ __device__ __forceinline__ float max_halves(float v) {
     return fmaxf(__builtin_bit_cast(float, low), __builtin_bit_cast(float, high));
 }
 
-// A wave's largest value, none below 0, in every lane.
+// A wave's values joined by op, `none` for a lane without one; in every lane.
+template <typename Op>
+__device__ __forceinline__ float wave_join(float v, float none, Op op) {
+    const int fill = __builtin_bit_cast(int, none);
+    auto moved = [&](int bits) { return __builtin_bit_cast(float, bits); };
+    v = op(v, moved(__builtin_amdgcn_update_dpp(fill, __builtin_bit_cast(int, v), 0x111, 0xF, 0xF, false)));   // row_shr 1, 2, 4, 8
+    v = op(v, moved(__builtin_amdgcn_update_dpp(fill, __builtin_bit_cast(int, v), 0x112, 0xF, 0xF, false)));
+    v = op(v, moved(__builtin_amdgcn_update_dpp(fill, __builtin_bit_cast(int, v), 0x114, 0xF, 0xF, false)));
+    v = op(v, moved(__builtin_amdgcn_update_dpp(fill, __builtin_bit_cast(int, v), 0x118, 0xF, 0xF, false)));
+    v = op(v, moved(__builtin_amdgcn_update_dpp(fill, __builtin_bit_cast(int, v), 0x142, 0xA, 0xF, false)));   // row_bcast 15 into rows 1 and 3
+    v = op(v, moved(__builtin_amdgcn_update_dpp(fill, __builtin_bit_cast(int, v), 0x143, 0xC, 0xF, false)));   // row_bcast 31 into rows 2 and 3
+    return moved(__builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
 __device__ __forceinline__ float wave_max(float v) {
-    int bits = __builtin_bit_cast(int, v);   // ordered as the values are
-    bits = max(bits, __builtin_amdgcn_update_dpp(0, bits, 0x111, 0xF, 0xF, false));   // row_shr 1, 2, 4, 8
-    bits = max(bits, __builtin_amdgcn_update_dpp(0, bits, 0x112, 0xF, 0xF, false));
-    bits = max(bits, __builtin_amdgcn_update_dpp(0, bits, 0x114, 0xF, 0xF, false));
-    bits = max(bits, __builtin_amdgcn_update_dpp(0, bits, 0x118, 0xF, 0xF, false));
-    bits = max(bits, __builtin_amdgcn_update_dpp(0, bits, 0x142, 0xA, 0xF, false));   // row_bcast 15 into rows 1 and 3
-    bits = max(bits, __builtin_amdgcn_update_dpp(0, bits, 0x143, 0xC, 0xF, false));   // row_bcast 31 into rows 2 and 3
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(bits, 63));
+    return wave_join(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    return wave_join(v, 0.f, [](float a, float b) { return a + b; });
 }
 
 // |v| as an integer, ordered as the values are, infinity and NaN above them.
@@ -905,13 +913,15 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
         }
 }
 
-// The splits that reach a token, in order; one wave a (token, head).
+// The splits that reach a token, 64 at most; one wave a (token, head): a lane has a
+// split's maximum and sum, then all lanes the dimensions, eight splits at a time
+// (read one after the other, 64 splits took 10 us longer).
 template <int HD>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
     const qk_paged_seq s = a.b.seqs[blockIdx.y];
     if (!paged_seq_ok(s, a.b, a.page_shift)) return;
     const int lane = threadIdx.x & 63;
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (at >= static_cast<int64_t>(s.count) * a.heads) return;
     const int tok = static_cast<int>(at / a.heads), head = static_cast<int>(at % a.heads);
     // As the kernel's: a tile's splits go to its last token's last row, and
@@ -920,17 +930,33 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
     if (a.splits[many] == 1) return;
     const int live = min(a.splits[many], (s.pos + tok) / a.split_rows[many] + 1);
     const float *p = a.parts + (static_cast<int64_t>(s.first + tok) * a.heads + head) * a.part_splits * part_floats(HD);
-    constexpr int kD = HD > 64 ? (HD + 63) / 64 : 1;
-    float m = -INFINITY, l = 0.f, o[kD] = {};
-    for (int i = 0; i < live; ++i) {
-        const float mo = p[i * part_floats(HD)], lo = p[i * part_floats(HD) + 1];
-        const float mn = fmaxf(m, mo), ref = mn == -INFINITY ? 0.f : mn;
-        const float f = __builtin_amdgcn_exp2f(m - ref), fo = __builtin_amdgcn_exp2f(mo - ref);
-        m = mn;
-        l = l * f + lo * fo;
+    constexpr int kD = (HD + 63) / 64, kBatch = 8;
+    float ms = -INFINITY, ls = 0.f;
+    if (lane < live) {
+        const float2 state = *reinterpret_cast<const float2 *>(p + lane * part_floats(HD));
+        ms = state.x;
+        ls = state.y;
+    }
+    const float *col[kD];
+    #pragma unroll
+    for (int d = 0; d < kD; ++d) col[d] = p + 4 + min(d * 64 + lane, HD - 1);
+    const float m = wave_max(ms);
+    const float fs = __builtin_amdgcn_exp2f(ms - (m == -INFINITY ? 0.f : m));
+    const float l = wave_sum(ls * fs);
+    float o[kD] = {};
+    for (int i0 = 0; i0 < live; i0 += kBatch) {
+        float v[kBatch][kD];
         #pragma unroll
-        for (int d = 0; d < kD; ++d)
-            if (d * 64 + lane < HD) o[d] = fmaf(p[i * part_floats(HD) + 4 + d * 64 + lane], fo, o[d] * f);
+        for (int i = 0; i < kBatch; ++i)
+            #pragma unroll
+            for (int d = 0; d < kD; ++d) v[i][d] = col[d][min(i0 + i, live - 1) * part_floats(HD)];
+        #pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const float f = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, fs), min(i0 + i, 63)));
+            if (i0 + i < live)
+                #pragma unroll
+                for (int d = 0; d < kD; ++d) o[d] = fmaf(v[i][d], f, o[d]);
+        }
     }
     const float norm = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
     float *out = a.out + (s.first + tok) * a.ldout + static_cast<int64_t>(head) * HD;
