@@ -257,7 +257,7 @@ __device__ __forceinline__ void query_units(int top, float scale, float &factor,
 // its four waves every fourth tile of 32 rows each; the waves' states meet in
 // LDS.
 template <int HD, int TYPE>
-__global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttn a) {
+__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel(PagedAttn a) {
     constexpr int NS = HD / 32, NC = HD / 16, kCode = code_bytes(TYPE);
     constexpr bool kScaled = TYPE != QK_TYPE_F16;
     __shared__ float meet[3][HD * 16 + 64];
@@ -982,11 +982,17 @@ int few_rows(const qk_paged_batch &b, int heads, int kv_heads, int head_dim) {
     return b.n_seqs == 1 ? 0 : kFewRows;
 }
 
-// Splits of a call's rows.  Few query rows: some 8 workgroups a CU, so that
-// sequences of different lengths even out, of at least 512 rows each while there
-// are enough of them to go round, at least one tile a wave.  Chunks: two
-// workgroups a CU, all at once, of at least four tiles; those that lie behind
-// all that a chunk's first tokens see end at once and do not count.
+// Splits of a call's rows, 64 at most.  Few query rows: the workgroups that the
+// chip holds at once, two a CU (one of 256 dimensions), of at least 128 rows, or
+// 256 in more than 32 splits, and none for 256 rows or less.  (One sequence, 8 KV
+// heads of 128 int8 values: 250 rows whole 8.2 us, in two splits 10.2; 2000 rows
+// in 16 splits 9.7, in eight 11.0; 8000 rows in 32 splits 12.5, in 63 14.0.  16
+// sequences of 8000 rows: in one round of workgroups 51 us, in two 55.)  Sequences
+// that fill the chip as they are even out in four splits, if those are long: 64
+// sequences of 1000 to 8000 rows 136 us, 146 whole (of equal lengths the other way
+// round, 217 and 197); of 125 to 1000 rows whole 24, in four splits 31.
+// Chunks: two workgroups a CU, all at once, of at least four tiles; those that lie
+// behind all that a chunk's first tokens see end at once and do not count.
 struct Splits {
     int few, many;
 };
@@ -996,8 +1002,11 @@ Splits wanted_splits(const qk_paged_batch &b, int heads, int kv_heads, int head_
     Splits splits{1, 1};
     if (few > 0) {
         const int64_t units = std::max<int64_t>((std::min(rows, few) + kRowTile - 1) / kRowTile * per_tile, 1);
-        const int64_t least = units * b.max_rows >= 512 * 1024 ? 512 : 4 * kTile;
-        splits.few = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({2048 / units, (b.max_rows + least - 1) / least, 64})));
+        const int64_t round = head_dim > 128 ? 256 : 512;
+        int64_t n = round / units;
+        if (b.max_rows >= 4096) n = std::max(n, std::min<int64_t>(4, 4 * round / units));
+        const int64_t most = std::max<int64_t>(std::min<int64_t>(32, (int64_t(b.max_rows) + 127) / 128), b.max_rows / 256);
+        splits.few = b.max_rows <= 256 ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({n, most, 64})));
     }
     if (rows > few) {
         const int64_t units = (rows + kChunkRows - 1) / kChunkRows * per_tile;
