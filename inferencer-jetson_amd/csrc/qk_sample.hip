@@ -38,6 +38,8 @@ constexpr int kMaxSegments = (1 << 19) / kSegment;
 constexpr int kOctave = 16, kBins = 48 * kOctave;
 constexpr int kFine = 128;   // steps of an octave in the weights' table
 constexpr int kList = 2048;
+constexpr int kRank = 8;     // of kList, whose end a step of them does not pass
+static_assert(kList % kRank == 0, "");
 constexpr int kGather = 8;   // segments whose bins a thread loads at once
 constexpr int kCopies = 2;   // of a segment's histogram in LDS: half the conflicts
 constexpr double kUnit = 17592186044416.;   // 2^44: sample_plain's weights, of which 2^19 stay below 2^64
@@ -124,6 +126,16 @@ __device__ __forceinline__ T wave_scan(T v) {
     v += dpp_part<0x142, 0xA>(v);   // row_bcast 15 into rows 1 and 3
     v += dpp_part<0x143, 0xC>(v);   // row_bcast 31 into rows 2 and 3
     return v;
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+    return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false)));
+}
+// The largest of a wave's values, in every lane.
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+    v = dpp_max<0x118, 0xF>(dpp_max<0x114, 0xF>(dpp_max<0x112, 0xF>(dpp_max<0x111, 0xF>(v))));
+    v = dpp_max<0x143, 0xC>(dpp_max<0x142, 0xA>(v));
+    return __builtin_amdgcn_readlane(static_cast<int>(v), 63);
 }
 // The last lane's value of a 64-bit type.
 template <class T>
@@ -748,11 +760,25 @@ __device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowPara
         return ldexp(static_cast<double>(m), -below);
     };
     constexpr double kWhole = 0x1p-16;   // 2^(e - 47) in units of 2^(e - 31)
+    // The first m tokens of a list, the largest first, into s.ordered: a token a
+    // thread, counting the larger ones, eight at a read's wait.
+    auto order = [&](uint64_t *from, int m) {
+        if (tid < kRank && m + tid < kList) from[m + tid] = 0;
+        __syncthreads();
+        for (int i = tid; i < m; i += kThreads) {
+            const uint64_t t = from[i];
+            int rank = 0;
+            for (int k = 0; k < m; k += kRank)
+                #pragma unroll
+                for (int j = 0; j < kRank; ++j) rank += from[k + j] > t;
+            s.ordered[rank] = t;
+        }
+        __syncthreads();
+    };
     // The last listed token that is kept, in the tokens' order: as many as
     // `left`, while the sum before is below the target and the weight is not
-    // below the least; ~0 if none is.  A list of some hundreds is cut into
-    // kThreads parts of its range first, of which one then holds the cut and is
-    // ordered by counting the larger tokens of each.
+    // below the least; ~0 if none is.  A list of more tokens than threads is cut
+    // into kThreads parts of its range first, of which one then holds the cut.
     auto cut_of = [&](double above, double target, int left, double least) -> uint64_t {
         const int n = s.listed;
         auto stays = [&](uint64_t t, uint64_t &w) { return weight_of(t, w) >= least; };
@@ -760,7 +786,7 @@ __device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowPara
         auto part_of = [&](uint64_t t) {
             return min(static_cast<int>((high - value_of(static_cast<uint32_t>(t >> 32))) * scale), kThreads - 1);
         };
-        const bool parts = n > 128;
+        const bool parts = n > kThreads;
         uint64_t base_mass = 0, base_count = 0;
         int part = 0;
         if (parts) {
@@ -779,7 +805,9 @@ __device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowPara
                 top = max(top, k);
                 low = min(low, k);
             }
-            if (tid < n) {
+            top = wave_max_u32(top);
+            low = ~wave_max_u32(~low);
+            if (lane == 0) {   // a wave at a time: 64 lanes' atomics on one word follow each other
                 atomicMax(&s.key_high, top);
                 atomicMin(&s.key_low, low);
             }
@@ -812,21 +840,19 @@ __device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowPara
             base_mass = s.base_mass;
             base_count = s.base_count;
         }
-        if (tid == 0) s.picked = 0;
-        __syncthreads();
-        for (int i = tid; i < n; i += kThreads) {
-            uint64_t w;
-            if (stays(s.list[i], w) && (!parts || part_of(s.list[i]) == part)) s.some[atomicAdd(&s.picked, 1)] = s.list[i];
+        const bool all = !parts && least <= 0.;
+        uint64_t *const some = all ? s.list : s.some;
+        if (!all) {
+            if (tid == 0) s.picked = 0;
+            __syncthreads();
+            for (int i = tid; i < n; i += kThreads) {
+                uint64_t w;
+                if (stays(s.list[i], w) && (!parts || part_of(s.list[i]) == part)) some[atomicAdd(&s.picked, 1)] = s.list[i];
+            }
+            __syncthreads();
         }
-        __syncthreads();
-        const int m = s.picked;
-        for (int i = tid; i < m; i += kThreads) {
-            const uint64_t t = s.some[i];
-            int rank = 0;
-            for (int k = 0; k < m; ++k) rank += s.some[k] > t;
-            s.ordered[rank] = t;
-        }
-        __syncthreads();
+        const int m = all ? n : s.picked;
+        order(some, m);
         if (tid == 0) s.found = -1;
         for (int i0 = 0; i0 < m; i0 += kThreads) {
             const int i = i0 + tid;
@@ -848,11 +874,7 @@ __device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowPara
     // All that top-k leaves is listed, a token a thread: both cuts from one order,
     // and the token from the kept ones themselves.
     if (st.bin_k < kBins && st.lo == 0 && listed <= kThreads) {
-        const uint64_t t = tid < listed ? s.list[tid] : 0;
-        int rank = 0;
-        for (int k = 0; k < listed; ++k) rank += s.list[k] > t;
-        if (tid < listed) s.ordered[rank] = t;
-        __syncthreads();
+        order(s.list, listed);
         const uint64_t mine = tid < listed ? s.ordered[tid] : 0;
         uint64_t own = 0, upto = 0, none = 0;
         bool stays = false;
