@@ -78,17 +78,6 @@ __device__ __forceinline__ half8 join(half2v a, half2v b, half2v c, half2v d) {
     return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-template <int BYTES>
-struct Bytes {
-    uint32_t w[(BYTES + 3) / 4];
-};
-template <int BYTES>
-__device__ __forceinline__ Bytes<BYTES> load_bytes(const char *p) {
-    Bytes<BYTES> r{};
-    __builtin_memcpy(r.w, p, BYTES);
-    return r;
-}
-
 // --------------------------------------------------------------- layouts --
 //
 // Key operand of step s (32 dimensions): lane (row l % 16, g = l / 16) holds
@@ -255,7 +244,13 @@ __device__ __forceinline__ void query_units(int top, float scale, float &factor,
 
 // A workgroup: 16 query rows of one (sequence, KV head) over a split's rows,
 // its four waves every fourth tile of 32 rows each; the waves' states meet in
-// LDS.
+// LDS.  Few query rows leave the cache as the bound, so nothing is staged: a lane
+// loads its own share of both operands, the next tile's while this one is
+// multiplied.  64 sequences over 1000 to 8000 rows, 8 KV heads of 128 int8 values:
+// 611 MB in 134 us, 4.6 TB/s (a copy reaches 4.7); one over 700 rows of 64 fp16
+// values: 5.8 us, the latency of its loads, and 3.4 of the merge.  Two workgroups a
+// CU up to 128 dimensions: left to itself the compiler takes registers beyond that
+// (fp16 rows of 128, 4 sequences of 8000: 33 us, with the bound 28).
 template <int HD, int TYPE>
 __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel(PagedAttn a) {
     constexpr int NS = HD / 32, NC = HD / 16, kCode = code_bytes(TYPE);
@@ -540,6 +535,14 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
 // are permuted as the scores' registers hold them: lane half hi has, of each 16
 // rows, 4 hi .. + 3 and 8 + 4 hi .. + 3.  While a tile is multiplied the next one
 // is in registers on its way from memory; two LDS buffers, a barrier a tile.
+//
+// The bound is the matrix instructions, twice the products of one fp16 pass: 2048
+// tokens over 8192 earlier rows, 32 heads of 128 float8 values, are 620 GFLOP of
+// them, in 620 to 650 us 1.0 PFLOP/s, where a library product of two fp16 matrices
+// of 8192 reaches 1.15 (both below the instructions' peak, at a clock of 1.9 GHz).
+// The 16-row kernel took 1150 us.  Short chunks are bound by the latency of a
+// workgroup's steps: 517 tokens over 600, 24 heads, 31 us and 7.5 of the merge,
+// where the matrix instructions are 10.
 constexpr int kChunkTile = 64, kChunkRows = 128;
 
 template <int HD, int TYPE>
@@ -965,20 +968,30 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
         if (d * 64 + lane < HD) out[d * 64 + lane] = o[d] * norm;
 }
 
-// A sequence of more query rows a KV head than this takes the chunk kernel, if the
-// call has at least so many pairs of a query row and a cache row.
-constexpr int kFewRows = 64;
-constexpr int64_t kFewPairs = 3 << 19;
+// A sequence of more query rows a KV head than kFewRows takes the chunk kernel,
+// if the call's chunks are kManyUnits workgroups of it unsplit, or have kManyPairs
+// pairs of a query row and a cache row.  Four query heads for each of eight KV
+// heads of 128 int8 values, the chunk kernel against the first, in us: one
+// sequence, 68 query rows a KV head over 4000 cache rows (2.2 million pairs) 24
+// and 18, 256 over 4000 (8.3 million) 29 and 29, 1600 over 500 (12 million) 36 and
+// 37, 512 over 4000 (17 million) 40 and 53, 2000 over none (8 million, 128
+// workgroups) 32 and 23; eight sequences, 256 over 500 (9.2 million, 128
+// workgroups) 35 and 32, 68 over 4000 (17 million) 51 and 72, 512 over none (256
+// workgroups) 19 and 27; 64 sequences, 68 over none (512 workgroups) 18 and 29.
+constexpr int kFewRows = 64, kManyUnits = 256;
+constexpr int64_t kManyPairs = 3 << 22;
 // The chunk kernel's queries and sums of a head fit the registers up to here
 // (at 256 it spilled 58 and more).
 constexpr int kChunkDim = 128;
 
 // Query rows a KV head up to which a sequence of this call takes the first
-// kernel: one sequence has the chunk kernel alone, if its bound calls for it.
+// kernel; a call of one sequence launches one of the two.
 int few_rows(const qk_paged_batch &b, int heads, int kv_heads, int head_dim) {
-    if (head_dim > kChunkDim || static_cast<int64_t>(b.max_count) * (heads / kv_heads) <= kFewRows ||
-        static_cast<double>(b.n_tokens) * heads * b.max_rows < kFewPairs)
-        return INT32_MAX;
+    const int64_t rows = static_cast<int64_t>(b.max_count) * (heads / kv_heads);
+    if (head_dim > kChunkDim || rows <= kFewRows) return INT32_MAX;
+    const int64_t units = (rows + kChunkRows - 1) / kChunkRows * kv_heads * b.n_seqs;
+    const double pairs = static_cast<double>(b.n_tokens) * heads * b.max_rows;
+    if (units < kManyUnits && pairs < kManyPairs) return INT32_MAX;
     return b.n_seqs == 1 ? 0 : kFewRows;
 }
 
