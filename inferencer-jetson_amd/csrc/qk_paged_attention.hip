@@ -1114,9 +1114,10 @@ int qk_paged_attention_f32(const qk_paged_kv *kv, const qk_paged_batch *batch, c
     const qk::Splits wanted = qk::wanted_splits(*batch, heads, kv->kv_heads, kv->head_dim);
     // Splits of whole rounds of a workgroup's tiles.
     auto plan = [&](int kind, int splits, int round) {
-        const int n = static_cast<int>(std::min<int64_t>(splits, fit < 2 ? 1 : fit));
-        a.split_rows[kind] = ((batch->max_rows + n - 1) / n + round - 1) / round * round;
-        a.splits[kind] = (batch->max_rows + a.split_rows[kind] - 1) / a.split_rows[kind];
+        const int64_t n = std::min<int64_t>(splits, fit < 2 ? 1 : fit), rows = batch->max_rows;
+        const int64_t each = ((rows + n - 1) / n + round - 1) / round * round;
+        a.split_rows[kind] = static_cast<int>(each);
+        a.splits[kind] = static_cast<int>((rows + each - 1) / each);
     };
     a.few_rows = qk::few_rows(*batch, heads, kv->kv_heads, kv->head_dim);
     plan(0, wanted.few, 4 * qk::kTile);

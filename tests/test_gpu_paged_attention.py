@@ -18,8 +18,22 @@ TOL = 3e-6
 LAYOUTS = [(32, 8, 64), (6, 6, 64), (16, 2, 96), (5, 1, 96), (24, 8, 128), (8, 8, 128), (20, 1, 128), (8, 1, 256), (4, 2, 256)]
 
 
+PAIRS = 3 << 22   # of a query row and a cache row: from there on chunks have a kernel of their own
+
+
+@pytest.fixture(params=["own bound", "wide bound"], autouse=True)
+def wide(request):
+    """Every test twice: max_rows as the batch has it, and so large that what is
+    chosen by it is what long contexts take."""
+    run.wide = request.param == "wide bound"
+
+
+def bound(pool, heads):
+    return {"max_rows": max(pool.max_rows, -(-PAIRS // (pool.n * heads)))} if run.wide else {}
+
+
 def run(qk, t, pool, q, heads, workspace=True, scale=0.0, **over):
-    kv, batch = pool.dev(qk, t, **over)
+    kv, batch = pool.dev(qk, t, **(bound(pool, heads) | over))
     out = t.full((batch.n_tokens, heads * pool.hd), np.nan, device="cuda")
     nb = qk.paged_attention_workspace_bytes(batch, heads, pool.kvh, pool.hd) if workspace is True else workspace
     ws = t.full((nb,), 0xFF, dtype=t.uint8, device="cuda") if nb else None   # stale partials are not numbers
@@ -233,7 +247,7 @@ def test_the_same_call_twice_and_captured(qk, torch_gpu, kind):
     t = torch_gpu
     rng = np.random.default_rng(11)
     pool = paged_ref.Pool(rng, kind, 2, 64, 32, [(1, 2000), (1, 50), (130, 20)])
-    kv, batch = pool.dev(qk, t)
+    kv, batch = pool.dev(qk, t, **bound(pool, 8))
     nb = qk.paged_attention_workspace_bytes(batch, 8, 2, 64)
     ws = [t.empty(max(nb, 16), dtype=t.uint8, device="cuda") for _ in range(2)]
     q = to_dev(t, queries(rng, pool, 8))
@@ -252,6 +266,65 @@ def test_the_same_call_twice_and_captured(qk, torch_gpu, kind):
         call(eager, ws[1])
         t.cuda.synchronize()
         assert t.equal(out, eager)
+
+
+@pytest.mark.parametrize("workspace", [0, True, 200000])
+def test_the_largest_bound(qk, torch_gpu, workspace):
+    """max_rows may be as large as rows can be counted."""
+    rng = np.random.default_rng(12)
+    pool = paged_ref.Pool(rng, "f16", 2, 64, 1024, [(1, 1500), (150, 900), (1, 0)])
+    q = queries(rng, pool, 4)
+    got = run(qk, torch_gpu, pool, q, 4, workspace=workspace, max_rows=2 ** 31 - 1 - 1024)
+    assert rel_l2(got, pool.attention(q, 4)) < TOL
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("count", [1, 150])
+def test_shared_pages_and_a_negative_scale(qk, torch_gpu, kind, count):
+    """Two sequences that begin with the same pages, and the same one twice, at
+    other positions; a scale that prefers the farthest rows."""
+    rng = np.random.default_rng(13)
+    pool = paged_ref.Pool(rng, kind, 2, 128, 16, [(count, 100), (count, 100), (count, 64)])
+    pool.table[1, :4] = pool.table[0, :4]
+    pool.seqs[2, 3] = 0
+    q = queries(rng, pool, 6)
+    for scale in (0.0, -0.05):
+        assert rel_l2(run(qk, torch_gpu, pool, q, 6, scale=scale), pool.attention(q, 6, scale or None)) < TOL   # 0: the default
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_two_calls_at_once(qk, torch_gpu, kind):
+    """On two streams, a workspace each, over the same cache."""
+    t = torch_gpu
+    rng = np.random.default_rng(14)
+    pool = paged_ref.Pool(rng, kind, 2, 64, 64, [(1, 3000), (140, 900), (1, 40)])
+    kv, batch = pool.dev(qk, t, **bound(pool, 8))
+    nb = qk.paged_attention_workspace_bytes(batch, 8, 2, 64)
+    qs = [to_dev(t, queries(rng, pool, 8)) for _ in range(2)]
+    outs, ws = [t.empty_like(x) for x in qs], [t.empty(max(nb, 16), dtype=t.uint8, device="cuda") for _ in qs]
+    streams = [t.cuda.Stream() for _ in qs]
+    t.cuda.synchronize()
+    for _ in range(20):
+        for x, o, w, s in zip(qs, outs, ws, streams):
+            with t.cuda.stream(s):
+                qk.paged_attention(kv, batch, x, o, 8, workspace=w)
+    t.cuda.synchronize()
+    for x, o in zip(qs, outs):
+        assert rel_l2(o.cpu().numpy(), pool.attention(x.cpu().numpy(), 8)) < TOL
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("count", [1, 150])
+def test_a_query_that_is_not_finite_and_sees_no_row(qk, torch_gpu, kind, count):
+    """Zeros like any that sees none."""
+    rng = np.random.default_rng(15)
+    pool = paged_ref.Pool(rng, kind, 1, 64, 16, [(count, 10), (1, 5)])
+    pool.table[0, :] = -1
+    q = queries(rng, pool, 2)
+    q[0, 3], q[count - 1, 70] = np.nan, np.inf
+    got = run(qk, torch_gpu, pool, q, 2)
+    assert not got[:count].any()
+    assert rel_l2(got[count:], pool.attention(np.nan_to_num(q, posinf=0), 2)[count:]) < TOL
 
 
 def test_refusals(qk, torch_gpu):
