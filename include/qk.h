@@ -481,7 +481,7 @@ typedef struct qk_rope_scaling {
    qk_rope_paged_write and the decode drivers' own rotation take.  scaling may
    be NULL (QK_ROPE_NONE); freq_factors (device, rot_dim / 2 values, or NULL)
    divide the frequencies before the scaling (a GGUF file's rope_freqs.weight).
-   rot_dim even, at most 512. */
+   rot_dim even, at most 512; at most 2^30 positions. */
 int qk_rope_tables_f32(float theta, int rot_dim, const qk_rope_scaling *scaling, const float *freq_factors,
                        int first_pos, int positions, float *cosine, float *sine, qk_stream stream);
 

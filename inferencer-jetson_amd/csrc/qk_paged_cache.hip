@@ -398,8 +398,8 @@ int qk_rope_tables_f32(float theta, int rot_dim, const qk_rope_scaling *scaling,
         return qk::fail(QK_ERR_INVALID_ARG, "qk_rope_tables_f32: null pointer or negative position");
     if (rot_dim < 2 || rot_dim % 2 || rot_dim > 512)
         return qk::fail(QK_ERR_LIMIT, "qk_rope_tables_f32: rot_dim must be even, 2 to 512");
-    if (positions > 0x7FFFFFFF - first_pos)
-        return qk::fail(QK_ERR_LIMIT, "qk_rope_tables_f32: positions beyond 2^31");
+    if (positions > 1 << 30 || positions > 0x7FFFFFFF - first_pos)
+        return qk::fail(QK_ERR_LIMIT, "qk_rope_tables_f32: more than 2^30 positions, or beyond 2^31");
     if (!(theta > 0.f) || !std::isfinite(theta))
         return qk::fail(QK_ERR_INVALID_ARG, "qk_rope_tables_f32: theta must be positive");
     qk::TableArgs a{};

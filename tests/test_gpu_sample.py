@@ -213,6 +213,41 @@ def test_captured(qk, torch_gpu):
         assert t.equal(outs[0], outs[2]) and t.equal(outs[1], outs[2])
 
 
+@pytest.mark.parametrize("count", [1, 2, 7, 8, 127, 129, 505, 511, 512, 513, 600, 1025, 2040, 2047, 2048, 2049, 4000])
+@pytest.mark.parametrize("min_p", [0.0, 0.993])
+def test_as_many_tokens_at_the_cut(qk, torch_gpu, count, min_p):
+    """So many tokens within a fiftieth of each other's weight, the rest far
+    below; a third, two thirds and nearly all of them kept."""
+    rng = np.random.default_rng(count)
+    x = np.full((6, 20000), -30, np.float32)
+    for r in x:
+        r[rng.choice(20000, count, replace=False)] = 3 + 0.02 * rng.random(count)
+    check(qk, torch_gpu, x, rng.random(6).astype(np.float32), top_p=np.float32([0.33, 0.67, 0.99] * 2),
+          min_p=np.full(6, min_p, np.float32), top_k=np.int32([0, 0, 0, 1, count // 2 + 1, count]))
+
+
+def test_two_calls_at_once(qk, torch_gpu):
+    """On two streams, a workspace each, over the same logits."""
+    t = torch_gpu
+    rng = np.random.default_rng(8)
+    x, n = to_dev(t, logits(rng, 24, 50000)), 50000
+    us, tops = [t.rand(24, device="cuda") for _ in range(2)], [t.full((24,), p, device="cuda") for p in (0.95, 0.6)]
+    outs = [[t.empty(24, dtype=t.int32, device="cuda") for _ in range(2)] for _ in range(2)]
+    ws = [t.empty(qk.sample_workspace_bytes(n, 24), dtype=t.uint8, device="cuda") for _ in range(2)]
+    streams = [t.cuda.Stream() for _ in range(2)]
+    t.cuda.synchronize()
+    for u, p, w, o in zip(us, tops, ws, outs):
+        qk.sample_rows(x, u, o[0], top_p=p, workspace=w)
+    t.cuda.synchronize()
+    for _ in range(20):
+        for u, p, w, o, s in zip(us, tops, ws, outs, streams):
+            with t.cuda.stream(s):
+                qk.sample_rows(x, u, o[1], top_p=p, workspace=w)
+    t.cuda.synchronize()
+    for o in outs:
+        assert t.equal(o[0], o[1])
+
+
 def test_refusals(qk, torch_gpu):
     t = torch_gpu
     x, u, o = t.zeros(2, 10, device="cuda"), t.zeros(2, device="cuda"), t.zeros(2, dtype=t.int32, device="cuda")

@@ -106,7 +106,7 @@ def test_empty_calls_are_no_ops(qk):
 @pytest.mark.parametrize("over,status", [
     (dict(theta=0.0), "INVALID_ARG"), (dict(theta=float("nan")), "INVALID_ARG"), (dict(rot_dim=63), "LIMIT"),
     (dict(rot_dim=514), "LIMIT"), (dict(first_pos=-1), "INVALID_ARG"), (dict(positions=-1), "INVALID_ARG"),
-    (dict(first_pos=0x7FFFFFF0), "LIMIT"), (dict(cosine=None), "INVALID_ARG")])
+    (dict(first_pos=0x7FFFFFF0), "LIMIT"), (dict(positions=(1 << 30) + 1), "LIMIT"), (dict(cosine=None), "INVALID_ARG")])
 def test_table_refusals(qk, over, status):
     d = dict(theta=10000.0, rot_dim=64, scaling=None, freq_factors=None, first_pos=0, positions=100, cosine=A, sine=A,
              stream=None) | over
