@@ -776,10 +776,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
         const auto &head = *reinterpret_cast<const typename C::Head *>(buf + C::kKeyBytes + C::kValueBytes);
         const int en = kScaled ? __builtin_amdgcn_readfirstlane(head.ev) : ev;
         const bool edge = t0 + kChunkTile - 1 > wave_seen || absent;   // some token does not see it whole
-        // Half a tile at a time: 32 scores a lane left too few registers.
-        #pragma unroll 1
-        for (int hf = 0; hf < 2; ++hf) {
-            float16v st;
+        auto scores = [&](int hf, float16v &st) {
             #pragma unroll
             for (int r = 0; r < 16; ++r) st[r] = 0.f;
             const char *keys = buf + (32 * hf + n) * C::kKeyStride + 16 * hi;
@@ -789,6 +786,14 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
                 st = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[x], st, 0, 0, 0);
                 st = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[x], st, 0, 0, 0);
             }
+        };
+        // Half a tile at a time, the second half's scores begun before the first
+        // one's weights, which run beside them: 2 % of a long chunk's time (all 32
+        // scores a lane at once left too few registers).
+        float16v st, ahead;
+        scores(0, st);
+        #pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
             // Register r: row t0 + 32 hf + 8 (r / 4) + 4 hi + r % 4.
             #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
@@ -838,6 +843,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
                         if ((bad >> (8 * (r / 4) + r % 4) & 1) && st[r] != -INFINITY) l = __builtin_nanf("");
                 }
             }
+            if (hf == 0) scores(1, ahead);
             const char *values = buf + C::kKeyBytes;
             #pragma unroll
             for (int b = 0; b < 2; ++b) {   // 16 rows
@@ -869,6 +875,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
                 #pragma unroll
                 for (int d = 0; d < ND; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], ph, o[d], 0, 0, 0);
             }
+            st = ahead;
         }
     };
 
