@@ -538,7 +538,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
 //
 // The bound is the matrix instructions, twice the products of one fp16 pass: 2048
 // tokens over 8192 earlier rows, 32 heads of 128 float8 values, are 620 GFLOP of
-// them, in 620 to 650 us 1.0 PFLOP/s, where a library product of two fp16 matrices
+// them, in 607 to 637 us 1.0 PFLOP/s, where a library product of two fp16 matrices
 // of 8192 reaches 1.15 (both below the instructions' peak, at a clock of 1.9 GHz).
 // The 16-row kernel took 1150 us.  Short chunks are bound by the latency of a
 // workgroup's steps: 517 tokens over 600, 24 heads, 31 us and 7.5 of the merge,
