@@ -719,6 +719,13 @@ __device__ __forceinline__ void block_scan(uint64_t &mass, uint64_t &count, Pick
     }
 }
 
+// The largest number i of the threads that say so (i grows with the thread), into
+// *found: one atomic a wave, since a word's follow each other.
+__device__ __forceinline__ void last_of(bool yes, int i, int *found) {
+    const uint64_t all = __builtin_amdgcn_ballot_w64(yes);
+    if (yes && !(all >> (threadIdx.x & 63) >> 1)) atomicMax(found, i);
+}
+
 // A row by its segments' histograms and its list, by all threads of the
 // workgroup; false: it is one for sample_plain.
 __device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowParams &r, const RowPlan &st, int row,
@@ -833,8 +840,9 @@ __device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowPara
             const uint64_t own_mass = mass, own_count = count;
             block_scan(mass, count, s);
             const uint64_t mass0 = mass - own_mass, count0 = count - own_count;
-            if (own_count > 0 && count0 < static_cast<uint64_t>(left) && above + static_cast<double>(mass0) * kWhole < target)
-                atomicMax(&s.found, tid);
+            last_of(own_count > 0 && count0 < static_cast<uint64_t>(left) &&
+                        above + static_cast<double>(mass0) * kWhole < target,
+                    tid, &s.found);
             __syncthreads();
             part = s.found;
             if (part < 0) return ~0ull;
@@ -869,9 +877,9 @@ __device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowPara
             uint64_t mass = own;
             block_scan(mass, count, s);
             mass += base_mass;
-            if (i < m && base_count + i < static_cast<uint64_t>(left) &&
-                above + static_cast<double>(mass - own) * kWhole < target)
-                atomicMax(&s.found, i);
+            last_of(i < m && base_count + i < static_cast<uint64_t>(left) &&
+                        above + static_cast<double>(mass - own) * kWhole < target,
+                    i, &s.found);
             base_mass = s.wave_mass[kWaves - 1] + base_mass;   // of full rounds only: the last has no next
             #pragma unroll
             for (int w = 0; w < kWaves - 1; ++w) base_mass += s.wave_mass[w];
@@ -897,7 +905,7 @@ __device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowPara
         s.some[tid] = stays ? own : 0;
         if (tid == 0) s.picked = 0;
         __syncthreads();
-        if (stays) atomicMax(&s.picked, tid + 1);
+        last_of(stays, tid + 1, &s.picked);
         __syncthreads();
         const int keep = s.picked;
         uint64_t z = 0, before = 0;
@@ -987,12 +995,16 @@ __device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowPara
     const bool any = cut != ~0ull;
     const float cut_x = any ? value_of(static_cast<uint32_t>(cut >> 32)) : INFINITY;
     const int cut_i = any ? static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(cut)) : -1;
+    // With a cut the kept tokens are those down to it, by the logits alone: a wave
+    // without any takes no exponentials.
     auto weights = [&](const float (&v)[4], int i, uint64_t (&w)[4]) {
         uint64_t sum = 0;
         #pragma unroll
         for (int k = 0; k < 4; ++k) {
+            w[k] = 0;
+            if (any && !(v[k] > cut_x || (v[k] == cut_x && i + k <= cut_i))) continue;
             const Depth d = depth_of(v[k], c, eg);
-            const bool kept = d.f >= 0 && (d.bin() + down < whole || v[k] > cut_x || (v[k] == cut_x && i + k <= cut_i));
+            const bool kept = d.f >= 0 && (any || d.bin() + down < whole);
             w[k] = kept ? static_cast<uint64_t>(unit_weight(d, s.table)) << 16 >> (d.f / kFine) : 0;
             sum += w[k];
         }
@@ -1004,7 +1016,8 @@ __device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowPara
     #pragma unroll
     for (int j = 0; j < kQuads; ++j) {
         uint64_t w[4];
-        const uint64_t t = wave_scan(weights(v[j], quad_at(seg, j), w));
+        const uint64_t own = weights(v[j], quad_at(seg, j), w);
+        const uint64_t t = __builtin_amdgcn_ballot_w64(own > 0) ? wave_scan(own) : 0;
         if (lane == 63) s.quads[j * kWaves + wave] = t;
     }
     __syncthreads();
