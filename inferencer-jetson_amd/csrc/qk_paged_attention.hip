@@ -1101,9 +1101,6 @@ int qk_paged_attention_f32(const qk_paged_kv *kv, const qk_paged_batch *batch, c
         return qk::fail(QK_ERR_INVALID_ARG, "qk_paged_attention_f32: leading dimension smaller than the row");
     if (!qk::aligned(q, 16) || !qk::aligned(out, 16) || !qk::aligned(workspace, 16) || ldq % 4 || ldout % 4)
         return qk::fail(QK_ERR_ALIGN, "qk_paged_attention_f32: q and out need 16-byte rows, workspace 16 bytes");
-    const int64_t tiles = (static_cast<int64_t>(batch->max_count) * (heads / kv->kv_heads) + qk::kRowTile - 1) / qk::kRowTile;
-    if (tiles * kv->kv_heads > 0x7FFFFFFF / 64)
-        return qk::fail(QK_ERR_LIMIT, "qk_paged_attention_f32: too many query rows in one launch");
     qk::PagedAttn a{};
     a.kv = *kv;
     a.b = *batch;
@@ -1130,6 +1127,10 @@ int qk_paged_attention_f32(const qk_paged_kv *kv, const qk_paged_batch *batch, c
     plan(0, wanted.few, 4 * qk::kTile);
     plan(1, wanted.many, qk::kChunkTile);
     a.part_splits = std::max(a.splits[0], a.splits[1]);
+    // A launch has fewer than 2^32 threads a dimension, of 256 a workgroup.
+    const int64_t tiles = (static_cast<int64_t>(batch->max_count) * a.group + qk::kRowTile - 1) / qk::kRowTile;
+    if (tiles * kv->kv_heads * std::max(a.part_splits, 4) >= 1 << 24)   // (the merge: four tokens' heads)
+        return qk::fail(QK_ERR_LIMIT, "qk_paged_attention_f32: too many query rows in one launch");
     switch (kv->head_dim) {
         case 64: return qk::launch_type<64>(a, qk::S(stream));
         case 96: return qk::launch_type<96>(a, qk::S(stream));

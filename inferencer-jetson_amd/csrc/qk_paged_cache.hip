@@ -347,10 +347,11 @@ struct Read {
     }
 };
 
-// Workgroups for max_count * R rows of a sequence; 0: more than a launch holds.
+// Workgroups for max_count * R rows of a sequence; 0: more than a launch holds
+// (fewer than 2^32 threads a dimension, of 256 a workgroup).
 unsigned row_blocks(int64_t max_count, int64_t R, int hd) {
     const int64_t per = 256 / row_lanes(hd) * kGroupRows, n = (max_count * R + per - 1) / per;
-    return n > 0x7FFFFFFF ? 0 : static_cast<unsigned>(n);
+    return n >= 1 << 24 ? 0 : static_cast<unsigned>(n);
 }
 
 }  // namespace

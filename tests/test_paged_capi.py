@@ -77,6 +77,8 @@ def test_too_many_rows(qk):
     assert write(qk, b=b, cache=kv(qk, head_dim=64, kv_heads=4096), q=None, q_out=None, rot_dim=64, ldk=1 << 18,
                  ldv=1 << 18) == qk.QK_ERR_LIMIT
     assert attend(qk, b=b) == qk.QK_ERR_LIMIT
+    b = batch(qk, max_count=1 << 27, max_rows=1 << 27, n_tokens=1 << 27)   # 2^32 threads
+    assert write(qk, b=b) == qk.QK_ERR_LIMIT and read(qk, b=b) == qk.QK_ERR_LIMIT and attend(qk, b=b) == qk.QK_ERR_LIMIT
 
 
 @pytest.mark.parametrize("over,status", [
