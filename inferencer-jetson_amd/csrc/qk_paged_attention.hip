@@ -566,13 +566,14 @@ struct Chunk {
     };
     static constexpr int kBuffer = kKeyBytes + kValueBytes + sizeof(Head);
 
+    // Of col + d, col a multiple of kValCols and d below it: that of col xor that of d.
     static __device__ __forceinline__ int exchange(int d) { return (d ^ (d >> 3)) & 7; }
 };
 
 typedef float float16v __attribute__((ext_vector_type(16)));
 
 template <int HD, int TYPE>
-__global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
+__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(PagedAttn a) {
     using C = Chunk<HD, TYPE>;
     constexpr int NS = HD / 16, ND = HD / 32, kCode = C::kCode;
     constexpr bool kScaled = TYPE != QK_TYPE_F16;
@@ -721,7 +722,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttn a) {
         }
         #pragma unroll
         for (int d = 0; d < C::kValCols; ++d)
-            *reinterpret_cast<uint2 *>(at + (exchanged ^ (d << 4)) + d * 2 * kChunkTile) = w[d];
+            *reinterpret_cast<uint2 *>(at + (exchanged ^ (C::exchange(d) << 4)) + d * 2 * kChunkTile) = w[d];
     };
 
     // ------------------------------------------------------- queries -----
@@ -985,17 +986,15 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
 // workgroups) 32 and 23; eight sequences, 256 over 500 (9.2 million, 128
 // workgroups) 35 and 32, 68 over 4000 (17 million) 51 and 72, 512 over none (256
 // workgroups) 19 and 27; 64 sequences, 68 over none (512 workgroups) 18 and 29.
+// Eight query heads of 256 for one KV head, one sequence of 2048 tokens over 4000:
+// int8 322 and 409, fp16 358 and 403; eight of 64 over 4000: 86 and 89, 97 and 84.
 constexpr int kFewRows = 64, kManyUnits = 256;
 constexpr int64_t kManyPairs = 3 << 22;
-// The chunk kernel's queries and sums of a head fit the registers up to here
-// (at 256 it spilled 58 and more).
-constexpr int kChunkDim = 128;
-
 // Query rows a KV head up to which a sequence of this call takes the first
 // kernel; a call of one sequence launches one of the two.
-int few_rows(const qk_paged_batch &b, int heads, int kv_heads, int head_dim) {
+int few_rows(const qk_paged_batch &b, int heads, int kv_heads) {
     const int64_t rows = static_cast<int64_t>(b.max_count) * (heads / kv_heads);
-    if (head_dim > kChunkDim || rows <= kFewRows) return INT32_MAX;
+    if (rows <= kFewRows) return INT32_MAX;
     const int64_t units = (rows + kChunkRows - 1) / kChunkRows * kv_heads * b.n_seqs;
     const double pairs = static_cast<double>(b.n_tokens) * heads * b.max_rows;
     if (units < kManyUnits && pairs < kManyPairs) return INT32_MAX;
@@ -1011,18 +1010,18 @@ int few_rows(const qk_paged_batch &b, int heads, int kv_heads, int head_dim) {
 // that fill the chip as they are even out in four splits, if those are long: 64
 // sequences of 1000 to 8000 rows 136 us, 146 whole (of equal lengths the other way
 // round, 217 and 197); of 125 to 1000 rows whole 24, in four splits 31.
-// Chunks: two workgroups a CU, all at once, of at least four tiles; those that lie
+// Chunks: a round of workgroups likewise, of at least four tiles; those that lie
 // behind all that a chunk's first tokens see end at once and do not count.
 struct Splits {
     int few, many;
 };
 Splits wanted_splits(const qk_paged_batch &b, int heads, int kv_heads, int head_dim) {
-    const int64_t few = few_rows(b, heads, kv_heads, head_dim), rows = static_cast<int64_t>(b.max_count) * (heads / kv_heads);
+    const int64_t few = few_rows(b, heads, kv_heads), rows = static_cast<int64_t>(b.max_count) * (heads / kv_heads);
     const int64_t per_tile = static_cast<int64_t>(kv_heads) * b.n_seqs;
+    const int64_t round = head_dim > 128 ? 256 : 512;
     Splits splits{1, 1};
     if (few > 0) {
         const int64_t units = std::max<int64_t>((std::min(rows, few) + kRowTile - 1) / kRowTile * per_tile, 1);
-        const int64_t round = head_dim > 128 ? 256 : 512;
         int64_t n = round / units;
         if (b.max_rows >= 4096) n = std::max(n, std::min<int64_t>(4, 4 * round / units));
         const int64_t most = std::max<int64_t>(std::min<int64_t>(32, (int64_t(b.max_rows) + 127) / 128), b.max_rows / 256);
@@ -1032,7 +1031,7 @@ Splits wanted_splits(const qk_paged_batch &b, int heads, int kv_heads, int head_
         const int64_t units = (rows + kChunkRows - 1) / kChunkRows * per_tile;
         const double mean = b.max_rows - 0.5 * std::min(b.max_count, b.max_rows);
         auto live = [&](int n) { return units * std::min<double>(n, mean * n / b.max_rows + 0.5); };
-        while (splits.many < 64 && live(splits.many + 1) <= 512 && b.max_rows > splits.many * 4 * kChunkTile) ++splits.many;
+        while (splits.many < 64 && live(splits.many + 1) <= round && b.max_rows > splits.many * 4 * kChunkTile) ++splits.many;
     }
     return splits;
 }
@@ -1050,12 +1049,10 @@ int launch(const PagedAttn &a, hipStream_t stream) {
     if (a.few_rows > 0)
         hipLaunchKernelGGL((paged_attention_kernel<HD, TYPE>),
                            grid(std::min<int64_t>(rows, a.few_rows), kRowTile, a.splits[0]), dim3(256), 0, stream, a);
-    if constexpr (HD <= kChunkDim) {
-        constexpr size_t kLds = 2 * Chunk<HD, TYPE>::kBuffer;
-        if (rows > a.few_rows)
-            hipLaunchKernelGGL((paged_chunk_kernel<HD, TYPE>), grid(rows, kChunkRows, a.splits[1]), dim3(256), kLds,
-                               stream, a);
-    }
+    constexpr size_t kLds = 2 * Chunk<HD, TYPE>::kBuffer;
+    if (rows > a.few_rows)
+        hipLaunchKernelGGL((paged_chunk_kernel<HD, TYPE>), grid(rows, kChunkRows, a.splits[1]), dim3(256), kLds, stream,
+                           a);
     if (a.part_splits > 1)
         hipLaunchKernelGGL((paged_merge_kernel<HD>),
                            dim3(static_cast<unsigned>((static_cast<int64_t>(a.b.max_count) * a.heads + 3) / 4),
@@ -1123,7 +1120,7 @@ int qk_paged_attention_f32(const qk_paged_kv *kv, const qk_paged_batch *batch, c
         a.split_rows[kind] = static_cast<int>(each);
         a.splits[kind] = static_cast<int>((rows + each - 1) / each);
     };
-    a.few_rows = qk::few_rows(*batch, heads, kv->kv_heads, kv->head_dim);
+    a.few_rows = qk::few_rows(*batch, heads, kv->kv_heads);
     plan(0, wanted.few, 4 * qk::kTile);
     plan(1, wanted.many, qk::kChunkTile);
     a.part_splits = std::max(a.splits[0], a.splits[1]);

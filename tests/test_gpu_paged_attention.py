@@ -72,7 +72,8 @@ def test_chunks(qk, torch_gpu, kind, heads, kvh, hd, seqs):
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("heads,kvh,hd,count,pos", [(32, 8, 64, 1, 5000), (24, 8, 128, 1, 9000), (8, 1, 256, 3, 4000),
-                                                    (16, 2, 96, 2, 3001), (8, 2, 128, 300, 1200), (8, 8, 64, 517, 300)])
+                                                    (16, 2, 96, 2, 3001), (8, 2, 128, 300, 1200), (8, 8, 64, 517, 300),
+                                                    (8, 1, 256, 130, 1700), (16, 2, 96, 150, 1500)])
 def test_long_rows_and_chunks(qk, torch_gpu, kind, heads, kvh, hd, count, pos):
     """Rows split over workgroups, and long chunks: a few tokens against the
     oracle, all of them against the call without a workspace (one split)."""
