@@ -836,7 +836,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
                 ev = en;
             }
             const float ref = c == INFINITY ? 0.f : c;   // nothing seen: weights of exp2(-inf)
-            if (edge && t0 + kChunkTile - 1 > seen) {
+            if (t0 + kChunkTile - 1 > seen) {   // flagged for all waves, those that see the whole tile too
                 const uint32_t bad = head.bad[hf] >> (4 * hi);
                 if (__builtin_amdgcn_ballot_w64(bad != 0)) {
                     #pragma unroll

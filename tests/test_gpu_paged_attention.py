@@ -341,3 +341,29 @@ def test_refusals(qk, torch_gpu):
         qk.paged_attention(kv, batch, x.half(), x.clone(), 4)
     with pytest.raises(qk.QKError, match="GPU"):
         qk.paged_attention(kv, batch, x.cpu(), x.clone(), 4)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("part", ["key", "value"])
+@pytest.mark.parametrize("group", [1, 2, 4])
+@pytest.mark.parametrize("pos", [0, 40, 63])
+def test_not_finite_rows_under_every_wave(qk, torch_gpu, kind, part, group, pos):
+    """A row that is not finite just behind a chunk's first tokens: later ones see
+    the whole tile that these see in part, and get no number either."""
+    count, at = 300, pos + 5
+    rng = np.random.default_rng(20)
+    pool = paged_ref.Pool(rng, kind, 1, 64, 16, [(count, pos)])
+    q = queries(rng, pool, group)
+    want = pool.attention(q, group).reshape(count, -1)
+    codes, scale, _ = getattr(pool, part)
+    page = pool.table[0, at // 16]
+    if kind == "f16":
+        codes[page, 0, at % 16, 5] = np.inf
+    elif kind == "i8":
+        scale[page, 0, at % 16] = np.nan
+    else:
+        codes[page, 0, at % 16, 5] = 0x7F
+    got = run(qk, torch_gpu, pool, q, group)
+    sees = np.arange(pos, pos + count) >= at
+    assert rel_l2(got[~sees], want[~sees]) < TOL
+    assert (~np.isfinite(got[sees].reshape(-1, 64))).any(-1).all()
