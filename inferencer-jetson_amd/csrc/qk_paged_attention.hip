@@ -374,10 +374,11 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
             #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 float x = st[hf][r] * qscale;
+                // An infinite key's score: not a number, whatever its sign.
                 if constexpr (kScaled)
-                    x *= t.ks[hf][r];
+                    x *= fmaf(t.ks[hf][r], 0.f, t.ks[hf][r]);
                 else
-                    x = fmaf(x, 0.f, x);   // an infinite key's score: not a number, whatever its sign
+                    x = fmaf(x, 0.f, x);
                 st[hf][r] = x;
             }
         if (edge) {
@@ -661,7 +662,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
                 head.vs[lane] = ldexpf(v, 14 - top_ev);
                 if (lane == 0) head.ev = top_ev;
             } else if (wave == 1) {
-                head.ks[lane] = g.scale;
+                head.ks[lane] = fmaf(g.scale, 0.f, g.scale);   // infinite: all its scores are not numbers
             }
         }
         #pragma unroll

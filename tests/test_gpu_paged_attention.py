@@ -367,3 +367,22 @@ def test_not_finite_rows_under_every_wave(qk, torch_gpu, kind, part, group, pos)
     sees = np.arange(pos, pos + count) >= at
     assert rel_l2(got[~sees], want[~sees]) < TOL
     assert (~np.isfinite(got[sees].reshape(-1, 64))).any(-1).all()
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+@pytest.mark.parametrize("count", [1, 40, 300])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf])
+def test_an_infinite_key_scale(qk, torch_gpu, kind, count, bad):
+    """Its product with a query is -inf half of the time: no number all the same,
+    to the tokens that see it."""
+    rng = np.random.default_rng(25)
+    pool = paged_ref.Pool(rng, kind, 1, 64, 16, [(count, 90)])
+    q = queries(rng, pool, 4)
+    want = pool.attention(q, 4)
+    at = 90 + count // 3
+    pool.key[1][pool.table[0, at // 16], 0, at % 16] = bad
+    got = run(qk, torch_gpu, pool, q, 4)
+    sees = np.arange(90, 90 + count) >= at
+    assert not np.isfinite(got[sees]).any()
+    if count > 1:
+        assert rel_l2(got[~sees], want[~sees]) < TOL
