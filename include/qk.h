@@ -511,8 +511,10 @@ int qk_paged_read_f32(const qk_paged_kv *kv, const qk_paged_batch *batch, float 
    position (which hold them already): out = softmax(scale q K^T) V, scale 1 /
    sqrt(head_dim) when 0.  q and out are [n_tokens] rows of heads * head_dim,
    ldq and ldout apart.  Rows of absent pages take no part; a token that sees
-   no row gets zeros.  Products keep 22 bits of q and of the probabilities, and
-   every bit of the cache.  A key or value that is not finite makes the outputs
+   no row gets zeros.  Products keep every bit of the cache, 22 bits of q, and of
+   a token's probabilities times value scales 22 bits or 2^-32 of the largest,
+   whatever the scales of rows that it does not see or gives no weight (value
+   scales of a sequence within 2^100 of each other).  A key or value that is not finite makes the outputs
    of the tokens that see it not finite, and reaches no other.  workspace holds
    partial results when a sequence's rows are split over workgroups; with less
    than the queried bytes (or none) the call takes fewer splits.  Calls sharing

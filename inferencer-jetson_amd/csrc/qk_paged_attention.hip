@@ -12,13 +12,15 @@
 //   score(row) = (K code . q 2^e) * 2^-e log2(e) scale * key_scale(row), e the
 //                exponent that brings a query row's largest value to 2^13;
 //   weight     = exp2(score - m), m the running maximum; its sum l in fp32;
-//   operand    = weight * value_scale(row) * 2^(14 - ev), ev the exponent of the
-//                largest value scale so far, so the halves neither overflow
-//                nor lose the bits of a small weight.
+//   operand    = weight * value_scale(row) * 2^(15 - e), e by the largest of these
+//                products of the query row so far (fp16 rows: 2^15): the halves do
+//                not overflow, and keep 22 bits of a product above 2^-10 of the
+//                largest and 2^-32 of that of any other.
 #include "qk_paged.h"
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace qk {
 namespace {
@@ -72,6 +74,21 @@ __device__ __forceinline__ void codes4(uint32_t w, half2v &a, half2v &b) {
         a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false);
         b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true);
     }
+}
+
+// The bits of four 8-bit codes that make them other than 0 (float8 has a -0).
+template <int TYPE>
+constexpr uint32_t code_bits = TYPE == QK_TYPE_I8 ? 0xFFFFFFFFu : 0x7F7F7F7Fu;
+
+// The bits of all lanes of each 16.
+__device__ __forceinline__ uint32_t or16(uint32_t bits) {
+    auto turned = [](uint32_t v, auto by) {
+        return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x120 + decltype(by)::value, 0xF, 0xF, false));
+    };
+    bits |= turned(bits, std::integral_constant<int, 8>{});   // row_ror
+    bits |= turned(bits, std::integral_constant<int, 4>{});
+    bits |= turned(bits, std::integral_constant<int, 2>{});
+    return bits | turned(bits, std::integral_constant<int, 1>{});
 }
 
 __device__ __forceinline__ half8 join(half2v a, half2v b, half2v c, half2v d) {
@@ -135,6 +152,18 @@ struct ValueTile {   // 8 rows a lane: slot j < 4 row 4 g + j, else 16 + 4 g + j
         } else {
             __builtin_memcpy(w[j], row + i * kB, kB);
         }
+    }
+    // Slots whose row is not all zeros (8-bit codes); by all lanes of 16 that hold it.
+    __device__ __forceinline__ uint32_t live() const {
+        uint32_t bits = 0;
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            uint32_t any = 0;
+            #pragma unroll
+            for (int d = 0; d < (kB + 3) / 4; ++d) any |= w[j][d];
+            if (any & code_bits<TYPE>) bits |= 1u << j;
+        }
+        return or16(bits);
     }
     // Operands of four dimensions (two of the rest of 96) from one dword of each
     // row: rows are interleaved in pairs, and a pair's bytes are as they stand
@@ -225,6 +254,26 @@ __device__ __forceinline__ float wave_join(float v, float none, Op op) {
 __device__ __forceinline__ float wave_max(float v) {
     return wave_join(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
 }
+// The largest and the least exponent of a wave's values that are not 0 (none:
+// below and above all others), each 2^(e - 1) to 2^e, in one go.
+__device__ __forceinline__ void wave_exponents(float v, int &top, int &low) {
+    typedef uint16_t two __attribute__((ext_vector_type(2)));
+    const int e = __builtin_amdgcn_frexp_expf(v) + 512;
+    two b = v != 0.f ? two{static_cast<uint16_t>(e), static_cast<uint16_t>(1024 - e)} : two{0, 0};
+    auto join = [&](auto ctrl, auto rows) {
+        const int moved = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, b), decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+        b = __builtin_elementwise_max(b, __builtin_bit_cast(two, moved));
+    };
+    join(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xF>{});   // row_shr 1, 2, 4, 8
+    join(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xF>{});
+    join(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xF>{});
+    join(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xF>{});
+    join(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});   // row_bcast 15 into rows 1 and 3
+    join(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});   // row_bcast 31 into rows 2 and 3
+    const uint32_t all = __builtin_amdgcn_readlane(__builtin_bit_cast(int, b), 63);
+    top = static_cast<int>(all & 0xFFFF) - 512;
+    low = 512 - static_cast<int>(all >> 16);
+}
 __device__ __forceinline__ float wave_sum(float v) {
     return wave_join(v, 0.f, [](float a, float b) { return a + b; });
 }
@@ -241,6 +290,36 @@ __device__ __forceinline__ void query_units(int top, float scale, float &factor,
     factor = fin ? ldexpf(1.f, e) : __builtin_nanf("");
     qscale = fin ? ldexpf(scale, -e) : 1.f;
 }
+
+// The units of one query row's products of weights and value scales, 2^(15 - e).
+// e follows the largest product, not the largest scale: a row that this query row
+// does not see, or gives no weight, may have a scale 2^40 times the others'.
+// Products are looked at where the maximum grows, and where the tile's largest
+// scale alone does not say that none overflows.  Nor do rows of zeros count, whose
+// scale says nothing: codes are looked at where a scale is 1, which the writer gives
+// such rows, or a product is 64 times what was known.
+constexpr int kLeastExponent = -112;   // the halves' least step is below fp32's then
+struct ValueUnits {
+    float known = 0.f;                // the largest product, by the present weights
+    float factor = 0x1p127f;          // 2^(15 - e)
+    __device__ __forceinline__ int exponent() const { return 16 - __builtin_amdgcn_frexp_expf(factor); }
+    __device__ __forceinline__ bool holds(float product) const { return product * factor <= 65504.f; }
+    __device__ __forceinline__ bool strange(float product) const { return product > 64.f * known; }
+    // New units by the largest product of a tile and its largest scale, for which
+    // they leave room (2^2); earlier weights (and known) times f: what the sums are
+    // multiplied by.  (Those that are not finite stay so in any units.)
+    __device__ __forceinline__ float renew(float product, float scale, float f) {
+        known = fmaxf(known, product);
+        const int old = exponent();
+        int e = kLeastExponent;
+        if (known > 0.f) {
+            const int ek = __builtin_amdgcn_frexp_expf(known);
+            e = known < INFINITY ? max(max(ek, min(ek + 2, __builtin_amdgcn_frexp_expf(scale))), kLeastExponent) : old;
+        }
+        factor = ldexpf(1.f, 15 - e);
+        return ldexpf(f, old - e);
+    }
+};
 
 // A workgroup: 16 query rows of one (sequence, KV head) over a split's rows,
 // its four waves every fourth tile of 32 rows each; the waves' states meet in
@@ -315,7 +394,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
     #pragma unroll
     for (int c = 0; c < NC; ++c) o[c] = float4v{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
-    int ev = -126;
+    ValueUnits units;
 
     const int32_t *table = a.b.page_table + static_cast<int64_t>(s.table) * a.b.table_stride;
     const int64_t page_stride = static_cast<int64_t>(kvh) * a.kv.page_rows, head_row = static_cast<int64_t>(h) * a.kv.page_rows;
@@ -368,6 +447,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
             }
         // Register r of half hf: row t0 + 16 hf + 4 g + r.
         float mx = -INFINITY, vtop = 0.f;
+        bool one = false;
         const bool edge = t0 + kTile - 1 > seen || !t.present[0] || !t.present[1];
         #pragma unroll
         for (int hf = 0; hf < 2; ++hf)
@@ -388,7 +468,6 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
                 for (int r = 0; r < 4; ++r) {
                     const int at = t0 + 16 * hf + 4 * g + r;
                     st[hf][r] = t.present[hf] && at <= mine ? st[hf][r] : -INFINITY;
-                    if constexpr (kScaled) t.vs[hf][r] = t.present[hf] && at <= last ? t.vs[hf][r] : 0.f;
                 }
         }
         #pragma unroll
@@ -396,43 +475,69 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
             #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 mx = fmaxf(mx, st[hf][r]);
-                if constexpr (kScaled) vtop = fmaxf(vtop, fabsf(t.vs[hf][r]));
+                if constexpr (kScaled) {
+                    vtop = fmaxf(vtop, fabsf(t.vs[hf][r]));
+                    one = one || t.vs[hf][r] == 1.f;
+                }
             }
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn;
-        int en = ev;
         if constexpr (kScaled) {
             vtop = fmaxf(vtop, __shfl_xor(vtop, 16));
             vtop = fmaxf(vtop, __shfl_xor(vtop, 32));
-            en = max(ev, vtop > 0.f ? __builtin_amdgcn_frexp_expf(vtop) : -126);
-            en = __builtin_amdgcn_readfirstlane(en);
         }
-        // The sums follow a larger maximum or exponent, of which there are few.
-        if (en != ev || __builtin_amdgcn_ballot_w64(mn > m)) {
-            const float f = __builtin_amdgcn_exp2f(m - ref);
+        const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn;
+        // The sums follow a larger maximum, of which there are few.
+        const bool more = __builtin_amdgcn_ballot_w64(mn > m);
+        float f = 1.f;
+        if (more) {
+            f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
             l *= f;
-            const float fo = kScaled ? ldexpf(f, ev - en) : f;
-            #pragma unroll
-            for (int c = 0; c < NC; ++c)
-                #pragma unroll
-                for (int r = 0; r < 4; ++r) o[c][r] *= fo;
             m = mn;
-            ev = en;
         }
-        half2v pu[4], pw[4];
         #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-            float y[4];
+        for (int hf = 0; hf < 2; ++hf)
             #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float w = __builtin_amdgcn_exp2f(st[hf][r] - ref);
                 l += w;
-                y[r] = w * (kScaled ? ldexpf(t.vs[hf][r], 14 - ev) : 0x1p14f);
-                if constexpr (kScaled) y[r] = st[hf][r] == -INFINITY ? 0.f : y[r];   // a masked row's scale may be NaN
+                if constexpr (kScaled)   // a masked row's scale may be anything
+                    st[hf][r] = st[hf][r] == -INFINITY ? 0.f : w * t.vs[hf][r];
+                else
+                    st[hf][r] = w;
             }
-            split_pair(y[0], y[1], pu[2 * hf], pw[2 * hf]);
-            split_pair(y[2], y[3], pu[2 * hf + 1], pw[2 * hf + 1]);
+        if (more || (kScaled && __builtin_amdgcn_ballot_w64(m != -INFINITY && !units.holds(vtop)))) {
+            float fo = f;
+            if constexpr (kScaled) {
+                auto largest = [&] {
+                    float y = 0.f;
+                    #pragma unroll
+                    for (int j = 0; j < 8; ++j) y = fmaxf(y, fabsf(st[j / 4][j % 4]));
+                    y = fmaxf(y, __shfl_xor(y, 16));
+                    return fmaxf(y, __shfl_xor(y, 32));
+                };
+                float y = largest();
+                units.known *= f;
+                if (__builtin_amdgcn_ballot_w64(one || units.strange(y))) {
+                    const uint32_t live = t.v.live();
+                    #pragma unroll
+                    for (int j = 0; j < 8; ++j)   // (a scale that is not finite stays)
+                        if (!(live >> j & 1) && fabsf(st[j / 4][j % 4]) < INFINITY) st[j / 4][j % 4] = 0.f;
+                    y = largest();
+                }
+                fo = units.renew(y, vtop, f);
+            }
+            #pragma unroll
+            for (int c = 0; c < NC; ++c)
+                #pragma unroll
+                for (int r = 0; r < 4; ++r) o[c][r] *= fo;
+        }
+        half2v pu[4], pw[4];
+        #pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+            const float k = kScaled ? units.factor : 0x1p15f;
+            split_pair(st[hf][0] * k, st[hf][1] * k, pu[2 * hf], pw[2 * hf]);
+            split_pair(st[hf][2] * k, st[hf][3] * k, pu[2 * hf + 1], pw[2 * hf + 1]);
         }
         const half8 ph = join(pu[0], pu[1], pu[2], pu[3]), pl = join(pw[0], pw[1], pw[2], pw[3]);
         // A row that some token does not see meets it as 0 * value.
@@ -478,7 +583,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     // The waves' states to a common exponent, then into wave 0, in wave order.
-    const float back = kScaled ? ldexpf(1.f, ev - 14) : 0x1p-14f;
+    const float back = kScaled ? ldexpf(1.f, units.exponent() - 15) : 0x1p-15f;
     #pragma unroll
     for (int c = 0; c < NC; ++c)
         #pragma unroll
@@ -546,6 +651,19 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
 // where the matrix instructions are 10.
 constexpr int kChunkTile = 64, kChunkRows = 128;
 
+// The units of products of weights and value scales are 2^(15 - ev), ev the exponent
+// of the largest scale so far, as long as no two scales of the split differ by more
+// than kAlike octaves (a query row's largest product, of its largest weight, is 2^8
+// of them then): nothing is to be done for a query row.  From the first tile on
+// where they do, a query row's weights are taken 2^lift as large, by an addend of
+// the exponential's argument: its own products count, where it sees and weighs the
+// rows and these are not all zeros, and are looked at when the largest known has
+// sunk below 2^8 by larger scores and scales, or when the tile may hold one of more
+// than 2^16.  (With a first row of 2^-8 of the others' values 517 tokens of int8 take
+// 44 us instead of 39, 2048 of float8 759 instead of 629.)
+constexpr int kAlike = 6;
+constexpr float kCoarse = 0x1p8f, kMostLift = 96.f;
+
 template <int HD, int TYPE>
 struct Chunk {
     static constexpr int kCode = code_bytes(TYPE), kWidth = HD == 96 ? 128 : HD;
@@ -561,9 +679,10 @@ struct Chunk {
     static constexpr int kKeyBytes = kChunkTile * kKeyStride, kValueBytes = HD * 2 * kChunkTile;
 
     struct Head {
-        float ks[kChunkTile], vs[kChunkTile];   // vs times 2^(14 - ev)
+        float ks[kChunkTile], vs[kChunkTile];   // vs times 2^(15 - ev)
         uint32_t bad[2];                        // rows that are not finite
-        int ev, pad;
+        int ev;                                 // the exponent of the largest value scale so far
+        int room;                               // 0, or, once scales are apart, 1 + octaves from the tile's largest to 2^ev
     };
     static constexpr int kBuffer = kKeyBytes + kValueBytes + sizeof(Head);
 
@@ -644,7 +763,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
             if (wave < 2)
                 g.scale = (wave == 0 ? a.kv.value_scale : a.kv.key_scale)[page * page_stride + head_row + (group & mask) + (tid & 15)];
     };
-    int top_ev = -126;   // wave 0's: the exponent of the largest value scale so far
+    int top_ev = kLeastExponent, low_ev = INT32_MAX;   // wave 0's: exponents of the value scales so far
     auto store = [&](const Stage &g, int t0, char *buf) {
         auto &head = *reinterpret_cast<typename C::Head *>(buf + C::kKeyBytes + C::kValueBytes);
         const bool edge = t0 + kChunkTile - 1 > seen;
@@ -657,10 +776,12 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
                 const uint64_t all_bad = __builtin_amdgcn_ballot_w64(bad);
                 if (lane < 2 && all_bad) atomicOr(&head.bad[lane], static_cast<uint32_t>(all_bad >> (32 * lane)));
                 const float v = there && !bad ? g.scale : 0.f;
-                const float top = wave_max(fabsf(v));
-                top_ev = max(top_ev, top > 0.f ? __builtin_amdgcn_frexp_expf(top) : -126);
-                head.vs[lane] = ldexpf(v, 14 - top_ev);
-                if (lane == 0) head.ev = top_ev;
+                int top, low;
+                wave_exponents(v, top, low);
+                top_ev = max(top_ev, top);
+                low_ev = min(low_ev, low);
+                head.vs[lane] = ldexpf(v, 15 - top_ev);
+                if (lane == 0) head.ev = top_ev, head.room = low_ev < top_ev - kAlike ? 1 + top_ev - max(top, kLeastExponent) : 0;
             } else if (wave == 1) {
                 head.ks[lane] = fmaf(g.scale, 0.f, g.scale);   // infinite: all its scores are not numbers
             }
@@ -772,11 +893,14 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
         for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
     // The largest score so far in the products' units, and in base 2 (-c).
     float m = -INFINITY, c = INFINITY, l = 0.f;
-    int ev = -126;
+    int ev = kLeastExponent;
+    float lift = 0.f, known = 0.f;   // once scales are apart: l is 2^lift as large; the row's largest product
+    bool apart = false;
 
-    auto take = [&](const char *buf, int t0, uint32_t absent) {
-        const auto &head = *reinterpret_cast<const typename C::Head *>(buf + C::kKeyBytes + C::kValueBytes);
+    auto take = [&](char *buf, int t0, uint32_t absent) {
+        auto &head = *reinterpret_cast<typename C::Head *>(buf + C::kKeyBytes + C::kValueBytes);
         const int en = kScaled ? __builtin_amdgcn_readfirstlane(head.ev) : ev;
+        const int room = kScaled ? __builtin_amdgcn_readfirstlane(head.room) : 0;
         const bool edge = t0 + kChunkTile - 1 > wave_seen || absent;   // some token does not see it whole
         auto scores = [&](int hf, float16v &st) {
             #pragma unroll
@@ -822,21 +946,63 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
             #pragma unroll
             for (int r = 0; r < 14; r += 2) mn = max3(mn, st[r], st[r + 1]);
             mn = max_halves(fmaxf(fmaxf(mn, st[14]), st[15]));
-            if (en != ev || __builtin_amdgcn_ballot_w64(mn > m)) {
+            const char *values = buf + C::kKeyBytes;
+            auto operand = [&](int b, int d) {   // 16 rows of 32 dimensions
+                return *reinterpret_cast<const half8 *>(
+                    values + (32 * d + n) * 2 * kChunkTile + (((4 * hf + 2 * b + hi) ^ C::exchange(32 * d + n)) << 4));
+            };
+            if (room && !apart) {
+                apart = true;
+                known = c == INFINITY ? 0.f : kCoarse;   // of alike scales, at least
+            }
+            // Besides: scales are apart, and the tile may hold a product beyond a row's units.
+            if (en != ev || __builtin_amdgcn_ballot_w64(mn > m || (room && c != INFINITY && lift > static_cast<float>(room)))) {
                 // c is what the weights so far were taken with, rounding and all.
                 const float cn = mn == -INFINITY ? INFINITY : -mn * qscale;
                 const float f = cn == INFINITY ? 1.f : __builtin_amdgcn_exp2f(cn - c);
                 l *= f;
-                const float fo = kScaled ? ldexpf(f, ev - en) : f;
+                float fo = kScaled ? ldexpf(f, ev - en) : f;
+                m = mn;
+                c = cn;
+                ev = en;
+                known *= fo;
+                if (__builtin_expect(room != 0, 0) &&
+                    __builtin_amdgcn_ballot_w64(c != INFINITY && (lift > static_cast<float>(room) || known < kCoarse))) {
+                    uint32_t live = 0;   // rows that are not all zeros, in the scores' order
+                    #pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        uint4v any = {0, 0, 0, 0};
+                        #pragma unroll
+                        for (int d = 0; d < ND; ++d) any |= __builtin_bit_cast(uint4v, operand(b, d));
+                        #pragma unroll
+                        for (int j = 0; j < 8; ++j) live |= any[j / 2] & (j & 1 ? 0x7FFF0000u : 0x7FFFu) ? 1u << (8 * b + j) : 0;
+                    }
+                    live = or16(live);
+                    live |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(live), 16));
+                    #pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        float &at = head.vs[32 * hf + 8 * (r / 4) + 4 * hi + r % 4];
+                        const float vs = at;
+                        // The scale of a row of zeros (a finite one) goes: no sum has
+                        // anything of it, whichever of the two another wave reads.
+                        const bool zeros = !(live >> r & 1) && fabsf(vs) < INFINITY;
+                        if (zeros && n == 0) at = 0.f;
+                        known = fmaxf(known, zeros ? 0.f : fabsf(__builtin_amdgcn_exp2f(fmaf(st[r], qscale, (c == INFINITY ? 0.f : c) + lift)) * vs));
+                    }
+                    known = max_halves(known);
+                    const float to = known > 0.f ? fminf(fmaxf(lift + static_cast<float>(12 - __builtin_amdgcn_frexp_expf(known)), 0.f), kMostLift) : kMostLift;
+                    const float up = known < INFINITY ? __builtin_amdgcn_exp2f(to - lift) : 1.f;
+                    lift = known < INFINITY ? to : lift;
+                    known *= up;
+                    l *= up;
+                    fo *= up;
+                }
                 #pragma unroll
                 for (int d = 0; d < ND; ++d)
                     #pragma unroll
                     for (int r = 0; r < 16; ++r) o[d][r] *= fo;
-                m = mn;
-                c = cn;
-                ev = en;
             }
-            const float ref = c == INFINITY ? 0.f : c;   // nothing seen: weights of exp2(-inf)
+            const float ref = (c == INFINITY ? 0.f : c) + lift;   // nothing seen: weights of exp2(-inf)
             if (t0 + kChunkTile - 1 > seen) {   // flagged for all waves, those that see the whole tile too
                 const uint32_t bad = head.bad[hf] >> (4 * hi);
                 if (__builtin_amdgcn_ballot_w64(bad != 0)) {
@@ -846,7 +1012,6 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
                 }
             }
             if (hf == 0) scores(1, ahead);
-            const char *values = buf + C::kKeyBytes;
             #pragma unroll
             for (int b = 0; b < 2; ++b) {   // 16 rows
                 half2v pu[4], pw[4];
@@ -861,7 +1026,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
                         const float x = st[8 * b + 4 * r4 + r];
                         const float w = __builtin_amdgcn_exp2f(fmaf(x, qscale, ref));
                         l += w;
-                        y[r] = w * (kScaled ? vs[r] : 0x1p14f);
+                        y[r] = w * (kScaled ? vs[r] : 0x1p15f);
                     }
                     split_pair(y[0], y[1], pu[2 * r4], pw[2 * r4]);
                     split_pair(y[2], y[3], pu[2 * r4 + 1], pw[2 * r4 + 1]);
@@ -870,8 +1035,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
                 half8 v[ND];
                 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
-                    v[d] = *reinterpret_cast<const half8 *>(
-                        values + (32 * d + n) * 2 * kChunkTile + (((4 * hf + 2 * b + hi) ^ C::exchange(32 * d + n)) << 4));
+                    v[d] = operand(b, d);
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], pl, o[d], 0, 0, 0);
                 }
                 #pragma unroll
@@ -907,21 +1071,25 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
     const int head = h * G + own;
     const bool none = m == -INFINITY && l == 0.f;
     float *dst;
-    float norm = kScaled ? ldexpf(1.f, ev - 14) : 0x1p-14f;
+    const int back = kScaled ? ev - 15 : -15;
+    float norm = 1.f;
     if (splits > 1) {
+        norm = kScaled ? __builtin_amdgcn_exp2f(-lift) : 1.f;
         dst = a.parts + ((static_cast<int64_t>(s.first + tok) * a.heads + head) * a.part_splits + split) * part_floats(HD);
-        if (hi == 0) *reinterpret_cast<float4 *>(dst) = make_float4(-c, l, 0.f, 0.f);
+        if (hi == 0) *reinterpret_cast<float4 *>(dst) = make_float4(-c, l * norm, 0.f, 0.f);
         dst += 4;
     } else {
         dst = a.out + (s.first + tok) * a.ldout + static_cast<int64_t>(head) * HD;
-        norm = none ? 0.f : norm / l;
+        norm = none ? 0.f : 1.f / l;
     }
     #pragma unroll
     for (int d = 0; d < ND; ++d)
         #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
-            float4 v = make_float4(o[d][4 * r4] * norm, o[d][4 * r4 + 1] * norm, o[d][4 * r4 + 2] * norm, o[d][4 * r4 + 3] * norm);
-            *reinterpret_cast<float4 *>(dst + 32 * d + 8 * r4 + 4 * hi) = v;
+            float v[4];
+            #pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = ldexpf(o[d][4 * r4 + r] * norm, back);
+            *reinterpret_cast<float4 *>(dst + 32 * d + 8 * r4 + 4 * hi) = make_float4(v[0], v[1], v[2], v[3]);
         }
 }
 

@@ -343,6 +343,44 @@ def test_refusals(qk, torch_gpu):
         qk.paged_attention(kv, batch, x.cpu(), x.clone(), 4)
 
 
+# --------------------------------------------- every token for itself --
+#
+# Scores of these cases are at most 8 |q| |k| / |q||k| in natural units (hd 64,
+# normal values): off by 8 * 1.45 * (2^-22 + 8 * 2^-24) = 8.3e-6 in base 2 were
+# all errors alike, 5.8e-6 of a weight, and so of its share; numerator and sum
+# both: 1.2e-5 of a token's sum of |weight * value|.  Halves and fp32 sums add
+# 2^-22 and some 2^-24.
+EACH = 1.3e-5
+
+
+def place(pool, part, t, rows, x):
+    """Rows of sequence t anew, encoded: x [rows, kvh, hd]."""
+    codes, scale, value = (getattr(pool, part) + [None])[:3]
+    c, s, v = paged_ref.encode(x, pool.kind)
+    for i, r in enumerate(rows):
+        page, slot = pool.table[t, r // pool.page_rows], r % pool.page_rows
+        codes[page, :, slot], value[page, :, slot] = c[i], v[i]
+        if scale is not None:
+            scale[page, :, slot] = s[i]
+
+
+def each(got, pool, q, heads):
+    """The largest error of any token and head, of its sum of |weight * value|."""
+    worst, hd, G = 0.0, pool.hd, heads // pool.kvh
+    got = got.reshape(pool.n, heads, hd)
+    for first, count, pos, t in pool.seqs:
+        k, v, present = pool.rows(t, pos + count)
+        for i in range(count):
+            seen = present & (np.arange(pos + count) <= pos + i)
+            for h in range(heads):
+                s = k[seen, h // G] @ q[first + i, h * hd:(h + 1) * hd].astype(np.float64) / np.sqrt(hd)
+                p = np.exp(s - s.max())
+                p /= p.sum()
+                size = (p @ np.abs(v[seen, h // G])).max()
+                worst = max(worst, np.nan_to_num(np.abs(got[first + i, h] - p @ v[seen, h // G]).max(), nan=np.inf) / size)
+    return worst
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("part", ["key", "value"])
 @pytest.mark.parametrize("group", [1, 2, 4])
@@ -370,6 +408,68 @@ def test_not_finite_rows_under_every_wave(qk, torch_gpu, kind, part, group, pos)
 
 
 @pytest.mark.parametrize("kind", ["i8", "e4m3"])
+@pytest.mark.parametrize("octaves", [20, 30, 40, 90])
+@pytest.mark.parametrize("count", [2, 70, 200])
+def test_a_large_value_row_of_later_tokens(qk, torch_gpu, kind, octaves, count):
+    """It costs the tokens before it nothing."""
+    rng = np.random.default_rng(21)
+    pool = paged_ref.Pool(rng, kind, 1, 64, 16, [(count, 50)])
+    at = 50 + count // 2
+    place(pool, "value", 0, [at], rng.standard_normal((1, 1, 64)) * 2.0 ** octaves)
+    q = queries(rng, pool, 2)
+    assert each(run(qk, torch_gpu, pool, q, 2), pool, q, 2) < EACH
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+@pytest.mark.parametrize("octaves", [24, 40])
+@pytest.mark.parametrize("count", [1, 100])
+@pytest.mark.parametrize("at", [0, 37, 300])
+def test_a_large_value_row_of_no_weight(qk, torch_gpu, kind, octaves, count, at):
+    """Every token sees it and gives it e^-80 of another's weight; what it adds,
+    2^40 e^-80, is below 2^-75."""
+    rng = np.random.default_rng(22)
+    pool = paged_ref.Pool(rng, kind, 1, 64, 16, [(count, 400)])
+    place(pool, "value", 0, [at], rng.standard_normal((1, 1, 64)) * 2.0 ** octaves)
+    place(pool, "key", 0, [at], np.full((1, 1, 64), -12.0))   # score -12 * 64 / 8 for q of ones
+    q = queries(rng, pool, 2) * np.float32(0.1) + 1
+    assert each(run(qk, torch_gpu, pool, q, 2), pool, q, 2) < EACH
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+@pytest.mark.parametrize("octaves", [-20, -40, -70])
+@pytest.mark.parametrize("count", [1, 130])
+def test_rows_of_zeros_among_small_values(qk, torch_gpu, kind, octaves, count):
+    """A row of zeros has scale 1, far above its neighbours' scales; and one has
+    every zero but its last."""
+    rng = np.random.default_rng(23)
+    small = lambda *s: rng.standard_normal(s) * 2.0 ** octaves
+    pool = paged_ref.Pool(rng, kind, 1, 64, 16, [(count, 300)])
+    total = 300 + count
+    place(pool, "value", 0, range(total), small(total, 1, 64))
+    zero = [0, 5, 31, 32, 100, 101, 102, 250, 300, total - 1]
+    place(pool, "value", 0, zero, np.zeros((len(zero), 1, 64)))
+    one = small(1, 1, 64)
+    one[..., :63] = 0
+    place(pool, "value", 0, [17], one)
+    q = queries(rng, pool, 2)
+    assert each(run(qk, torch_gpu, pool, q, 2), pool, q, 2) < EACH
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+@pytest.mark.parametrize("count", [1, 200])
+def test_value_scales_far_apart_token_by_token(qk, torch_gpu, kind, count):
+    """Scales over 2^100, in any order and falling with the position."""
+    for order in ("any", "falling", "rising"):
+        rng = np.random.default_rng(24)
+        pool = paged_ref.Pool(rng, kind, 1, 64, 16, [(count, 200)])
+        e = rng.uniform(-60, 40, 200 + count)
+        e = {"any": e, "falling": -np.sort(-e), "rising": np.sort(e)}[order]
+        place(pool, "value", 0, range(200 + count), rng.standard_normal((200 + count, 1, 64)) * 2.0 ** np.floor(e)[:, None, None])
+        q = queries(rng, pool, 2)
+        assert each(run(qk, torch_gpu, pool, q, 2), pool, q, 2) < EACH, order
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
 @pytest.mark.parametrize("count", [1, 40, 300])
 @pytest.mark.parametrize("bad", [np.inf, -np.inf])
 def test_an_infinite_key_scale(qk, torch_gpu, kind, count, bad):
@@ -386,3 +486,39 @@ def test_an_infinite_key_scale(qk, torch_gpu, kind, count, bad):
     assert not np.isfinite(got[sees]).any()
     if count > 1:
         assert rel_l2(got[~sees], want[~sees]) < TOL
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+@pytest.mark.parametrize("heads,kvh,hd", [(4, 2, 64), (3, 1, 96), (4, 2, 128), (8, 1, 256)])
+@pytest.mark.parametrize("count,pos", [(1, 1700), (130, 1500)])
+@pytest.mark.parametrize("workspace", [True, 0])
+def test_value_scales_apart_in_every_head_size(qk, torch_gpu, kind, heads, kvh, hd, count, pos, workspace):
+    """Rows split over workgroups, whole and by one workgroup: a first row far
+    below the others, zeros, rows from some tile on 2^7 and 2^30 as large, the
+    largest seen by later tokens alone."""
+    rng = np.random.default_rng(29)
+    pool = paged_ref.Pool(rng, kind, kvh, hd, 64, [(count, pos)])
+    total = pos + count
+    e = np.zeros(total)
+    e[0], e[500:520], e[1000], e[pos + count // 2:] = -9, 7, -40, 30
+    x = rng.standard_normal((total, kvh, hd)) * 2.0 ** e[:, None, None]
+    x[[3, 64, 700, 1100]] = 0
+    place(pool, "value", 0, range(total), x * 2.0 ** -10)
+    q = queries(rng, pool, heads)
+    got = run(qk, torch_gpu, pool, q, heads, workspace=workspace)
+    assert each(got, pool, q, heads) < EACH * (hd / 64) ** 0.5
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+@pytest.mark.parametrize("octaves", [4, 5, 6, 7, 8, 12])
+@pytest.mark.parametrize("count", [1, 150])
+def test_value_scales_about_the_limit_of_alike(qk, torch_gpu, kind, octaves, count):
+    """Every other row's values so many octaves below the rest, and tokens that see
+    only small ones first."""
+    rng = np.random.default_rng(30)
+    pool = paged_ref.Pool(rng, kind, 1, 64, 16, [(count, 300)])
+    total = 300 + count
+    e = np.where((np.arange(total) % 2 == 0) & (np.arange(total) > 70), 0.0, -octaves)
+    place(pool, "value", 0, range(total), rng.standard_normal((total, 1, 64)) * 2.0 ** e[:, None, None])
+    q = queries(rng, pool, 2)
+    assert each(run(qk, torch_gpu, pool, q, 2), pool, q, 2) < EACH
