@@ -683,7 +683,10 @@ struct Chunk {
         uint32_t bad[2];                        // rows that are not finite
         int ev;                                 // the exponent of the largest value scale so far
         int room;                               // 0, or, once scales are apart, 1 + octaves from the tile's largest to 2^ev
+        int big;                                // ks are times 2^-24: there is one above 2^96
+        int pad[3];
     };
+    static_assert(sizeof(Head) % 16 == 0, "the second buffer's 16-byte reads");
     static constexpr int kBuffer = kKeyBytes + kValueBytes + sizeof(Head);
 
     // Of col + d, col a multiple of kValCols and d below it: that of col xor that of d.
@@ -783,7 +786,12 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
                 head.vs[lane] = ldexpf(v, 15 - top_ev);
                 if (lane == 0) head.ev = top_ev, head.room = low_ev < top_ev - kAlike ? 1 + top_ev - max(top, kLeastExponent) : 0;
             } else if (wave == 1) {
-                head.ks[lane] = fmaf(g.scale, 0.f, g.scale);   // infinite: all its scores are not numbers
+                // Products without it are 2^31 at most (2^14 by 448 by 256 dimensions),
+                // with it 2^14 by 2^128 by 256: 2^126 in the units of such tiles.
+                const bool big = __builtin_amdgcn_ballot_w64(fabsf(g.scale) > 0x1p96f);
+                const float v = big ? g.scale * 0x1p-24f : g.scale;
+                head.ks[lane] = fmaf(v, 0.f, v);   // infinite: all its scores are not numbers
+                if (lane == 0) head.big = big;
             }
         }
         #pragma unroll
@@ -870,7 +878,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
         // would turn: its sign goes to the queries.
         float factor;
         query_units(top, fabsf(a.scale), factor, qscale);
-        qscale = fmaxf(qscale, 0x1p-126f);   // one that underflows is as good as 2^-126
+        qscale = fmaxf(qscale, 0x1p-149f);   // one that underflows is as good as that
         factor = a.scale < 0.f ? -factor : factor;
         #pragma unroll
         for (int x = 0; x < NS; ++x) {
@@ -891,7 +899,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
     for (int d = 0; d < ND; ++d)
         #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
-    // The largest score so far in the products' units, and in base 2 (-c).
+    // The largest score so far, in base 2 (-c) and in the products' units (after large
+    // key scales: that or less).
     float m = -INFINITY, c = INFINITY, l = 0.f;
     int ev = kLeastExponent;
     float lift = 0.f, known = 0.f;   // once scales are apart: l is 2^lift as large; the row's largest product
@@ -901,6 +910,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
         auto &head = *reinterpret_cast<typename C::Head *>(buf + C::kKeyBytes + C::kValueBytes);
         const int en = kScaled ? __builtin_amdgcn_readfirstlane(head.ev) : ev;
         const int room = kScaled ? __builtin_amdgcn_readfirstlane(head.room) : 0;
+        const bool big = kScaled && __builtin_amdgcn_readfirstlane(head.big);
+        const float unit = big ? fminf(qscale * 0x1p24f, 0x1.fffffep127f) : qscale;   // a score's, of the products
         const bool edge = t0 + kChunkTile - 1 > wave_seen || absent;   // some token does not see it whole
         auto scores = [&](int hf, float16v &st) {
             #pragma unroll
@@ -942,7 +953,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
                     st[r] = at <= left && !(hide >> at & 1) ? st[r] : -INFINITY;
                 }
             }
-            float mn = m;
+            float mn = big ? -INFINITY : m;
             #pragma unroll
             for (int r = 0; r < 14; r += 2) mn = max3(mn, st[r], st[r + 1]);
             mn = max_halves(fmaxf(fmaxf(mn, st[14]), st[15]));
@@ -956,13 +967,13 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
                 known = c == INFINITY ? 0.f : kCoarse;   // of alike scales, at least
             }
             // Besides: scales are apart, and the tile may hold a product beyond a row's units.
-            if (en != ev || __builtin_amdgcn_ballot_w64(mn > m || (room && c != INFINITY && lift > static_cast<float>(room)))) {
+            if (en != ev || big || __builtin_amdgcn_ballot_w64(mn > m || (room && c != INFINITY && lift > static_cast<float>(room)))) {
                 // c is what the weights so far were taken with, rounding and all.
-                const float cn = mn == -INFINITY ? INFINITY : -mn * qscale;
+                const float cn = kScaled ? fminf(c, -mn * unit) : mn == -INFINITY ? INFINITY : -mn * qscale;
                 const float f = cn == INFINITY ? 1.f : __builtin_amdgcn_exp2f(cn - c);
                 l *= f;
                 float fo = kScaled ? ldexpf(f, ev - en) : f;
-                m = mn;
+                m = big ? -INFINITY : mn;
                 c = cn;
                 ev = en;
                 known *= fo;
@@ -987,7 +998,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
                         // anything of it, whichever of the two another wave reads.
                         const bool zeros = !(live >> r & 1) && fabsf(vs) < INFINITY;
                         if (zeros && n == 0) at = 0.f;
-                        known = fmaxf(known, zeros ? 0.f : fabsf(__builtin_amdgcn_exp2f(fmaf(st[r], qscale, (c == INFINITY ? 0.f : c) + lift)) * vs));
+                        known = fmaxf(known, zeros ? 0.f : fabsf(__builtin_amdgcn_exp2f(fmaf(st[r], unit, (c == INFINITY ? 0.f : c) + lift)) * vs));
                     }
                     known = max_halves(known);
                     const float to = known > 0.f ? fminf(fmaxf(lift + static_cast<float>(12 - __builtin_amdgcn_frexp_expf(known)), 0.f), kMostLift) : kMostLift;
@@ -1005,7 +1016,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
             const float ref = (c == INFINITY ? 0.f : c) + lift;   // nothing seen: weights of exp2(-inf)
             if (t0 + kChunkTile - 1 > seen) {   // flagged for all waves, those that see the whole tile too
                 const uint32_t bad = head.bad[hf] >> (4 * hi);
-                if (__builtin_amdgcn_ballot_w64(bad != 0)) {
+                if (__builtin_expect(__builtin_amdgcn_ballot_w64(bad != 0) != 0, 0)) {
                     #pragma unroll
                     for (int r = 0; r < 16; ++r)
                         if ((bad >> (8 * (r / 4) + r % 4) & 1) && st[r] != -INFINITY) l = __builtin_nanf("");
@@ -1024,7 +1035,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
                     #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const float x = st[8 * b + 4 * r4 + r];
-                        const float w = __builtin_amdgcn_exp2f(fmaf(x, qscale, ref));
+                        const float w = __builtin_amdgcn_exp2f(fmaf(x, unit, ref));
                         l += w;
                         y[r] = w * (kScaled ? vs[r] : 0x1p15f);
                     }
@@ -1069,7 +1080,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
     l += __shfl_xor(l, 32);
     if (!have) return;
     const int head = h * G + own;
-    const bool none = m == -INFINITY && l == 0.f;
+    const bool none = c == INFINITY && l == 0.f;
     float *dst;
     const int back = kScaled ? ev - 15 : -15;
     float norm = 1.f;

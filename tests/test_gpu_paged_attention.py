@@ -489,6 +489,21 @@ def test_an_infinite_key_scale(qk, torch_gpu, kind, count, bad):
 
 
 @pytest.mark.parametrize("kind", ["i8", "e4m3"])
+@pytest.mark.parametrize("count", [1, 130])
+@pytest.mark.parametrize("octaves", [60, 112])
+def test_large_keys_and_small_queries(qk, torch_gpu, kind, count, octaves):
+    """Ordinary scores of keys some 2^112 and queries some 2^-112, next to rows of
+    2^-20 of such keys."""
+    rng = np.random.default_rng(26)
+    pool = paged_ref.Pool(rng, kind, 1, 64, 16, [(count, 150)])
+    total = 150 + count
+    g = np.where(rng.random(total) < 0.3, -20.0, 0.0) + octaves
+    place(pool, "key", 0, range(total), rng.standard_normal((total, 1, 64)) * 2.0 ** g[:, None, None])
+    q = queries(rng, pool, 2) * np.float32(2.0 ** -octaves)
+    assert each(run(qk, torch_gpu, pool, q, 2), pool, q, 2) < EACH
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
 @pytest.mark.parametrize("heads,kvh,hd", [(4, 2, 64), (3, 1, 96), (4, 2, 128), (8, 1, 256)])
 @pytest.mark.parametrize("count,pos", [(1, 1700), (130, 1500)])
 @pytest.mark.parametrize("workspace", [True, 0])
