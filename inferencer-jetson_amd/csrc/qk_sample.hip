@@ -362,10 +362,13 @@ __device__ __forceinline__ Slope slope_of(float t) {
 }
 
 // The power of two above a segment's weights by its largest logit: t = x c is
-// below it for every x, since p is monotone.
+// below it for every x, since p is monotone.  Slopes below 2^-60 (temperatures of
+// 2^60 and more) are out of range too: x c ends in 0 for an x that the bins'
+// intervals still tell from 0, and an infinite temperature leaves these without
+// numbers.
 __device__ __forceinline__ int exponent_of(float best, const Slope &c) {
     const float p = best * c.hi;
-    return best == -INFINITY ? kNone : !(fabsf(p) < 4096.f) ? kFar : static_cast<int>(floorf(p)) + 1;
+    return best == -INFINITY ? kNone : !(fabsf(p) < 4096.f) || c.hi < 0x1p-60f ? kFar : static_cast<int>(floorf(p)) + 1;
 }
 
 // t = x c = p + lo to some 48 bits, p = (g + 1/2) / 128 + y with y exact, f = 128
@@ -986,9 +989,10 @@ __device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowPara
     // The segment of the random number's token, and the share of its weight that
     // lies before that token.
     const double mine = lane < a.segments ? s.kept_all[lane] : 0., upto = wave_scan(mine), z = wave_last(upto);
+    if (!(z > 0.)) return false;
     const double u = a.uniform[row], goal = u > 0. ? fmin(u, 1.) * z : 0.;
     const uint64_t some = __builtin_amdgcn_ballot_w64(mine > 0.), over = __builtin_amdgcn_ballot_w64(mine > 0. && goal < upto);
-    const int seg = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : 0;
+    const int seg = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
     const double share = (goal - (__shfl(upto, seg) - __shfl(mine, seg))) / __shfl(mine, seg);
     // The segment again, weights as integers: wave sums by quads, then the token.
     const int eg = s.head[seg].e, down = kOctave * octaves_down(e, eg);
@@ -1023,6 +1027,7 @@ __device__ __forceinline__ bool sample_binned(const SampleArgs &a, const RowPara
     __syncthreads();
     static_assert(kQuads * kWaves == 64, "a lane for each sum");
     const uint64_t sum = s.quads[lane], sums = wave_scan(sum), all = wave_last(sums);
+    if (all == 0) return false;
     const double inside = fmax(share, 0.) * static_cast<double>(all);
     const uint64_t want = inside < static_cast<double>(all) ? min(static_cast<uint64_t>(inside), all - 1) : all - 1;
     const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sums > want));

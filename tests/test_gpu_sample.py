@@ -261,3 +261,33 @@ def test_refusals(qk, torch_gpu):
         qk.sample_rows(x.half(), u, o)
     with pytest.raises(qk.QKError, match="contiguous"):
         qk.sample_rows(x.t().contiguous().t(), u, o)
+
+
+@pytest.mark.parametrize("n", [5, 1000, 3000, 20000, 40000])
+@pytest.mark.parametrize("t", [np.inf, 3e38, 1e30, 2e18, 1e15])
+def test_flat_temperatures_with_filters(qk, torch_gpu, n, t):
+    """A temperature that leaves all logits alike, up to an infinite one: top-k and
+    top-p cut by the logits' order; logits of 0 and next to it among them."""
+    rng = np.random.default_rng(n)
+    x = logits(rng, 8, n)
+    x[:, ::5] = 0
+    x[:, 1::5] = rng.choice(np.float32([-1e-20, 1e-20, -1e-30, -0.0, 1e-40, -1e-40]), x[:, 1::5].shape)
+    x[7, : n // 2] = -np.inf
+    half = max(n // 2, 1)
+    params = dict(temperature=[t] * 8, top_k=[0, 2, half, n, 0, 77, 0, 0], top_p=[0.5, 1.0, 0.75, 0.25, 1.0, 0.9, 0.999, 0.5],
+                  min_p=[0, 0, 0, 0, 1.0, 0, 0.5, 0])
+    # Row 4's filter is at the weights' border: they are e^(-d / t), d the distance
+    # to the largest logit, at t = 1e15 below 2^-45 t (28): within 2^-45 of 1, far
+    # closer than the 2^-30 that a weight is held to (at 2e18 and more they are 1 in
+    # 64 bits).  Any token may be kept there.
+    edge = 4 if t == 1e15 else -1
+    rows = [r for r in range(8) if r != edge]
+    for u in (0.0, 0.37, 1 - 2.0 ** -24):
+        check(qk, torch_gpu, x[rows], [u] * len(rows), **{k: [v[r] for r in rows] for k, v in params.items()})
+    if edge >= 0:
+        assert x[4].max() - x[4].min() < 2.0 ** -45 * t
+        got = torch_gpu.empty(1, dtype=torch_gpu.int32, device="cuda")
+        ws = torch_gpu.empty(qk.sample_workspace_bytes(n, 1), dtype=torch_gpu.uint8, device="cuda")
+        one = lambda v: to_dev(torch_gpu, np.float32([v]))
+        qk.sample_rows(to_dev(torch_gpu, x[4:5]), one(0.37), got, temperature=one(t), min_p=one(1.0), workspace=ws)
+        assert 0 <= int(got[0]) < n
