@@ -434,8 +434,9 @@ typedef struct qk_paged_kv {
 } qk_paged_kv;
 
 /* One sequence of a call: its new tokens are rows first .. first + count - 1
-   of q, k, v and out, at positions pos .. pos + count - 1; its row r lies in
-   page page_table[table * table_stride + r / page_rows]. */
+   of q, k, v and out (rows of no other sequence), at positions pos .. pos +
+   count - 1; its row r lies in page page_table[table * table_stride + r /
+   page_rows]. */
 typedef struct qk_paged_seq {
     int32_t first, count, pos, table;
 } qk_paged_seq;
@@ -487,39 +488,40 @@ int qk_rope_tables_f32(float theta, int rot_dim, const qk_rope_scaling *scaling,
 
 /* Rotates every new token's q and k at its position and writes k and v into
    the pages.  q is [n_tokens] rows of heads * head_dim values, ldq apart, its
-   rotation goes to q_out (which may be q with ldq_out = ldq, or NULL with q
-   NULL: no queries); k and v are rows of kv_heads * head_dim.  The first
-   rot_dim values of a head rotate (0: none, and no tables), in pairs (2 i, 2 i
-   + 1) or, with `half`, (i, i + rot_dim / 2), by the tables' row of the token's
-   position, in 64 bits, rounded once.  Tables have `positions` rows of rot_dim
-   / 2 values; a sequence that reaches beyond them is left out.  A token whose
-   page is absent writes no row (its q is rotated).  No two tokens of a call may
-   have the same row.  q, q_out, k, v 16-byte aligned with leading dimensions
-   multiples of 4. */
+   rotation goes to q_out (which may be q with ldq_out = ldq, but share nothing
+   else with q, k or v; or NULL with q NULL: no queries); k and v are rows of
+   kv_heads * head_dim.  The first rot_dim values of a head rotate (0: none, and
+   no tables), in pairs (2 i, 2 i + 1) or, with `half`, (i, i + rot_dim / 2), by
+   the tables' row of the token's position, in 64 bits, rounded once.  Tables
+   have `positions` rows of rot_dim / 2 values; a sequence that reaches beyond
+   them is left out.  A token whose page is absent writes no row (its q is
+   rotated).  No two tokens of a call may have the same row.  q, q_out, k, v
+   16-byte aligned with leading dimensions multiples of 4. */
 int qk_rope_paged_write(const qk_paged_kv *kv, const qk_paged_batch *batch, const float *q, int ldq, float *q_out,
                         int ldq_out, const float *k, int ldk, const float *v, int ldv, int heads, const float *cosine,
                         const float *sine, int positions, int rot_dim, int half, qk_stream stream);
 
 /* The rows of every sequence's count tokens as fp32: row pos + i of a sequence
    goes to row first + i of key_out and value_out (rows of kv_heads * head_dim,
-   ldk and ldv apart; either may be NULL).  Rows of absent pages are 0.
-   16-byte aligned, leading dimensions multiples of 4. */
+   ldk and ldv apart, that share nothing; either may be NULL).  Rows of absent
+   pages are 0.  16-byte aligned, leading dimensions multiples of 4. */
 int qk_paged_read_f32(const qk_paged_kv *kv, const qk_paged_batch *batch, float *key_out, int ldk, float *value_out,
                       int ldv, qk_stream stream);
 
 /* GQA attention of every new token over its sequence's rows 0 .. its own
    position (which hold them already): out = softmax(scale q K^T) V, scale 1 /
    sqrt(head_dim) when 0.  q and out are [n_tokens] rows of heads * head_dim,
-   ldq and ldout apart.  Rows of absent pages take no part; a token that sees
-   no row gets zeros.  Products keep every bit of the cache, 22 bits of q, and of
-   a token's probabilities times value scales 22 bits or 2^-32 of the largest,
-   whatever the scales of rows that it does not see or gives no weight (value
-   scales of a sequence within 2^100 of each other).  A key or value that is not finite makes the outputs
-   of the tokens that see it not finite, and reaches no other.  workspace holds
-   partial results when a sequence's rows are split over workgroups; with less
-   than the queried bytes (or none) the call takes fewer splits.  Calls sharing
-   a workspace must not overlap.  Base alignments 16 bytes, leading dimensions
-   multiples of 4. */
+   ldq and ldout apart; out may be q with ldout = ldq, or shares nothing with it.
+   Rows of absent pages take no part; a token that sees no row gets zeros.
+   Products keep every bit of the cache, 22 bits of q, and of a token's
+   probabilities times value scales 22 bits or 2^-32 of the largest, whatever the
+   scales of rows that it does not see or gives no weight (value scales of a
+   sequence within 2^100 of each other).  A key or value that is not finite makes
+   the outputs of the tokens that see it not finite, and reaches no other.
+   workspace holds partial results when a sequence's rows are split over
+   workgroups; with less than the queried bytes (or none) the call takes fewer
+   splits.  Calls sharing a workspace must not overlap.  Base alignments 16 bytes,
+   leading dimensions multiples of 4. */
 size_t qk_paged_attention_workspace_bytes(const qk_paged_batch *batch, int heads, int kv_heads, int head_dim);
 int qk_paged_attention_f32(const qk_paged_kv *kv, const qk_paged_batch *batch, const float *q, int ldq, float *out,
                            int ldout, int heads, float scale, void *workspace, size_t workspace_bytes,

@@ -10,7 +10,8 @@ namespace qk {
 int check_paged_kv(const char *where, const qk_paged_kv *kv);
 int check_paged_batch(const char *where, const qk_paged_batch *batch);
 
-inline int64_t paged_type_bytes(int type) { return type == QK_TYPE_F16 ? 2 : 1; }
+// Whether n rows of wa values, lda apart from a on, share one with n of wb, ldb apart.
+bool rows_meet(const float *a, int64_t lda, int64_t wa, const float *b, int64_t ldb, int64_t wb, int64_t n);
 
 // Whether a sequence of a batch takes part (qk.h).
 __device__ __forceinline__ bool paged_seq_ok(const qk_paged_seq &s, const qk_paged_batch &b, int page_shift) {

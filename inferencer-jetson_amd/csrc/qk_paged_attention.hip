@@ -1308,6 +1308,9 @@ int qk_paged_attention_f32(const qk_paged_kv *kv, const qk_paged_batch *batch, c
     const int64_t tiles = (static_cast<int64_t>(batch->max_count) * a.group + qk::kRowTile - 1) / qk::kRowTile;
     if (tiles * kv->kv_heads * std::max(a.part_splits, 4) >= 1 << 24)   // (the merge: four tokens' heads)
         return qk::fail(QK_ERR_LIMIT, "qk_paged_attention_f32: too many query rows in one launch");
+    // (In place it may be: a workgroup reads its query rows before it writes them.)
+    if ((q != out || ldq != ldout) && qk::rows_meet(q, ldq, dim, out, ldout, dim, batch->n_tokens))
+        return qk::fail(QK_ERR_INVALID_ARG, "qk_paged_attention_f32: out overlaps a part of q");
     switch (kv->head_dim) {
         case 64: return qk::launch_type<64>(a, qk::S(stream));
         case 96: return qk::launch_type<96>(a, qk::S(stream));

@@ -235,6 +235,8 @@ __global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a) {
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
         if (r < heads) {
             if (active) {
+                // In place too: a row's lanes are of one wave, so all have loaded their
+                // pairs before any of them stores.
                 x = rotate4(a.q + tok * a.ldq + r * HD, c, cosine, sine, a.rot, a.half);
                 *reinterpret_cast<float4 *>(a.q_out + tok * a.ldq_out + r * HD + c) = x;
             }
@@ -356,6 +358,19 @@ unsigned row_blocks(int64_t max_count, int64_t R, int hd) {
 
 }  // namespace
 
+bool rows_meet(const float *a, int64_t lda, int64_t wa, const float *b, int64_t ldb, int64_t wb, int64_t n) {
+    if (!a || !b || n < 1) return false;
+    const int64_t d = (reinterpret_cast<intptr_t>(b) - reinterpret_cast<intptr_t>(a)) / static_cast<int64_t>(sizeof(float));
+    if (d >= (n - 1) * lda + wa || -d >= (n - 1) * ldb + wb) return false;
+    for (int64_t i = d < wa ? 0 : (d - wa) / lda; i < n; ++i) {
+        // The first row of b that ends behind the start of row i of a.
+        const int64_t from = i * lda - d - wb + 1, j = from <= 0 ? 0 : (from + ldb - 1) / ldb;
+        if (j < n && d + j * ldb < i * lda + wa) return true;
+        if (lda == ldb && j > 0 && j < n - 1) return false;   // the rows behind meet alike
+    }
+    return false;
+}
+
 int check_paged_kv(const char *where, const qk_paged_kv *kv) {
     const std::string w(where);
     if (!kv || !kv->key || !kv->value) return fail(QK_ERR_INVALID_ARG, w + ": null cache pointer");
@@ -440,6 +455,9 @@ int qk_rope_tables_f32(float theta, int rot_dim, const qk_rope_scaling *scaling,
         }
     }
     if (positions == 0) return qk::ok();
+    const int64_t values = static_cast<int64_t>(positions) * (rot_dim / 2);
+    if (qk::rows_meet(cosine, values, values, sine, values, values, 1))
+        return qk::fail(QK_ERR_INVALID_ARG, "qk_rope_tables_f32: cosine overlaps sine");
     a.type = type;
     a.rot = rot_dim;
     a.half = rot_dim / 2;
@@ -481,6 +499,10 @@ int qk_rope_paged_write(const qk_paged_kv *kv, const qk_paged_batch *batch, cons
     const int R = (q ? heads : 0) + 2 * kv->kv_heads;
     const unsigned blocks = qk::row_blocks(batch->max_count, R, kv->head_dim);
     if (!blocks) return qk::fail(QK_ERR_LIMIT, "qk_rope_paged_write: too many rows in one launch");
+    if (q && ((q != q_out && qk::rows_meet(q_out, ldq_out, q_dim, q, ldq, q_dim, batch->n_tokens)) ||
+              qk::rows_meet(q_out, ldq_out, q_dim, k, ldk, kv_dim, batch->n_tokens) ||
+              qk::rows_meet(q_out, ldq_out, q_dim, v, ldv, kv_dim, batch->n_tokens)))
+        return qk::fail(QK_ERR_INVALID_ARG, "qk_rope_paged_write: q_out overlaps k, v or a part of q");
     const qk::WriteArgs a{*kv, *batch, q,   k,     v,         cosine,  sine, q_out, ldq,
                           ldq_out, ldk, ldv, heads, positions, rot_dim, half, __builtin_ctz(kv->page_rows)};
     return qk::by_shape<qk::Write>(kv->head_dim, kv->type, a, dim3(blocks, batch->n_seqs), qk::S(stream));
@@ -501,6 +523,8 @@ int qk_paged_read_f32(const qk_paged_kv *kv, const qk_paged_batch *batch, float 
     const int R = ((key_out ? 1 : 0) + (value_out ? 1 : 0)) * kv->kv_heads;
     const unsigned blocks = qk::row_blocks(batch->max_count, R, kv->head_dim);
     if (!blocks) return qk::fail(QK_ERR_LIMIT, "qk_paged_read_f32: too many rows in one launch");
+    if (qk::rows_meet(key_out, ldk, kv_dim, value_out, ldv, kv_dim, batch->n_tokens))
+        return qk::fail(QK_ERR_INVALID_ARG, "qk_paged_read_f32: key_out overlaps value_out");
     const qk::ReadArgs a{*kv, *batch, key_out, value_out, ldk, ldv, __builtin_ctz(kv->page_rows)};
     return qk::by_shape<qk::Read>(kv->head_dim, kv->type, a, dim3(blocks, batch->n_seqs), qk::S(stream));
 }

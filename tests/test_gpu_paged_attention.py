@@ -537,3 +537,21 @@ def test_value_scales_about_the_limit_of_alike(qk, torch_gpu, kind, octaves, cou
     place(pool, "value", 0, range(total), rng.standard_normal((total, 1, 64)) * 2.0 ** e[:, None, None])
     q = queries(rng, pool, 2)
     assert each(run(qk, torch_gpu, pool, q, 2), pool, q, 2) < EACH
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("workspace", [True, 0])
+def test_in_place(qk, torch_gpu, kind, workspace):
+    """Outputs over their queries, bit for bit those elsewhere: both kernels, rows
+    split and whole."""
+    t = torch_gpu
+    rng = np.random.default_rng(31)
+    pool = paged_ref.Pool(rng, kind, 2, 128, 32, [(1, 2000), (170, 900), (1, 50), (3, 700)])
+    q = queries(rng, pool, 8)
+    want = run(qk, t, pool, q, 8, workspace=workspace)
+    kv, batch = pool.dev(qk, t, **bound(pool, 8))
+    nb = qk.paged_attention_workspace_bytes(batch, 8, 2, 128) if workspace else 0
+    ws = t.empty(nb, dtype=t.uint8, device="cuda") if nb else None
+    x = to_dev(t, q)
+    qk.paged_attention(kv, batch, x, x, 8, workspace=ws)
+    assert np.array_equal(x.cpu().numpy(), want)

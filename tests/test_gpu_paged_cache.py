@@ -270,3 +270,23 @@ def test_refusals(qk, torch_gpu):
         qk.paged_read(kv, batch, t.zeros(129, device="cuda")[1:].view(1, 128), None)
     with pytest.raises(qk.QKError, match="contiguous"):
         qk.paged_read(kv, batch, t.zeros(1, 256, device="cuda")[:, ::2], None)
+
+
+def test_queries_beside_their_rotation(qk, torch_gpu):
+    """q and q_out as the two halves of one buffer's rows, and k and v behind."""
+    t = torch_gpu
+    rng = np.random.default_rng(11)
+    heads, kvh, hd = 4, 2, 64
+    pool = paged_ref.Pool(rng, "f16", kvh, hd, 16, [(7, 3), (1, 20)])
+    cos, sin = tables(rng, 21, hd)
+    kv, batch = pool.dev(qk, t)
+    w, kw = heads * hd, kvh * hd
+    f = to_dev(t, rng.standard_normal((pool.n, 2 * w + 2 * kw)).astype(np.float32))
+    before = f.cpu().numpy()
+    qk.rope_paged_write(kv, batch, f[:, :w], f[:, w: 2 * w], f[:, 2 * w: 2 * w + kw], f[:, 2 * w + kw:], to_dev(t, cos), to_dev(t, sin), heads)
+    got, pos = f.cpu().numpy(), np.r_[3:10, 20]
+    want = paged_ref.rotate(before[:, :w].reshape(pool.n, -1, hd), cos[pos], sin[pos], hd, False).reshape(pool.n, -1)
+    assert np.array_equal(bits(got[:, w: 2 * w]), bits(want))
+    assert np.array_equal(got[:, :w], before[:, :w]) and np.array_equal(got[:, 2 * w:], before[:, 2 * w:])
+    with pytest.raises(qk.QKError, match="overlaps"):
+        qk.rope_paged_write(kv, batch, f[:, :w], f[:, hd: w + hd], f[:, 2 * w: 2 * w + kw], f[:, 2 * w + kw:], to_dev(t, cos), to_dev(t, sin), heads)

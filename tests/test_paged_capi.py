@@ -173,3 +173,26 @@ def test_float8_values_and_rows():
         assert s[0] == s[1] == 1 and np.isnan(s[2]) and not x[:2].any() and np.isnan(x[2]).all()
     _, s, x = paged_ref.encode(np.array([[127.0, 0.5, 1.5, -2.5]], dtype=np.float32), "i8")
     assert s[0] == 1 and x[0].tolist() == [127, 0, 2, -2]
+
+
+@pytest.mark.parametrize("over", [
+    dict(q_out=A + 16),                                        # a few values on
+    dict(q_out=A + 4 * 4096 + 16, k=4 * A, v=4 * A),           # a row and a few values on
+    dict(q_out=A - 4 * 4096 + 16, k=4 * A, v=4 * A),
+    dict(q=2 * A, q_out=4 * A, k=4 * A + 4 * (4096 - 4), v=8 * A),   # q_out's last values
+    dict(q=2 * A, q_out=4 * A, k=8 * A, v=4 * A - 4 * 1020),   # and its first
+    dict(q=2 * A, q_out=4 * A, ldq_out=5120, k=4 * A + 4 * 4096, ldk=5000, v=8 * A),   # other strides: from the second row on
+])
+def test_write_refuses_overlaps(qk, over):
+    """q_out may be q, and nothing else of q, k or v (sizes are floats: q rows of
+    4096, k and v rows of 1024, four tokens)."""
+    assert write(qk, **over) == qk.QK_ERR_INVALID_ARG
+    assert b"overlaps" in qk.lib().qk_last_error()
+
+
+def test_read_attention_and_tables_refuse_overlaps(qk):
+    assert read(qk) == read(qk, value_out=A + 4 * 1020) == read(qk, value_out=A + 16 * 1023, ldv=2048) == qk.QK_ERR_INVALID_ARG
+    assert b"overlaps" in qk.lib().qk_last_error()
+    assert attend(qk, out=A + 16) == attend(qk, ldout=4100) == attend(qk, out=A - 16 * 4000, ldout=4100) == qk.QK_ERR_INVALID_ARG
+    assert b"overlaps" in qk.lib().qk_last_error()
+    assert qk.lib().qk_rope_tables_f32(10000.0, 64, None, None, 0, 100, A, A + 4 * 3199, None) == qk.QK_ERR_INVALID_ARG
