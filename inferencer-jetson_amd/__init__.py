@@ -454,6 +454,18 @@ def _torch():
     return _TORCH
 
 
+_INT_MAX = 0x7FFFFFFF
+
+
+def _int(where: str, name: str, n) -> int:
+    """n for an int of the C interface, where a larger one would lose its upper bits
+    (QKError)."""
+    n = int(n)
+    if not -_INT_MAX <= n <= _INT_MAX:
+        raise QKError(where, QK_ERR_LIMIT, f"{name} of {n} is beyond 2^31 - 1")
+    return n
+
+
 def _gpu(where: str, name: str, t):
     """The GPU a tensor is on (QKError if it is on none)."""
     if not t.is_cuda:
@@ -461,13 +473,17 @@ def _gpu(where: str, name: str, t):
     return t.device
 
 
-def _rows(where: str, name: str, t, n: int, w: int, device) -> int:
+def _rows(where: str, name: str, t, n: int, w: int, device, most: int = _INT_MAX) -> int:
     """The leading dimension of a float32 matrix [n][w] of contiguous rows on
-    the device (QKError for anything else)."""
+    the device (QKError for anything else), `most` at most; w of a single row."""
     if t is not None and t.dtype is _TORCH.float32 and t.device == device and t.shape == (n, w):
         ld, one = t.stride()
         if (one == 1 or w == 1) and (ld >= w or n == 1):
-            return ld if ld >= w else w
+            if n == 1:
+                return w
+            if ld > most:
+                raise QKError(where, QK_ERR_LIMIT, f"rows of {name} are {ld} apart, more than 2^31 - 1")
+            return ld
     _want(where, name, t, ("torch.float32",), (n, w), last_contiguous=True)
     raise QKError(where, QK_ERR_INVALID_ARG, f"{name} is on {t.device}, the call's other tensors on {device}")
 
@@ -498,6 +514,8 @@ def _launch(device, stream, fn, *args) -> int:
     if stream is None:
         stream = _TORCH._C._cuda_getCurrentRawStream(index)
     elif not isinstance(stream, int):
+        if stream.device != device:
+            raise QKError(fn.__name__, QK_ERR_INVALID_ARG, f"stream of {stream.device}, tensors on {device}")
         stream = stream.cuda_stream
     if cuda.current_device() == index:
         return fn(*args, stream)
@@ -556,9 +574,10 @@ class PagedBatch:
         _want(where, "seqs", seqs, ("torch.int32",), (None, 4))
         if page_table.device != seqs.device:
             raise QKError(where, QK_ERR_INVALID_ARG, f"tensors on {page_table.device} and {seqs.device}")
-        self.page_table, self.seqs, self.n_tokens = page_table, seqs, int(n_tokens)
-        self.max_count, self.max_rows = int(max_count), int(max_rows)
-        self.desc = qk_paged_batch(ptr(page_table), page_table.shape[0], page_table.shape[1], ptr(seqs), seqs.shape[0],
+        self.page_table, self.seqs, self.n_tokens = page_table, seqs, _int(where, "n_tokens", n_tokens)
+        self.max_count, self.max_rows = _int(where, "max_count", max_count), _int(where, "max_rows", max_rows)
+        rows, stride = (_int(where, "page_table", n) for n in page_table.shape)
+        self.desc = qk_paged_batch(ptr(page_table), rows, stride, ptr(seqs), _int(where, "seqs", seqs.shape[0]),
                                    self.n_tokens, self.max_count, self.max_rows)
         self.ref, self.device = ctypes.byref(self.desc), seqs.device
 
@@ -580,6 +599,8 @@ def rope_tables(theta: float, rot_dim: int, cosine, sine, first_pos: int = 0, sc
     where = "rope_tables"
     f32 = _torch().float32
     positions = cosine.shape[0] if cosine.dim() == 2 else -1
+    if not 0 <= first_pos <= _INT_MAX - positions:
+        raise QKError(where, QK_ERR_LIMIT, f"{positions} positions from {first_pos} on: beyond 0 to 2^31 - 1")
     device = _gpu(where, "cosine", cosine)
     c_ptr = _dense(where, "cosine", cosine, f32, (positions, rot_dim // 2), device)
     s_ptr = _dense(where, "sine", sine, f32, (positions, rot_dim // 2), device)
@@ -612,7 +633,7 @@ def rope_paged_write(kv: PagedKV, batch: PagedBatch, q, q_out, k, v, cosine, sin
     ldk, ldv = _rows(where, "k", k, n, w, device), _rows(where, "v", v, n, w, device)
     if rot_dim:
         f32 = _TORCH.float32
-        positions = cosine.shape[0] if cosine is not None and cosine.dim() == 2 else -1
+        positions = _int(where, "positions", cosine.shape[0]) if cosine is not None and cosine.dim() == 2 else -1
         c_ptr = _dense(where, "cosine", cosine, f32, (positions, rot_dim // 2), device)
         s_ptr = _dense(where, "sine", sine, f32, (positions, rot_dim // 2), device)
     check(_launch(device, stream, lib().qk_rope_paged_write, kv.ref, batch.ref, q_ptr, ldq, qo_ptr, ldq_out,
@@ -636,7 +657,10 @@ def paged_read(kv: PagedKV, batch: PagedBatch, key_out, value_out, stream=None) 
 
 def paged_attention_workspace_bytes(batch: PagedBatch, heads: int, kv_heads: int, head_dim: int) -> int:
     """Workspace bytes of paged_attention."""
-    return int(lib().qk_paged_attention_workspace_bytes(batch.ref, heads, kv_heads, head_dim))
+    where = "paged_attention_workspace_bytes"
+    return int(lib().qk_paged_attention_workspace_bytes(batch.ref, _int(where, "heads", heads),
+                                                        _int(where, "kv_heads", kv_heads),
+                                                        _int(where, "head_dim", head_dim)))
 
 
 def paged_attention(kv: PagedKV, batch: PagedBatch, q, out, heads: int, scale: float = 0.0, workspace=None,
@@ -654,7 +678,8 @@ def paged_attention(kv: PagedKV, batch: PagedBatch, q, out, heads: int, scale: f
 
 def sample_workspace_bytes(n: int, rows: int) -> int:
     """Workspace bytes of sample_rows for rows of n logits."""
-    return int(lib().qk_sample_rows_workspace_bytes(n, rows))
+    where = "sample_workspace_bytes"
+    return int(lib().qk_sample_rows_workspace_bytes(_int(where, "n", n), _int(where, "rows", rows)))
 
 
 def sample_rows(logits, uniform, out, temperature=None, top_k=None, top_p=None, min_p=None, prob=None, workspace=None,
@@ -669,7 +694,7 @@ def sample_rows(logits, uniform, out, temperature=None, top_k=None, top_p=None, 
         raise QKError(where, QK_ERR_SHAPE, f"logits has shape {tuple(logits.shape)}, expected rows of logits")
     rows, n = logits.shape
     device = _gpu(where, "logits", logits)
-    ldv = _rows(where, "logits", logits, rows, n, device)
+    ldv = _rows(where, "logits", logits, _int(where, "rows", rows), _int(where, "logits a row", n), device, most=1 << 62)
     f32, i32, shape = torch.float32, torch.int32, (rows,)
     of = lambda name, t, dt: None if t is None else _dense(where, name, t, dt, shape, device)
     u_ptr, o_ptr = _dense(where, "uniform", uniform, f32, shape, device), _dense(where, "out", out, i32, shape, device)

@@ -290,3 +290,27 @@ def test_queries_beside_their_rotation(qk, torch_gpu):
     assert np.array_equal(got[:, :w], before[:, :w]) and np.array_equal(got[:, 2 * w:], before[:, 2 * w:])
     with pytest.raises(qk.QKError, match="overlaps"):
         qk.rope_paged_write(kv, batch, f[:, :w], f[:, hd: w + hd], f[:, 2 * w: 2 * w + kw], f[:, 2 * w + kw:], to_dev(t, cos), to_dev(t, sin), heads)
+
+
+def test_sizes_beyond_an_int(qk, torch_gpu):
+    """Bounds and strides whose lower 32 bits would be fine are refused; a single
+    row has no stride to refuse."""
+    t = torch_gpu
+    kv = qk.PagedKV.empty(qk.F16, 4, 2, 16, 64)
+    table, seqs = t.zeros(1, 4, dtype=t.int32, device="cuda"), t.tensor([[0, 2, 0, 0]], dtype=t.int32, device="cuda")
+    for sizes in ((2 ** 32 + 2, 2, 2), (2, 2 ** 32 + 2, 2), (2, 2, 2 ** 32 + 2)):
+        with pytest.raises(qk.QKError, match="beyond"):
+            qk.PagedBatch(table, seqs, *sizes)
+    batch = qk.PagedBatch(table, seqs, 2, 2, 2)
+    far = t.empty(2 ** 32 + 256, device="cuda")      # 17 GB, never touched
+    with pytest.raises(qk.QKError, match="apart"):
+        qk.paged_read(kv, batch, far.as_strided((2, 128), (2 ** 32 + 128, 1)), None)
+    with pytest.raises(qk.QKError, match="beyond"):
+        qk.rope_tables(1e4, 64, t.empty(2, 32, device="cuda"), t.empty(2, 32, device="cuda"), first_pos=2 ** 32)
+    one = qk.PagedBatch(table, t.tensor([[0, 1, 0, 0]], dtype=t.int32, device="cuda"), 1, 1, 1)
+    odd = t.full((1, 131), 7.0, device="cuda")
+    kv.key.zero_()
+    qk.paged_read(kv, one, odd[:, :128], None)
+    assert not odd[:, :128].any() and (odd[:, 128:] == 7).all()
+    qk.paged_read(kv, one, far.as_strided((1, 128), (2 ** 32 + 128, 1)), None)
+    assert not far[:128].any()

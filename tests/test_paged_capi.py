@@ -196,3 +196,22 @@ def test_read_attention_and_tables_refuse_overlaps(qk):
     assert attend(qk, out=A + 16) == attend(qk, ldout=4100) == attend(qk, out=A - 16 * 4000, ldout=4100) == qk.QK_ERR_INVALID_ARG
     assert b"overlaps" in qk.lib().qk_last_error()
     assert qk.lib().qk_rope_tables_f32(10000.0, 64, None, None, 0, 100, A, A + 4 * 3199, None) == qk.QK_ERR_INVALID_ARG
+
+
+def test_wrappers_refuse_what_an_int_does_not_hold(qk):
+    """ctypes would pass the lower 32 bits on."""
+    for call in (lambda: qk.sample_workspace_bytes(1000, 2 ** 32 + 1), lambda: qk.sample_workspace_bytes(2 ** 32 + 1000, 1)):
+        with pytest.raises(qk.QKError, match="beyond"):
+            call()
+
+
+def test_wrappers_refuse_a_stream_of_another_device(qk):
+    torch = qk._torch()
+
+    class Stream:
+        device, cuda_stream = torch.device("cuda", 1), 0
+
+    def launched(*args):
+        raise AssertionError("launched")
+    with pytest.raises(qk.QKError, match="stream of cuda:1"):
+        qk._launch(torch.device("cuda", 0), Stream, launched)
