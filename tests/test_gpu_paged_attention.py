@@ -503,6 +503,45 @@ def test_large_keys_and_small_queries(qk, torch_gpu, kind, count, octaves):
     assert each(run(qk, torch_gpu, pool, q, 2), pool, q, 2) < EACH
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("count", [1, 130])
+def test_peaked_rows_element_by_element(qk, torch_gpu, kind, count):
+    """One row of far the highest score: its value, to the halves' bits."""
+    rng = np.random.default_rng(27)
+    pool = paged_ref.Pool(rng, kind, 1, 64, 16, [(count, 350)])
+    q = queries(rng, pool, 1)
+    best = rng.integers(0, 350, count)
+    best = best if count == 1 else np.arange(count) * 350 // count   # a row each
+    place(pool, "key", 0, best, q.reshape(count, 1, 64) * 20)        # score 20 |q|^2 / 8, of others some 20 |q| at most
+    k, v, _ = pool.rows(0, 350 + count)
+    got = run(qk, torch_gpu, pool, q, 1)
+    for i in range(count):
+        s = np.sort(k[: 351 + i, 0] @ q[i].astype(np.float64) / 8)
+        assert s[-1] - s[-2] > 40   # e^-40 = 2^-57
+        assert np.abs(got[i] - v[best[i], 0]).max() <= 2.0 ** -21 * np.abs(v[best[i], 0]).max()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("count", [1, 150])
+def test_absent_pages_read_nothing_of_the_first_page(qk, torch_gpu, kind, count):
+    """Page 0, which no sequence holds, is full of what is not finite."""
+    rng = np.random.default_rng(28)
+    pool = paged_ref.Pool(rng, kind, 2, 64, 16, [(count, 200), (1, 40)])
+    held = pool.table == 0
+    free = np.setdiff1d(np.arange(pool.pages), pool.table[pool.table >= 0])[0]
+    for part in (pool.key, pool.value):       # page 0 changes places with a free one
+        for a in part:
+            if a is not None:
+                a[[0, free]] = a[[free, 0]]
+    pool.table[held] = free
+    pool.table[0, 3:7] = -1
+    pool.table[0, 9] = pool.pages
+    assert not (pool.table == 0).any()
+    pool.poison(pool.unused())
+    q = queries(rng, pool, 4)
+    assert rel_l2(run(qk, torch_gpu, pool, q, 4), pool.attention(q, 4)) < TOL
+
+
 @pytest.mark.parametrize("kind", ["i8", "e4m3"])
 @pytest.mark.parametrize("heads,kvh,hd", [(4, 2, 64), (3, 1, 96), (4, 2, 128), (8, 1, 256)])
 @pytest.mark.parametrize("count,pos", [(1, 1700), (130, 1500)])

@@ -291,3 +291,46 @@ def test_flat_temperatures_with_filters(qk, torch_gpu, n, t):
         one = lambda v: to_dev(torch_gpu, np.float32([v]))
         qk.sample_rows(to_dev(torch_gpu, x[4:5]), one(0.37), got, temperature=one(t), min_p=one(1.0), workspace=ws)
         assert 0 <= int(got[0]) < n
+
+
+@pytest.mark.parametrize("n", [131073, 151936, 262144, 524288])
+def test_rows_of_many_segments(qk, torch_gpu, n):
+    """More than eight segments of 16384 logits, whose heads and histograms are
+    gone through by eights; the largest logits in the first, the last or any."""
+    rng = np.random.default_rng(n)
+    x = logits(rng, 6, n)
+    x[1, -100:] = 20 + rng.random(100)
+    x[2, :100] = 20 + rng.random(100)
+    x[3, 16384 * 8: 16384 * 8 + 1] = 30
+    x[4, : n - 16384 - 3] = -np.inf
+    for params in (dict(), dict(top_k=[40] * 6, top_p=[0.9] * 6), dict(top_p=[0.9, 0.6, 0.99, 0.999, 0.5, 0.95], temperature=[1.5, 1, 0.7, 3, 1, 2]),
+                   dict(min_p=[0.05] * 6), dict(top_k=[3000] * 6, min_p=[1e-4] * 6)):
+        for u in (0.1, 0.6, 1 - 2.0 ** -24):
+            check(qk, torch_gpu, x, [u] * 6, **params)
+
+
+@pytest.mark.parametrize("low", [-1e4, -1e9, float(np.finfo(np.float32).min), -np.inf])
+def test_masked_vocabularies(qk, torch_gpu, low):
+    """All but a few tokens at a finite value or -inf, over whole segments of the
+    row, next to a row without a mask."""
+    rng = np.random.default_rng(12)
+    n = 128256
+    x = logits(rng, 5, n)
+    keep = rng.choice(n, 200, replace=False)
+    for r in (0, 2):
+        masked = np.full(n, low, np.float32)
+        masked[keep] = x[r, keep]
+        x[r] = masked
+    x[1, 16384: 5 * 16384] = low
+    x[4, :] = low
+    for params in (dict(), dict(top_k=[50] * 5, top_p=[0.9] * 5), dict(top_p=[0.95] * 5, temperature=[0.7] * 5), dict(min_p=[0.1] * 5)):
+        for u in (0.0, 0.5, 1 - 2.0 ** -24):
+            check(qk, torch_gpu, x, [u] * 5, **params)
+
+
+@pytest.mark.parametrize("n,spread,t,p", [(151936, 2.2, 2.0, 0.9), (262144, 2.2, 1.5, 0.9), (128256, 1.5, 1.5, 0.9), (128256, 2.2, 3.0, 0.9)])
+def test_more_tokens_at_the_cut_than_its_list(qk, torch_gpu, n, spread, t, p):
+    """Ordinary logits at high temperatures: some thousands share the cut's bin."""
+    rng = np.random.default_rng(13)
+    x = (rng.standard_normal((3, n)) * spread).astype(np.float32)
+    check(qk, torch_gpu, x, [0.3, 0.9, 0.999], temperature=[t] * 3, top_p=[p] * 3)
