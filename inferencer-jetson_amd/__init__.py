@@ -475,12 +475,13 @@ def _gpu(where: str, name: str, t):
 
 def _rows(where: str, name: str, t, n: int, w: int, device, most: int = _INT_MAX) -> int:
     """The leading dimension of a float32 matrix [n][w] of contiguous rows on
-    the device (QKError for anything else), `most` at most; w of a single row."""
+    the device (QKError for anything else), `most` at most; of a single row w
+    where its own would be refused."""
     if t is not None and t.dtype is _TORCH.float32 and t.device == device and t.shape == (n, w):
         ld, one = t.stride()
         if (one == 1 or w == 1) and (ld >= w or n == 1):
             if n == 1:
-                return w
+                return ld if w <= ld <= most and ld % 4 == 0 else w
             if ld > most:
                 raise QKError(where, QK_ERR_LIMIT, f"rows of {name} are {ld} apart, more than 2^31 - 1")
             return ld
@@ -514,7 +515,7 @@ def _launch(device, stream, fn, *args) -> int:
     if stream is None:
         stream = _TORCH._C._cuda_getCurrentRawStream(index)
     elif not isinstance(stream, int):
-        if stream.device != device:
+        if getattr(stream, "device", device) != device:
             raise QKError(fn.__name__, QK_ERR_INVALID_ARG, f"stream of {stream.device}, tensors on {device}")
         stream = stream.cuda_stream
     if cuda.current_device() == index:
