@@ -478,11 +478,12 @@ typedef struct qk_rope_scaling {
 } qk_rope_scaling;
 
 /* cosine[p * rot_dim / 2 + i] and sine[...] of (first_pos + p) * f_i for p <
-   positions, in 64 bits, rounded once: the tables that qk_rope_kv_write*,
-   qk_rope_paged_write and the decode drivers' own rotation take.  scaling may
-   be NULL (QK_ROPE_NONE); freq_factors (device, rot_dim / 2 values, or NULL)
-   divide the frequencies before the scaling (a GGUF file's rope_freqs.weight).
-   rot_dim even, at most 512; at most 2^30 positions. */
+   positions, in 64 bits, rounded once: the tables that qk_rope_kv_write* and
+   qk_rope_paged_write take.  (The decode drivers build their own from rope_theta
+   and take none.)  scaling may be NULL (QK_ROPE_NONE); freq_factors (device,
+   rot_dim / 2 values, or NULL) divide the frequencies before the scaling (a GGUF
+   file's rope_freqs.weight).  rot_dim even, at most 512; at most 2^30 positions;
+   cosine and sine share nothing. */
 int qk_rope_tables_f32(float theta, int rot_dim, const qk_rope_scaling *scaling, const float *freq_factors,
                        int first_pos, int positions, float *cosine, float *sine, qk_stream stream);
 
@@ -528,9 +529,9 @@ int qk_paged_attention_f32(const qk_paged_kv *kv, const qk_paged_batch *batch, c
                            qk_stream stream);
 
 /* The next token of each of `rows` rows of n logits (row r at logits + r *
-   ldv).  Of row r, with w_i = exp((logit_i - max) / temperature[r]) held to
-   2^-30 of itself (a token below 2^-45 may have no weight), tokens in descending
-   order of their logits (equal ones by index):
+   ldv).  Of row r, with w_i = exp((logit_i - max) / temperature[r]) held to 2^-30
+   of itself and 2^-45 (a token below that may have no weight), tokens in
+   descending order of their logits (equal ones by index):
      top_k[r]  keeps the first top_k (<= 0: all),
      top_p[r]  of those the shortest run whose weights reach top_p of their sum
                (1: all),
@@ -540,11 +541,14 @@ int qk_paged_attention_f32(const qk_paged_kv *kv, const qk_paged_batch *batch, c
    prob (or NULL) receives its share of that sum.  temperature[r] <= 0, or a
    parameter that is NaN, keeps the first alone.  NaN logits count as -inf;
    where a logit is +inf, those that are share the weight.  A row without a
-   logit above -inf gives 0 with prob 0.  A row's
-   token does not depend on the other rows.  All arrays are on
-   the device; temperature, top_k, top_p and min_p hold `rows` values, or are
-   NULL: 1, and no filter.  workspace: qk_sample_rows_workspace_bytes(n, rows)
-   bytes, 256-byte aligned; calls sharing it must not overlap. */
+   logit above -inf gives 0 with prob 0.  A row's token does not depend on the
+   other rows.  All arrays are on the device; temperature, top_k, top_p and min_p
+   hold `rows` values, or are NULL: 1, and no filter.  At most 2^19 logits.  A row
+   with thousands of tokens of like weight at the cut, with 16384 aligned logits
+   that are all finite but far from its others (|logit / temperature| above some
+   2800) or with a temperature of 2^60 takes ten to thirty times as long as others.
+   workspace: qk_sample_rows_workspace_bytes(n, rows) bytes, 256-byte aligned;
+   calls sharing it must not overlap. */
 size_t qk_sample_rows_workspace_bytes(int n, int rows);
 int qk_sample_rows_f32(const float *logits, int n, int64_t ldv, int rows, const float *temperature,
                        const int32_t *top_k, const float *top_p, const float *min_p, const float *uniform,

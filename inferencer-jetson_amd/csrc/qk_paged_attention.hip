@@ -326,10 +326,11 @@ struct ValueUnits {
 // LDS.  Few query rows leave the cache as the bound, so nothing is staged: a lane
 // loads its own share of both operands, the next tile's while this one is
 // multiplied.  64 sequences over 1000 to 8000 rows, 8 KV heads of 128 int8 values:
-// 611 MB in 134 us, 4.6 TB/s (a copy reaches 4.7); one over 700 rows of 64 fp16
-// values: 5.8 us, the latency of its loads, and 3.4 of the merge.  Two workgroups a
-// CU up to 128 dimensions: left to itself the compiler takes registers beyond that
-// (fp16 rows of 128, 4 sequences of 8000: 33 us, with the bound 28).
+// 611 MB in 136 us, 4.5 TB/s (a copy reaches 4.7, a plain reading 6.15); one over
+// 700 rows of 64 fp16 values: 5.9 us, the latency of its loads, and 3.1 of the
+// merge.  Two workgroups a CU up to 128 dimensions: left to itself the compiler
+// takes registers beyond that (fp16 rows of 128, 4 sequences of 8000: 33 us, with
+// the bound 28).
 template <int HD, int TYPE>
 __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel(PagedAttn a) {
     constexpr int NS = HD / 32, NC = HD / 16, kCode = code_bytes(TYPE);
@@ -644,7 +645,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
 //
 // The bound is the matrix instructions, twice the products of one fp16 pass: 2048
 // tokens over 8192 earlier rows, 32 heads of 128 float8 values, are 620 GFLOP of
-// them, in 607 to 637 us 1.0 PFLOP/s, where a library product of two fp16 matrices
+// them, in 616 to 645 us 1.0 PFLOP/s, where a library product of two fp16 matrices
 // of 8192 reaches 1.15 (both below the instructions' peak, at a clock of 1.9 GHz).
 // The 16-row kernel took 1150 us.  Short chunks are bound by the latency of a
 // workgroup's steps: 517 tokens over 600, 24 heads, 31 us and 7.5 of the merge,
@@ -1160,14 +1161,16 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
 // if the call's chunks are kManyUnits workgroups of it unsplit, or have kManyPairs
 // pairs of a query row and a cache row.  Four query heads for each of eight KV
 // heads of 128 int8 values, the chunk kernel against the first, in us: one
-// sequence, 68 query rows a KV head over 4000 cache rows (2.2 million pairs) 24
-// and 18, 256 over 4000 (8.3 million) 29 and 29, 1600 over 500 (12 million) 36 and
-// 37, 512 over 4000 (17 million) 40 and 53, 2000 over none (8 million, 128
+// sequence, 68 query rows a KV head over 4000 cache rows (2.2 million pairs) 23
+// and 19, 256 over 4000 (8.3 million) 30 and 30, 1600 over 500 (12 million) 36 and
+// 38, 512 over 4000 (17 million) 40 and 56, 2000 over none (8 million, 128
 // workgroups) 32 and 23; eight sequences, 256 over 500 (9.2 million, 128
-// workgroups) 35 and 32, 68 over 4000 (17 million) 51 and 72, 512 over none (256
-// workgroups) 19 and 27; 64 sequences, 68 over none (512 workgroups) 18 and 29.
+// workgroups) 33 and 33, 68 over 4000 (17 million) 48 and 76, 512 over none (256
+// workgroups) 16 and 28; 64 sequences, 68 over none (512 workgroups) 15 and 30.
 // Eight query heads of 256 for one KV head, one sequence of 2048 tokens over 4000:
-// int8 322 and 409, fp16 358 and 403; eight of 64 over 4000: 86 and 89, 97 and 84.
+// int8 344 and 413, fp16 355 and 405; eight of 64 over 4000: 88 and 87, 95 and 85,
+// where the first kernel would be the faster one: the rule sees neither head size
+// nor type.
 constexpr int kFewRows = 64, kManyUnits = 256;
 constexpr int64_t kManyPairs = 3 << 22;
 // Query rows a KV head up to which a sequence of this call takes the first
@@ -1188,7 +1191,7 @@ int few_rows(const qk_paged_batch &b, int heads, int kv_heads) {
 // in 16 splits 9.7, in eight 11.0; 8000 rows in 32 splits 12.5, in 63 14.0.  16
 // sequences of 8000 rows: in one round of workgroups 51 us, in two 55.)  Sequences
 // that fill the chip as they are even out in four splits, if those are long: 64
-// sequences of 1000 to 8000 rows 136 us, 146 whole (of equal lengths the other way
+// sequences of 1000 to 8000 rows 137 us, 146 whole (of equal lengths the other way
 // round, 217 and 197); of 125 to 1000 rows whole 24, in four splits 31.
 // Chunks: a round of workgroups likewise, of at least four tiles; those that lie
 // behind all that a chunk's first tokens see end at once and do not count.
