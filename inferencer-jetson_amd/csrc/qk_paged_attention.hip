@@ -49,8 +49,8 @@ struct PagedAttn {
 constexpr int kTile = 32;      // cache rows of a tile
 constexpr int kRowTile = 16;   // query rows of a workgroup
 
-// A split's partial of one (token, head): the running maximum and the sum (in
-// base-2 units), padded to 4, then head_dim sums.
+// A split's partial of one (token, head): the largest score and the sum of weights
+// (in base-2 units), padded to 4, then head_dim means.
 constexpr int part_floats(int hd) { return 4 + hd; }
 
 constexpr int code_bytes(int type) { return type == QK_TYPE_F16 ? 2 : 1; }
@@ -583,12 +583,14 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    // The waves' states to a common exponent, then into wave 0, in wave order.
-    const float back = kScaled ? ldexpf(1.f, units.exponent() - 15) : 0x1p-15f;
+    // The waves' means (sums could pass fp32's range), then into wave 0, in wave order.
+    auto share_of = [](float l) { return l == 0.f ? 0.f : 1.f / l; };   // no row seen: zeros
+    const int back = (kScaled ? units.exponent() : 0) - 15;
+    const float inverse = share_of(l);
     #pragma unroll
     for (int c = 0; c < NC; ++c)
         #pragma unroll
-        for (int r = 0; r < 4; ++r) o[c][r] *= back;
+        for (int r = 0; r < 4; ++r) o[c][r] = ldexpf(o[c][r] * inverse, back);
     if (wave > 0) {
         float *mineat = meet[wave - 1];
         #pragma unroll
@@ -600,37 +602,46 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
     }
     __syncthreads();
     if (wave > 0) return;
-    #pragma unroll 1
+    float mw[4] = {m}, lw[4] = {l};
+    #pragma unroll
     for (int w = 0; w < 3; ++w) {
-        const float *other = meet[w];
-        const float mo = other[HD * 16 + 2 * n], lo = other[HD * 16 + 2 * n + 1];
-        const float mn = fmaxf(m, mo), ref = mn == -INFINITY ? 0.f : mn;
-        const float f = __builtin_amdgcn_exp2f(m - ref), fo = __builtin_amdgcn_exp2f(mo - ref);
-        m = mn;
-        l = l * f + lo * fo;
+        mw[w + 1] = meet[w][HD * 16 + 2 * n];
+        lw[w + 1] = meet[w][HD * 16 + 2 * n + 1];
+    }
+    m = fmaxf(fmaxf(mw[0], mw[1]), fmaxf(mw[2], mw[3]));
+    l = 0.f;
+    #pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        lw[w] *= __builtin_amdgcn_exp2f(mw[w] - (m == -INFINITY ? 0.f : m));
+        l += lw[w];
+    }
+    const float whole = share_of(l);
+    #pragma unroll
+    for (int c = 0; c < NC; ++c)
+        #pragma unroll
+        for (int r = 0; r < 4; ++r) o[c][r] *= lw[0] * whole;
+    #pragma unroll
+    for (int w = 0; w < 3; ++w) {
+        const float f = lw[w + 1] * whole;
         #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const float4v po = *reinterpret_cast<const float4v *>(other + (c * 64 + lane) * 4);
+            const float4v po = *reinterpret_cast<const float4v *>(meet[w] + (c * 64 + lane) * 4);
             #pragma unroll
-            for (int r = 0; r < 4; ++r) o[c][r] = fmaf(po[r], fo, o[c][r] * f);
+            for (int r = 0; r < 4; ++r) o[c][r] = fmaf(po[r], f, o[c][r]);
         }
     }
     if (!have) return;
     const int head = h * G + own;
-    float *dst;
-    float norm = 1.f;
+    float *dst = a.out + (s.first + tok) * a.ldout + static_cast<int64_t>(head) * HD;
     if (splits > 1) {
         dst = a.parts + ((static_cast<int64_t>(s.first + tok) * a.heads + head) * a.part_splits + split) * part_floats(HD);
         if (g == 0) *reinterpret_cast<float4 *>(dst) = make_float4(m, l, 0.f, 0.f);
         dst += 4;
-    } else {
-        dst = a.out + (s.first + tok) * a.ldout + static_cast<int64_t>(head) * HD;
-        norm = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;   // no row seen: zeros
     }
     #pragma unroll
     for (int r = 0; r < 4; ++r)
         #pragma unroll
-        for (int c = 0; c < NC; ++c) dst[value_dim<HD, TYPE>(4 * g + r, c)] = o[c][r] * norm;
+        for (int c = 0; c < NC; ++c) dst[value_dim<HD, TYPE>(4 * g + r, c)] = o[c][r];
 }
 
 // -------------------------------------------------------------- chunks --
@@ -1081,18 +1092,13 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
     l += __shfl_xor(l, 32);
     if (!have) return;
     const int head = h * G + own;
-    const bool none = c == INFINITY && l == 0.f;
-    float *dst;
     const int back = kScaled ? ev - 15 : -15;
-    float norm = 1.f;
+    const float inverse = l == 0.f ? 0.f : 1.f / l;   // no row seen: zeros
+    float *dst = a.out + (s.first + tok) * a.ldout + static_cast<int64_t>(head) * HD;
     if (splits > 1) {
-        norm = kScaled ? __builtin_amdgcn_exp2f(-lift) : 1.f;
         dst = a.parts + ((static_cast<int64_t>(s.first + tok) * a.heads + head) * a.part_splits + split) * part_floats(HD);
-        if (hi == 0) *reinterpret_cast<float4 *>(dst) = make_float4(-c, l * norm, 0.f, 0.f);
+        if (hi == 0) *reinterpret_cast<float4 *>(dst) = make_float4(-c, kScaled ? l * __builtin_amdgcn_exp2f(-lift) : l, 0.f, 0.f);
         dst += 4;
-    } else {
-        dst = a.out + (s.first + tok) * a.ldout + static_cast<int64_t>(head) * HD;
-        norm = none ? 0.f : 1.f / l;
     }
     #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -1100,7 +1106,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
         for (int r4 = 0; r4 < 4; ++r4) {
             float v[4];
             #pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = ldexpf(o[d][4 * r4 + r] * norm, back);
+            for (int r = 0; r < 4; ++r) v[r] = ldexpf(o[d][4 * r4 + r] * inverse, back);
             *reinterpret_cast<float4 *>(dst + 32 * d + 8 * r4 + 4 * hi) = make_float4(v[0], v[1], v[2], v[3]);
         }
 }
@@ -1133,8 +1139,9 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
     #pragma unroll
     for (int d = 0; d < kD; ++d) col[d] = p + 4 + min(d * 64 + lane, HD - 1);
     const float m = wave_max(ms);
-    const float fs = __builtin_amdgcn_exp2f(ms - (m == -INFINITY ? 0.f : m));
-    const float l = wave_sum(ls * fs);
+    float fs = ls * __builtin_amdgcn_exp2f(ms - (m == -INFINITY ? 0.f : m));
+    const float l = wave_sum(fs);
+    fs *= l == 0.f ? 0.f : 1.f / l;   // no row seen: zeros
     float o[kD] = {};
     for (int i0 = 0; i0 < live; i0 += kBatch) {
         float v[kBatch][kD];
@@ -1150,11 +1157,10 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
                 for (int d = 0; d < kD; ++d) o[d] = fmaf(v[i][d], f, o[d]);
         }
     }
-    const float norm = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
     float *out = a.out + (s.first + tok) * a.ldout + static_cast<int64_t>(head) * HD;
     #pragma unroll
     for (int d = 0; d < kD; ++d)
-        if (d * 64 + lane < HD) out[d * 64 + lane] = o[d] * norm;
+        if (d * 64 + lane < HD) out[d * 64 + lane] = o[d];
 }
 
 // A sequence of more query rows a KV head than kFewRows takes the chunk kernel,

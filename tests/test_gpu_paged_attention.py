@@ -594,3 +594,17 @@ def test_in_place(qk, torch_gpu, kind, workspace):
     x = to_dev(t, q)
     qk.paged_attention(kv, batch, x, x, 8, workspace=ws)
     assert np.array_equal(x.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+@pytest.mark.parametrize("count,pos", [(1, 3), (1, 3000), (1, 400), (150, 800)])
+@pytest.mark.parametrize("workspace", [True, 0])
+def test_values_next_to_the_largest(qk, torch_gpu, kind, count, pos, workspace):
+    """Values of up to 3e38, which sums of many would pass: their mean does not."""
+    rng = np.random.default_rng(32)
+    pool = paged_ref.Pool(rng, kind, 1, 64, 64, [(count, pos)])
+    x = rng.uniform(0.5, 1, (pos + count, 1, 64)) * 3e38
+    place(pool, "value", 0, range(pos + count), x)
+    q = queries(rng, pool, 2)
+    got = run(qk, torch_gpu, pool, q, 2, workspace=workspace)
+    assert np.isfinite(got).all() and each(got, pool, q, 2) < EACH
