@@ -1197,7 +1197,7 @@ int few_rows(const qk_paged_batch &b, int heads, int kv_heads) {
 // in 16 splits 9.7, in eight 11.0; 8000 rows in 32 splits 12.5, in 63 14.0.  16
 // sequences of 8000 rows: in one round of workgroups 51 us, in two 55.)  Sequences
 // that fill the chip as they are even out in four splits, if those are long: 64
-// sequences of 1000 to 8000 rows 137 us, 146 whole (of equal lengths the other way
+// sequences of 1000 to 8000 rows 136 us, 146 whole (of equal lengths the other way
 // round, 217 and 197); of 125 to 1000 rows whole 24, in four splits 31.
 // Chunks: a round of workgroups likewise, of at least four tiles; those that lie
 // behind all that a chunk's first tokens see end at once and do not count.
