@@ -49,6 +49,7 @@ extern "C" {
 /* Types of paged cache rows (besides QK_TYPE_F16); no weights have them. */
 #define QK_TYPE_I8 24
 #define QK_TYPE_F8_E4M3 120
+#define QK_TYPE_I4 121
 
 /* Status codes. */
 #define QK_OK 0
@@ -421,9 +422,19 @@ int qk_argmax_rows_f32(const float *v, int n, int64_t ldv, int rows, int32_t *ou
                       code * scale; written with scale the least power of two
                       that keeps the row within 448, code = x / scale to
                       nearest even.
+     QK_TYPE_I4       4-bit code * multiplier * scale.  Codes are of two's
+                      complement, two a byte, the earlier value in the low half:
+                      a row is head_dim / 2 bytes.  A row's entry of key_scale
+                      (value_scale) is 8 bytes: the fp32 scale, then a multiplier
+                      (one byte, 1 to 255) for each quarter of the row's values.
+                      Written with scale the least number of 13 significant bits
+                      with 1785 scale >= max|x| (and finite), the multiplier the
+                      least with 7 multiplier scale >= its quarter's max|x|, code
+                      = x / (multiplier scale) to nearest even, -7 to 7: a value
+                      as written is an fp32 number.
    A row whose largest magnitude is below 2^-100 is written as zeros with scale
-   1, one that holds a value that is not finite as zeros with scale NaN (I8,
-   E4M3).  head_dim 64, 96, 128 or 256; page_rows a power of two, 16 to 1024;
+   1 (multipliers 1), one that holds a value that is not finite as zeros with
+   scale NaN (I8, I4, E4M3).  head_dim 64, 96, 128 or 256; page_rows a power of two, 16 to 1024;
    every base 16-byte aligned. */
 typedef struct qk_paged_kv {
     int type;
@@ -527,6 +538,88 @@ size_t qk_paged_attention_workspace_bytes(const qk_paged_batch *batch, int heads
 int qk_paged_attention_f32(const qk_paged_kv *kv, const qk_paged_batch *batch, const float *q, int ldq, float *out,
                            int ldout, int heads, float scale, void *workspace, size_t workspace_bytes,
                            qk_stream stream);
+
+/* What a model adds to the scores of attention and which rows its tokens see.  Of
+   a token at position p and a row r, with s = scale q k:
+     cap     s = cap tanh(s / cap); 0: not.  From 2^-64 to 2^64.
+     slopes  s - slopes[head] |p - r| (after the cap); a device array of `heads`
+             finite values, or NULL.
+     window  rows with p - r < window alone; 0: all.
+     prefix  besides rows 0 .. p, those below prefix[sequence] (a device array of
+             n_seqs values, in the order of seqs; or NULL) that the sequence has
+             by the end of the call: its first rows see each other.
+   All zeros: none. */
+typedef struct qk_attention_terms {
+    float cap;
+    int window;
+    const float *slopes;
+    const int32_t *prefix;
+} qk_attention_terms;
+
+/* qk_paged_attention_f32 with terms (NULL: none).  A row that a token does not see
+   takes no part in it, whatever it holds; rows that no token of a call sees are
+   not read beyond the tile (32 or 64 rows) that a seen one shares with them. */
+size_t qk_paged_attention_terms_workspace_bytes(const qk_paged_batch *batch, int heads, int kv_heads, int head_dim,
+                                                int window);
+int qk_paged_attention_terms_f32(const qk_paged_kv *kv, const qk_paged_batch *batch, const float *q, int ldq, float *out,
+                                 int ldout, int heads, float scale, const qk_attention_terms *terms, void *workspace,
+                                 size_t workspace_bytes, qk_stream stream);
+
+/* A pool of pages and the table of the sequences that hold them: page_table
+   [table_rows][table_stride] (what qk_paged_batch takes) and refs, of each page the
+   number of table entries that name it; both on the device, with all entries -1 and
+   all refs 0 an empty pool.  layers is a host array of n_layers caches of these pages
+   (0: none; contents then stay where they are).  At most 2^30 pages and table
+   entries, refs 16-byte aligned.  The calls below keep refs right; entries that name
+   no page count as absent.  They run on the device alone (no value comes back to the
+   host) and give the same result for the same table and refs. */
+typedef struct qk_page_pool {
+    int32_t *page_table;
+    int table_rows, table_stride;
+    int32_t *refs;
+    int64_t pages;
+    int page_rows;
+    const qk_paged_kv *layers;
+    int n_layers;
+} qk_page_pool;
+
+/* Workspace of the three calls below, 16-byte aligned; calls sharing it, or the
+   pool, must not overlap. */
+size_t qk_pages_workspace_bytes(const qk_page_pool *pool);
+
+/* Every table row r with lengths[r] >= 0 comes to hold the pages of its rows
+   begins[r] .. lengths[r] - 1 (begins NULL: from 0) and no others: entries before
+   begins[r] / page_rows and from ceil(lengths[r] / page_rows) on give their pages
+   back (0: the whole row), absent ones between take free pages, in order of table
+   rows and entries the lowest page first.  Pages that the call takes back are free for
+   it.  lengths and begins are device arrays of table_rows values.  missing (device,
+   or NULL) receives the number of entries that got no page (and stay absent), those
+   beyond the table's stride included. */
+int qk_pages_resize(const qk_page_pool *pool, const int32_t *begins, const int32_t *lengths, int32_t *missing,
+                    void *workspace, size_t workspace_bytes, qk_stream stream);
+
+/* Every table row c whose parents[c] is another table row becomes a fork of that row
+   as it was before the call, of its first lengths[c] rows: it gives its own pages back,
+   shares the pages that these rows fill, and the contents of the last page, where they
+   fill a part of it, are copied in every layer into a page that was free before the
+   call (lowest first, in order of c).  Other rows (parents[c] out of range, or c
+   itself) stay as they are.  Entries absent in the parent are absent.  Rows may be
+   forked from rows that are forked themselves.  missing as above: forks without a
+   page for the last part. */
+int qk_pages_fork(const qk_page_pool *pool, const int32_t *parents, const int32_t *lengths, int32_t *missing,
+                  void *workspace, size_t workspace_bytes, qk_stream stream);
+
+/* Of n pages that are held, those numbered n and more move to the free ones below, in
+   order: contents in every layer, table entries and refs.  moved (device, or NULL)
+   receives their number. */
+int qk_pages_compact(const qk_page_pool *pool, int32_t *moved, void *workspace, size_t workspace_bytes,
+                     qk_stream stream);
+
+/* The contents of page source[i] into page target[i], i < n, in every layer (device
+   arrays; pairs that name no page are left out).  No page is a target twice, or a
+   target and a source. */
+int qk_pages_copy(const qk_paged_kv *layers, int n_layers, const int32_t *source, const int32_t *target, int n,
+                  qk_stream stream);
 
 /* The next token of each of `rows` rows of n logits (row r at logits + r *
    ldv).  Of row r, with w_i = exp((logit_i - max) / temperature[r]) held to 2^-30

@@ -29,7 +29,7 @@ QUANT_TYPES = (Q4_K, Q6_K, Q6_K_SPLIT)
 STORAGE_NAMES = {F32: "FP32", F16: "FP16", Q4_K: "Q4_K", Q6_K: "Q6_K", Q6_K_SPLIT: "Q6_K (split)"}
 MAX_FUSED = 8
 # Types of paged cache rows, besides F16.
-I8, F8_E4M3 = 24, 120
+I8, F8_E4M3, I4 = 24, 120, 121
 ROPE_SCALING = {"none": 0, "linear": 1, "llama3": 2, "yarn": 3}
 
 QK_OK = 0
@@ -107,6 +107,19 @@ class qk_paged_batch(ctypes.Structure):
                [(n, ctypes.c_int) for n in ("n_seqs", "n_tokens", "max_count", "max_rows")]
 
 
+class qk_attention_terms(ctypes.Structure):
+    """What attention adds to its scores and which rows tokens see (include/qk.h)."""
+    _fields_ = [("cap", ctypes.c_float), ("window", ctypes.c_int), ("slopes", ctypes.c_void_p),
+                ("prefix", ctypes.c_void_p)]
+
+
+class qk_page_pool(ctypes.Structure):
+    """A pool of pages and the table of those that hold them (include/qk.h)."""
+    _fields_ = [("page_table", ctypes.c_void_p), ("table_rows", ctypes.c_int), ("table_stride", ctypes.c_int),
+                ("refs", ctypes.c_void_p), ("pages", ctypes.c_int64), ("page_rows", ctypes.c_int),
+                ("layers", ctypes.POINTER(qk_paged_kv)), ("n_layers", ctypes.c_int)]
+
+
 class qk_rope_scaling(ctypes.Structure):
     """Scaling of rotary frequencies (include/qk.h)."""
     _fields_ = [("type", ctypes.c_int)] + \
@@ -158,6 +171,14 @@ SIGNATURES = {
     "qk_paged_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(qk_paged_batch), _i, _i, _i]),
     "qk_paged_attention_f32": (_i, [ctypes.POINTER(qk_paged_kv), ctypes.POINTER(qk_paged_batch), _vp, _i, _vp, _i, _i,
                                     _f, _vp, ctypes.c_size_t, _vp]),
+    "qk_paged_attention_terms_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(qk_paged_batch), _i, _i, _i, _i]),
+    "qk_paged_attention_terms_f32": (_i, [ctypes.POINTER(qk_paged_kv), ctypes.POINTER(qk_paged_batch), _vp, _i, _vp, _i,
+                                          _i, _f, ctypes.POINTER(qk_attention_terms), _vp, ctypes.c_size_t, _vp]),
+    "qk_pages_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(qk_page_pool)]),
+    "qk_pages_resize": (_i, [ctypes.POINTER(qk_page_pool), _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "qk_pages_fork": (_i, [ctypes.POINTER(qk_page_pool), _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "qk_pages_compact": (_i, [ctypes.POINTER(qk_page_pool), _vp, _vp, ctypes.c_size_t, _vp]),
+    "qk_pages_copy": (_i, [ctypes.POINTER(qk_paged_kv), _i, _vp, _vp, _i, _vp]),
     "qk_sample_rows_workspace_bytes": (ctypes.c_size_t, [_i, _i]),
     "qk_sample_rows_f32": (_i, [_vp, _i, ctypes.c_int64, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t,
                                 _vp]),
@@ -424,7 +445,7 @@ def matvec_i8(t: Tensor, xq, xscale, out, cols: int, rows: int, n_tokens: int = 
 
 # ------------------------------------------ paged cache of a serving step --
 
-_KV_DTYPES = {F16: "torch.float16", I8: "torch.int8", F8_E4M3: "torch.float8_e4m3fn"}
+_KV_DTYPES = {F16: "torch.float16", I8: "torch.int8", F8_E4M3: "torch.float8_e4m3fn", I4: "torch.uint8"}
 
 
 def _want(where: str, name: str, t, dtypes, shape=None, last_contiguous: bool = False):
@@ -528,25 +549,29 @@ class PagedKV:
     """One layer's paged cache (qk_paged_kv): key and value are tensors [pages]
     [kv_heads][page_rows][head_dim] of the type's dtype (F16 float16, I8 int8,
     F8_E4M3 float8_e4m3fn), the scales [pages][kv_heads][page_rows] float32 (I8,
-    F8_E4M3)."""
+    F8_E4M3).  I4: key and value uint8 [...][head_dim / 2], two codes a byte, the
+    scales uint8 [pages][kv_heads][page_rows][8], a row's fp32 scale and its four
+    multipliers."""
 
     def __init__(self, type: int, key, value, key_scale=None, value_scale=None):
         where = "PagedKV"
         _torch()
         if type not in _KV_DTYPES:
-            raise QKError(where, QK_ERR_TYPE, f"cache type {type} is not F16, I8 or F8_E4M3")
+            raise QKError(where, QK_ERR_TYPE, f"cache type {type} is not F16, I8, I4 or F8_E4M3")
         _want(where, "key", key, (_KV_DTYPES[type],), (None,) * 4)
         _want(where, "value", value, (_KV_DTYPES[type],), tuple(key.shape))
         if (type == F16) != (key_scale is None) or (type == F16) != (value_scale is None):
-            raise QKError(where, QK_ERR_INVALID_ARG, "scales belong to I8 and F8_E4M3 caches, and only to them")
+            raise QKError(where, QK_ERR_INVALID_ARG, "scales belong to I8, I4 and F8_E4M3 caches, and only to them")
+        scales, shape = ("torch.uint8", (8,)) if type == I4 else ("torch.float32", ())
         for name, t in (("key_scale", key_scale), ("value_scale", value_scale)):
             if t is not None:
-                _want(where, name, t, ("torch.float32",), tuple(key.shape[:3]))
+                _want(where, name, t, (scales,), tuple(key.shape[:3]) + shape)
         for t in (value, key_scale, value_scale):
             if t is not None and t.device != key.device:
                 raise QKError(where, QK_ERR_INVALID_ARG, f"tensors on {key.device} and {t.device}")
         self.type, self.key, self.value, self.key_scale, self.value_scale = type, key, value, key_scale, value_scale
         self.pages, self.kv_heads, self.page_rows, self.head_dim = (int(n) for n in key.shape)
+        self.head_dim *= 2 if type == I4 else 1
         self.desc = qk_paged_kv(type, self.kv_heads, self.head_dim, self.page_rows, self.pages, ptr(key), ptr(value),
                                 ptr(key_scale), ptr(value_scale))
         self.ref, self.device, self.width = ctypes.byref(self.desc), key.device, self.kv_heads * self.head_dim
@@ -556,10 +581,15 @@ class PagedKV:
         """A cache whose rows are not written yet."""
         torch = _torch()
         if type not in _KV_DTYPES:
-            raise QKError("PagedKV", QK_ERR_TYPE, f"cache type {type} is not F16, I8 or F8_E4M3")
+            raise QKError("PagedKV", QK_ERR_TYPE, f"cache type {type} is not F16, I8, I4 or F8_E4M3")
+        if type == I4 and head_dim % 2:
+            raise QKError("PagedKV", QK_ERR_LIMIT, "head_dim must be 64, 96, 128 or 256")
         dtype = getattr(torch, _KV_DTYPES[type].split(".")[1])
-        new = lambda: torch.empty(pages, kv_heads, page_rows, head_dim, dtype=dtype, device=device)
-        scale = lambda: None if type == F16 else torch.empty(pages, kv_heads, page_rows, device=device)
+        width = head_dim // 2 if type == I4 else head_dim
+        new = lambda: torch.empty(pages, kv_heads, page_rows, width, dtype=dtype, device=device)
+        entry = dict(dtype=torch.uint8) if type == I4 else dict(dtype=torch.float32)
+        shape = (pages, kv_heads, page_rows) + ((8,) if type == I4 else ())
+        scale = lambda: None if type == F16 else torch.empty(*shape, device=device, **entry)
         return cls(type, new(), new(), scale(), scale())
 
 
@@ -656,25 +686,127 @@ def paged_read(kv: PagedKV, batch: PagedBatch, key_out, value_out, stream=None) 
           "paged cache read launch")
 
 
-def paged_attention_workspace_bytes(batch: PagedBatch, heads: int, kv_heads: int, head_dim: int) -> int:
+def paged_attention_workspace_bytes(batch: PagedBatch, heads: int, kv_heads: int, head_dim: int,
+                                    window: int = 0) -> int:
     """Workspace bytes of paged_attention."""
     where = "paged_attention_workspace_bytes"
-    return int(lib().qk_paged_attention_workspace_bytes(batch.ref, _int(where, "heads", heads),
-                                                        _int(where, "kv_heads", kv_heads),
-                                                        _int(where, "head_dim", head_dim)))
+    return int(lib().qk_paged_attention_terms_workspace_bytes(batch.ref, _int(where, "heads", heads),
+                                                              _int(where, "kv_heads", kv_heads),
+                                                              _int(where, "head_dim", head_dim),
+                                                              _int(where, "window", window)))
 
 
 def paged_attention(kv: PagedKV, batch: PagedBatch, q, out, heads: int, scale: float = 0.0, workspace=None,
-                    stream=None) -> None:
+                    stream=None, cap: float = 0.0, window: int = 0, slopes=None, prefix=None) -> None:
     """qk_paged_attention_f32: attention of every new token (rows of q, [n_tokens]
-    [heads * head_dim]) over its sequence's pages up to its own position, into
-    out.  scale: 1 / sqrt(head_dim) when 0."""
+    [heads * head_dim], into out) over its sequence's rows up to its own.  With terms
+    (qk_attention_terms): scores capped by cap * tanh(score / cap), less slopes[head]
+    (float32 [heads]) times the distance; rows of the last `window` positions alone;
+    and those below prefix[sequence] (int32 [n_seqs]) seen from before them too."""
     where = "paged_attention"
-    device, n, w = _one_device(where, kv, batch), batch.n_tokens, heads * kv.head_dim
+    device, heads, window = _one_device(where, kv, batch), _int(where, "heads", heads), _int(where, "window", window)
+    n, w = batch.n_tokens, heads * kv.head_dim
     ldq, ldout = _rows(where, "q", q, n, w, device), _rows(where, "out", out, n, w, device)
     ws, nbytes = _space(where, workspace, device)
-    check(_launch(device, stream, lib().qk_paged_attention_f32, kv.ref, batch.ref, q.data_ptr(), ldq, out.data_ptr(),
-                  ldout, heads, scale, ws, nbytes), "paged attention launch")
+    slopes_ptr = None if slopes is None else _dense(where, "slopes", slopes, _TORCH.float32, (heads,), device)
+    prefix_ptr = None if prefix is None else _dense(where, "prefix", prefix, _TORCH.int32, (batch.seqs.shape[0],), device)
+    terms = qk_attention_terms(cap, window, slopes_ptr, prefix_ptr)
+    check(_launch(device, stream, lib().qk_paged_attention_terms_f32, kv.ref, batch.ref, q.data_ptr(), ldq,
+                  out.data_ptr(), ldout, heads, scale, ctypes.byref(terms), ws, nbytes), "paged attention launch")
+
+
+class PagePool:
+    """A pool of pages (qk_page_pool): page_table int32 [table_rows][table_stride]
+    (the one of PagedBatch), refs int32 [pages], of each page the entries that name
+    it, and the PagedKV of every layer whose contents follow."""
+
+    def __init__(self, page_table, refs, page_rows: int, layers: Sequence[PagedKV] = ()):
+        where = "PagePool"
+        _torch()
+        _want(where, "page_table", page_table, ("torch.int32",), (None, None))
+        _want(where, "refs", refs, ("torch.int32",), (None,))
+        for t in (refs, *layers):
+            if t.device != page_table.device:
+                raise QKError(where, QK_ERR_INVALID_ARG, f"tensors on {page_table.device} and {t.device}")
+        self.page_table, self.refs, self.page_rows, self.layers = page_table, refs, _int(where, "page_rows", page_rows), tuple(layers)
+        rows, stride = (_int(where, "page_table", n) for n in page_table.shape)
+        self._layers = (qk_paged_kv * max(len(self.layers), 1))(*(kv.desc for kv in self.layers))
+        self.desc = qk_page_pool(ptr(page_table), rows, stride, ptr(refs), int(refs.shape[0]), self.page_rows,
+                                 self._layers, len(self.layers))
+        self.ref, self.device, self.rows = ctypes.byref(self.desc), page_table.device, rows
+
+    @classmethod
+    def empty(cls, table_rows: int, table_stride: int, pages: int, page_rows: int, layers: Sequence[PagedKV] = (),
+              device="cuda") -> "PagePool":
+        """A pool of which no page is held."""
+        torch = _torch()
+        table = torch.full((table_rows, table_stride), -1, dtype=torch.int32, device=device)
+        return cls(table, torch.zeros(pages, dtype=torch.int32, device=device), page_rows, layers)
+
+
+def pages_workspace_bytes(pool: PagePool) -> int:
+    """Workspace bytes of pages_resize, pages_fork and pages_compact."""
+    n = int(lib().qk_pages_workspace_bytes(pool.ref))
+    if n == 0:
+        raise QKError("pages_workspace_bytes", QK_ERR_INVALID_ARG, lib().qk_last_error().decode())
+    return n
+
+
+def _row_numbers(where: str, name: str, t, pool: PagePool) -> int:
+    return _dense(where, name, t, _TORCH.int32, (pool.rows,), pool.device)
+
+
+def _one_number(where: str, name: str, t, pool: PagePool):
+    return None if t is None else _dense(where, name, t, _TORCH.int32, (1,), pool.device)
+
+
+def pages_resize(pool: PagePool, lengths, begins=None, missing=None, workspace=None, stream=None) -> None:
+    """qk_pages_resize: table row r comes to hold the pages of rows begins[r] ..
+    lengths[r] - 1 (int32 [table_rows]; a negative length leaves the row as it is);
+    missing (int32 [1]) receives the entries that got none."""
+    where = "pages_resize"
+    first = None if begins is None else _row_numbers(where, "begins", begins, pool)
+    ws, nbytes = _space(where, workspace, pool.device)
+    check(_launch(pool.device, stream, lib().qk_pages_resize, pool.ref, first, _row_numbers(where, "lengths", lengths, pool),
+                  _one_number(where, "missing", missing, pool), ws, nbytes), "pages resize launch")
+
+
+def pages_fork(pool: PagePool, parents, lengths, missing=None, workspace=None, stream=None) -> None:
+    """qk_pages_fork: table row c becomes a fork of the first lengths[c] rows of table
+    row parents[c] (int32 [table_rows]; a negative parent, or c, leaves the row as it
+    is): full pages are shared, the last part of one is copied."""
+    where = "pages_fork"
+    ws, nbytes = _space(where, workspace, pool.device)
+    check(_launch(pool.device, stream, lib().qk_pages_fork, pool.ref, _row_numbers(where, "parents", parents, pool),
+                  _row_numbers(where, "lengths", lengths, pool), _one_number(where, "missing", missing, pool), ws, nbytes),
+          "pages fork launch")
+
+
+def pages_compact(pool: PagePool, moved=None, workspace=None, stream=None) -> None:
+    """qk_pages_compact: the pages that are held move to the pool's front; moved
+    (int32 [1]) receives how many did."""
+    where = "pages_compact"
+    ws, nbytes = _space(where, workspace, pool.device)
+    check(_launch(pool.device, stream, lib().qk_pages_compact, pool.ref, _one_number(where, "moved", moved, pool), ws,
+                  nbytes), "pages compact launch")
+
+
+def pages_copy(layers: Sequence[PagedKV], source, target, stream=None) -> None:
+    """qk_pages_copy: the contents of pages source into pages target (int32 [n]) in
+    every layer."""
+    where = "pages_copy"
+    _torch()
+    if not layers:
+        return
+    device = layers[0].device
+    for kv in layers:
+        if kv.device != device:
+            raise QKError(where, QK_ERR_INVALID_ARG, f"caches on {device} and {kv.device}")
+    _want(where, "source", source, ("torch.int32",), (None,))
+    n = _int(where, "source", source.shape[0])
+    array = (qk_paged_kv * len(layers))(*(kv.desc for kv in layers))
+    check(_launch(device, stream, lib().qk_pages_copy, array, len(layers), _dense(where, "source", source, _TORCH.int32, (n,), device),
+                  _dense(where, "target", target, _TORCH.int32, (n,), device), n), "pages copy launch")
 
 
 def sample_workspace_bytes(n: int, rows: int) -> int:

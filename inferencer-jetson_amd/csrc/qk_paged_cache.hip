@@ -161,9 +161,49 @@ __device__ __forceinline__ int round_quotient(float x, float scale, float inv) {
 
 constexpr uint32_t kTinyBits = (127u - 100u) << 23;   // 2^-100
 
+// Bytes of n codes, and floats of a row's scale entry.
+constexpr int code_bytes(int type, int n) { return type == QK_TYPE_F16 ? 2 * n : type == QK_TYPE_I4 ? n / 2 : n; }
+constexpr int scale_floats(int type) { return type == QK_TYPE_I4 ? 2 : 1; }
+
+// The scale of a 4-bit row of largest magnitude top: the least number of 13
+// significant bits s with 1785 s >= top (a product of 24 bits: exact), found by two
+// comparisons from a quotient that is off by less than a step of 13 bits.
+__device__ __forceinline__ float scale_of_13(float top) {
+    uint32_t b = (__builtin_bit_cast(uint32_t, top * (1.f / 1785.f)) + 0x7FFu) & ~0x7FFu;
+    auto value = [](uint32_t bits) { return __builtin_bit_cast(float, bits); };
+    if (1785.f * value(b) < top) b += 0x800u;
+    if (1785.f * value(b - 0x800u) >= top) b -= 0x800u;
+    // (Next to fp32's largest: the one below, whose values are finite.)
+    return 1785.f * value(b) < INFINITY ? value(b) : value(b - 0x800u);
+}
+// The least positive integer m with m step >= top, step of 16 significant bits, at
+// most 255.
+__device__ __forceinline__ float multiplier(float top, float step) {
+    float m = ceilf(top * (1.f / step));
+    if ((m - 1.f) * step >= top) m -= 1.f;
+    if (m * step < top) m += 1.f;
+    return fminf(fmaxf(m, 1.f), 255.f);
+}
+
+// The largest of the lanes of a row's quarter (HD / 16 of them).
+template <int HD>
+__device__ __forceinline__ uint32_t quarter_max(uint32_t v) {
+    constexpr int kLanes = HD / 16;
+    if constexpr (kLanes & (kLanes - 1)) {   // 6 of 96 values
+        const int row = threadIdx.x & 32, first = row + (threadIdx.x & 31) / kLanes * kLanes;
+        uint32_t top = 0;   // (lanes past the row's 24 hold zeros, and read within the wave)
+        #pragma unroll
+        for (int i = 0; i < kLanes; ++i) top = max(top, static_cast<uint32_t>(__shfl(static_cast<int>(v), first + i)));
+        return top;
+    }
+    #pragma unroll
+    for (int off = 1; off < kLanes; off <<= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), off)));
+    return v;
+}
+
 // One row's four values of a lane (zeros past head_dim) into its page; all
 // row_lanes lanes call it.
-template <int TYPE, int LANES>
+template <int HD, int TYPE, int LANES>
 __device__ __forceinline__ void store_codes(const float4 &x, bool active, char *row, float *scale_at, int c) {
     if constexpr (TYPE == QK_TYPE_F16) {
         if (!active) return;
@@ -177,6 +217,8 @@ __device__ __forceinline__ void store_codes(const float4 &x, bool active, char *
     uint32_t amax = 0;
     #pragma unroll
     for (int e = 0; e < 4; ++e) amax = max(amax, __builtin_bit_cast(uint32_t, v[e]) & 0x7FFFFFFFu);
+    uint32_t part = 0;
+    if constexpr (TYPE == QK_TYPE_I4) part = quarter_max<HD>(amax);
     #pragma unroll
     for (int off = 1; off < LANES; off <<= 1) amax = max(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), off)));
     const float top = __builtin_bit_cast(float, amax);
@@ -189,6 +231,26 @@ __device__ __forceinline__ void store_codes(const float4 &x, bool active, char *
         #pragma unroll
         for (int e = 0; e < 4; ++e)
             codes |= (static_cast<uint32_t>(round_quotient(v[e], scale, inv)) & 0xFFu) << (8 * e);
+    } else if constexpr (TYPE == QK_TYPE_I4) {
+        scale = none ? 1.f : scale_of_13(top);
+        const float m = bad || none ? 1.f : multiplier(__builtin_bit_cast(float, part), 7.f * scale);
+        const float step = m * scale, inv = 1.f / step;   // a product of 21 bits; its code's is of 24
+        #pragma unroll
+        for (int e = 0; e < 4; ++e)
+            codes |= (static_cast<uint32_t>(round_quotient(v[e], step, inv)) & 0xFu) << (4 * e);
+        // The multipliers of all quarters in the row's first lane.
+        const int first = threadIdx.x & (64 - LANES);
+        uint32_t mults = 0;
+        #pragma unroll
+        for (int q = 0; q < 4; ++q)
+            mults |= static_cast<uint32_t>(__shfl(static_cast<int>(m), first + q * (HD / 16))) << (8 * q);
+        if (bad) scale = __builtin_nanf("");
+        if (bad || none) codes = 0;
+        if (!active) return;
+        const uint16_t two = static_cast<uint16_t>(codes);
+        __builtin_memcpy(row + c / 2, &two, 2);
+        if (c == 0) *reinterpret_cast<float2 *>(scale_at) = make_float2(scale, __builtin_bit_cast(float, mults));
+        return;
     } else {
         // 448 = 0.875 * 2^9: the least power of two with top / scale <= 448.
         const int s = __builtin_amdgcn_frexp_expf(top) - (__builtin_amdgcn_frexp_mantf(top) > 0.875f ? 8 : 9);
@@ -250,9 +312,9 @@ __global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a) {
         const int64_t page = paged_page(a.b.page_table + static_cast<int64_t>(s.table) * a.b.table_stride,
                                         pos >> a.page_shift, a.kv.pages);
         const int64_t row = (max(page, int64_t(0)) * kvh + h) * a.kv.page_rows + (pos & (a.kv.page_rows - 1));
-        char *base = static_cast<char *>(key ? a.kv.key : a.kv.value) + row * HD * (TYPE == QK_TYPE_F16 ? 2 : 1);
-        store_codes<TYPE, L>(x, active && page >= 0, base,
-                             TYPE == QK_TYPE_F16 ? nullptr : (key ? a.kv.key_scale : a.kv.value_scale) + row, c);
+        char *base = static_cast<char *>(key ? a.kv.key : a.kv.value) + row * code_bytes(TYPE, HD);
+        float *scale_at = TYPE == QK_TYPE_F16 ? nullptr : (key ? a.kv.key_scale : a.kv.value_scale) + row * scale_floats(TYPE);
+        store_codes<HD, TYPE, L>(x, active && page >= 0, base, scale_at, c);
     }
 }
 
@@ -266,9 +328,16 @@ struct ReadArgs {
     int page_shift;
 };
 
+// (4-bit codes: mult the multiplier of their quarter; code * mult is exact.)
 template <int TYPE>
-__device__ __forceinline__ float4 decode4(const char *p, float scale) {
-    if constexpr (TYPE == QK_TYPE_F16) {
+__device__ __forceinline__ float4 decode4(const char *p, float scale, float mult) {
+    if constexpr (TYPE == QK_TYPE_I4) {
+        uint16_t two;
+        __builtin_memcpy(&two, p, 2);
+        const uint32_t w = two ^ 0x8888u;
+        auto at = [&](int e) { return (static_cast<float>(w >> (4 * e) & 15) - 8.f) * mult * scale; };
+        return make_float4(at(0), at(1), at(2), at(3));
+    } else if constexpr (TYPE == QK_TYPE_F16) {
         _Float16 h[4];
         __builtin_memcpy(h, p, 8);
         return make_float4(h[0], h[1], h[2], h[3]);
@@ -308,9 +377,12 @@ __global__ __launch_bounds__(256) void paged_read_kernel(ReadArgs a) {
         if (page >= 0) {
             const int64_t row = (page * kvh + h) * a.kv.page_rows + (pos & (a.kv.page_rows - 1));
             const char *base = static_cast<const char *>(key ? a.kv.key : a.kv.value);
-            constexpr int kBytes = TYPE == QK_TYPE_F16 ? 2 : 1;
-            const float scale = TYPE == QK_TYPE_F16 ? 1.f : (key ? a.kv.key_scale : a.kv.value_scale)[row];
-            x = decode4<TYPE>(base + (row * HD + c) * kBytes, scale);
+            const float *scales = key ? a.kv.key_scale : a.kv.value_scale;
+            const float scale = TYPE == QK_TYPE_F16 ? 1.f : scales[row * scale_floats(TYPE)];
+            float mult = 1.f;
+            if constexpr (TYPE == QK_TYPE_I4)
+                mult = static_cast<float>(__builtin_bit_cast(uint32_t, scales[row * 2 + 1]) >> (8 * (c / (HD / 4))) & 0xFFu);
+            x = decode4<TYPE>(base + row * code_bytes(TYPE, HD) + code_bytes(TYPE, c), scale, mult);
         }
         float *out = key ? a.key_out + (s.first + i) * a.ldk : a.value_out + (s.first + i) * a.ldv;
         *reinterpret_cast<float4 *>(out + h * HD + c) = x;
@@ -323,6 +395,7 @@ int by_shape(int hd, int type, A &&...args) {
         constexpr int kHd = decltype(HD)::value;
         if (type == QK_TYPE_F16) return Launch<kHd, QK_TYPE_F16>::run(args...);
         if (type == QK_TYPE_I8) return Launch<kHd, QK_TYPE_I8>::run(args...);
+        if (type == QK_TYPE_I4) return Launch<kHd, QK_TYPE_I4>::run(args...);
         return Launch<kHd, QK_TYPE_F8_E4M3>::run(args...);
     };
     switch (hd) {
@@ -374,8 +447,8 @@ bool rows_meet(const float *a, int64_t lda, int64_t wa, const float *b, int64_t 
 int check_paged_kv(const char *where, const qk_paged_kv *kv) {
     const std::string w(where);
     if (!kv || !kv->key || !kv->value) return fail(QK_ERR_INVALID_ARG, w + ": null cache pointer");
-    if (kv->type != QK_TYPE_F16 && kv->type != QK_TYPE_I8 && kv->type != QK_TYPE_F8_E4M3)
-        return fail(QK_ERR_TYPE, w + ": cache type " + std::to_string(kv->type) + " is not F16, I8 or F8_E4M3");
+    if (kv->type != QK_TYPE_F16 && kv->type != QK_TYPE_I8 && kv->type != QK_TYPE_F8_E4M3 && kv->type != QK_TYPE_I4)
+        return fail(QK_ERR_TYPE, w + ": cache type " + std::to_string(kv->type) + " is not F16, I8, I4 or F8_E4M3");
     if (kv->type != QK_TYPE_F16 && (!kv->key_scale || !kv->value_scale))
         return fail(QK_ERR_INVALID_ARG, w + ": null scale pointer");
     if (kv->head_dim != 64 && kv->head_dim != 96 && kv->head_dim != 128 && kv->head_dim != 256)
