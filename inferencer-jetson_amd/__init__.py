@@ -704,13 +704,17 @@ def paged_attention(kv: PagedKV, batch: PagedBatch, q, out, heads: int, scale: f
     (float32 [heads]) times the distance; rows of the last `window` positions alone;
     and those below prefix[sequence] (int32 [n_seqs]) seen from before them too."""
     where = "paged_attention"
-    device, heads, window = _one_device(where, kv, batch), _int(where, "heads", heads), _int(where, "window", window)
+    device, heads = _one_device(where, kv, batch), _int(where, "heads", heads)
     n, w = batch.n_tokens, heads * kv.head_dim
     ldq, ldout = _rows(where, "q", q, n, w, device), _rows(where, "out", out, n, w, device)
     ws, nbytes = _space(where, workspace, device)
+    if not cap and not window and slopes is None and prefix is None:
+        check(_launch(device, stream, lib().qk_paged_attention_f32, kv.ref, batch.ref, q.data_ptr(), ldq,
+                      out.data_ptr(), ldout, heads, scale, ws, nbytes), "paged attention launch")
+        return
     slopes_ptr = None if slopes is None else _dense(where, "slopes", slopes, _TORCH.float32, (heads,), device)
     prefix_ptr = None if prefix is None else _dense(where, "prefix", prefix, _TORCH.int32, (batch.seqs.shape[0],), device)
-    terms = qk_attention_terms(cap, window, slopes_ptr, prefix_ptr)
+    terms = qk_attention_terms(cap, _int(where, "window", window), slopes_ptr, prefix_ptr)
     check(_launch(device, stream, lib().qk_paged_attention_terms_f32, kv.ref, batch.ref, q.data_ptr(), ldq,
                   out.data_ptr(), ldout, heads, scale, ctypes.byref(terms), ws, nbytes), "paged attention launch")
 

@@ -106,9 +106,10 @@ __device__ __forceinline__ void codes4(uint32_t w, half2v &a, half2v &b) {
     }
 }
 
-// 4-bit codes become code * multiplier in fp16, a whole number of at most 2040: a
-// nibble u (code + 8) in bits 6 to 9 of 0x4C00 is 16 + u, and (16 + u) m - 24 m is
-// one packed fma, exact (24 m is 8 times a number of ten bits).
+// 4-bit codes become code * multiplier in fp16, a whole number of at most 2040: with
+// u = code + 8, a nibble of two's complement but for its upper bit, in bits 6 to 9 of
+// 0x4C00 it is 16 + u, and (16 + u) m - 24 m is one packed fma, exact (24 m is 8 times
+// a number of ten bits).
 struct Mult {
     half2v m, off;
     // Of each half, the byte of its dword that sel names.
@@ -121,20 +122,28 @@ struct Mult {
 };
 // The selector of byte k of both dwords.
 __device__ __forceinline__ uint32_t mult_sel(int k) { return 0x0C040C00u + 0x10001u * k; }
-__device__ __forceinline__ half2v coded(uint32_t at6, const Mult &m) {   // nibbles in bits 6 to 9 of each half
-    return __builtin_elementwise_fma(__builtin_bit_cast(half2v, (at6 & 0x03C003C0u) | 0x4C004C00u), m.m, m.off);
-}
-// Eight codes of one dword w (xor 0x88888888): pair k holds values k and k + 4.
-__device__ __forceinline__ half8 codes8(uint32_t w, const Mult &m) {
-    const half2v a = coded(w << 6, m), b = coded(w << 2, m), c = coded(w >> 2, m), d = coded(w >> 6, m);
-    return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-// Two bytes (of two rows, in bits 0 to 7 of each half): the pairs of their lower
-// and of their upper nibbles.
-__device__ __forceinline__ void codes2x2(uint32_t w, const Mult &m, half2v &lower, half2v &upper) {
-    lower = coded(w << 6, m);
-    upper = coded(w << 2, m);
-}
+// The constants in registers: a nibble's bits are then cut out and joined with them in
+// one instruction, which takes no literals (one in a scalar and one in a vector
+// register; they are made anew where the compiler likes).
+struct Nibbles {
+    uint32_t mask = 0x03C003C0u, base = 0x4E004E00u;
+    __device__ __forceinline__ Nibbles() { asm("" : "+s"(mask), "+v"(base)); }
+    __device__ __forceinline__ half2v code(uint32_t at6, const Mult &m) const {   // in bits 6 to 9 of each half
+        return __builtin_elementwise_fma(__builtin_bit_cast(half2v, (at6 & mask) ^ base), m.m, m.off);
+    }
+    // Eight codes of one dword: pair k holds values k and k + 4.
+    __device__ __forceinline__ half8 eight(uint32_t w, const Mult &m) const {
+        const half2v a = code(w << 6, m), b = code(w << 2, m), c = code(w >> 2, m), d = code(w >> 6, m);
+        return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+    }
+    // Four of two rows each, x and y: pair k their values k.
+    __device__ __forceinline__ void four(uint32_t x, uint32_t y, uint32_t sel, const Mult &m, half2v (&p)[4]) const {
+        const uint32_t w = __builtin_amdgcn_perm(y, x, sel);
+        p[0] = code(w << 6, m), p[1] = code(w << 2, m), p[2] = code(w >> 2, m), p[3] = code(w >> 6, m);
+    }
+};
+// The selector of the lower or upper two bytes of two rows, for four().
+__device__ __forceinline__ constexpr uint32_t four_sel(int half) { return half ? 0x07060302u : 0x05040100u; }
 // Query values of one step in the order in which its key codes stand.
 template <int TYPE>
 __device__ __forceinline__ half8 key_order(half2v a, half2v b, half2v c, half2v d) {
@@ -198,9 +207,9 @@ struct KeyTile {   // 32 rows: two halves of 16
         for (int j = 0; j < kB / 16; ++j) __builtin_memcpy(&w[h][j], row + j * 64 + g * 16, 16);
         if constexpr (kB % 16 != 0) __builtin_memcpy(&w[h][kB / 16], row + kB / 16 * 64 + g * 8, 8);
     }
-    __device__ __forceinline__ half8 operand(int h, int s, const Mult &m) const {
+    __device__ __forceinline__ half8 operand(int h, int s, const Mult &m, const Nibbles &codes) const {
         if constexpr (TYPE == QK_TYPE_I4) {
-            return codes8(w[h][s / 4][s % 4] ^ 0x88888888u, m);
+            return codes.eight(w[h][s / 4][s % 4], m);
         } else if constexpr (TYPE == QK_TYPE_F16) {
             return __builtin_bit_cast(half8, w[h][s]);
         } else {
@@ -255,18 +264,13 @@ struct ValueTile {   // 8 rows a lane: slot j < 4 row 4 g + j, else 16 + 4 g + j
     // what a conversion takes.
     // (4-bit codes: from two bytes of each row, times the multipliers of the rows'
     // pairs, of the quarter that holds these dimensions.)
-    __device__ __forceinline__ void operands(int d, half8 (&v)[4], const Mult (&m)[4]) const {
+    __device__ __forceinline__ void operands(int d, half8 (&v)[4], const Mult (&m)[4], const Nibbles &codes) const {
         if constexpr (TYPE == QK_TYPE_I4) {
-            half2v p[4][4];
+            half2v p[4][4];   // [pair of rows][dimension]
             #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint32_t x = w[2 * k][d / 2] ^ 0x88888888u, y = w[2 * k + 1][d / 2] ^ 0x88888888u;
-                const uint32_t sel = 0x0C040C00u + 0x10001u * (2 * (d & 1));
-                codes2x2(__builtin_amdgcn_perm(y, x, sel), m[k], p[0][k], p[1][k]);
-                codes2x2(__builtin_amdgcn_perm(y, x, sel + 0x10001u), m[k], p[2][k], p[3][k]);
-            }
+            for (int k = 0; k < 4; ++k) codes.four(w[2 * k][d / 2], w[2 * k + 1][d / 2], four_sel(d & 1), m[k], p[k]);
             #pragma unroll
-            for (int c = 0; c < 4; ++c) v[c] = join(p[c][0], p[c][1], p[c][2], p[c][3]);
+            for (int c = 0; c < 4; ++c) v[c] = join(p[0][c], p[1][c], p[2][c], p[3][c]);
         } else if constexpr (TYPE == QK_TYPE_F16) {
             #pragma unroll
             for (int c = 0; c < 4 && 4 * d + c < HD / 16; ++c) {
@@ -380,34 +384,42 @@ __device__ __forceinline__ float wave_sum(float v) {
 // 0.55 of the cap, which is where trained scores lie, by y + y^3 P(y^2), P the
 // minimax polynomial of (tanh(y) / y - 1) / y^2 there (its error is below fp32's
 // rounding): eight operations instead of two quarter-rate ones and eight.
+// (Four at a time: all of a tile's side by side would take the registers of the sums.)
 template <int N, typename V>
 __device__ __forceinline__ void cap_scores(V &x, float cap, float inverse) {
+    constexpr int kBy = N < 4 ? N : 4;
     float top = 0.f;
     #pragma unroll
     for (int r = 0; r < N; ++r) top = fmaxf(top, fabsf(x[r]));
+    auto cubic = [](float z) {
+        float p = fmaf(-0.00661022774875164f, z, 0.021309388801455498f);
+        p = fmaf(p, z, -0.05390942841768265f);
+        p = fmaf(p, z, 0.13333113491535187f);
+        return fmaf(p, z, -0.3333333134651184f);
+    };
     if (__builtin_amdgcn_ballot_w64(top * inverse > 0.55f)) {
         #pragma unroll
-        for (int r = 0; r < N; ++r) {
-            const float y = x[r] * inverse, e = __builtin_amdgcn_exp2f(-2.8853900817779268f * fabsf(y));
-            const float t = (1.f - e) * __builtin_amdgcn_rcpf(1.f + e), z = y * y;
-            float p = fmaf(-0.00661022774875164f, z, 0.021309388801455498f);
-            p = fmaf(p, z, -0.05390942841768265f);
-            p = fmaf(p, z, 0.13333113491535187f);
-            p = fmaf(p, z, -0.3333333134651184f);
-            const float small = fmaf(p, z * y, y);
-            x[r] = cap * (fabsf(y) > 0.55f ? copysignf(t, y) : small);
+        for (int r0 = 0; r0 < N; r0 += kBy) {
+            __builtin_amdgcn_sched_barrier(0);
+            #pragma unroll
+            for (int r = r0; r < r0 + kBy; ++r) {
+                const float y = x[r] * inverse, e = __builtin_amdgcn_exp2f(-2.8853900817779268f * fabsf(y));
+                const float t = (1.f - e) * __builtin_amdgcn_rcpf(1.f + e), z = y * y;
+                x[r] = cap * (fabsf(y) > 0.55f ? copysignf(t, y) : fmaf(cubic(z), z * y, y));
+            }
         }
     } else {
         #pragma unroll
-        for (int r = 0; r < N; ++r) {
-            const float y = x[r] * inverse, z = y * y;
-            float p = fmaf(-0.00661022774875164f, z, 0.021309388801455498f);
-            p = fmaf(p, z, -0.05390942841768265f);
-            p = fmaf(p, z, 0.13333113491535187f);
-            p = fmaf(p, z, -0.3333333134651184f);
-            x[r] = fmaf(cap * p, z * y, x[r]);
+        for (int r0 = 0; r0 < N; r0 += kBy) {
+            __builtin_amdgcn_sched_barrier(0);
+            #pragma unroll
+            for (int r = r0; r < r0 + kBy; ++r) {
+                const float y = x[r] * inverse, z = y * y;
+                x[r] = fmaf(cap * cubic(z), z * y, x[r]);
+            }
         }
     }
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // |v| as an integer, ordered as the values are, infinity and NaN above them.
@@ -452,6 +464,39 @@ struct ValueUnits {
         return ldexpf(f, old - e);
     }
 };
+
+// A query row as the operands of the scores' product, lane group g's dimensions of
+// it: two halves each, times what qscale undoes.
+template <int HD, int TYPE, int NS>
+__device__ __forceinline__ void load_query(const float *qrow, int g, float scale, half8 (&qh)[NS], half8 (&ql)[NS],
+                                           float &qscale) {
+    float v[NS][8];
+    #pragma unroll
+    for (int st = 0; st < NS; ++st)
+        #pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+            const float4 x = *reinterpret_cast<const float4 *>(qrow + key_dim<HD, TYPE>(st, g) + e);
+            v[st][e] = x.x, v[st][e + 1] = x.y, v[st][e + 2] = x.z, v[st][e + 3] = x.w;
+        }
+    int top = 0;
+    #pragma unroll
+    for (int st = 0; st < NS; ++st)
+        #pragma unroll
+        for (int k = 0; k < 8; ++k) top = max(top, magnitude(v[st][k]));
+    top = max(top, __shfl_xor(top, 16));
+    top = max(top, __shfl_xor(top, 32));
+    float factor;
+    query_units(top, scale, factor, qscale);
+    #pragma unroll
+    for (int st = 0; st < NS; ++st) {
+        half2v u[4], w[4];
+        #pragma unroll
+        for (int k = 0; k < 4; ++k)
+            split_pair(factor * v[st][2 * k], factor * v[st][2 * k + 1], u[k], w[k]);
+        qh[st] = key_order<TYPE>(u[0], u[1], u[2], u[3]);
+        ql[st] = key_order<TYPE>(w[0], w[1], w[2], w[3]);
+    }
+}
 
 // A workgroup: 16 query rows of one (sequence, KV head) over a split's rows,
 // its four waves every fourth tile of 32 rows each; the waves' states meet in
@@ -509,45 +554,21 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
 
     half8 qh[NS], ql[NS];
     float qscale;
-    {
-        const float *qrow = a.q + (s.first + tok) * a.ldq + static_cast<int64_t>(h * G + own) * HD;
-        float v[NS][8];
-        #pragma unroll
-        for (int st = 0; st < NS; ++st)
-            #pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-                const float4 x = *reinterpret_cast<const float4 *>(qrow + key_dim<HD, TYPE>(st, g) + e);
-                v[st][e] = x.x, v[st][e + 1] = x.y, v[st][e + 2] = x.z, v[st][e + 3] = x.w;
-            }
-        int top = 0;
-        #pragma unroll
-        for (int st = 0; st < NS; ++st)
-            #pragma unroll
-            for (int k = 0; k < 8; ++k) top = max(top, magnitude(v[st][k]));
-        top = max(top, __shfl_xor(top, 16));
-        top = max(top, __shfl_xor(top, 32));
-        float factor;
-        query_units(top, a.scale, factor, qscale);
-        #pragma unroll
-        for (int st = 0; st < NS; ++st) {
-            half2v u[4], w[4];
-            #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                split_pair(factor * v[st][2 * k], factor * v[st][2 * k + 1], u[k], w[k]);
-            qh[st] = key_order<TYPE>(u[0], u[1], u[2], u[3]);
-            ql[st] = key_order<TYPE>(w[0], w[1], w[2], w[3]);
-        }
-    }
+    load_query<HD, TYPE, NS>(a.q + (s.first + tok) * a.ldq + static_cast<int64_t>(h * G + own) * HD, g, a.scale, qh, ql, qscale);
 
     float4v o[NC];
     #pragma unroll
     for (int c = 0; c < NC; ++c) o[c] = float4v{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
     ValueUnits units;
+    const Nibbles codes;
     const float slope = TERMS && a.slopes ? 1.4426950408889634f * a.slopes[h * G + own] : 0.f;
     const float inverse_cap = TERMS && a.cap > 0.f ? 1.f / a.cap : 0.f;
 
-    const int32_t *table = a.b.page_table + static_cast<int64_t>(s.table) * a.b.table_stride;
+    // (Of the constant address space: looked up by scalar loads, which no wait for a
+    // tile's loads includes.)
+    typedef const __attribute__((address_space(4))) int32_t *Table;
+    const Table table = (Table)(a.b.page_table + static_cast<int64_t>(s.table) * a.b.table_stride);
     const int64_t page_stride = static_cast<int64_t>(kvh) * a.kv.page_rows, head_row = static_cast<int64_t>(h) * a.kv.page_rows;
     // Each half of a tile lies in one page; rows past the sequence's last are
     // read from the first page (in bounds, masked).  A tile's pages are looked up
@@ -565,11 +586,18 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
     // Scales (and multipliers) of rows base + 4 g .. + 3.
     auto scales4 = [&](const float *at, int64_t base, float4v &scale, uint32_t *mults) {
         if constexpr (TYPE == QK_TYPE_I4) {
-            const uint4v *e = reinterpret_cast<const uint4v *>(at + 2 * (base + 4 * g));
-            const uint4v lo = e[0], hi = e[1];
-            const uint32_t s[4] = {lo[0], lo[2], hi[0], hi[2]};   // (a cast of an element of a vector is one of its first)
-            scale = __builtin_bit_cast(float4v, s);
-            if (mults) mults[0] = lo[1], mults[1] = lo[3], mults[2] = hi[1], mults[3] = hi[3];
+            // (No part of a load unused: its register would be given to something else,
+            // which then waits for the load.)
+            if (mults) {
+                const uint4v *e = reinterpret_cast<const uint4v *>(at + 2 * (base + 4 * g));
+                const uint4v lo = e[0], hi = e[1];
+                const uint32_t s[4] = {lo[0], lo[2], hi[0], hi[2]};   // (a cast of an element of a vector is one of its first)
+                scale = __builtin_bit_cast(float4v, s);
+                mults[0] = lo[1], mults[1] = lo[3], mults[2] = hi[1], mults[3] = hi[3];
+            } else {
+                #pragma unroll
+                for (int r = 0; r < 4; ++r) scale[r] = at[2 * (base + 4 * g + r)];
+            }
         } else {
             scale = *reinterpret_cast<const float4v *>(at + base + 4 * g);
         }
@@ -579,8 +607,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
         #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
             const int r = min(t0 + 16 * hf, last);
-            const int64_t page = paged_page(table, r >> a.page_shift, a.kv.pages);
-            p.id[hf] = t0 + 16 * hf <= last ? page : -1;
+            const int64_t page = table[r >> a.page_shift];
+            p.id[hf] = t0 + 16 * hf <= last && page >= 0 && page < a.kv.pages ? page : -1;
         }
         return p;
     };
@@ -611,7 +639,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
         for (int x = 0; x < NS; ++x)
             #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
-                const half8 k = t.k.operand(hf, x, km[hf]);
+                const half8 k = t.k.operand(hf, x, km[hf], codes);
                 st[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[x], st[hf], 0, 0, 0);
                 st[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[x], st[hf], 0, 0, 0);
             }
@@ -735,7 +763,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
                     #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         vm[k].set(t.vm[2 * k], t.vm[2 * k + 1], mult_sel(value_dim<HD, TYPE>(n, 4 * d) / (HD / 4)));
-            t.v.operands(d, v, vm);
+            t.v.operands(d, v, vm, codes);
             #pragma unroll
             for (int k = 0; k < 4 && 4 * d + k < NC; ++k) {
                 if (!whole_codes(TYPE) && edge) clear_not_finite(v[k], bad);
@@ -757,18 +785,29 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
                         l = __builtin_nanf("");
         }
     };
+    // Two tiles in registers by turns, one multiplied while the other loads; a tile's
+    // pages are looked up before its turn to load comes.  Past the wave's last tile
+    // that one again: loads that may be left out would have every wait for a tile wait
+    // for all that is under way.
     constexpr int kStep = 4 * kTile;
     int t0 = begin + wave * kTile;
     if (t0 < end) {
-        Tile cur;
-        load(cur, t0, pages_of(t0));
-        Pages ahead = pages_of(t0 + kStep);
-        for (; t0 < end; t0 += kStep) {
-            Tile next;
-            if (t0 + kStep < end) load(next, t0 + kStep, ahead);
-            ahead = pages_of(t0 + 2 * kStep);
-            take(cur, t0);
-            cur = next;
+        const int final = t0 + (end - 1 - t0) / kStep * kStep;
+        Tile tiles[2];
+        load(tiles[0], t0, pages_of(t0));
+        Pages ahead = pages_of(min(t0 + kStep, final));
+        for (bool more = true; more;) {
+            #pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                load(tiles[i ^ 1], min(t0 + kStep, final), ahead);
+                asm volatile("" ::: "memory");   // or they would sink to where the tile is known to be needed
+                ahead = pages_of(min(t0 + 2 * kStep, final));
+                take(tiles[i], t0);
+                if ((t0 += kStep) >= end) {
+                    more = false;
+                    break;
+                }
+            }
         }
     }
     l += __shfl_xor(l, 16);
@@ -821,6 +860,414 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
         }
     }
     if (!have) return;
+    const int head = h * G + own;
+    float *dst = a.out + (s.first + tok) * a.ldout + static_cast<int64_t>(head) * HD;
+    if (splits > 1) {
+        dst = a.parts + ((static_cast<int64_t>(s.first + tok) * a.heads + head) * a.part_splits + split) * part_floats(HD);
+        if (g == 0) *reinterpret_cast<float4 *>(dst) = make_float4(m, l, 0.f, 0.f);
+        dst += 4;
+    }
+    #pragma unroll
+    for (int r = 0; r < 4; ++r)
+        #pragma unroll
+        for (int c = 0; c < NC; ++c) dst[value_dim<HD, TYPE>(4 * g + r, c)] = o[c][r];
+}
+
+// ---------------------------------------------------------- few rows --
+//
+// Sequences of at most 16 / DUP query rows a KV head (single tokens, mostly): each
+// query row stands in DUP neighbouring columns of the scores' product, so a lane of
+// them need take no more than 4 / DUP of each four scores through the softmax, and
+// the lanes share what the 16-row kernel does DUP times over.  Of the second
+// product's columns the first of a query row's holds the weights' upper halves, the
+// second the lower ones, added at the end: one matrix instruction for two.  Rows
+// pair as 4 g + k of a tile's two halves, so that a lane's weights are whole pairs.
+// Lanes of four: the value of lane `from` of each.
+template <int A, int B, int C, int D>
+__device__ __forceinline__ uint32_t quad(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), A | B << 2 | C << 4 | D << 6, 0xF, 0xF, true));
+}
+template <int A, int B, int C, int D>
+__device__ __forceinline__ float quad(float v) {
+    return __builtin_bit_cast(float, quad<A, B, C, D>(__builtin_bit_cast(uint32_t, v)));
+}
+// Joined over the DUP lanes of a query row and the four groups of 16 lanes.
+template <int DUP, typename Op>
+__device__ __forceinline__ float join_row(float v, Op op) {
+    v = op(v, quad<1, 0, 3, 2>(v));
+    if constexpr (DUP == 4) v = op(v, quad<2, 3, 0, 1>(v));
+    uint32_t bits = __builtin_bit_cast(uint32_t, v);
+    const auto rows = __builtin_amdgcn_permlane16_swap(bits, bits, false, false);
+    const uint32_t even = rows[0], odd = rows[1];
+    v = op(__builtin_bit_cast(float, even), __builtin_bit_cast(float, odd));
+    bits = __builtin_bit_cast(uint32_t, v);
+    const auto halves = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
+    const uint32_t low = halves[0], high = halves[1];
+    return op(__builtin_bit_cast(float, low), __builtin_bit_cast(float, high));
+}
+
+template <int HD, int TYPE, bool TERMS, int DUP>
+__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_decode_kernel(PagedAttn a) {
+    constexpr int NS = HD / 32, NC = HD / 16, kRow = code_bytes(TYPE, HD), kRows = 16 / DUP, kOwn = 4 / DUP;
+    constexpr bool kScaled = TYPE != QK_TYPE_F16;
+    __shared__ float meet[3][kRows * (HD + 4)];
+    __shared__ half8 queries[2][NS][64];
+    const qk_paged_seq s = a.b.seqs[blockIdx.y];
+    if (!paged_seq_ok(s, a.b, a.page_shift)) return;
+    const int kvh = a.kv.kv_heads, G = a.group;
+    // A chip's XCDs take workgroups in turn: the splits rotate, or the first ones
+    // (which every sequence has) would all fall to the same XCDs.
+    const int splits = a.splits[0], h = blockIdx.x / splits, split = (blockIdx.x + h + blockIdx.y) % splits;
+    const int rows = s.count * G;
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, part = n % DUP;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+    // This lane's query row (past the last: that one again, masked and not written),
+    // the cache rows low .. up that it sees, those that all of them do, hidden .. seen.
+    const int row = n / DUP, tok = min(row, rows - 1) / G, own = min(row, rows - 1) - tok * G;
+    const bool have = row < rows;
+    const int mine = have ? s.pos + tok : -1;
+    int last = s.pos + s.count - 1, seen = s.pos, up = mine, low = 0, hidden = 0;
+    int64_t begin64 = static_cast<int64_t>(split) * a.split_rows[0];
+    if constexpr (TERMS) {
+        const int prefix = prefix_rows(a, s);
+        up = have ? max(mine, prefix - 1) : -1;
+        low = a.window ? mine - a.window + 1 : 0;
+        hidden = a.window ? last - a.window + 1 : 0;
+        begin64 += first_row(a, s);
+        last = max(last, prefix - 1);
+        seen = max(seen, prefix - 1);
+    }
+    if (begin64 > last) return;   // the merge takes the splits that reach a token
+    int begin = static_cast<int>(begin64);
+    const int end = static_cast<int>(min(begin64 + a.split_rows[0], int64_t(last) + 1));
+    if constexpr (TERMS)
+        if (a.window) begin = max(begin, (s.pos - a.window + 1) & ~(kTile - 1));   // no tile before the first token's window
+
+    // The queries in LDS, read for each tile (the same for all four waves): 8 NS
+    // registers fewer.
+    float qscale;
+    {
+        half8 qh[NS], ql[NS];
+        load_query<HD, TYPE, NS>(a.q + (s.first + tok) * a.ldq + static_cast<int64_t>(h * G + own) * HD, g, a.scale, qh, ql, qscale);
+        if (wave == 0)
+            #pragma unroll
+            for (int x = 0; x < NS; ++x) queries[0][x][lane] = qh[x], queries[1][x][lane] = ql[x];
+        __syncthreads();
+    }
+
+    float4v o[NC];
+    #pragma unroll
+    for (int c = 0; c < NC; ++c) o[c] = float4v{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    ValueUnits units;
+    const Nibbles codes;
+    const float slope = TERMS && a.slopes ? 1.4426950408889634f * a.slopes[h * G + own] : 0.f;
+    const float inverse_cap = TERMS && a.cap > 0.f ? 1.f / a.cap : 0.f;
+
+    // (Of the constant address space: looked up by scalar loads, which no wait for a
+    // tile's loads includes.)
+    typedef const __attribute__((address_space(4))) int32_t *Table;
+    const Table table = (Table)(a.b.page_table + static_cast<int64_t>(s.table) * a.b.table_stride);
+    const int64_t page_stride = static_cast<int64_t>(kvh) * a.kv.page_rows, head_row = static_cast<int64_t>(h) * a.kv.page_rows;
+    struct Pages {
+        int64_t id[2];
+    };
+    struct Tile {
+        KeyTile<HD, TYPE> k;
+        ValueTile<HD, TYPE> v;   // slot 2 k + hf: row 4 g + k of half hf
+        float ks[2][kOwn], vs[2][kOwn];   // of rows 4 g + part * kOwn ..
+        uint4v entry[2][2];               // 4-bit codes: scales and multipliers of value rows 4 g .. + 3
+        bool present[2];
+    };
+    auto pages_of = [&](int t0) {
+        Pages p;
+        #pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+            const int r = min(t0 + 16 * hf, last);
+            const int64_t page = table[r >> a.page_shift];
+            p.id[hf] = t0 + 16 * hf <= last && page >= 0 && page < a.kv.pages ? page : -1;
+        }
+        return p;
+    };
+    auto load = [&](Tile &t, int t0, const Pages &p) {
+        #pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+            t.present[hf] = p.id[hf] >= 0;
+            const int64_t base = max(p.id[hf], int64_t(0)) * page_stride + head_row + ((t0 + 16 * hf) & (a.kv.page_rows - 1));
+            t.k.load(hf, static_cast<const char *>(a.kv.key) + base * kRow + n * kRow, g);
+            #pragma unroll
+            for (int k = 0; k < 4; ++k)
+                t.v.load(2 * k + hf, static_cast<const char *>(a.kv.value) + base * kRow + (4 * g + k) * kRow, n);
+            if constexpr (kScaled) {
+                constexpr int kEntry = TYPE == QK_TYPE_I4 ? 2 : 1;
+                #pragma unroll
+                for (int i = 0; i < kOwn; ++i) {
+                    t.ks[hf][i] = (a.kv.key_scale + base * kEntry)[(4 * g + part * kOwn + i) * kEntry];
+                    if constexpr (TYPE != QK_TYPE_I4) t.vs[hf][i] = (a.kv.value_scale + base)[4 * g + part * kOwn + i];
+                }
+            }
+            if constexpr (TYPE == QK_TYPE_I4) {
+                t.k.mults[hf] = __builtin_bit_cast(uint32_t, (a.kv.key_scale + base * 2)[2 * n + 1]);
+                // (Whole entries, and all of them used: a register of a load that is not
+                // would be given to something else, which then waits for the load.)
+                const uint4v *e = reinterpret_cast<const uint4v *>(a.kv.value_scale + base * 2) + 2 * g;
+                t.entry[hf][0] = e[0];
+                t.entry[hf][1] = e[1];
+            }
+        }
+    };
+    // Of four values of rows 4 g + 0 .. 3 this lane's.
+    auto pick = [&](float r0, float r1, float r2, float r3, float *x) {
+        if constexpr (DUP == 4) {
+            const float even = part & 2 ? r2 : r0, odd = part & 2 ? r3 : r1;
+            x[0] = part & 1 ? odd : even;
+        } else {
+            x[0] = part ? r2 : r0;
+            x[1] = part ? r3 : r1;
+        }
+    };
+    auto take = [&](Tile &t, int t0) {
+        if constexpr (TYPE == QK_TYPE_I4)
+            #pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const uint32_t s[4] = {t.entry[hf][0][0], t.entry[hf][0][2], t.entry[hf][1][0], t.entry[hf][1][2]};
+                const float4v scale = __builtin_bit_cast(float4v, s);
+                pick(scale[0], scale[1], scale[2], scale[3], t.vs[hf]);
+            }
+        float4v st[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        Mult km[2];
+        if constexpr (TYPE == QK_TYPE_I4)
+            #pragma unroll
+            for (int hf = 0; hf < 2; ++hf) km[hf].set(t.k.mults[hf], t.k.mults[hf], mult_sel(g));
+        #pragma unroll
+        for (int x = 0; x < NS; ++x) {
+            const half8 qh = queries[0][x][lane], ql = queries[1][x][lane];
+            #pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const half8 k = t.k.operand(hf, x, km[hf], codes);
+                st[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql, st[hf], 0, 0, 0);
+                st[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh, st[hf], 0, 0, 0);
+            }
+        }
+        // Of rows t0 + 16 hf + 4 g + 0 .. 3 this lane's: x[kOwn hf + i] of row part * kOwn + i.
+        float x[2 * kOwn];
+        #pragma unroll
+        for (int hf = 0; hf < 2; ++hf) pick(st[hf][0], st[hf][1], st[hf][2], st[hf][3], x + hf * kOwn);
+        const bool edge = t0 + kTile - 1 > seen || !t.present[0] || !t.present[1] || (TERMS && t0 < hidden);
+        #pragma unroll
+        for (int i = 0; i < 2 * kOwn; ++i) {
+            // An infinite key's score: not a number, whatever its sign.
+            x[i] *= qscale;
+            if constexpr (kScaled)
+                x[i] *= fmaf(t.ks[i / kOwn][i % kOwn], 0.f, t.ks[i / kOwn][i % kOwn]);
+            else
+                x[i] = fmaf(x[i], 0.f, x[i]);
+        }
+        const int first = t0 + 4 * g + part * kOwn;   // the row of x[0]
+        if constexpr (TERMS) {
+            if (a.cap > 0.f) cap_scores<2 * kOwn>(x, a.cap, inverse_cap);
+            if (a.slopes) {
+                const float far = static_cast<float>(mine - first);
+                #pragma unroll
+                for (int i = 0; i < 2 * kOwn; ++i)
+                    x[i] = fmaf(-slope, fabsf(far - static_cast<float>(i / kOwn * 16 + i % kOwn)), x[i]);
+            }
+        }
+        if (edge) {
+            #pragma unroll
+            for (int i = 0; i < 2 * kOwn; ++i) {
+                const int at = first + i / kOwn * 16 + i % kOwn;
+                x[i] = t.present[i / kOwn] && at <= up && (!TERMS || at >= low) ? x[i] : -INFINITY;
+            }
+        }
+        // A larger maximum, or a product beyond the units, is met in few tiles: lanes look
+        // at their own rows, and join what they have only then.
+        auto larger = [](float a, float b) { return fmaxf(a, b); };
+        float mx = x[0], vtop = 0.f, f = 1.f;
+        #pragma unroll
+        for (int i = 1; i < 2 * kOwn; ++i) mx = fmaxf(mx, x[i]);
+        const bool more = __builtin_amdgcn_ballot_w64(mx > m);
+        if (more) {
+            const float mn = fmaxf(m, join_row<DUP>(mx, larger));
+            f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            l *= f;
+            m = mn;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        #pragma unroll
+        for (int i = 0; i < 2 * kOwn; ++i) {
+            const float w = __builtin_amdgcn_exp2f(x[i] - ref);
+            l += w;
+            if constexpr (kScaled) {   // a masked row's scale may be anything
+                x[i] = x[i] == -INFINITY ? 0.f : w * t.vs[i / kOwn][i % kOwn];
+                vtop = fmaxf(vtop, fabsf(t.vs[i / kOwn][i % kOwn]));
+            } else {
+                x[i] = w;
+            }
+        }
+        if (more || (kScaled && __builtin_amdgcn_ballot_w64(m != -INFINITY && !units.holds(vtop)))) {
+            float fo = f;
+            if constexpr (kScaled) {
+                bool one = false;
+                #pragma unroll
+                for (int i = 0; i < 2 * kOwn; ++i) one = one || t.vs[i / kOwn][i % kOwn] == 1.f;
+                auto largest = [&] {
+                    float y = 0.f;
+                    #pragma unroll
+                    for (int i = 0; i < 2 * kOwn; ++i) y = fmaxf(y, fabsf(x[i]));
+                    return join_row<DUP>(y, larger);
+                };
+                float y = largest();
+                units.known *= f;
+                if (__builtin_amdgcn_ballot_w64(one || units.strange(y))) {
+                    const uint32_t live = t.v.live();
+                    #pragma unroll
+                    for (int i = 0; i < 2 * kOwn; ++i)   // (a scale that is not finite stays)
+                        if (!(live >> (2 * (part * kOwn + i % kOwn) + i / kOwn) & 1) && fabsf(x[i]) < INFINITY) x[i] = 0.f;
+                    y = largest();
+                }
+                fo = units.renew(y, join_row<DUP>(vtop, larger), f);
+            }
+            #pragma unroll
+            for (int c = 0; c < NC; ++c)
+                #pragma unroll
+                for (int r = 0; r < 4; ++r) o[c][r] *= fo;
+        }
+        // Pairs of this lane, then of all four rows: upper halves in a query row's
+        // first column, lower ones in its others.
+        uint4v p;
+        {
+            const float k = kScaled ? units.factor : 0x1p15f;
+            uint32_t hi[kOwn], lo[kOwn];
+            #pragma unroll
+            for (int i = 0; i < kOwn; ++i) {
+                half2v ph, pl;
+                split_pair(x[i] * k, x[kOwn + i] * k, ph, pl);
+                hi[i] = __builtin_bit_cast(uint32_t, ph);
+                lo[i] = __builtin_bit_cast(uint32_t, pl);
+            }
+            // (Both sides of a choice are taken before it: lanes have to be active to be read.)
+            auto choose = [&](uint32_t up, uint32_t down) { return part == 0 ? up : down; };
+            if constexpr (DUP == 4) {
+                p[0] = choose(quad<0, 0, 0, 0>(hi[0]), quad<0, 0, 0, 0>(lo[0]));
+                p[1] = choose(quad<1, 1, 1, 1>(hi[0]), quad<1, 1, 1, 1>(lo[0]));
+                p[2] = choose(quad<2, 2, 2, 2>(hi[0]), quad<2, 2, 2, 2>(lo[0]));
+                p[3] = choose(quad<3, 3, 3, 3>(hi[0]), quad<3, 3, 3, 3>(lo[0]));
+            } else {
+                p[0] = choose(quad<0, 0, 2, 2>(hi[0]), quad<0, 0, 2, 2>(lo[0]));
+                p[1] = choose(quad<0, 0, 2, 2>(hi[1]), quad<0, 0, 2, 2>(lo[1]));
+                p[2] = choose(quad<1, 1, 3, 3>(hi[0]), quad<1, 1, 3, 3>(lo[0]));
+                p[3] = choose(quad<1, 1, 3, 3>(hi[1]), quad<1, 1, 3, 3>(lo[1]));
+            }
+        }
+        const half8 weights = __builtin_bit_cast(half8, p);
+        // A row that some token does not see meets it as 0 * value.
+        uint32_t bad = 0;
+        Mult vm[4];
+        #pragma unroll
+        for (int d = 0; d < (NC + 3) / 4; ++d) {
+            half8 v[4];
+            if constexpr (TYPE == QK_TYPE_I4)
+                if (d == 0 || HD == 96)   // (of 96 values a lane's first four and last two lie apart)
+                    #pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        vm[k].set(t.entry[0][k / 2][k % 2 * 2 + 1], t.entry[1][k / 2][k % 2 * 2 + 1],
+                                  mult_sel(value_dim<HD, TYPE>(n, 4 * d) / (HD / 4)));
+            t.v.operands(d, v, vm, codes);
+            #pragma unroll
+            for (int k = 0; k < 4 && 4 * d + k < NC; ++k) {
+                if (!whole_codes(TYPE) && edge) clear_not_finite(v[k], bad);
+                o[4 * d + k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[k], weights, o[4 * d + k], 0, 0, 0);
+            }
+        }
+        if (!whole_codes(TYPE) && edge && __builtin_amdgcn_ballot_w64(bad != 0)) {
+            // The tokens that see such a row: not finite.
+            #pragma unroll
+            for (int off = 1; off < 16; off <<= 1) bad |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(bad), off));
+            #pragma unroll
+            for (int hf = 0; hf < 2; ++hf)
+                #pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int at = t0 + 16 * hf + 4 * g + r;
+                    if ((bad >> (2 * r + hf) & 1) && t.present[hf] && at <= up && (!TERMS || at >= low)) l = __builtin_nanf("");
+                }
+        }
+    };
+    // Tiles in registers by turns, one multiplied while the others load; a tile's
+    // pages are looked up before its turn to load comes.  Past the wave's last tile
+    // that one again: loads that may be left out would have every wait for a tile wait
+    // for all that is under way.
+    constexpr int kStep = 4 * kTile;
+    int t0 = begin + wave * kTile;
+    if (t0 < end) {
+        const int final = t0 + (end - 1 - t0) / kStep * kStep;
+        Tile tiles[2];
+        load(tiles[0], t0, pages_of(t0));
+        Pages ahead = pages_of(min(t0 + kStep, final));
+        for (bool more = true; more;) {
+            #pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                load(tiles[i ^ 1], min(t0 + kStep, final), ahead);
+                asm volatile("" ::: "memory");   // or they would sink to where the tile is known to be needed
+                ahead = pages_of(min(t0 + 2 * kStep, final));
+                take(tiles[i], t0);
+                if ((t0 += kStep) >= end) {
+                    more = false;
+                    break;
+                }
+            }
+        }
+    }
+    l = join_row<DUP>(l, [](float a, float b) { return a + b; });
+    // The waves' means (sums could pass fp32's range), then into wave 0, in wave order.
+    auto share_of = [](float l) { return l == 0.f ? 0.f : 1.f / l; };   // no row seen: zeros
+    const int back = (kScaled ? units.exponent() : 0) - 15;
+    const float inverse = share_of(l);
+    #pragma unroll
+    for (int c = 0; c < NC; ++c)
+        #pragma unroll
+        for (int r = 0; r < 4; ++r) o[c][r] = ldexpf((o[c][r] + quad<1, 0, 3, 2>(o[c][r])) * inverse, back);
+    // Of a query row's lanes the first has all of its dimensions 4 g + r of 16.
+    if (wave > 0 && part == 0) {
+        float *mineat = meet[wave - 1] + row * (HD + 4);
+        #pragma unroll
+        for (int c = 0; c < NC; ++c) *reinterpret_cast<float4v *>(mineat + (c * 4 + g) * 4) = o[c];
+        if (g == 0) {
+            mineat[HD] = m;
+            mineat[HD + 1] = l;
+        }
+    }
+    __syncthreads();
+    if (wave > 0 || part != 0 || !have) return;
+    float mw[4] = {m}, lw[4] = {l};
+    #pragma unroll
+    for (int w = 0; w < 3; ++w) {
+        mw[w + 1] = meet[w][row * (HD + 4) + HD];
+        lw[w + 1] = meet[w][row * (HD + 4) + HD + 1];
+    }
+    m = fmaxf(fmaxf(mw[0], mw[1]), fmaxf(mw[2], mw[3]));
+    l = 0.f;
+    #pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        lw[w] *= __builtin_amdgcn_exp2f(mw[w] - (m == -INFINITY ? 0.f : m));
+        l += lw[w];
+    }
+    const float whole = share_of(l);
+    #pragma unroll
+    for (int c = 0; c < NC; ++c)
+        #pragma unroll
+        for (int r = 0; r < 4; ++r) o[c][r] *= lw[0] * whole;
+    #pragma unroll
+    for (int w = 0; w < 3; ++w) {
+        const float f = lw[w + 1] * whole;
+        #pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const float4v po = *reinterpret_cast<const float4v *>(meet[w] + row * (HD + 4) + (c * 4 + g) * 4);
+            #pragma unroll
+            for (int r = 0; r < 4; ++r) o[c][r] = fmaf(po[r], f, o[c][r]);
+        }
+    }
     const int head = h * G + own;
     float *dst = a.out + (s.first + tok) * a.ldout + static_cast<int64_t>(head) * HD;
     if (splits > 1) {
@@ -906,6 +1353,11 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
     using C = Chunk<HD, TYPE>;
     constexpr int NS = HD / 16, ND = HD / 32, kRow = code_bytes(TYPE, HD);
     constexpr bool kScaled = TYPE != QK_TYPE_F16;
+    // Scores in base-2 units of rows without scales: the maximum that weights are taken
+    // from follows only when it has grown by 2^kSlack, so the sums are seldom rescaled
+    // (of 32 query rows some one's maximum grows in most tiles); weights are below
+    // 2^kSlack then and their halves in units of 2^(kSlack - 15).
+    constexpr float kSlack = TERMS && !kScaled ? 8.f : 0.f, kUnit = TERMS && !kScaled ? 0x1p7f : 0x1p15f;
     extern __shared__ __align__(16) char lds[];
     const qk_paged_seq s = a.b.seqs[blockIdx.y];
     if (!paged_seq_ok(s, a.b, a.page_shift)) return;
@@ -994,9 +1446,9 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
             for (int i = 0; i < C::kKeyRegs; ++i)
                 __builtin_memcpy(&g.key[i], keys + 16 * i, kB - 16 * i < 16 ? kB - 16 * i : 16);
             g.key_mults = __builtin_bit_cast(uint32_t, a.kv.key_scale[2 * (first + (tid / 4 & 15)) + 1]);
-            const uint4v *e = reinterpret_cast<const uint4v *>(a.kv.value_scale + 2 * (first + 4 * (quad & 3)));
-            const uint4v lo = e[0], hi = e[1];
-            g.value_mults[0] = lo[1], g.value_mults[1] = lo[3], g.value_mults[2] = hi[1], g.value_mults[3] = hi[3];
+            const float *entries = a.kv.value_scale + 2 * (first + 4 * (quad & 3));
+            #pragma unroll
+            for (int r = 0; r < 4; ++r) g.value_mults[r] = __builtin_bit_cast(uint32_t, entries[2 * r + 1]);
         } else {
             #pragma unroll
             for (int i = 0; i < C::kKeys; ++i) {
@@ -1024,6 +1476,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
                     [(page * page_stride + head_row + (group & mask) + (tid & 15)) * (TYPE == QK_TYPE_I4 ? 2 : 1)];
     };
     int top_ev = kLeastExponent, low_ev = INT32_MAX;   // wave 0's: exponents of the value scales so far
+    const Nibbles codes;
     auto store = [&](const Stage &g, int t0, char *buf) {
         auto &head = *reinterpret_cast<typename C::Head *>(buf + C::kKeyBytes + C::kValueBytes);
         const bool edge = cut(t0);
@@ -1058,7 +1511,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
             m.set(g.key_mults, g.key_mults, mult_sel(tid % 4));
             #pragma unroll
             for (int w = 0; w < C::kKeyCols / 8; ++w)
-                *reinterpret_cast<half8 *>(at + 16 * w) = codes8(g.key[w / 4][w % 4] ^ 0x88888888u, m);
+                *reinterpret_cast<half8 *>(at + 16 * w) = codes.eight(g.key[w / 4][w % 4], m);
         }
         #pragma unroll
         for (int i = 0; i < (TYPE == QK_TYPE_I4 ? 0 : C::kKeys); ++i) {
@@ -1091,10 +1544,10 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
             if constexpr (TYPE == QK_TYPE_I4) {
                 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    const uint32_t x = g.value[2 * k][d4 / 2] ^ 0x88888888u, y = g.value[2 * k + 1][d4 / 2] ^ 0x88888888u;
-                    const uint32_t sel = 0x0C040C00u + 0x10001u * (2 * (d4 & 1));
-                    codes2x2(__builtin_amdgcn_perm(y, x, sel), vm[k], p[0][k], p[1][k]);
-                    codes2x2(__builtin_amdgcn_perm(y, x, sel + 0x10001u), vm[k], p[2][k], p[3][k]);
+                    half2v four[4];
+                    codes.four(g.value[2 * k][d4 / 2], g.value[2 * k + 1][d4 / 2], four_sel(d4 & 1), vm[k], four);
+                    #pragma unroll
+                    for (int c = 0; c < 4; ++c) p[c][k] = four[c];
                 }
             } else if constexpr (TYPE == QK_TYPE_F16) {
                 #pragma unroll
@@ -1208,10 +1661,12 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
         // Half a tile at a time, the second half's scores begun before the first
         // one's weights, which run beside them: 2 % of a long chunk's time (all 32
         // scores a lane at once left too few registers).
+        // (With terms there are too few registers for that.)
         float16v st, ahead;
         scores(0, st);
         #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
+            if (TERMS && hf == 1) scores(1, st);
             // Register r: row t0 + 32 hf + 8 (r / 4) + 4 hi + r % 4.
             #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
@@ -1259,7 +1714,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
                 known = c == INFINITY ? 0.f : kCoarse;   // of alike scales, at least
             }
             // Besides: scales are apart, and the tile may hold a product beyond a row's units.
-            if (en != ev || renew || __builtin_amdgcn_ballot_w64(mn > m || (room && c != INFINITY && lift > static_cast<float>(room)))) {
+            if (en != ev || renew || __builtin_amdgcn_ballot_w64(mn > m + kSlack || (room && c != INFINITY && lift > static_cast<float>(room)))) {
                 // c is what the weights so far were taken with, rounding and all.
                 const float cn = kScaled ? fminf(c, -mn * by) : mn == -INFINITY ? INFINITY : -mn * (TERMS ? 1.f : qscale);
                 const float f = cn == INFINITY ? 1.f : __builtin_amdgcn_exp2f(cn - c);
@@ -1314,7 +1769,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
                         if ((bad >> (8 * (r / 4) + r % 4) & 1) && st[r] != -INFINITY) l = __builtin_nanf("");
                 }
             }
-            if (hf == 0) scores(1, ahead);
+            if (!TERMS && hf == 0) scores(1, ahead);
             #pragma unroll
             for (int b = 0; b < 2; ++b) {   // 16 rows
                 half2v pu[4], pw[4];
@@ -1329,7 +1784,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
                         const float x = st[8 * b + 4 * r4 + r];
                         const float w = __builtin_amdgcn_exp2f(fmaf(x, by, ref));
                         l += w;
-                        y[r] = w * (kScaled ? vs[r] : 0x1p15f);
+                        y[r] = w * (kScaled ? vs[r] : kUnit);
                     }
                     split_pair(y[0], y[1], pu[2 * r4], pw[2 * r4]);
                     split_pair(y[2], y[3], pu[2 * r4 + 1], pw[2 * r4 + 1]);
@@ -1344,7 +1799,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
                 #pragma unroll
                 for (int d = 0; d < ND; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], ph, o[d], 0, 0, 0);
             }
-            st = ahead;
+            if constexpr (!TERMS) st = ahead;
         }
     };
 
@@ -1372,7 +1827,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
     l += __shfl_xor(l, 32);
     if (!have) return;
     const int head = h * G + own;
-    const int back = kScaled ? ev - 15 : -15;
+    const int back = kScaled ? ev - 15 : TERMS ? -7 : -15;
     const float inverse = l == 0.f ? 0.f : 1.f / l;   // no row seen: zeros
     float *dst = a.out + (s.first + tok) * a.ldout + static_cast<int64_t>(head) * HD;
     if (splits > 1) {
@@ -1397,6 +1852,18 @@ int attend_launch(const PagedAttn &a, hipStream_t stream) {
     auto grid = [&](int64_t n, int tile, int splits) {
         return dim3(static_cast<unsigned>((n + tile - 1) / tile * a.kv.kv_heads * splits), a.b.n_seqs);
     };
+    // Few rows: 64 sequences over 1000 to 8000 4-bit rows, eight KV heads of 128, in us,
+    // against the 16-row kernel: 4 query rows 90 and 124, 8 102 and 128; 16 sequences over
+    // 4000 of 256, 2 query rows 45 and 68.  With terms, 32 sequences of int8 over windows
+    // of 4096: 60 and 67; of 1000: 23 and 26; float8, 8 query rows over 3000: 52 and 54.
+    // Of fp16 rows the loads alone take the time: 32 sequences over 3000 86 and 80.
+    if constexpr (TYPE == QK_TYPE_I4 || (TERMS && TYPE != QK_TYPE_F16)) {
+        if (rows <= 8) {
+            auto kernel = rows <= 4 ? paged_decode_kernel<HD, TYPE, TERMS, 4> : paged_decode_kernel<HD, TYPE, TERMS, 2>;
+            hipLaunchKernelGGL(kernel, grid(1, 1, a.splits[0]), dim3(256), 0, stream, a);
+            return launch_status("qk_paged_attention_f32 launch");
+        }
+    }
     if (a.few_rows > 0)
         hipLaunchKernelGGL((paged_attention_kernel<HD, TYPE, TERMS>),
                            grid(std::min<int64_t>(rows, a.few_rows), kRowTile, a.splits[0]), dim3(256), 0, stream, a);

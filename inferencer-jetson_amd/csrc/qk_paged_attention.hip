@@ -83,6 +83,9 @@ constexpr int64_t kManyPairs = 3 << 22;
 int few_rows(const qk_paged_batch &b, int heads, int kv_heads) {
     const int64_t rows = static_cast<int64_t>(b.max_count) * (heads / kv_heads);
     if (rows <= kFewRows) return INT32_MAX;
+#ifdef QK_FORCE
+    return QK_FORCE ? (b.n_seqs == 1 ? 0 : kFewRows) : INT32_MAX;
+#endif
     const int64_t units = (rows + kChunkRows - 1) / kChunkRows * kv_heads * b.n_seqs;
     const double pairs = static_cast<double>(b.n_tokens) * heads * b.max_rows;
     if (units < kManyUnits && pairs < kManyPairs) return INT32_MAX;
