@@ -1,13 +1,15 @@
 // qk_pages.hip - a pool of cache pages: given out and taken back, forked, compacted,
 // and copied, all on the device.
 //
-// A call is a few launches: one over the table's rows (a workgroup each) that says
-// what each row gives back and lacks, one of a single workgroup that adds up what is
-// lacking and lists as many free pages (or, compacting, pairs pages to move with
-// free ones before them), one over the rows again that fills them in, and the copies
-// of contents.  Pages are given in the order of table rows and their entries, lowest
-// page first: what a call does depends on the table and the counts alone, and the
-// atomics on the counts are sums of whole numbers.
+// A call is a few launches.  One over the table's rows (a wave each) says what each
+// row gives back and lacks; one adds up what rows lack, in order, and writes down which
+// pages are free, a bit each, and how many of each segment of the pool; one over the
+// rows again in which a wave finds the free pages of its ranks and fills them in; and
+// the copies of contents.
+// (Compacting, one workgroup pairs pages to move with free ones before them.)  Pages
+// are given in the order of table rows and their entries, lowest page first: what a
+// call does depends on the table and the counts alone, and the atomics on the counts
+// are sums of whole numbers.
 #include "qk_paged.h"
 
 #include <algorithm>
@@ -20,39 +22,49 @@ hipStream_t S(qk_stream s) { return static_cast<hipStream_t>(s); }
 // ---------------------------------------------------------- workspace --
 
 // What the launches of a call leave each other, in 32-bit numbers: how many pages
-// are given (or moved), then for each table row what it lacks and the rank of its
-// first page, the pages given, the sources of their copies, and the rows that a fork
-// makes (or, compacting, the new number of each page).
+// are given (or moved), the free pages of each segment, and all of them a bit each
+// (the counts change while pages are given), for each table row what it
+// lacks and the rank of its first page, the pages given by rank, the sources of their
+// copies, and the rows that a fork makes (or, compacting, the new number of each page).
 struct Space {
-    int32_t *counts, *need, *base, *list, *source, *next;
+    int32_t *counts, *free;
+    uint64_t *bits;
+    int32_t *need, *base, *list, *source, *next;
 };
-constexpr int kCounts = 16;   // counts[0]: pages given; [1]: pages moved; [2]: live pages
+constexpr int kCounts = 16;   // counts[0]: pages given or moved; [1]: wanted; [2]: live pages
+
+// Segments of the pool: 4096 pages, or as many times that as make 256 of them.
+constexpr int kSegments = 256, kSegment = 4096;
+constexpr int64_t segment_pages(int64_t pages) {
+    return (pages + int64_t(kSegments) * kSegment - 1) / (int64_t(kSegments) * kSegment) * kSegment;
+}
 
 int64_t list_entries(const qk_page_pool &p) {
-    return std::min<int64_t>(p.pages, static_cast<int64_t>(p.table_rows) * p.table_stride);
+    return std::max<int64_t>(std::min<int64_t>(p.pages, static_cast<int64_t>(p.table_rows) * p.table_stride), p.pages / 2 + 1);
 }
+int64_t bit_words(const qk_page_pool &p) { return (p.pages + kSegment - 1) / kSegment * (kSegment / 64); }
 int64_t next_entries(const qk_page_pool &p) {
     return std::max<int64_t>(p.pages, static_cast<int64_t>(p.table_rows) * p.table_stride);
 }
 int64_t space_entries(const qk_page_pool &p) {
-    return kCounts + 2 * static_cast<int64_t>(p.table_rows) + 2 * std::max<int64_t>(list_entries(p), p.pages / 2 + 1) +
-           next_entries(p);
+    return kCounts + kSegments + 2 * bit_words(p) + 2 * static_cast<int64_t>(p.table_rows) + 2 * list_entries(p) + next_entries(p);
 }
 Space space_of(const qk_page_pool &p, void *workspace) {
     Space s;
-    const int64_t list = std::max<int64_t>(list_entries(p), p.pages / 2 + 1);
     s.counts = static_cast<int32_t *>(workspace);
-    s.need = s.counts + kCounts;
+    s.free = s.counts + kCounts;
+    s.bits = reinterpret_cast<uint64_t *>(s.free + kSegments);
+    s.need = reinterpret_cast<int32_t *>(s.bits + bit_words(p));
     s.base = s.need + p.table_rows;
     s.list = s.base + p.table_rows;
-    s.source = s.list + list;
-    s.next = s.source + list;
+    s.source = s.list + list_entries(p);
+    s.next = s.source + list_entries(p);
     return s;
 }
 
 struct Pool {
     int32_t *table, *refs;
-    int rows, stride, pages, page_rows;
+    int rows, stride, pages, page_rows, segment;
     __device__ __forceinline__ bool is_page(int32_t p) const { return p >= 0 && p < pages; }
     __device__ __forceinline__ int32_t *row(int r) const { return table + static_cast<int64_t>(r) * stride; }
 };
@@ -147,33 +159,118 @@ __device__ __forceinline__ int rank_pages(const int32_t *refs, int pages, int mo
     return min(found, most);
 }
 
-// What the rows lack, in order, and the free pages for it.
-__global__ __launch_bounds__(kScanThreads) void give_kernel(Pool p, Space s, int32_t *missing) {
+// Workgroup 0: the rank of each row's first page; the others: the free pages of a
+// segment each.
+__global__ __launch_bounds__(kScanThreads) void count_kernel(Pool p, Space s) {
     __shared__ u64 part[kScanThreads / 64];
-    u64 need = 0, over = 0;   // entries; those that the table has no place for
-    for (int r0 = 0; r0 < p.rows; r0 += kScanThreads) {
-        const int r = r0 + threadIdx.x;
-        u64 total;
-        const u64 mine = r < p.rows ? static_cast<uint32_t>(s.need[r]) | static_cast<u64>(static_cast<uint32_t>(s.base[r])) << 32 : 0;
-        const u64 before = block_sums<kScanThreads / 64>(mine & 0xFFFFFFFFull, total, part);
-        if (r < p.rows) s.base[r] = static_cast<int32_t>(need + before);
-        need += total;
-        block_sums<kScanThreads / 64>(mine >> 32, total, part);
-        over += total;
+    u64 total;
+    if (blockIdx.x == 0) {
+        u64 need = 0;
+        for (int r0 = 0; r0 < p.rows; r0 += kScanThreads) {
+            const int r = r0 + threadIdx.x;
+            const u64 before = block_sums<kScanThreads / 64>(r < p.rows ? s.need[r] : 0, total, part);
+            if (r < p.rows) s.base[r] = static_cast<int32_t>(need + before);
+            need += total;
+        }
+        if (threadIdx.x == 0) s.counts[1] = static_cast<int32_t>(need);
+        return;
     }
-    int32_t *const list = s.list;
-    const int found = need == 0 ? 0 : rank_pages(
-        p.refs, p.pages, static_cast<int>(need), part, [](int32_t count, int) { return count == 0; },
-        [&](int rank, int page) { list[rank] = page; });
-    if (threadIdx.x == 0) {
-        s.counts[0] = found;
-        if (missing) *missing = static_cast<int32_t>(min(need - found + over, u64(0x7FFFFFFF)));
+    // A wave 64 pages at a time, a bit a lane.
+    const int segment = blockIdx.x - 1, lane = threadIdx.x & 63;
+    const int64_t first = static_cast<int64_t>(segment) * p.segment, end = min(first + p.segment, int64_t(p.pages));
+    int count = 0;
+    constexpr int kLoads = 4;
+    for (int64_t w0 = first + threadIdx.x - lane; w0 < end; w0 += kScanThreads * kLoads) {
+        int32_t c[kLoads];
+        #pragma unroll
+        for (int k = 0; k < kLoads; ++k) c[k] = w0 + k * kScanThreads + lane < end ? p.refs[w0 + k * kScanThreads + lane] : 1;
+        #pragma unroll
+        for (int k = 0; k < kLoads; ++k) {
+            const uint64_t word = __builtin_amdgcn_ballot_w64(c[k] == 0);
+            if (lane == 0 && w0 + k * kScanThreads < end) s.bits[(w0 + k * kScanThreads) / 64] = word;
+            count += __popcll(word);
+        }
     }
+    block_sums<kScanThreads / 64>(lane == 0 ? static_cast<u64>(count) : 0, total, part);
+    if (threadIdx.x == 0) s.free[segment] = static_cast<int32_t>(total);
+}
+
+// How many lanes before this one a mask holds.
+__device__ __forceinline__ int lanes_before(uint64_t mask) {
+    return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+}
+
+// A wave lists the free pages of ranks base .. base + n - 1 (kFound at most), as far as
+// there are, in `found` (LDS of its own); the number of free pages.  From the segment that holds the first one
+// on it looks at 4096 pages at a time, a word of 64 a lane.
+constexpr int kFound = 256;
+__device__ __forceinline__ int find_pages(const Pool &p, const Space &s, int base, int n, int32_t *found) {
+    const int lane = threadIdx.x & 63, segments = (p.pages + p.segment - 1) / p.segment;
+    int all = 0, segment = 0, skipped = 0;   // the free pages of segments before `segment`
+    for (int g0 = 0; g0 < segments; g0 += 64) {
+        const int own = g0 + lane < segments ? s.free[g0 + lane] : 0;
+        int upto = own;
+        #pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int other = __shfl_up(upto, off);
+            if (lane >= off) upto += other;
+        }
+        upto += all;
+        const int whole = __popcll(__builtin_amdgcn_ballot_w64(g0 + lane < segments && upto <= base));   // (a run of lanes)
+        if (whole > 0) segment = g0 + whole, skipped = __shfl(upto, whole - 1);
+        all = __shfl(upto, 63);
+    }
+    int64_t at = static_cast<int64_t>(segment) * p.segment;
+    for (int rank = skipped; at < p.pages && rank < base + n; at += kSegment) {
+        const int64_t first = at + lane * 64;
+        uint64_t word = first < p.pages ? s.bits[first / 64] : 0;
+        const int own = __popcll(word);
+        int upto = own;
+        #pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int other = __shfl_up(upto, off);
+            if (lane >= off) upto += other;
+        }
+        const int k = rank + upto - own;   // the rank of this lane's first
+        if (k < base + n && k + own > base) {
+            // Without the ones before rank base: where that many lower bits end, by halves.
+            int skip = max(base - k, 0), at_bit = 0;
+            const int from = max(k, base) - base, upto_here = min(k + own, base + n) - base;
+            for (int width = 32; width > 0; width >>= 1) {
+                const int lower = __popcll(word >> at_bit & ((1ull << width) - 1));
+                if (skip >= lower) skip -= lower, at_bit += width;
+            }
+            word = word >> at_bit << at_bit;
+            for (int i = from; i < upto_here; ++i, word &= word - 1) found[i] = static_cast<int32_t>(first + __builtin_ctzll(word));
+        }
+        rank += __shfl(upto, 63);
+    }
+    asm volatile("" ::: "memory");   // other lanes read it, in the order of the wave's LDS accesses
+    return all;
 }
 
 // ------------------------------------------------------------- resize --
 
-constexpr int kRowThreads = 256;
+constexpr int kRowWaves = 4;   // rows of a workgroup, a wave each
+
+__device__ __forceinline__ int row_of_wave() {
+    return blockIdx.x * kRowWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+}
+
+// The row's entries in order, 256 at a time, four loads under way: use(entry, page)
+// by the lane that has it, for all lanes at once (entry may be beyond the row).
+template <typename Use>
+__device__ __forceinline__ void each_entry(const int32_t *row, int first, int end, Use use) {
+    const int lane = threadIdx.x & 63;
+    constexpr int kLoads = 4;
+    for (int e0 = first; e0 < end; e0 += 64 * kLoads) {
+        int32_t page[kLoads];
+        #pragma unroll
+        for (int k = 0; k < kLoads; ++k) page[k] = e0 + k * 64 + lane < end ? row[e0 + k * 64 + lane] : -1;
+        #pragma unroll
+        for (int k = 0; k < kLoads; ++k) use(e0 + k * 64 + lane, page[k]);
+    }
+}
 
 // Entries first .. last - 1 are those that row r is to have (last may lie beyond the
 // table); false: the row stays as it is.
@@ -186,53 +283,63 @@ __device__ __forceinline__ bool wanted(const Pool &p, const int32_t *begins, con
     return true;
 }
 
-__global__ __launch_bounds__(kRowThreads) void resize_look_kernel(Pool p, Space s, const int32_t *begins, const int32_t *lengths) {
-    __shared__ int lacks;
-    const int r = blockIdx.x;
-    int first = 0, last = 0;
-    const bool change = wanted(p, begins, lengths, r, first, last);
-    if (threadIdx.x == 0) lacks = 0;
-    __syncthreads();
-    int lack = 0;
-    if (change)
-        for (int e = threadIdx.x; e < p.stride; e += kRowThreads) {
-            const int32_t page = p.row(r)[e];
-            const bool want = e >= first && e < last;
+__global__ __launch_bounds__(64 * kRowWaves) void resize_look_kernel(Pool p, Space s, const int32_t *begins, const int32_t *lengths) {
+    const int r = row_of_wave();
+    if (r >= p.rows) return;
+    int first = 0, last = 0, lacks = 0;
+    if (wanted(p, begins, lengths, r, first, last))
+        each_entry(p.row(r), 0, p.stride, [&](int e, int32_t page) {
+            const bool want = e >= first && e < min(last, p.stride);
             if (p.is_page(page) && !want) {
                 atomicSub(p.refs + page, 1);
                 p.row(r)[e] = -1;
             }
-            lack += want && !p.is_page(page);
-        }
-    if (lack) atomicAdd(&lacks, lack);
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        s.need[r] = lacks;
-        s.base[r] = change ? max(last - max(first, p.stride), 0) : 0;
-    }
+            lacks += __popcll(__builtin_amdgcn_ballot_w64(want && !p.is_page(page)));
+        });
+    if ((threadIdx.x & 63) == 0) s.need[r] = lacks;
 }
 
-__global__ __launch_bounds__(kRowThreads) void resize_fill_kernel(Pool p, Space s, const int32_t *begins, const int32_t *lengths) {
-    __shared__ u64 part[kRowThreads / 64];
-    const int r = blockIdx.x;
-    if (s.need[r] == 0) return;
+// (What row 0's wave says: the entries that got no page, and those that the table has
+// no place for.)
+__global__ __launch_bounds__(64 * kRowWaves) void resize_fill_kernel(Pool p, Space s, const int32_t *begins, const int32_t *lengths,
+                                                                      int32_t *missing) {
+    __shared__ int32_t pages[kRowWaves][kFound];
+    int32_t *const found = pages[threadIdx.x >> 6];
+    const int r = row_of_wave(), lane = threadIdx.x & 63;
+    if (r >= p.rows) return;
+    const int n = s.need[r];
+    if (n == 0 && (r > 0 || !missing)) return;
+    const int base = s.base[r];
+    int all = find_pages(p, s, base, min(n, kFound), found);
+    if (r == 0 && missing) {
+        int64_t over = 0;
+        for (int i = lane; i < p.rows; i += 64) {
+            int first = 0, last = 0;
+            if (wanted(p, begins, lengths, i, first, last)) over += max(last - max(first, p.stride), 0);
+        }
+        #pragma unroll
+        for (int off = 32; off > 0; off >>= 1) over += __shfl_xor(over, off);
+        if (lane == 0) *missing = static_cast<int32_t>(min(max(s.counts[1] - all, 0) + over, int64_t(0x7FFFFFFF)));
+    }
+    if (n == 0) return;
     int first = 0, last = 0;
     wanted(p, begins, lengths, r, first, last);
-    const int given = s.counts[0];
-    int rank = s.base[r];
-    const int end = min(last, p.stride);
-    for (int e0 = first; e0 < end; e0 += kRowThreads) {
-        const int e = e0 + threadIdx.x;
-        const bool lacks = e < end && !p.is_page(p.row(r)[e]);
-        u64 total;
-        const int k = rank + static_cast<int>(block_sums<kRowThreads / 64>(lacks, total, part));
-        if (lacks) {
-            const int32_t page = k < given ? s.list[k] : -1;
-            p.row(r)[e] = page;
-            if (page >= 0) p.refs[page] = 1;   // it was free, and is given once
+    int rank = 0, listed = 0;   // of the row's own; those before `listed` are no longer in LDS
+    each_entry(p.row(r), first, min(last, p.stride), [&](int e, int32_t page) {
+        const bool lacks = e < min(last, p.stride) && !p.is_page(page);
+        const uint64_t mask = __builtin_amdgcn_ballot_w64(lacks);
+        if (rank + __popcll(mask) > listed + kFound) {   // the next ones, from this entry on
+            listed = rank;
+            find_pages(p, s, base + listed, min(n - listed, kFound), found);
         }
-        rank += static_cast<int>(total);
-    }
+        const int k = rank + lanes_before(mask);
+        if (lacks) {
+            const int32_t given = base + k < all ? found[k - listed] : -1;
+            p.row(r)[e] = given;
+            if (given >= 0) p.refs[given] = 1;   // it was free, and is given once
+        }
+        rank += __popcll(mask);
+    });
 }
 
 // --------------------------------------------------------------- fork --
@@ -243,43 +350,53 @@ __device__ __forceinline__ bool forks(const Pool &p, const int32_t *parents, int
 
 // The rows of the forks as they will be but for fresh pages (parents may be forks
 // themselves: all rows are read before any is written).
-__global__ __launch_bounds__(kRowThreads) void fork_look_kernel(Pool p, Space s, const int32_t *parents, const int32_t *lengths) {
-    const int r = blockIdx.x;
-    if (!forks(p, parents, r)) {
-        if (threadIdx.x == 0) s.need[r] = s.base[r] = 0;
-        return;
+__global__ __launch_bounds__(64 * kRowWaves) void fork_look_kernel(Pool p, Space s, const int32_t *parents, const int32_t *lengths) {
+    const int r = row_of_wave(), lane = threadIdx.x & 63;
+    if (r >= p.rows) return;
+    int need = 0;
+    if (forks(p, parents, r)) {
+        const int length = max(lengths[r], 0), full = length / p.page_rows;
+        const bool part = length % p.page_rows != 0;
+        int32_t *next = s.next + static_cast<int64_t>(r) * p.stride;
+        each_entry(p.row(parents[r]), 0, p.stride, [&](int e, int32_t page) {
+            const bool held = p.is_page(page) && (e < full || (e == full && part));
+            if (e < p.stride) next[e] = held ? page : -1;
+            need += __builtin_amdgcn_ballot_w64(held && e == full) != 0;
+        });
     }
-    const int length = max(lengths[r], 0), full = length / p.page_rows;
-    const int32_t *from = p.row(parents[r]);
-    if (threadIdx.x == 0) {
-        s.need[r] = length % p.page_rows && full < p.stride && p.is_page(from[full]);
-        s.base[r] = 0;
-    }
-    int32_t *next = s.next + static_cast<int64_t>(r) * p.stride;
-    for (int e = threadIdx.x; e < p.stride; e += kRowThreads) {
-        const int32_t page = from[e];
-        next[e] = p.is_page(page) && (e < full || (e == full && length % p.page_rows)) ? page : -1;
-    }
+    if (lane == 0) s.need[r] = need;
 }
 
-__global__ __launch_bounds__(kRowThreads) void fork_fill_kernel(Pool p, Space s, const int32_t *parents, const int32_t *lengths) {
-    const int r = blockIdx.x;
-    if (!forks(p, parents, r)) return;
-    const int full = max(lengths[r], 0) / p.page_rows, k = s.base[r];
-    const bool fresh = s.need[r] != 0;
+__global__ __launch_bounds__(64 * kRowWaves) void fork_fill_kernel(Pool p, Space s, const int32_t *parents, const int32_t *lengths,
+                                                                    int32_t *missing) {
+    const int r = row_of_wave(), lane = threadIdx.x & 63;
+    if (r >= p.rows) return;
+    const bool fork = forks(p, parents, r);
+    if (!fork && r > 0) return;
+    const int n = s.need[r], k = s.base[r];
+    __shared__ int32_t pages[kRowWaves][kFound];
+    int32_t *const found = pages[threadIdx.x >> 6];   // (n is 1 at most)
+    int all = 0;
+    if (n > 0 || r == 0) all = find_pages(p, s, k, n, found);
+    if (r == 0 && lane == 0) {
+        s.counts[0] = min(s.counts[1], all);   // pairs to copy
+        if (missing) *missing = max(s.counts[1] - all, 0);
+    }
+    if (!fork) return;
+    const int full = max(lengths[r], 0) / p.page_rows;
+    const int32_t fresh = n > 0 && k < all ? found[0] : -1;
     const int32_t *next = s.next + static_cast<int64_t>(r) * p.stride;
-    for (int e = threadIdx.x; e < p.stride; e += kRowThreads) {
-        const int32_t old = p.row(r)[e];
+    each_entry(p.row(r), 0, p.stride, [&](int e, int32_t old) {
+        if (e >= p.stride) return;
         int32_t page = next[e];
-        if (fresh && e == full) {
-            const int32_t source = page;
-            page = k < s.counts[0] ? s.list[k] : -1;
-            if (page >= 0) s.source[k] = source;
+        if (n > 0 && e == full) {
+            if (fresh >= 0) s.source[k] = page, s.list[k] = fresh;
+            page = fresh;
         }
         if (p.is_page(old)) atomicSub(p.refs + old, 1);
         if (page >= 0) atomicAdd(p.refs + page, 1);
         p.row(r)[e] = page;
-    }
+    });
 }
 
 // ------------------------------------------------------------ compact --
@@ -437,7 +554,8 @@ int check_space(const char *where, const qk_page_pool *p, const void *workspace,
 }
 
 Pool pool_of(const qk_page_pool &p) {
-    return Pool{p.page_table, p.refs, p.table_rows, p.table_stride, static_cast<int>(p.pages), p.page_rows};
+    return Pool{p.page_table, p.refs, p.table_rows, p.table_stride, static_cast<int>(p.pages), p.page_rows,
+                static_cast<int>(segment_pages(p.pages))};
 }
 
 }  // namespace
@@ -460,10 +578,10 @@ int qk_pages_resize(const qk_page_pool *pool, const int32_t *begins, const int32
     if (int s = qk::check_space(where, pool, workspace, workspace_bytes)) return s;
     const qk::Pool p = qk::pool_of(*pool);
     const qk::Space s = qk::space_of(*pool, workspace);
-    const dim3 rows(pool->table_rows);
-    hipLaunchKernelGGL(qk::resize_look_kernel, rows, dim3(qk::kRowThreads), 0, qk::S(stream), p, s, begins, lengths);
-    hipLaunchKernelGGL(qk::give_kernel, dim3(1), dim3(qk::kScanThreads), 0, qk::S(stream), p, s, missing);
-    hipLaunchKernelGGL(qk::resize_fill_kernel, rows, dim3(qk::kRowThreads), 0, qk::S(stream), p, s, begins, lengths);
+    const dim3 rows((pool->table_rows + qk::kRowWaves - 1) / qk::kRowWaves), threads(64 * qk::kRowWaves);
+    hipLaunchKernelGGL(qk::resize_look_kernel, rows, threads, 0, qk::S(stream), p, s, begins, lengths);
+    hipLaunchKernelGGL(qk::count_kernel, dim3(1 + (p.pages - 1) / p.segment + 1), dim3(qk::kScanThreads), 0, qk::S(stream), p, s);
+    hipLaunchKernelGGL(qk::resize_fill_kernel, rows, threads, 0, qk::S(stream), p, s, begins, lengths, missing);
     return qk::launch_status("qk_pages_resize launch");
 }
 
@@ -477,10 +595,10 @@ int qk_pages_fork(const qk_page_pool *pool, const int32_t *parents, const int32_
     if (int s = qk::check_space(where, pool, workspace, workspace_bytes)) return s;
     const qk::Pool p = qk::pool_of(*pool);
     const qk::Space s = qk::space_of(*pool, workspace);
-    const dim3 rows(pool->table_rows);
-    hipLaunchKernelGGL(qk::fork_look_kernel, rows, dim3(qk::kRowThreads), 0, qk::S(stream), p, s, parents, lengths);
-    hipLaunchKernelGGL(qk::give_kernel, dim3(1), dim3(qk::kScanThreads), 0, qk::S(stream), p, s, missing);
-    hipLaunchKernelGGL(qk::fork_fill_kernel, rows, dim3(qk::kRowThreads), 0, qk::S(stream), p, s, parents, lengths);
+    const dim3 rows((pool->table_rows + qk::kRowWaves - 1) / qk::kRowWaves), threads(64 * qk::kRowWaves);
+    hipLaunchKernelGGL(qk::fork_look_kernel, rows, threads, 0, qk::S(stream), p, s, parents, lengths);
+    hipLaunchKernelGGL(qk::count_kernel, dim3(1 + (p.pages - 1) / p.segment + 1), dim3(qk::kScanThreads), 0, qk::S(stream), p, s);
+    hipLaunchKernelGGL(qk::fork_fill_kernel, rows, threads, 0, qk::S(stream), p, s, parents, lengths, missing);
     if (int status = qk::launch_status("qk_pages_fork launch")) return status;
     const int most = static_cast<int>(std::min<int64_t>(pool->table_rows, pool->pages));
     if (int status = qk::copy_pages(pool->layers, pool->n_layers, pool->pages, s.source, s.list, s.counts, most, qk::S(stream)))
