@@ -509,7 +509,7 @@ __device__ __forceinline__ void load_query(const float *qrow, int g, float scale
 // takes registers beyond that (fp16 rows of 128, 4 sequences of 8000: 33 us, with
 // the bound 28).
 template <int HD, int TYPE, bool TERMS>
-__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel(PagedAttn a) {
+__global__ __launch_bounds__(256, 2) void paged_attention_kernel(PagedAttn a) {
     constexpr int NS = HD / 32, NC = HD / 16, kRow = code_bytes(TYPE, HD);
     constexpr bool kScaled = TYPE != QK_TYPE_F16;
     __shared__ float meet[3][HD * 16 + 64];
@@ -552,9 +552,19 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
         seen = max(seen, prefix_rows(a, s) - 1);
     }
 
+    // (Of 256 dimensions in LDS, read for each tile: two workgroups a CU then, and 1340
+    // tokens in four prompts over float8 rows, 8 heads, take 36 us, not 47.)
+    constexpr bool kShared = HD > 128;
     half8 qh[NS], ql[NS];
     float qscale;
     load_query<HD, TYPE, NS>(a.q + (s.first + tok) * a.ldq + static_cast<int64_t>(h * G + own) * HD, g, a.scale, qh, ql, qscale);
+    __shared__ half8 queries[kShared ? 2 : 1][kShared ? NS : 1][64];
+    if constexpr (kShared) {
+        if (wave == 0)
+            #pragma unroll
+            for (int x = 0; x < NS; ++x) queries[0][x][lane] = qh[x], queries[1][x][lane] = ql[x];
+        __syncthreads();
+    }
 
     float4v o[NC];
     #pragma unroll
@@ -636,13 +646,15 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
             #pragma unroll
             for (int hf = 0; hf < 2; ++hf) km[hf].set(t.k.mults[hf], t.k.mults[hf], mult_sel(g));
         #pragma unroll
-        for (int x = 0; x < NS; ++x)
+        for (int x = 0; x < NS; ++x) {
+            const half8 upper = kShared ? queries[0][kShared ? x : 0][lane] : qh[x], lower = kShared ? queries[kShared ? 1 : 0][kShared ? x : 0][lane] : ql[x];
             #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
                 const half8 k = t.k.operand(hf, x, km[hf], codes);
-                st[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[x], st[hf], 0, 0, 0);
-                st[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[x], st[hf], 0, 0, 0);
+                st[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, lower, st[hf], 0, 0, 0);
+                st[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, upper, st[hf], 0, 0, 0);
             }
+        }
         // Register r of half hf: row t0 + 16 hf + 4 g + r.
         float mx = -INFINITY, vtop = 0.f;
         bool one = false;
@@ -793,19 +805,29 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_attention_kernel
     int t0 = begin + wave * kTile;
     if (t0 < end) {
         const int final = t0 + (end - 1 - t0) / kStep * kStep;
-        Tile tiles[2];
-        load(tiles[0], t0, pages_of(t0));
-        Pages ahead = pages_of(min(t0 + kStep, final));
-        for (bool more = true; more;) {
-            #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                load(tiles[i ^ 1], min(t0 + kStep, final), ahead);
-                asm volatile("" ::: "memory");   // or they would sink to where the tile is known to be needed
-                ahead = pages_of(min(t0 + 2 * kStep, final));
-                take(tiles[i], t0);
-                if ((t0 += kStep) >= end) {
-                    more = false;
-                    break;
+        if constexpr (kShared) {   // the other workgroup of the CU hides the loads
+            Pages ahead = pages_of(t0);
+            for (; t0 < end; t0 += kStep) {
+                Tile tile;
+                load(tile, t0, ahead);
+                ahead = pages_of(min(t0 + kStep, final));
+                take(tile, t0);
+            }
+        } else {
+            Tile tiles[2];
+            load(tiles[0], t0, pages_of(t0));
+            Pages ahead = pages_of(min(t0 + kStep, final));
+            for (bool more = true; more;) {
+                #pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    load(tiles[i ^ 1], min(t0 + kStep, final), ahead);
+                    asm volatile("" ::: "memory");   // or they would sink to where the tile is known to be needed
+                    ahead = pages_of(min(t0 + 2 * kStep, final));
+                    take(tiles[i], t0);
+                    if ((t0 += kStep) >= end) {
+                        more = false;
+                        break;
+                    }
                 }
             }
         }
@@ -1867,10 +1889,12 @@ int attend_launch(const PagedAttn &a, hipStream_t stream) {
     if (a.few_rows > 0)
         hipLaunchKernelGGL((paged_attention_kernel<HD, TYPE, TERMS>),
                            grid(std::min<int64_t>(rows, a.few_rows), kRowTile, a.splits[0]), dim3(256), 0, stream, a);
-    constexpr size_t kLds = 2 * Chunk<HD, TYPE>::kBuffer;
-    if (rows > a.few_rows)
-        hipLaunchKernelGGL((paged_chunk_kernel<HD, TYPE, TERMS>), grid(rows, kChunkRows, a.splits[1]), dim3(256), kLds,
-                           stream, a);
+    if constexpr (HD <= 128 || !(TERMS || TYPE == QK_TYPE_I4)) {   // (the others have no chunks)
+        constexpr size_t kLds = 2 * Chunk<HD, TYPE>::kBuffer;
+        if (rows > a.few_rows)
+            hipLaunchKernelGGL((paged_chunk_kernel<HD, TYPE, TERMS>), grid(rows, kChunkRows, a.splits[1]), dim3(256), kLds,
+                               stream, a);
+    }
     return launch_status("qk_paged_attention_f32 launch");
 }
 

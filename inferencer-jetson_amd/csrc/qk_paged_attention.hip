@@ -78,14 +78,16 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
 // nor type.
 constexpr int kFewRows = 64, kManyUnits = 256;
 constexpr int64_t kManyPairs = 3 << 22;
+// Heads of 256 dimensions of 4-bit rows, or with terms, all take the first (all_few),
+// whose workgroups are two a CU, not one: 2048 tokens over 4000 4-bit rows 530 us and
+// 583 by the chunk kernel, 8 sequences of 300 over 1000 187 and 266, 2048 over 4000
+// float8 rows with capped scores 283 and 380; of fp16 ones 383 and 385, through a
+// window 307 and 348 or (1024) 184 and 169, over none 207 and 252.
 // Query rows a KV head up to which a sequence of this call takes the first
 // kernel; a call of one sequence launches one of the two.
-int few_rows(const qk_paged_batch &b, int heads, int kv_heads) {
+int few_rows(const qk_paged_batch &b, int heads, int kv_heads, bool all_few) {
     const int64_t rows = static_cast<int64_t>(b.max_count) * (heads / kv_heads);
-    if (rows <= kFewRows) return INT32_MAX;
-#ifdef QK_FORCE
-    return QK_FORCE ? (b.n_seqs == 1 ? 0 : kFewRows) : INT32_MAX;
-#endif
+    if (rows <= kFewRows || all_few) return INT32_MAX;
     const int64_t units = (rows + kChunkRows - 1) / kChunkRows * kv_heads * b.n_seqs;
     const double pairs = static_cast<double>(b.n_tokens) * heads * b.max_rows;
     if (units < kManyUnits && pairs < kManyPairs) return INT32_MAX;
@@ -106,8 +108,8 @@ int few_rows(const qk_paged_batch &b, int heads, int kv_heads) {
 struct Splits {
     int few, many;
 };
-Splits wanted_splits(const qk_paged_batch &b, int heads, int kv_heads, int head_dim) {
-    const int64_t few = few_rows(b, heads, kv_heads), rows = static_cast<int64_t>(b.max_count) * (heads / kv_heads);
+Splits wanted_splits(const qk_paged_batch &b, int heads, int kv_heads, int head_dim, bool all_few) {
+    const int64_t few = few_rows(b, heads, kv_heads, all_few), rows = static_cast<int64_t>(b.max_count) * (heads / kv_heads);
     const int64_t per_tile = static_cast<int64_t>(kv_heads) * b.n_seqs;
     const int64_t round = head_dim > 128 ? 256 : 512;
     Splits splits{1, 1};
@@ -163,9 +165,16 @@ qk_paged_batch planned(const qk_paged_batch &b, int window) {
     return p;
 }
 
+// Whether all query rows of a call take the first kernel.
+bool all_few(int type, bool terms, int head_dim) { return head_dim > 128 && (terms || type == QK_TYPE_I4); }
+
+// (Of any cache type, with any terms of this window.)
 size_t workspace_bytes(const qk_paged_batch &batch, int heads, int kv_heads, int head_dim, int window) {
-    const Splits splits = wanted_splits(planned(batch, window), heads, kv_heads, head_dim);
-    const int most = std::max(splits.few, splits.many);
+    int most = 1;
+    for (const bool few : {false, all_few(QK_TYPE_I4, true, head_dim)}) {
+        const Splits splits = wanted_splits(planned(batch, window), heads, kv_heads, head_dim, few);
+        most = std::max({most, splits.few, splits.many});
+    }
     return most > 1 ? most * split_bytes(batch, heads, head_dim) : 0;
 }
 
@@ -233,7 +242,9 @@ int qk_paged_attention_terms_f32(const qk_paged_kv *kv, const qk_paged_batch *ba
     const qk_paged_batch plan_batch = qk::planned(*batch, t.window);
     const size_t per = qk::split_bytes(*batch, heads, kv->head_dim);
     const int64_t fit = workspace ? static_cast<int64_t>(workspace_bytes / per) : 0;
-    const qk::Splits wanted = qk::wanted_splits(plan_batch, heads, kv->kv_heads, kv->head_dim);
+    const bool with_terms = t.cap > 0.f || t.window > 0 || t.slopes || t.prefix;
+    const bool few = qk::all_few(kv->type, with_terms, kv->head_dim);
+    const qk::Splits wanted = qk::wanted_splits(plan_batch, heads, kv->kv_heads, kv->head_dim, few);
     // Splits of whole rounds of a workgroup's tiles.
     auto plan = [&](int kind, int splits, int round) {
         const int64_t n = std::min<int64_t>(splits, fit < 2 ? 1 : fit), rows = plan_batch.max_rows;
@@ -241,7 +252,7 @@ int qk_paged_attention_terms_f32(const qk_paged_kv *kv, const qk_paged_batch *ba
         a.split_rows[kind] = static_cast<int>(each);
         a.splits[kind] = static_cast<int>((rows + each - 1) / each);
     };
-    a.few_rows = qk::few_rows(plan_batch, heads, kv->kv_heads);
+    a.few_rows = qk::few_rows(plan_batch, heads, kv->kv_heads, few);
     plan(0, wanted.few, 4 * qk::kTile);
     plan(1, wanted.many, qk::kChunkTile);
     a.part_splits = std::max(a.splits[0], a.splits[1]);
@@ -252,7 +263,7 @@ int qk_paged_attention_terms_f32(const qk_paged_kv *kv, const qk_paged_batch *ba
     // (In place it may be: a workgroup reads its query rows before it writes them.)
     if ((q != out || ldq != ldout) && qk::rows_meet(q, ldq, dim, out, ldout, dim, batch->n_tokens))
         return qk::fail(QK_ERR_INVALID_ARG, "qk_paged_attention_f32: out overlaps a part of q");
-    return qk::launch(a, t.cap > 0.f || t.window > 0 || t.slopes || t.prefix, qk::S(stream));
+    return qk::launch(a, with_terms, qk::S(stream));
 }
 
 }  // extern "C"
