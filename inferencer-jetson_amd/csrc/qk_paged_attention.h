@@ -55,9 +55,9 @@ int attend_i8(const PagedAttn &a, bool terms, hipStream_t stream);
 int attend_e4m3(const PagedAttn &a, bool terms, hipStream_t stream);
 int attend_i4(const PagedAttn &a, bool terms, hipStream_t stream);
 
-// Rows of a sequence's prefix that there are.
+// Rows of a sequence's prefix that there are (a negative one is none).
 __device__ __forceinline__ int prefix_rows(const PagedAttn &a, const qk_paged_seq &s) {
-    return a.prefix ? min(a.prefix[blockIdx.y], s.pos + s.count) : 0;
+    return a.prefix ? max(min(a.prefix[blockIdx.y], s.pos + s.count), 0) : 0;
 }
 // Where the rows that a windowed sequence's splits divide begin: a multiple of 64
 // (a tile's rows lie in whole groups of 16 of a page), no row that a token sees

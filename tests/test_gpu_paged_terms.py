@@ -140,6 +140,20 @@ def test_masked_rows_may_hold_anything(qk, torch_gpu, kind, seqs, wide):
     assert rel_l2(got[~sees], want[~sees]) < 4 * TOL
 
 
+@pytest.mark.parametrize("kind", ["f16", "i4"])
+@pytest.mark.parametrize("seqs", ["decode", "chunk", "mixed"])
+def test_prefixes_at_the_ends_of_the_range(qk, torch_gpu, kind, seqs, wide):
+    """The least and the largest number: no prefix, and all rows that there are."""
+    rng = np.random.default_rng(7)
+    s = SEQS[seqs]
+    pool = ref.Pool(rng, kind, 2, 64, 16, s)
+    pool.poison(pool.unused())
+    q = queries(rng, pool, 8)
+    for window in (0, 2 ** 31 - 1):
+        t = dict(prefix=np.array([(-2 ** 31, 2 ** 31 - 1, -1)[i % 3] for i in range(len(s))], dtype=np.int32), window=window)
+        assert rel_l2(run(qk, torch_gpu, pool, q, 8, wide, **t), pool.attention(q, 8, **t)) < TOL
+
+
 def test_rows_that_see_nothing(qk, torch_gpu, wide):
     """A window of which every page is absent: zeros."""
     rng = np.random.default_rng(5)
