@@ -188,3 +188,49 @@ def test_large_keys(qk, torch_gpu, wide):
         q = queries(rng, pool, 4) * np.float32(1e-36)
         t = dict(cap=10.0, window=100, slopes=slopes(4))
         assert rel_l2(run(qk, torch_gpu, pool, q, 4, wide, **t), pool.attention(q, 4, **t)) < TOL
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3", "i4"])
+@pytest.mark.parametrize("seqs", ["decode", "chunk", "mixed"])
+@pytest.mark.parametrize("terms", ["window", "all"])
+def test_values_far_apart(qk, torch_gpu, kind, seqs, terms, wide):
+    """Value rows 2^60 apart: each token's own, by the rows that it sees.  A product of
+    weight and value is within the score's error of itself (or 2^-32 of the token's
+    largest), and few of them make up a token's sum: three times TOL of each head's."""
+    rng = np.random.default_rng(11)
+    s = SEQS[seqs]
+    pool = ref.Pool(rng, kind, 2, 64, 16, s)
+    pool.value = list((ref.encode4 if kind == "i4" else lambda x: ref.paged_ref.encode(x, kind))(
+        (rng.standard_normal((pool.pages, 2, 16, 64)) * np.exp2(rng.uniform(-30, 30, (pool.pages, 1, 16, 1)))).astype(np.float32)))
+    q = queries(rng, pool, 8)
+    t = of(TERMS[terms], 8, s)
+    got, want = run(qk, torch_gpu, pool, q, 8, wide, **t).reshape(-1, 64), pool.attention(q, 8, **t).reshape(-1, 64)
+    norm = np.linalg.norm(want, axis=1)
+    assert (np.linalg.norm(got - want, axis=1) <= 3 * TOL * norm).all()
+
+
+@pytest.mark.parametrize("kind", ["f16", "i8", "i4"])
+@pytest.mark.parametrize("heads", [8, 16])
+def test_rows_apart_in_place_and_left_out(qk, torch_gpu, kind, heads):
+    """Strided queries and outputs, outputs in the queries' place, a sequence that does
+    not fit the batch and tokens of none: as they were."""
+    t = torch_gpu
+    rng = np.random.default_rng(12)
+    pool = ref.Pool(rng, kind, 2, 64, 16, [(1, 40), (1, 300), (1, 0), (1, 90)])
+    q = queries(rng, pool, heads)
+    terms = dict(cap=10.0, window=200)
+    want = pool.attention(q, heads, **terms)
+    pool.seqs[1, 2] = 2 ** 31 - 2   # its position
+    kv, batch = pool.dev(qk, t, max_rows=400, n_tokens=6)
+    big = t.full((6, heads * 64 + 12), 7.0, device="cuda")
+    rows = big[:, 4: 4 + heads * 64]
+    rows[:4] = to_dev(t, q)
+    out = t.full((6, heads * 64 + 8), np.nan, device="cuda")[:, : heads * 64]
+    ws = t.full((qk.paged_attention_workspace_bytes(batch, heads, 2, 64, window=200),), 0xFF, dtype=t.uint8, device="cuda")
+    qk.paged_attention(kv, batch, rows, out, heads, workspace=ws, **terms)
+    got = out.cpu().numpy()
+    assert rel_l2(got[[0, 2, 3]], want[[0, 2, 3]]) < TOL and np.isnan(got[[1, 4, 5]]).all()
+    qk.paged_attention(kv, batch, rows, rows, heads, workspace=ws, **terms)
+    assert np.array_equal(rows.cpu().numpy()[[0, 2, 3]], got[[0, 2, 3]])
+    assert np.array_equal(rows.cpu().numpy()[1], q[1]) and (rows[4:] == 7).all()
+    assert (big[:, :4] == 7).all() and (big[:, 4 + heads * 64:] == 7).all()
