@@ -503,11 +503,10 @@ __device__ __forceinline__ void load_query(const float *qrow, int g, float scale
 // LDS.  Few query rows leave the cache as the bound, so nothing is staged: a lane
 // loads its own share of both operands, the next tile's while this one is
 // multiplied.  64 sequences over 1000 to 8000 rows, 8 KV heads of 128 int8 values:
-// 611 MB in 136 us, 4.5 TB/s (a copy reaches 4.7, a plain reading 6.15); one over
+// 611 MB in 124 us, 4.9 TB/s (a copy reaches 4.95, a plain reading 6.15); one over
 // 700 rows of 64 fp16 values: 5.9 us, the latency of its loads, and 3.1 of the
-// merge.  Two workgroups a CU up to 128 dimensions: left to itself the compiler
-// takes registers beyond that (fp16 rows of 128, 4 sequences of 8000: 33 us, with
-// the bound 28).
+// merge.  Two workgroups a CU: left to itself the compiler takes registers beyond
+// that (fp16 rows of 128, 4 sequences of 8000: 33 us, with the bound 28).
 template <int HD, int TYPE, bool TERMS>
 __global__ __launch_bounds__(256, 2) void paged_attention_kernel(PagedAttn a) {
     constexpr int NS = HD / 32, NC = HD / 16, kRow = code_bytes(TYPE, HD);
@@ -904,6 +903,9 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(PagedAttn a) {
 // product's columns the first of a query row's holds the weights' upper halves, the
 // second the lower ones, added at the end: one matrix instruction for two.  Rows
 // pair as 4 g + k of a tile's two halves, so that a lane's weights are whole pairs.
+// 64 sequences over 1000 to 8000 4-bit rows, 8 KV heads of 128: 332 MB in 90 us, the
+// vector instructions 55 % of the issue slots (404 a tile; the 16-row kernel's 640
+// took 124 us); its loads alone take 75.
 // Lanes of four: the value of lane `from` of each.
 template <int A, int B, int C, int D>
 __device__ __forceinline__ uint32_t quad(uint32_t v) {
@@ -1317,7 +1319,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_decode_kernel(Pa
 // tokens over 8192 earlier rows, 32 heads of 128 float8 values, are 620 GFLOP of
 // them, in 616 to 645 us 1.0 PFLOP/s, where a library product of two fp16 matrices
 // of 8192 reaches 1.15 (both below the instructions' peak, at a clock of 1.9 GHz).
-// The 16-row kernel took 1150 us.  Short chunks are bound by the latency of a
+// The 16-row kernel took 1150 us.  Of 4-bit rows 671 us, three instructions a pair of
+// codes where float8 takes one.  Short chunks are bound by the latency of a
 // workgroup's steps: 517 tokens over 600, 24 heads, 31 us and 7.5 of the merge,
 // where the matrix instructions are 10.
 constexpr int kChunkTile = 64, kChunkRows = 128;

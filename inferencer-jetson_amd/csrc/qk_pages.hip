@@ -251,7 +251,10 @@ __device__ __forceinline__ int find_pages(const Pool &p, const Space &s, int bas
 
 // ------------------------------------------------------------- resize --
 
-constexpr int kRowWaves = 4;   // rows of a workgroup, a wave each
+// Rows of a workgroup, a wave each.  256 rows of 512 entries over 65536 pages: 3.4 us to
+// look, 4.3 to count, 4.8 to fill, all of them a launch and a chain of three or four
+// loads.  (Bits walked one by one up to a row's first rank: 8.5 to fill.)
+constexpr int kRowWaves = 4;
 
 __device__ __forceinline__ int row_of_wave() {
     return blockIdx.x * kRowWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -402,7 +405,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void fork_fill_kernel(Pool p, Space
 // ------------------------------------------------------------ compact --
 
 // Of `live` pages held, those numbered live and more move, in order, to the free
-// ones below.
+// ones below.  Three looks at all counts: 5000 pages in 16 us, beside 900 of copies.
 __global__ __launch_bounds__(kScanThreads) void compact_look_kernel(Pool p, Space s, int32_t *moved) {
     __shared__ u64 part[kScanThreads / 64];
     auto nothing = [](int, int) {};
@@ -445,7 +448,9 @@ __global__ __launch_bounds__(256) void compact_table_kernel(Pool p, Space s) {
 // ------------------------------------------------------------- copies --
 
 // A launch copies what up to kParts arrays (keys, values and scales of layers) hold
-// of each pair of pages, in pieces of kPiece bytes, a workgroup a piece.
+// of each pair of pages, in pieces of kPiece bytes, a workgroup a piece, 2048 of them
+// at once.  4.7 GB in and out in 900 us, 5.2 TB/s (torch's copy 4.95); 47 MB, in pieces
+// of 4 and 16 KB, in 21 (with 8192 workgroups 24, and 947 the former).
 constexpr int kParts = 128, kPieceLoads = 4, kPiece = 256 * 16 * kPieceLoads;
 struct Copies {
     char *base[kParts];
