@@ -605,7 +605,10 @@ int qk_pages_resize(const qk_page_pool *pool, const int32_t *begins, const int32
    call (lowest first, in order of c).  Other rows (parents[c] out of range, or c
    itself) stay as they are.  Entries absent in the parent are absent.  Rows may be
    forked from rows that are forked themselves.  missing as above: forks without a
-   page for the last part. */
+   page for the last part.
+   Rows that follow a fork's or its parent's lie in pages of their own.  A row that is
+   cut back (qk_pages_resize) into a page that others hold too still shares it: before
+   new rows are written there, it is to be forked from one of those that hold it. */
 int qk_pages_fork(const qk_page_pool *pool, const int32_t *parents, const int32_t *lengths, int32_t *missing,
                   void *workspace, size_t workspace_bytes, qk_stream stream);
 

@@ -232,3 +232,20 @@ def test_wrapper_refusals(qk, torch_gpu):
                   dict(slopes=t.zeros(4, device="cuda", dtype=t.float64)), dict(window=1 << 31)):
         with pytest.raises(qk.QKError):
             qk.paged_attention(kv, batch, q, out, 4, **terms)
+
+
+def test_a_row_cut_back_into_a_shared_page(qk, torch_gpu):
+    """Forked again from one that holds the page, it goes on without touching it."""
+    rng = np.random.default_rng(4)
+    s = Server(qk, torch_gpu, qk.I4)
+    s.step(rng, [(0, 64)])
+    s.fork([-1, 0] + [-1] * 6, [0, 64] + [0] * 6)
+    s.step(rng, [(1, 5), (0, 1)])
+    s.resize([-1, 40] + [-1] * 6)
+    for layer in s.rows:
+        layer[1] = layer[1][:40]
+    assert int((s.pool.refs > 1).sum()) == 3   # 40 rows of the prompt's 64, in pages of 16
+    s.fork([-1, 0] + [-1] * 6, [0, 40] + [0] * 6)
+    assert int((s.pool.refs > 1).sum()) == 2
+    s.step(rng, [(1, 30), (0, 1)])
+    s.step(rng, [(0, 1), (1, 1)], window=50)
