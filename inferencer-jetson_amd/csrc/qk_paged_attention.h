@@ -506,9 +506,12 @@ __device__ __forceinline__ void load_query(const float *qrow, int g, float scale
 // 611 MB in 124 us, 4.9 TB/s (a copy reaches 4.95, a plain reading 6.15); one over
 // 700 rows of 64 fp16 values: 5.9 us, the latency of its loads, and 3.1 of the
 // merge.  Two workgroups a CU: left to itself the compiler takes registers beyond
-// that (fp16 rows of 128, 4 sequences of 8000: 33 us, with the bound 28).
-template <int HD, int TYPE, bool TERMS>
-__global__ __launch_bounds__(256, 2) void paged_attention_kernel(PagedAttn a) {
+// that (fp16 rows of 128, 4 sequences of 8000: 33 us, with the bound 28).  Heads of 256
+// need all of a CU's registers for two tiles and the query; SHARED has the query in LDS,
+// read for each tile, and one tile in registers, whose loads a second workgroup hides
+// (attend_launch says when).
+template <int HD, int TYPE, bool TERMS, bool SHARED>
+__global__ __launch_bounds__(256, HD <= 128 || SHARED ? 2 : 1) void paged_attention_kernel(PagedAttn a) {
     constexpr int NS = HD / 32, NC = HD / 16, kRow = code_bytes(TYPE, HD);
     constexpr bool kScaled = TYPE != QK_TYPE_F16;
     __shared__ float meet[3][HD * 16 + 64];
@@ -521,7 +524,8 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(PagedAttn a) {
     const int h = unit % kvh, row0 = unit / kvh * kRowTile;
     const int rows = s.count * G;
     if (row0 >= rows || rows > a.few_rows) return;
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63;
+    int n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
     // This lane's query row, the last row it sees, and the rows the tile sees.
@@ -551,14 +555,11 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(PagedAttn a) {
         seen = max(seen, prefix_rows(a, s) - 1);
     }
 
-    // (Of 256 dimensions in LDS, read for each tile: two workgroups a CU then, and 1340
-    // tokens in four prompts over float8 rows, 8 heads, take 36 us, not 47.)
-    constexpr bool kShared = HD > 128;
     half8 qh[NS], ql[NS];
     float qscale;
     load_query<HD, TYPE, NS>(a.q + (s.first + tok) * a.ldq + static_cast<int64_t>(h * G + own) * HD, g, a.scale, qh, ql, qscale);
-    __shared__ half8 queries[kShared ? 2 : 1][kShared ? NS : 1][64];
-    if constexpr (kShared) {
+    __shared__ half8 queries[SHARED ? 2 : 1][SHARED ? NS : 1][64];
+    if constexpr (SHARED) {
         if (wave == 0)
             #pragma unroll
             for (int x = 0; x < NS; ++x) queries[0][x][lane] = qh[x], queries[1][x][lane] = ql[x];
@@ -593,7 +594,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(PagedAttn a) {
         bool present[2];
     };
     // Scales (and multipliers) of rows base + 4 g .. + 3.
-    auto scales4 = [&](const float *at, int64_t base, float4v &scale, uint32_t *mults) {
+    auto scales4 = [&](const float *at, int64_t base, int g, float4v &scale, uint32_t *mults) {
         if constexpr (TYPE == QK_TYPE_I4) {
             // (No part of a load unused: its register would be given to something else,
             // which then waits for the load.)
@@ -621,7 +622,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(PagedAttn a) {
         }
         return p;
     };
-    auto load = [&](Tile &t, int t0, const Pages &p) {
+    auto load = [&](Tile &t, int t0, const Pages &p, int n, int g) {
         #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
             t.present[hf] = p.id[hf] >= 0;
@@ -631,8 +632,8 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(PagedAttn a) {
             for (int j = 0; j < 4; ++j)
                 t.v.load(4 * hf + j, static_cast<const char *>(a.kv.value) + (base + 4 * g + j) * kRow, n);
             if constexpr (kScaled) {
-                scales4(a.kv.key_scale, base, t.ks[hf], nullptr);
-                scales4(a.kv.value_scale, base, t.vs[hf], t.vm + 4 * hf);
+                scales4(a.kv.key_scale, base, g, t.ks[hf], nullptr);
+                scales4(a.kv.value_scale, base, g, t.vs[hf], t.vm + 4 * hf);
             }
             if constexpr (TYPE == QK_TYPE_I4)
                 t.k.mults[hf] = __builtin_bit_cast(uint32_t, a.kv.key_scale[2 * (base + n) + 1]);
@@ -646,7 +647,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(PagedAttn a) {
             for (int hf = 0; hf < 2; ++hf) km[hf].set(t.k.mults[hf], t.k.mults[hf], mult_sel(g));
         #pragma unroll
         for (int x = 0; x < NS; ++x) {
-            const half8 upper = kShared ? queries[0][kShared ? x : 0][lane] : qh[x], lower = kShared ? queries[kShared ? 1 : 0][kShared ? x : 0][lane] : ql[x];
+            const half8 upper = SHARED ? queries[0][SHARED ? x : 0][lane] : qh[x], lower = SHARED ? queries[SHARED ? 1 : 0][SHARED ? x : 0][lane] : ql[x];
             #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
                 const half8 k = t.k.operand(hf, x, km[hf], codes);
@@ -798,28 +799,38 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(PagedAttn a) {
     };
     // Two tiles in registers by turns, one multiplied while the other loads; a tile's
     // pages are looked up before its turn to load comes.  Past the wave's last tile
-    // that one again: loads that may be left out would have every wait for a tile wait
-    // for all that is under way.
+    // a line of it again, by all lanes: loads that may be left out would have every wait
+    // for a tile wait for all that is under way.
     constexpr int kStep = 4 * kTile;
     int t0 = begin + wave * kTile;
     if (t0 < end) {
         const int final = t0 + (end - 1 - t0) / kStep * kStep;
-        if constexpr (kShared) {   // the other workgroup of the CU hides the loads
+        if constexpr (SHARED) {
             Pages ahead = pages_of(t0);
             for (; t0 < end; t0 += kStep) {
                 Tile tile;
-                load(tile, t0, ahead);
+                load(tile, t0, ahead, n, g);
                 ahead = pages_of(min(t0 + kStep, final));
                 take(tile, t0);
             }
+        } else if (t0 == final) {
+            // One tile, as of short splits: nothing is loaded beside it (8 sequences of 700
+            // rows, 8 KV heads of 128 fp16 values, 11.0 us, with a second tile's loads 12.8).
+            // What follows from the lane's numbers is computed for it alone: shared with the
+            // loop's it spills (64 sequences of 3000 rows 154 us, 138 without).
+            asm volatile("" : "+v"(n), "+v"(g));
+            Tile tile;
+            load(tile, t0, pages_of(t0), n, g);
+            take(tile, t0);
         } else {
             Tile tiles[2];
-            load(tiles[0], t0, pages_of(t0));
+            load(tiles[0], t0, pages_of(t0), n, g);
             Pages ahead = pages_of(min(t0 + kStep, final));
             for (bool more = true; more;) {
                 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    load(tiles[i ^ 1], min(t0 + kStep, final), ahead);
+                    const int keep = t0 == final ? 0 : 63;
+                    load(tiles[i ^ 1], min(t0 + kStep, final), ahead, n & keep, g & keep);
                     asm volatile("" ::: "memory");   // or they would sink to where the tile is known to be needed
                     ahead = pages_of(min(t0 + 2 * kStep, final));
                     take(tiles[i], t0);
@@ -1889,9 +1900,21 @@ int attend_launch(const PagedAttn &a, hipStream_t stream) {
             return launch_status("qk_paged_attention_f32 launch");
         }
     }
-    if (a.few_rows > 0)
-        hipLaunchKernelGGL((paged_attention_kernel<HD, TYPE, TERMS>),
-                           grid(std::min<int64_t>(rows, a.few_rows), kRowTile, a.splits[0]), dim3(256), 0, stream, a);
+    if (a.few_rows > 0) {
+        const int64_t few = std::min<int64_t>(rows, a.few_rows);
+        const dim3 blocks = grid(few, kRowTile, a.splits[0]);
+        // Heads of 256 without terms: SHARED where there are more workgroups than CUs, of fp16
+        // rows only if they share the cache rows of a sequence.  In us, SHARED second: 16
+        // single tokens over 2000, 16 heads on 8, int8 32.4 and 35.5, fp16 49.9 and 50.5; 64
+        // over 1000, int8 54.8 and 49.2, float8 56.0 and 51.4; 64 over 4500, int8 233 and 228,
+        // fp16 402 and 417; four prompts of 300 over 100, 8 heads on 1, int8 41.6 and 31.3, fp16
+        // 45.6 and 38.7.
+        auto kernel = paged_attention_kernel<HD, TYPE, TERMS, (HD > 128)>;
+        if constexpr (HD > 128 && !TERMS && TYPE != QK_TYPE_I4)
+            if (static_cast<int64_t>(blocks.x) * blocks.y <= 256 || (TYPE == QK_TYPE_F16 && few <= kRowTile))
+                kernel = paged_attention_kernel<HD, TYPE, TERMS, false>;
+        hipLaunchKernelGGL(kernel, blocks, dim3(256), 0, stream, a);
+    }
     if constexpr (HD <= 128 || !(TERMS || TYPE == QK_TYPE_I4)) {   // (the others have no chunks)
         constexpr size_t kLds = 2 * Chunk<HD, TYPE>::kBuffer;
         if (rows > a.few_rows)
