@@ -1436,7 +1436,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
     int up = mine, low = 0, wave_hidden = 0, wave_first = 0;
     if constexpr (TERMS) {
         up = have ? max(mine, prefix - 1) : -1;
-        low = a.window ? mine - a.window + 1 : 0;
+        low = a.window ? max(mine - a.window + 1, 0) : 0;   // (a tile's row is taken off it below)
         wave_hidden = a.window ? wave_last - a.window + 1 : 0;
         wave_first = a.window ? wave_seen - a.window + 1 : 0;
         wave_seen = max(wave_seen, prefix - 1);
