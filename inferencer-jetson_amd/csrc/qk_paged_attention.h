@@ -944,7 +944,7 @@ __device__ __forceinline__ float join_row(float v, Op op) {
 template <int HD, int TYPE, bool TERMS, int DUP>
 __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_decode_kernel(PagedAttn a) {
     constexpr int NS = HD / 32, NC = HD / 16, kRow = code_bytes(TYPE, HD), kRows = 16 / DUP, kOwn = 4 / DUP;
-    constexpr bool kScaled = TYPE != QK_TYPE_F16;
+    static_assert(TYPE != QK_TYPE_F16, "rows have scales");
     __shared__ float meet[3][kRows * (HD + 4)];
     __shared__ half8 queries[2][NS][64];
     const qk_paged_seq s = a.b.seqs[blockIdx.y];
@@ -1034,13 +1034,11 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_decode_kernel(Pa
             #pragma unroll
             for (int k = 0; k < 4; ++k)
                 t.v.load(2 * k + hf, static_cast<const char *>(a.kv.value) + base * kRow + (4 * g + k) * kRow, n);
-            if constexpr (kScaled) {
-                constexpr int kEntry = TYPE == QK_TYPE_I4 ? 2 : 1;
-                #pragma unroll
-                for (int i = 0; i < kOwn; ++i) {
-                    t.ks[hf][i] = (a.kv.key_scale + base * kEntry)[(4 * g + part * kOwn + i) * kEntry];
-                    if constexpr (TYPE != QK_TYPE_I4) t.vs[hf][i] = (a.kv.value_scale + base)[4 * g + part * kOwn + i];
-                }
+            constexpr int kEntry = TYPE == QK_TYPE_I4 ? 2 : 1;
+            #pragma unroll
+            for (int i = 0; i < kOwn; ++i) {
+                t.ks[hf][i] = (a.kv.key_scale + base * kEntry)[(4 * g + part * kOwn + i) * kEntry];
+                if constexpr (TYPE != QK_TYPE_I4) t.vs[hf][i] = (a.kv.value_scale + base)[4 * g + part * kOwn + i];
             }
             if constexpr (TYPE == QK_TYPE_I4) {
                 t.k.mults[hf] = __builtin_bit_cast(uint32_t, (a.kv.key_scale + base * 2)[2 * n + 1]);
@@ -1094,10 +1092,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_decode_kernel(Pa
         for (int i = 0; i < 2 * kOwn; ++i) {
             // An infinite key's score: not a number, whatever its sign.
             x[i] *= qscale;
-            if constexpr (kScaled)
-                x[i] *= fmaf(t.ks[i / kOwn][i % kOwn], 0.f, t.ks[i / kOwn][i % kOwn]);
-            else
-                x[i] = fmaf(x[i], 0.f, x[i]);
+            x[i] *= fmaf(t.ks[i / kOwn][i % kOwn], 0.f, t.ks[i / kOwn][i % kOwn]);
         }
         const int first = t0 + 4 * g + part * kOwn;   // the row of x[0]
         if constexpr (TERMS) {
@@ -1134,36 +1129,29 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_decode_kernel(Pa
         for (int i = 0; i < 2 * kOwn; ++i) {
             const float w = __builtin_amdgcn_exp2f(x[i] - ref);
             l += w;
-            if constexpr (kScaled) {   // a masked row's scale may be anything
-                x[i] = x[i] == -INFINITY ? 0.f : w * t.vs[i / kOwn][i % kOwn];
-                vtop = fmaxf(vtop, fabsf(t.vs[i / kOwn][i % kOwn]));
-            } else {
-                x[i] = w;
-            }
+            x[i] = x[i] == -INFINITY ? 0.f : w * t.vs[i / kOwn][i % kOwn];   // a masked row's scale may be anything
+            vtop = fmaxf(vtop, fabsf(t.vs[i / kOwn][i % kOwn]));
         }
-        if (more || (kScaled && __builtin_amdgcn_ballot_w64(m != -INFINITY && !units.holds(vtop)))) {
-            float fo = f;
-            if constexpr (kScaled) {
-                bool one = false;
+        if (more || __builtin_amdgcn_ballot_w64(m != -INFINITY && !units.holds(vtop))) {
+            bool one = false;
+            #pragma unroll
+            for (int i = 0; i < 2 * kOwn; ++i) one = one || t.vs[i / kOwn][i % kOwn] == 1.f;
+            auto largest = [&] {
+                float y = 0.f;
                 #pragma unroll
-                for (int i = 0; i < 2 * kOwn; ++i) one = one || t.vs[i / kOwn][i % kOwn] == 1.f;
-                auto largest = [&] {
-                    float y = 0.f;
-                    #pragma unroll
-                    for (int i = 0; i < 2 * kOwn; ++i) y = fmaxf(y, fabsf(x[i]));
-                    return join_row<DUP>(y, larger);
-                };
-                float y = largest();
-                units.known *= f;
-                if (__builtin_amdgcn_ballot_w64(one || units.strange(y))) {
-                    const uint32_t live = t.v.live();
-                    #pragma unroll
-                    for (int i = 0; i < 2 * kOwn; ++i)   // (a scale that is not finite stays)
-                        if (!(live >> (2 * (part * kOwn + i % kOwn) + i / kOwn) & 1) && fabsf(x[i]) < INFINITY) x[i] = 0.f;
-                    y = largest();
-                }
-                fo = units.renew(y, join_row<DUP>(vtop, larger), f);
+                for (int i = 0; i < 2 * kOwn; ++i) y = fmaxf(y, fabsf(x[i]));
+                return join_row<DUP>(y, larger);
+            };
+            float y = largest();
+            units.known *= f;
+            if (__builtin_amdgcn_ballot_w64(one || units.strange(y))) {
+                const uint32_t live = t.v.live();
+                #pragma unroll
+                for (int i = 0; i < 2 * kOwn; ++i)   // (a scale that is not finite stays)
+                    if (!(live >> (2 * (part * kOwn + i % kOwn) + i / kOwn) & 1) && fabsf(x[i]) < INFINITY) x[i] = 0.f;
+                y = largest();
             }
+            const float fo = units.renew(y, join_row<DUP>(vtop, larger), f);
             #pragma unroll
             for (int c = 0; c < NC; ++c)
                 #pragma unroll
@@ -1173,7 +1161,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_decode_kernel(Pa
         // first column, lower ones in its others.
         uint4v p;
         {
-            const float k = kScaled ? units.factor : 0x1p15f;
+            const float k = units.factor;
             uint32_t hi[kOwn], lo[kOwn];
             #pragma unroll
             for (int i = 0; i < kOwn; ++i) {
@@ -1257,7 +1245,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_decode_kernel(Pa
     l = join_row<DUP>(l, [](float a, float b) { return a + b; });
     // The waves' means (sums could pass fp32's range), then into wave 0, in wave order.
     auto share_of = [](float l) { return l == 0.f ? 0.f : 1.f / l; };   // no row seen: zeros
-    const int back = (kScaled ? units.exponent() : 0) - 15;
+    const int back = units.exponent() - 15;
     const float inverse = share_of(l);
     #pragma unroll
     for (int c = 0; c < NC; ++c)
