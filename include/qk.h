@@ -592,9 +592,11 @@ size_t qk_pages_workspace_bytes(const qk_page_pool *pool);
    begins[r] / page_rows and from ceil(lengths[r] / page_rows) on give their pages
    back (0: the whole row), absent ones between take free pages, in order of table
    rows and entries the lowest page first.  Pages that the call takes back are free for
-   it.  lengths and begins are device arrays of table_rows values.  missing (device,
-   or NULL) receives the number of entries that got no page (and stay absent), those
-   beyond the table's stride included. */
+   it.  lengths and begins are device arrays of table_rows values.  (Before a step
+   through a window of w rows begins[r] is its first new token's position less w - 1:
+   that token sees the rows from there on.)  missing (device, or NULL) receives the
+   number of entries that got no page (and stay absent), those beyond the table's
+   stride included. */
 int qk_pages_resize(const qk_page_pool *pool, const int32_t *begins, const int32_t *lengths, int32_t *missing,
                     void *workspace, size_t workspace_bytes, qk_stream stream);
 
