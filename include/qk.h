@@ -584,7 +584,8 @@ typedef struct qk_page_pool {
 } qk_page_pool;
 
 /* Workspace of the three calls below, 16-byte aligned; calls sharing it, or the
-   pool, must not overlap. */
+   pool, must not overlap.  What a call writes (table, refs, its number, workspace)
+   may share no memory with its other arguments. */
 size_t qk_pages_workspace_bytes(const qk_page_pool *pool);
 
 /* Every table row r with lengths[r] >= 0 comes to hold the pages of its rows

@@ -558,6 +558,26 @@ int check_space(const char *where, const qk_page_pool *p, const void *workspace,
     return QK_OK;
 }
 
+// Whether what a call writes (table, counts, its number, workspace) lies apart from all
+// else that it takes: rows read their lengths while others write.
+int check_apart(const char *where, const qk_page_pool &p, const int32_t *one, const int32_t *two, const int32_t *number,
+                const void *workspace) {
+    struct Span {
+        const void *at;
+        int64_t bytes;
+    };
+    const int64_t rows = static_cast<int64_t>(p.table_rows) * 4;
+    const Span all[] = {{p.page_table, rows * p.table_stride}, {p.refs, p.pages * 4}, {number, 4},
+                        {workspace, space_entries(p) * 4}, {one, rows}, {two, rows}};
+    for (int i = 0; i < 4; ++i)
+        for (int j = i + 1; j < 6; ++j) {
+            const auto a = reinterpret_cast<uintptr_t>(all[i].at), b = reinterpret_cast<uintptr_t>(all[j].at);
+            if (a && b && (a < b ? b - a < static_cast<uintptr_t>(all[i].bytes) : a - b < static_cast<uintptr_t>(all[j].bytes)))
+                return fail(QK_ERR_INVALID_ARG, std::string(where) + ": page table, refs, number returned or workspace overlaps another argument");
+        }
+    return QK_OK;
+}
+
 Pool pool_of(const qk_page_pool &p) {
     return Pool{p.page_table, p.refs, p.table_rows, p.table_stride, static_cast<int>(p.pages), p.page_rows,
                 static_cast<int>(segment_pages(p.pages))};
@@ -581,6 +601,7 @@ int qk_pages_resize(const qk_page_pool *pool, const int32_t *begins, const int32
     if (!qk::aligned(begins, 4) || !qk::aligned(lengths, 4) || !qk::aligned(missing, 4))
         return qk::fail(QK_ERR_ALIGN, "qk_pages_resize: begins, lengths and missing must be 4-byte aligned");
     if (int s = qk::check_space(where, pool, workspace, workspace_bytes)) return s;
+    if (int s = qk::check_apart(where, *pool, begins, lengths, missing, workspace)) return s;
     const qk::Pool p = qk::pool_of(*pool);
     const qk::Space s = qk::space_of(*pool, workspace);
     const dim3 rows((pool->table_rows + qk::kRowWaves - 1) / qk::kRowWaves), threads(64 * qk::kRowWaves);
@@ -598,6 +619,7 @@ int qk_pages_fork(const qk_page_pool *pool, const int32_t *parents, const int32_
     if (!qk::aligned(parents, 4) || !qk::aligned(lengths, 4) || !qk::aligned(missing, 4))
         return qk::fail(QK_ERR_ALIGN, "qk_pages_fork: parents, lengths and missing must be 4-byte aligned");
     if (int s = qk::check_space(where, pool, workspace, workspace_bytes)) return s;
+    if (int s = qk::check_apart(where, *pool, parents, lengths, missing, workspace)) return s;
     const qk::Pool p = qk::pool_of(*pool);
     const qk::Space s = qk::space_of(*pool, workspace);
     const dim3 rows((pool->table_rows + qk::kRowWaves - 1) / qk::kRowWaves), threads(64 * qk::kRowWaves);
@@ -616,6 +638,7 @@ int qk_pages_compact(const qk_page_pool *pool, int32_t *moved, void *workspace, 
     if (int s = qk::check_pool(where, pool)) return s;
     if (!qk::aligned(moved, 4)) return qk::fail(QK_ERR_ALIGN, "qk_pages_compact: moved must be 4-byte aligned");
     if (int s = qk::check_space(where, pool, workspace, workspace_bytes)) return s;
+    if (int s = qk::check_apart(where, *pool, nullptr, nullptr, moved, workspace)) return s;
     const qk::Pool p = qk::pool_of(*pool);
     const qk::Space s = qk::space_of(*pool, workspace);
     const int64_t entries = static_cast<int64_t>(pool->table_rows) * pool->table_stride;
