@@ -383,7 +383,10 @@ __device__ __forceinline__ float wave_sum(float v) {
 // cap tanh(x / cap) of N scores, inverse 1 / cap.  Where all of a wave are below
 // 0.55 of the cap, which is where trained scores lie, by y + y^3 P(y^2), P the
 // minimax polynomial of (tanh(y) / y - 1) / y^2 there (its error is below fp32's
-// rounding): eight operations instead of two quarter-rate ones and eight.
+// rounding): eight operations instead of two quarter-rate ones and eight.  Why 0.55: the
+// quotient (1 - e) / (1 + e) passes the rounding of e on 1 / sinh(2 y) times, less than
+// once from y = 0.44 on (five times at 0.1), and the polynomial, fitted to a little more
+// than that, has there an error of 4.9e-9 of tanh(y) / y, a twelfth of a rounding.
 // (Four at a time: all of a tile's side by side would take the registers of the sums.)
 template <int N, typename V>
 __device__ __forceinline__ void cap_scores(V &x, float cap, float inverse) {
@@ -503,8 +506,8 @@ __device__ __forceinline__ void load_query(const float *qrow, int g, float scale
 // LDS.  Few query rows leave the cache as the bound, so nothing is staged: a lane
 // loads its own share of both operands, the next tile's while this one is
 // multiplied.  64 sequences over 1000 to 8000 rows, 8 KV heads of 128 int8 values:
-// 611 MB in 124 us, 4.9 TB/s (a copy reaches 4.95, a plain reading 6.15); one over
-// 700 rows of 64 fp16 values: 5.9 us, the latency of its loads, and 3.1 of the
+// 611 MB in 127 us, 4.8 TB/s (a copy reaches 4.95, a plain reading 6.15); one over
+// 700 rows of 64 fp16 values: 5.5 us, the latency of its loads, and 3.7 of the
 // merge.  Two workgroups a CU: left to itself the compiler takes registers beyond
 // that (fp16 rows of 128, 4 sequences of 8000: 33 us, with the bound 28).  Heads of 256
 // need all of a CU's registers for two tiles and the query; SHARED has the query in LDS,
@@ -916,7 +919,7 @@ __global__ __launch_bounds__(256, HD <= 128 || SHARED ? 2 : 1) void paged_attent
 // pair as 4 g + k of a tile's two halves, so that a lane's weights are whole pairs.
 // 64 sequences over 1000 to 8000 4-bit rows, 8 KV heads of 128: 332 MB in 90 us, the
 // vector instructions 55 % of the issue slots (404 a tile; the 16-row kernel's 640
-// took 124 us); its loads alone take 75.
+// take 114 us); its loads alone take 75.
 // Lanes of four: the value of lane `from` of each.
 template <int A, int B, int C, int D>
 __device__ __forceinline__ uint32_t quad(uint32_t v) {
@@ -1318,7 +1321,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_decode_kernel(Pa
 // tokens over 8192 earlier rows, 32 heads of 128 float8 values, are 620 GFLOP of
 // them, in 616 to 645 us 1.0 PFLOP/s, where a library product of two fp16 matrices
 // of 8192 reaches 1.15 (both below the instructions' peak, at a clock of 1.9 GHz).
-// The 16-row kernel took 1150 us.  Of 4-bit rows 671 us, three instructions a pair of
+// The 16-row kernel took 1150 us.  Of 4-bit rows 659 us, three instructions a pair of
 // codes where float8 takes one.  Short chunks are bound by the latency of a
 // workgroup's steps: 517 tokens over 600, 24 heads, 31 us and 7.5 of the merge,
 // where the matrix instructions are 10.
@@ -1877,10 +1880,10 @@ int attend_launch(const PagedAttn &a, hipStream_t stream) {
         return dim3(static_cast<unsigned>((n + tile - 1) / tile * a.kv.kv_heads * splits), a.b.n_seqs);
     };
     // Few rows: 64 sequences over 1000 to 8000 4-bit rows, eight KV heads of 128, in us,
-    // against the 16-row kernel: 4 query rows 90 and 124, 8 102 and 128; 16 sequences over
-    // 4000 of 256, 2 query rows 45 and 68.  With terms, 32 sequences of int8 over windows
-    // of 4096: 60 and 67; of 1000: 23 and 26; float8, 8 query rows over 3000: 52 and 54.
-    // Of fp16 rows the loads alone take the time: 32 sequences over 3000 86 and 80.
+    // against the 16-row kernel: 4 query rows 95 and 114, 8 105 and 111; 16 sequences over
+    // 4000 of 256, 2 query rows 42 and 49.  With terms, 32 sequences of int8 over windows
+    // of 4096: 53 and 57; of 1000: 22.9 and 23.5; float8, 8 query rows over 3000: 42.7 and
+    // 43.1.  Of fp16 rows the loads alone take the time (32 sequences over 3000 86 and 80).
     if constexpr (TYPE == QK_TYPE_I4 || (TERMS && TYPE != QK_TYPE_F16)) {
         if (rows <= 8) {
             auto kernel = rows <= 4 ? paged_decode_kernel<HD, TYPE, TERMS, 4> : paged_decode_kernel<HD, TYPE, TERMS, 2>;

@@ -66,23 +66,26 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
 // if the call's chunks are kManyUnits workgroups of it unsplit, or have kManyPairs
 // pairs of a query row and a cache row.  Four query heads for each of eight KV
 // heads of 128 int8 values, the chunk kernel against the first, in us: one
-// sequence, 68 query rows a KV head over 4000 cache rows (2.2 million pairs) 23
-// and 19, 256 over 4000 (8.3 million) 30 and 30, 1600 over 500 (12 million) 36 and
-// 38, 512 over 4000 (17 million) 40 and 56, 2000 over none (8 million, 128
+// sequence, 68 query rows a KV head over 4000 cache rows (2.2 million pairs) 24
+// and 19, 256 over 4000 (8.3 million) 31 and 29, 1600 over 500 (12 million) 36 and
+// 36, 512 over 4000 (17 million) 42 and 53, 2000 over none (8 million, 128
 // workgroups) 32 and 23; eight sequences, 256 over 500 (9.2 million, 128
-// workgroups) 33 and 33, 68 over 4000 (17 million) 48 and 76, 512 over none (256
-// workgroups) 16 and 28; 64 sequences, 68 over none (512 workgroups) 15 and 30.
+// workgroups) 36 and 31, 68 over 4000 (17 million) 52 and 68, 512 over none (256
+// workgroups) 19 and 28; 64 sequences, 68 over none (512 workgroups) 20 and 30.
 // Eight query heads of 256 for one KV head, one sequence of 2048 tokens over 4000:
-// int8 344 and 413, fp16 355 and 405; eight of 64 over 4000: 88 and 87, 95 and 85,
-// where the first kernel would be the faster one: the rule sees neither head size
-// nor type.
+// int8 344 and 280, fp16 348 and 380; eight of 64 over 4000: 91 and 83, 97 and 83,
+// where the first kernel would be the faster one three times of four: the rule sees
+// neither head size nor type.
 constexpr int kFewRows = 64, kManyUnits = 256;
 constexpr int64_t kManyPairs = 3 << 22;
 // Heads of 256 dimensions of 4-bit rows, or with terms, all take the first (all_few),
-// whose workgroups are two a CU, not one: 2048 tokens over 4000 4-bit rows 530 us and
-// 583 by the chunk kernel, 8 sequences of 300 over 1000 187 and 266, 2048 over 4000
-// float8 rows with capped scores 283 and 380; of fp16 ones 383 and 385, through a
-// window 307 and 348 or (1024) 184 and 169, over none 207 and 252.
+// whose workgroups are two a CU, not one.  In us, and by the chunk kernel: 4-bit rows, 16
+// heads on 8, 2048 tokens over 4000 530 and 583, 8 sequences of 300 over 1000 192 and 264;
+// 8 heads on one, 2048 over 4000 with capped scores, float8 rows 306 and 375, fp16 381 and
+// 384; fp16, 16 heads on 8, capped, over none 208 and 251, 1024 over 6000 and a window of
+// 4096 310 and 353.  The other way round for longer fp16 chunks of 16 heads on 8, which
+// the rule does not see: 2048 over 4000 capped 740 and 712, over 6000 through a window
+// of 4096 602 and 506, of 1024 189 and 163.
 // Query rows a KV head up to which a sequence of this call takes the first
 // kernel; a call of one sequence launches one of the two.
 int few_rows(const qk_paged_batch &b, int heads, int kv_heads, bool all_few) {
@@ -95,14 +98,16 @@ int few_rows(const qk_paged_batch &b, int heads, int kv_heads, bool all_few) {
 }
 
 // Splits of a call's rows, 64 at most.  Few query rows: the workgroups that the
-// chip holds at once, two a CU (one of 256 dimensions), of at least 128 rows, or
-// 256 in more than 32 splits, and none for 256 rows or less.  (One sequence, 8 KV
-// heads of 128 int8 values: 250 rows whole 8.2 us, in two splits 10.2; 2000 rows
-// in 16 splits 9.7, in eight 11.0; 8000 rows in 32 splits 12.5, in 63 14.0.  16
-// sequences of 8000 rows: in one round of workgroups 51 us, in two 55.)  Sequences
-// that fill the chip as they are even out in four splits, if those are long: 64
-// sequences of 1000 to 8000 rows 136 us, 146 whole (of equal lengths the other way
-// round, 217 and 197); of 125 to 1000 rows whole 24, in four splits 31.
+// chip holds at once, two a CU (one of 256 dimensions: 512 of those that are two a CU
+// were no faster), of at least 128 rows, or 256 in more than 32 splits, and none for 256
+// rows or less.  (One sequence, 8 KV heads of 128 int8 values: 250 rows whole 8.0 us, in
+// two splits 9.8; 2000 rows in 16 splits 10.5, in eight 11.6; 8000 rows in 32 splits
+// 13.4, in 63 15.0.  16 sequences of 8000 rows: in one round of workgroups 50 us, in two
+// 52.)  Sequences that fill the chip as they are even out in four splits, if those are
+// long.  64 sequences of 1000 to 8000 rows: 4-bit 91 us and whole 103, int8 130 and 132,
+// fp16 222 and 223; of equal lengths the other way round, of 4500 91 and 78, 126 and 110,
+// 212 and 202, which no call can tell from the others on the host; of 125 to 1000 int8
+// rows whole 22, in four splits 31.
 // Chunks: a round of workgroups likewise, of at least four tiles; those that lie
 // behind all that a chunk's first tokens see end at once and do not count.
 struct Splits {
