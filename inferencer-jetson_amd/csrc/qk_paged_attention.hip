@@ -12,7 +12,9 @@ hipStream_t S(qk_stream s) { return static_cast<hipStream_t>(s); }
 // The splits that reach a token, 64 at most; one wave a (token, head): a lane has a
 // split's maximum and sum, then all lanes the dimensions, eight splits at a time
 // (read one after the other, 64 splits took 10 us longer).
-template <int HD>
+// (MASKED: with a window or a prefix.  Asked for by every wave, of calls without them
+// too, the two took 2 us of 10: four chunks of 512 tokens, 32 heads.)
+template <int HD, bool MASKED>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
     const qk_paged_seq s = a.b.seqs[blockIdx.y];
     if (!paged_seq_ok(s, a.b, a.page_shift)) return;
@@ -24,7 +26,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
     // those beyond this token's own hold nothing of it.
     const int many = static_cast<int64_t>(s.count) * a.group > a.few_rows;
     if (a.splits[many] == 1) return;
-    const int upto = max(s.pos + tok, prefix_rows(a, s) - 1) - first_row(a, s);
+    const int upto = MASKED ? max(s.pos + tok, prefix_rows(a, s) - 1) - first_row(a, s) : s.pos + tok;
     const int live = min(a.splits[many], upto / a.split_rows[many] + 1);
     const float *p = a.parts + (static_cast<int64_t>(s.first + tok) * a.heads + head) * a.part_splits * part_floats(HD);
     constexpr int kD = (HD + 63) / 64, kBatch = 8;
@@ -140,7 +142,8 @@ size_t split_bytes(const qk_paged_batch &b, int heads, int hd) {
 
 template <int HD>
 int merge(const PagedAttn &a, hipStream_t stream) {
-    hipLaunchKernelGGL((paged_merge_kernel<HD>),
+    auto kernel = a.window || a.prefix ? paged_merge_kernel<HD, true> : paged_merge_kernel<HD, false>;
+    hipLaunchKernelGGL(kernel,
                        dim3(static_cast<unsigned>((static_cast<int64_t>(a.b.max_count) * a.heads + 3) / 4), a.b.n_seqs),
                        dim3(256), 0, stream, a);
     return launch_status("qk_paged_attention_f32 launch");
