@@ -1324,7 +1324,9 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_decode_kernel(Pa
 // The 16-row kernel took 1150 us.  Of 4-bit rows 659 us, three instructions a pair of
 // codes where float8 takes one.  Short chunks are bound by the latency of a
 // workgroup's steps: 517 tokens over 600, 24 heads, 31 us and 7.5 of the merge,
-// where the matrix instructions are 10.
+// where the matrix instructions are 10.  Two workgroups a CU; of 64 fp16 values three,
+// for which the compiler has to be asked (8 sequences of 300 tokens over 1000, 32 heads:
+// 89 us, of two 102).
 constexpr int kChunkTile = 64, kChunkRows = 128;
 
 // The units of products of weights and value scales are 2^(15 - ev), ev the exponent
@@ -1376,7 +1378,7 @@ struct Chunk {
 typedef float float16v __attribute__((ext_vector_type(16)));
 
 template <int HD, int TYPE, bool TERMS>
-__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(PagedAttn a) {
+__global__ __launch_bounds__(256, HD > 128 ? 1 : HD == 64 && TYPE == QK_TYPE_F16 && !TERMS ? 3 : 2) void paged_chunk_kernel(PagedAttn a) {
     using C = Chunk<HD, TYPE>;
     constexpr int NS = HD / 16, ND = HD / 32, kRow = code_bytes(TYPE, HD);
     constexpr bool kScaled = TYPE != QK_TYPE_F16;
@@ -1741,7 +1743,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void paged_chunk_kernel(Pag
                 known = c == INFINITY ? 0.f : kCoarse;   // of alike scales, at least
             }
             // Besides: scales are apart, and the tile may hold a product beyond a row's units.
-            if (en != ev || renew || __builtin_amdgcn_ballot_w64(mn > m + kSlack || (room && c != INFINITY && lift > static_cast<float>(room)))) {
+            if (en != ev || renew || __builtin_amdgcn_ballot_w64(mn > (kSlack > 0.f ? m + kSlack : m) || (room && c != INFINITY && lift > static_cast<float>(room)))) {
                 // c is what the weights so far were taken with, rounding and all.
                 const float cn = kScaled ? fminf(c, -mn * by) : mn == -INFINITY ? INFINITY : -mn * (TERMS ? 1.f : qscale);
                 const float f = cn == INFINITY ? 1.f : __builtin_amdgcn_exp2f(cn - c);
