@@ -506,8 +506,8 @@ __device__ __forceinline__ void load_query(const float *qrow, int g, float scale
 // LDS.  Few query rows leave the cache as the bound, so nothing is staged: a lane
 // loads its own share of both operands, the next tile's while this one is
 // multiplied.  64 sequences over 1000 to 8000 rows, 8 KV heads of 128 int8 values:
-// 611 MB in 127 us, 4.8 TB/s (a copy reaches 4.95, a plain reading 6.15); one over
-// 700 rows of 64 fp16 values: 5.5 us, the latency of its loads, and 3.7 of the
+// 611 MB in 126 us, 4.8 TB/s (a copy reaches 4.95, a plain reading 6.15); one over
+// 700 rows of 64 fp16 values: 5.5 us, the latency of its loads, and 3.4 of the
 // merge.  Two workgroups a CU: left to itself the compiler takes registers beyond
 // that (fp16 rows of 128, 4 sequences of 8000: 33 us, with the bound 28).  Heads of 256
 // need all of a CU's registers for two tiles and the query; SHARED has the query in LDS,
